@@ -1,0 +1,307 @@
+// Cross attention, backward.  With P = exp2(scale * log2e * Q K^T - LSE), dP = dO V^T, delta = rowsum(O * dO), dS = P * (dP - delta):
+//   cross_dq_kernel     dQ = scale * dS K               a lane owns a row, the keys go by
+//   cross_dkdv_kernel   dV = P^T dO, dK = scale * dS^T Q  a lane owns a key, the rows of all query heads that share it go by, so
+//                                                       that the sum over the heads is part of the product
+// The first one forms delta and leaves it, beside the log-sum-exp, in the order of the rows for the second.  No atomics: a
+// sum over workgroups (few rows and many keys, or the reverse) goes through float32 parts that are added up in order.
+#pragma once
+#include "sa_bwd.h"
+#include "kv_fwd.h"
+
+namespace kv {
+
+// dQ^T += K^T dS^T, negated, for the tile of TK keys whose first is k0: float32 (16-bit elements: sa::dq2_tile).  g holds -dO.
+template <typename T, int D, int TK, int NF, int DB>
+SA_DEV void dq_tile_f32(f32x16 (&acc)[DB], const T* keys, const T* values, int k0, int L, const typename Elem<T>::Frag (&q)[NF],
+                        const typename Elem<T>::Frag (&g)[NF], float sl2e, float lse, float delta, int lane) {
+#pragma unroll
+  for (int n = 0; n < TK / 32; ++n) {
+    if (k0 + n * 32 >= L) continue;
+    f32x16 s[1], dp[1];
+    clear(s);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) dp[0][i] = delta;
+    mul_rows<T, D>(s, keys, n * 32, q, lane);
+    mul_rows<T, D>(dp, values, n * 32, g, lane);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) s[0][i] = sa::fast_exp2(__builtin_fmaf(s[0][i], sl2e, -lse)) * dp[0][i];
+    if (k0 + n * 32 + 32 > L) {
+      const uint32_t mask = sa::row_mask(0, L - k0 - n * 32, lane >> 5);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) s[0][i] = sa::keep_or_zero(s[0][i], sa::keep_bits(mask, i));
+    }
+    mul_tr<T, D>(acc, keys, n * 32, s[0], lane);
+  }
+}
+
+template <typename T> SA_DEV float dot(typename Elem<T>::Frag a, typename Elem<T>::Frag b, float acc) {
+  if constexpr (Elem<T>::HALF) return sa::dot_frag(a, b, acc);
+  else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) acc = __builtin_fmaf(a[e], b[e], acc);
+    return acc;
+  }
+}
+
+template <typename T, int D, int NW>
+__global__ __launch_bounds__(NW * 64) void cross_dq_kernel(const BwdParams p) {
+  using G = Geom<T, D>;
+  using Frag = typename Elem<T>::Frag;
+  constexpr int TK = fwd_tile<T, D>(), TQ = NW * 32, NT = NW * 64, NF = G::NF, DB = G::DB, STAGE = 2 * TK * D;
+  extern __shared__ __attribute__((aligned(16))) char smem_raw[];
+  T* smem = reinterpret_cast<T*>(smem_raw);   // [stage][K | V][TK][D]
+
+  const int tid = threadIdx.x, lane = tid & 63, c = lane & 31, h = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  int bh, tile;
+  sa::tile_coords(blockIdx.x, gridDim.x, p.tiles, bh, tile);
+  int split = 0;
+  if (p.splits > 1) {
+    const int t = div_by(tile, p.by_splits);
+    split = tile - t * p.splits, tile = t;
+  }
+  const int b = div_by(bh, p.tiles.by_heads), hk = bh - b * p.map.Hkv;
+  const int L = clamped_length(p.lens, p.lens_stride, b, p.Tk);
+  const int rows = p.map.rows(), live = clamped_length(p.q_lens, p.q_lens_stride, b, p.map.T) * p.map.G;
+  const int r0 = tile * TQ, wr0 = r0 + wave * 32, row = wr0 + c;
+  T* const out = reinterpret_cast<T*>(p.dq);
+  if (r0 >= live) {
+    if (p.splits == 1) zero_rows<T, D, NT>(out, p.map, bh, r0, r0 + TQ < rows ? r0 + TQ : rows, tid);
+    return;
+  }
+  int t0, t1;
+  share((L + TK - 1) / TK, p.splits, split, t0, t1);
+  PairCopy<T, D, TK, NW> tiles;
+  if (t0 < t1) {
+    tiles.init(reinterpret_cast<const T*>(p.k) + b * p.k_sb + hk * p.k_sh, p.k_st,
+               reinterpret_cast<const T*>(p.v) + b * p.v_sb + hk * p.v_sh, p.v_st, L - 1, wave, lane);
+    tiles.issue(smem, t0, wave);
+  }
+
+  const float sl2e = fabsf(p.scale_log2e);
+  Frag qf[NF], gf[NF];
+  float lse, delta = 0.0f;
+  {
+    const int r = row < live ? row : live - 1;
+    int t, g;
+    p.map.split(r, t, g);
+    const int64_t head = (int64_t)hk * p.map.G + g;
+    load_row<T, D>(qf, reinterpret_cast<const T*>(p.q) + b * p.q_sb + head * p.q_sh + t * p.q_st, true, lane);
+    load_row<T, D>(gf, reinterpret_cast<const T*>(p.d_o) + b * p.g_sb + head * p.g_sh + t * p.g_st, true, lane);
+    const T* o = reinterpret_cast<const T*>(p.o) + b * p.o_sb + head * p.o_sh + t * p.o_st;
+#pragma unroll
+    for (int i = 0; i < NF; ++i)
+      delta = dot<T>(gf[i], *reinterpret_cast<const Frag*>(o + (i * 2 + h) * Elem<T>::VEC), delta);
+    delta = sa::half_sum(delta);
+    lse = p.lse[p.map.flat(bh, r)];
+    if (lse == -INFINITY || row >= live) lse = INFINITY;   // P = exp2(-inf) = 0: no key is seen, or padding
+    if (split == 0 && h == 0 && row < live) {
+      p.row_lse[(int64_t)bh * rows + row] = lse;
+      p.row_delta[(int64_t)bh * rows + row] = delta;
+    }
+#pragma unroll
+    for (int i = 0; i < NF; ++i) {
+      if (p.scale_log2e < 0.0f) qf[i] = sa::negate<T>(qf[i]);
+      gf[i] = sa::negate<T>(gf[i]);   // the dP accumulator starts at delta and ends at delta - dP
+    }
+  }
+  f32x16 acc[DB], dinit;
+  clear(acc);
+#pragma unroll
+  for (int i = 0; i < 16; ++i) dinit[i] = delta;
+  const sa::WaveWindow win{0, L, 0, L, 0, L};
+  for (int t = t0; t < t1; ++t) {
+    sa::wait_loads<0>();
+    __syncthreads();
+    if (t + 1 < t1) tiles.issue(smem + ((t + 1 - t0) & 1) * STAGE, t + 1, wave);
+    if (wr0 >= live) continue;
+    const T* keys = smem + ((t - t0) & 1) * STAGE;
+    if constexpr (!Elem<T>::HALF)
+      dq_tile_f32<T, D, TK>(acc, keys, keys + TK * D, t * TK, L, qf, gf, sl2e, lse, delta, lane);
+    else
+      sa::dq2_tile<T, D, TK>(acc, keys, keys + TK * D, t * TK, win, qf, gf, sl2e, lse, dinit, lane);
+  }
+  if (p.splits > 1) {
+    if (row < live)
+      sa::store_acc_T<float, D, DB>(p.part + ((int64_t)split * p.B * p.map.Hkv * rows + (int64_t)bh * rows + row) * D, acc, -p.scale, h);
+    return;
+  }
+  if (row >= live) clear(acc);
+  __syncthreads();   // the patches lie over the tile stages
+  store_rows<T, D, DB>(out, p.map, bh, wr0, smem + wave * sa::RowPatch<T, D>::ELEMS, acc, -p.scale, lane);
+}
+
+// dV^T += dO^T P and dK^T += Q^T dS, negated, for the TQ rows from r0 on, or one of them (16-bit elements up to head dimension 128:
+// sa::dkdv2_tile).  v holds -V.
+template <typename T, int D, int TQ, bool WITH_DK, bool WITH_DV, int NF, int NV, int DK, int DV>
+SA_DEV void dkdv_rows(f32x16 (&dk)[DK], f32x16 (&dv)[DV], const T* qt, const T* gt, int r0, int live,
+                          const typename Elem<T>::Frag (&k)[NF], const typename Elem<T>::Frag (&v)[NV], float scale_log2e,
+                          const float* stats, int lane) {   // stats: {lse, delta} of RPW rows after one another
+  constexpr int RPW = TQ / 4;
+  auto place = [](int r) { return r / RPW * 2 * RPW + r % RPW; };
+  const int h = lane >> 5;
+#pragma unroll
+  for (int n = 0; n < TQ / 32; ++n) {
+    if (r0 + n * 32 >= live) continue;
+    f32x16 s[1], dp[1];
+    clear(s);
+    mul_rows<T, D>(s, qt, n * 32, k, lane);
+    if constexpr (WITH_DK) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) dp[0][i] = stats[place(n * 32 + sa::crow(i, h)) + RPW];
+      mul_rows<T, D>(dp, gt, n * 32, v, lane);
+    }
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      s[0][i] = sa::fast_exp2(__builtin_fmaf(s[0][i], scale_log2e, -stats[place(n * 32 + sa::crow(i, h))]));
+      if constexpr (WITH_DK) dp[0][i] *= s[0][i];
+    }
+    if (r0 + n * 32 + 32 > live) {
+      const uint32_t mask = sa::row_mask(0, live - r0 - n * 32, h);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        s[0][i] = sa::keep_or_zero(s[0][i], sa::keep_bits(mask, i));
+        if constexpr (WITH_DK) dp[0][i] = sa::keep_or_zero(dp[0][i], sa::keep_bits(mask, i));
+      }
+    }
+    if constexpr (WITH_DV) mul_tr<T, D>(dv, gt, n * 32, s[0], lane);
+    if constexpr (WITH_DK) mul_tr<T, D>(dk, qt, n * 32, dp[0], lane);
+  }
+}
+
+template <typename T, int D> constexpr int dkdv_tile() { return D * (int)sizeof(T) <= 256 ? 64 : 32; }
+// Bytes of a stage: Q and dO tiles, and lse and delta of their rows.
+template <typename T, int D> constexpr int dkdv_stage() { return 2 * dkdv_tile<T, D>() * (D * (int)sizeof(T) + (int)sizeof(float)); }
+
+// PASS: 0 both gradients, 1 dV, 2 dK.  Head dimension 256 takes a launch for each: two accumulators of 32 x 256 are 256 registers of a
+// lane, the rows of K and V another 128 (float32: 256) of its 512, and in one launch 444 values were spilled.
+template <typename T, int D, int NW, int PASS>
+__global__ __launch_bounds__(NW * 64, (sizeof(T) == 2 && D == 64 ? 3 : 1)) void cross_dkdv_kernel(const BwdParams p) {
+  using G = Geom<T, D>;
+  using Frag = typename Elem<T>::Frag;
+  constexpr bool WITH_DV = PASS != 2, WITH_DK = PASS != 1;
+  constexpr int TQ = dkdv_tile<T, D>(), TKB = NW * 32, NT = NW * 64, NF = G::NF, DB = G::DB, TILE = TQ * D;
+  constexpr int RPW = TQ / NW, STAGE = dkdv_stage<T, D>();
+  extern __shared__ __attribute__((aligned(16))) char smem_raw[];   // [stage]{[Q | dO][TQ][D], [wave]{lse, delta}[RPW]}
+
+  const int tid = threadIdx.x, lane = tid & 63, c = lane & 31, h = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  int bh, tile;
+  sa::tile_coords(blockIdx.x, gridDim.x, p.tiles, bh, tile);
+  int split = 0;
+  if (p.splits > 1) {
+    const int t = div_by(tile, p.by_splits);
+    split = tile - t * p.splits, tile = t;
+  }
+  const int b = div_by(bh, p.tiles.by_heads), hk = bh - b * p.map.Hkv;
+  const int L = clamped_length(p.lens, p.lens_stride, b, p.Tk);
+  const int rows = p.map.rows(), live = clamped_length(p.q_lens, p.q_lens_stride, b, p.map.T) * p.map.G;
+  const int k0 = tile * TKB, wk0 = k0 + wave * 32, key = wk0 + c;
+  const RowMap keys{1, 1, p.Tk, chunk_div(1)};   // K's gradients are rows of one head each
+  T* const dk_out = reinterpret_cast<T*>(p.dk);
+  T* const dv_out = reinterpret_cast<T*>(p.dv);
+  if (k0 >= L || live == 0) {
+    if (p.splits == 1) {
+      const int k1 = k0 + TKB < p.Tk ? k0 + TKB : p.Tk;
+      if constexpr (WITH_DK) zero_rows<T, D, NT>(dk_out, keys, bh, k0, k1, tid);
+      if constexpr (WITH_DV) zero_rows<T, D, NT>(dv_out, keys, bh, k0, k1, tid);
+    }
+    return;
+  }
+  int t0, t1;
+  share((live + TQ - 1) / TQ, p.splits, split, t0, t1);
+
+  const T* const q = reinterpret_cast<const T*>(p.q) + b * p.q_sb + (int64_t)hk * p.map.G * p.q_sh;
+  const T* const g = reinterpret_cast<const T*>(p.d_o) + b * p.g_sb + (int64_t)hk * p.map.G * p.g_sh;
+  const float* const lse_rows = p.row_lse + (int64_t)bh * rows;
+  const float* const delta_rows = p.row_delta + (int64_t)bh * rows;
+  // one head: whole tiles at a constant stride, rows past the last one as zeros.  Several: rows at addresses of their own, the last
+  // one again in place of those past it
+  PairCopy<T, D, TQ, NW> whole;
+  const bool one_head = p.map.G == 1;
+  if (one_head) whole.init(q, p.q_st, g, p.g_st, live - 1, wave, lane);
+  auto issue_tile = [&](int t) {
+    char* const stage = smem_raw + ((t - t0) & 1) * STAGE;
+    T* const dst = reinterpret_cast<T*>(stage);
+    if (lane < 2 * RPW) {   // lanes [0, RPW) fetch lse, [RPW, 2 * RPW) delta
+      int r = t * TQ + wave * RPW + lane % RPW;
+      r = r < live ? r : live - 1;
+      sa::async_copy_f32((lane < RPW ? lse_rows : delta_rows) + r, reinterpret_cast<float*>(stage + 2 * TILE * sizeof(T)) + wave * 2 * RPW);
+    }
+    if (one_head) {
+      whole.issue(dst, t, wave);
+    } else {
+#pragma unroll
+      for (int i = 0; i < (TQ / G::RPI + NW - 1) / NW; ++i) {
+        const int first = (i * NW + wave) * G::RPI;
+        if (first < TQ) {
+          const int in_tile = first + lane / G::CPR;
+          int r = t * TQ + in_tile, tok, head;
+          r = r < live ? r : live - 1;
+          p.map.split(r, tok, head);
+          const int chunk = ((lane % G::CPR) ^ G::swz(in_tile)) * G::VEC;
+          __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(q + (tok * p.q_st + head * p.q_sh + chunk)),
+                                           (SA_LDS void*)(dst + first * D), 16, 0, 0);
+          __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(g + (tok * p.g_st + head * p.g_sh + chunk)),
+                                           (SA_LDS void*)(dst + TILE + first * D), 16, 0, 0);
+        }
+      }
+    }
+  };
+  if (t0 < t1) issue_tile(t0);
+
+  Frag kf[NF], vf[WITH_DK ? NF : 1];
+  {
+    const bool valid = key < L;
+    const int k = valid ? key : L - 1;
+    load_row<T, D>(kf, reinterpret_cast<const T*>(p.k) + b * p.k_sb + hk * p.k_sh + k * p.k_st, valid, lane);
+    if constexpr (WITH_DK) {
+      load_row<T, D>(vf, reinterpret_cast<const T*>(p.v) + b * p.v_sb + hk * p.v_sh + k * p.v_st, valid, lane);
+#pragma unroll
+      for (int i = 0; i < NF; ++i) vf[i] = sa::negate<T>(vf[i]);
+    }
+    if constexpr (Elem<T>::HALF && PASS == 0)
+#pragma unroll
+      for (int i = 0; i < NF; ++i) kf[i] = sa::dkdv2_keys<T, D>(kf[i], p.scale_log2e);
+  }
+  f32x16 dk[WITH_DK ? DB : 1], dv[WITH_DV ? DB : 1];
+  clear(dk);
+  clear(dv);
+  sa::wait_all_loads();
+  const sa::WaveWindow win{0, live, 0, live, 0, wk0 < L ? live : 0};
+  for (int t = t0; t < t1; ++t) {
+    sa::wait_loads<0>();
+    __syncthreads();
+    if (t + 1 < t1) issue_tile(t + 1);
+    const char* const stage = smem_raw + ((t - t0) & 1) * STAGE;
+    const T* const qt = reinterpret_cast<const T*>(stage);
+    const float* const stats = reinterpret_cast<const float*>(stage + 2 * TILE * sizeof(T));
+    if (!win.seen(t * TQ, TQ)) continue;
+    if constexpr (Elem<T>::HALF && PASS == 0) {
+      sa::dkdv2_tile<T, D, TQ, (D == 64 ? 2 : 4)>(dk, dv, qt, qt + TILE, t * TQ, win, kf, vf, p.scale_log2e,
+                                                   [&](int r, f32x4& l4, f32x4& d4) {
+        const float* chunk = stats + (r / RPW) * 2 * RPW + r % RPW;
+        l4 = *reinterpret_cast<const f32x4*>(chunk);
+        d4 = *reinterpret_cast<const f32x4*>(chunk + RPW);
+      }, lane);
+    } else {
+      dkdv_rows<T, D, TQ, WITH_DK, WITH_DV>(dk, dv, qt, qt + TILE, t * TQ, live, kf, vf, p.scale_log2e, stats, lane);
+    }
+  }
+  if (p.splits > 1) {
+    const int64_t each = (int64_t)p.B * p.map.Hkv * p.Tk;
+    if (key < L) {
+      float* part = p.part + ((int64_t)split * 2 * each + (int64_t)bh * p.Tk + key) * D;
+      if constexpr (WITH_DK) sa::store_acc_T<float, D, DB>(part, dk, -p.scale, h);
+      if constexpr (WITH_DV) sa::store_acc_T<float, D, DB>(part + each * D, dv, 1.0f, h);
+    }
+    return;
+  }
+  if (key >= L) clear(dk), clear(dv);
+  __syncthreads();   // the patches lie over the tile stages
+  T* patch = reinterpret_cast<T*>(smem_raw) + wave * sa::RowPatch<T, D>::ELEMS;
+  if constexpr (WITH_DK) store_rows<T, D, DB>(dk_out, keys, bh, wk0, patch, dk, -p.scale, lane);
+  if constexpr (WITH_DV) store_rows<T, D, DB>(dv_out, keys, bh, wk0, patch, dv, 1.0f, lane);
+}
+
+}  // namespace kv

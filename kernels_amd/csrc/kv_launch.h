@@ -1,0 +1,37 @@
+// Launches of the kernels for keys that are not the queries' own, one explicit instantiation per element type and group of head
+// dimensions (1: 256), and the rules by which work is divided.  Each returns 0, a hipError_t or a KV_ERR_* code.
+#pragma once
+#include <algorithm>
+#include "../../include/kv_attention.h"
+#include "kv_bwd.h"
+#include "kv_rows.h"
+
+namespace kv {
+
+template <typename T, int DGROUP> int launch_cross_fwd(const FwdParams& p, int D, hipStream_t st);
+template <typename T, int DGROUP> int launch_cross_dq(const BwdParams& p, int D, hipStream_t st);
+template <typename T, int DGROUP> int launch_cross_dkdv(const BwdParams& p, int D, hipStream_t st);
+template <typename T, int DGROUP> int launch_rows(const RowsParams& p, int D, hipStream_t st);
+template <typename T, int DGROUP> int launch_rows_paged(const RowsParams& p, int D, hipStream_t st);
+template <typename T, int DGROUP> int launch_join(const JoinParams& p, int D, hipStream_t st);
+template <typename T, int DGROUP> int launch_sum(const SumParams& p, int D, hipStream_t st);
+
+constexpr int64_t kMostBlocks = 0x7fffffff;
+inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+constexpr int TILE_ROWS = 128;   // rows (or keys) of a workgroup of the tile kernels: four waves of 32
+constexpr int CUS = 256;
+
+// The tile kernels: with fewer workgroups than CUs the keys (or rows) that each goes through are divided, into shares of at least
+// four tiles, so that there are two workgroups per CU.
+inline int tile_splits(int64_t workgroups, int64_t tiles) {
+  if (workgroups >= CUS || workgroups == 0) return 1;
+  return (int)std::max<int64_t>(1, std::min<int64_t>(2 * CUS / workgroups, tiles / 4));
+}
+
+// The rows kernel serves up to 32 rows of a key head.  Its keys are divided into shares of a fixed length, not by the number of workgroups: a
+// sequence has the same bits alone and in any batch.
+inline bool few_rows(int64_t rows) { return rows <= 32; }
+inline int rows_share(int64_t tiles) { return (int)std::max<int64_t>(16, ceil_div(tiles, 64)); }
+
+}  // namespace kv

@@ -1,0 +1,265 @@
+"""Cross attention on the GPU against the float64 oracle, element by element within bounds counted in roundings
+(oracle/kv_oracle.py), at the sizes, lengths and layouts where it can go wrong."""
+import pytest
+import torch
+
+from cross_attention import cross_attention, cross_attention_reference
+from oracle import kv_oracle
+
+pytestmark = pytest.mark.gpu
+DTYPES = [torch.float32, torch.float16, torch.bfloat16]
+DEV = "cuda:0"
+
+
+def _inputs(B, Hq, Hkv, Tq, Tk, D, dtype, seed=3):
+    g = torch.Generator().manual_seed(seed)
+    return [torch.randn(*s, generator=g).to(dtype) for s in ((B, Hq, Tq, D), (B, Hkv, Tk, D), (B, Hkv, Tk, D), (B, Hq, Tq, D))]
+
+
+def _lens(x):
+    return None if x is None else torch.tensor(x, dtype=torch.int32)
+
+
+def _run(q, k, v, d_o, lens, q_lens, scale=None):
+    leaves = [t.to(DEV).requires_grad_() for t in (q, k, v)]
+    on = [None if x is None else x.to(DEV) for x in (lens, q_lens)]
+    o, lse = cross_attention(*leaves, *on, sm_scale=scale, return_lse=True)
+    grads = torch.autograd.grad(o, leaves, d_o.to(DEV))
+    return dict(zip(("o", "lse", "dq", "dk", "dv"), (o, lse, *grads)))
+
+
+def _check(q, k, v, d_o, lens=None, q_lens=None, scale=None):
+    lens, q_lens = _lens(lens), _lens(q_lens)
+    want = kv_oracle.cross(q, k, v, lens, q_lens, scale, d_o)
+    got = _run(q, k, v, d_o, lens, q_lens, scale)
+    torch.cuda.synchronize()
+    for name in want:
+        kv_oracle.assert_within(name, got[name], want[name])
+    return got
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("D", [16, 32, 64, 128, 256])
+@pytest.mark.parametrize("B,Hq,Hkv,Tq,Tk,lens,q_lens", [
+    (2, 2, 2, 40, 70, [70, 33], [40, 1]),          # one tile and a part of one
+    (3, 4, 2, 150, 200, [1, 0, 200], [150, 7, 0]),   # shared heads, lengths of none and one
+    (1, 6, 2, 67, 129, None, None),                # three heads to a key head: rows cross the tiles
+])
+def test_against_oracle(dtype, D, B, Hq, Hkv, Tq, Tk, lens, q_lens):
+    _check(*_inputs(B, Hq, Hkv, Tq, Tk, D, dtype), lens, q_lens)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("D", [16, 32, 64, 128, 256])
+@pytest.mark.parametrize("Hq,Hkv,Tq,Tk,lens", [(2, 2, 1, 300, [300, 0]), (8, 2, 1, 1100, [1100, 513]), (4, 2, 7, 37, [1, 36]),
+                                               (32, 1, 1, 65, None), (2, 1, 16, 2100, [2100, 31])])
+def test_few_rows(dtype, D, Hq, Hkv, Tq, Tk, lens):
+    """Up to 32 rows of a key head run a kernel of their own, long keys in shares that are joined."""
+    _check(*_inputs(2, Hq, Hkv, Tq, Tk, D, dtype), lens, None if Tq == 1 else [Tq, Tq - 3])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("D", [32, 64, 128, 256])
+@pytest.mark.parametrize("Tq,Tk,lens,q_lens", [(40, 1500, [1500, 260], None), (1500, 40, [40, 3], [1300, 1500]),
+                                               (700, 900, [900, 0], [1, 700])])
+def test_split_work(dtype, D, Tq, Tk, lens, q_lens):
+    """Few workgroups: the keys (for dK and dV the rows) are divided and float32 parts added up."""
+    from kv_attention import _lib
+
+    dt = DTYPES.index(dtype)
+    plain = 2 * ((4 * 2 * Tq * 4 + 255) // 256 * 256)   # lse and delta of all rows
+    assert _lib.load().kv_cross_backward_workspace(2, 4, 2, Tq, Tk, D, dt) > plain
+    _check(*_inputs(2, 4, 2, Tq, Tk, D, dtype), lens, q_lens)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("scale", [-0.3, 0.0, 1.7])
+def test_scales(dtype, scale):
+    q, k, v, d_o = _inputs(1, 2, 1, 70, 90, 64, dtype)
+    _check(q * 0.5, k * 0.5, v, d_o, scale=scale)
+    _check(q[:, :, :5] * 0.5, k * 0.5, v, d_o[:, :, :5], scale=scale)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("Tq", [3, 100])
+def test_large_scores(dtype, Tq):
+    """Scores whose exponentials pass every range, with a maximum that keeps moving."""
+    q, k, v, d_o = _inputs(1, 1, 1, Tq, 333, 64, dtype)
+    k = (k.float() * torch.linspace(0.1, 8, 333)[:, None]).to(dtype)
+    _check(q, k, v, d_o)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("Tq", [5, 140])
+@pytest.mark.parametrize("D", [16, 64, 128, 256])
+@pytest.mark.parametrize("junk", [float("nan"), float("inf"), -float("inf")])
+def test_padding_is_never_used(dtype, Tq, D, junk):
+    q, k, v, d_o = _inputs(3, 4, 2, Tq, 150, D, dtype)
+    lens, q_lens = [150, 41, 0], [Tq - 2, Tq, 3]
+    clean = _run(q, k, v, d_o, _lens(lens), _lens(q_lens))
+    for b in range(3):
+        k[b, :, lens[b]:], v[b, :, lens[b]:] = junk, junk
+        q[b, :, q_lens[b]:], d_o[b, :, q_lens[b]:] = junk, junk
+    dirty = _run(q, k, v, d_o, _lens(lens), _lens(q_lens))
+    for name in clean:
+        assert torch.equal(clean[name], dirty[name]), name
+    for b in range(3):
+        assert not dirty["o"][b, :, q_lens[b]:].any() and not dirty["dq"][b, :, q_lens[b]:].any()
+        assert not dirty["lse"][b, :, q_lens[b]:].any()
+        assert not dirty["dk"][b, :, lens[b]:].any() and not dirty["dv"][b, :, lens[b]:].any()
+    assert (dirty["lse"][2, :, :3] == -float("inf")).all() and not dirty["o"][2].any() and not dirty["dq"][2].any()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("Tq,Tk", [(1, 1), (1, 33), (130, 1), (0, 40), (40, 0), (1, 0)])
+def test_smallest(dtype, Tq, Tk):
+    got = _check(*_inputs(2, 2, 1, Tq, Tk, 64, dtype))
+    if Tk == 0:
+        assert not got["o"].any() and (got["lse"] == -float("inf")).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
+@pytest.mark.parametrize("Tq", [6, 90])
+def test_strides(dtype, Tq):
+    """Views of projection outputs, broadcast heads and batch entries, strides that have to be copied."""
+    B, H, Tk, D = 2, 4, 120, 64
+    g = torch.Generator().manual_seed(8)
+    kv = torch.randn(B, Tk, 2, H, D, generator=g).to(dtype).to(DEV)
+    qs = torch.randn(B, Tq, H, D, generator=g).to(dtype).to(DEV)
+    d_o = torch.randn(B, Tq, H, D, generator=g).to(dtype).to(DEV)
+    wide = torch.randn(B, H, Tk, D + 1, generator=g).to(dtype).to(DEV)
+    one = torch.randn(1, 1, Tk, D, generator=g).to(dtype).to(DEV)
+    lens = torch.tensor([[120, 7], [33, 9]], dtype=torch.int32, device=DEV)[:, 0]
+    for k, v in ((kv[:, :, 0].transpose(1, 2), kv[:, :, 1].transpose(1, 2)), (wide[..., 1:], wide[..., :-1]),
+                 (one.expand(B, H, Tk, D), one.expand(B, H, Tk, D)), (wide[:, :2, :, :D], wide[:, :2, ::1, 1:])):
+        q = qs.transpose(1, 2)
+        leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+        grads = torch.autograd.grad(cross_attention(*leaves, lens), leaves, d_o.transpose(1, 2))
+        plain = [t.detach().contiguous().requires_grad_() for t in (q, k, v)]
+        out = cross_attention(*plain, lens.contiguous())
+        for a, b in zip(grads, torch.autograd.grad(out, plain, d_o.transpose(1, 2).contiguous())):
+            assert torch.equal(a, b)
+        assert torch.equal(out, cross_attention(*leaves, lens))
+
+
+def test_gradients_are_those_of_differences():
+    """Directional derivatives of the float32 forward against the gradients."""
+    q, k, v, d_o = (t.to(DEV) for t in _inputs(2, 4, 2, 45, 60, 32, torch.float32))
+    lens, q_lens = (torch.tensor(x, dtype=torch.int32, device=DEV) for x in ([60, 31], [45, 20]))
+    leaves = [t.clone().requires_grad_() for t in (q, k, v)]
+    grads = torch.autograd.grad(cross_attention(*leaves, lens, q_lens), leaves, d_o)
+    g = torch.Generator().manual_seed(9)
+    for i in range(3):
+        step = torch.randn(leaves[i].shape, generator=g).to(DEV)
+        h = 2.0 ** -6
+        side = []
+        for sign in (1, -1):
+            moved = [t + sign * h * step if j == i else t for j, t in enumerate((q, k, v))]
+            side.append((cross_attention(*moved, lens, q_lens).double() * d_o.double()).sum())
+        slope, want = (side[0] - side[1]) / (2 * h), (grads[i].double() * step.double()).sum()
+        # third derivatives, h^2 / 6 of them, and the float32 rounding of about 8000 outputs, divided by 2 h
+        assert abs(slope - want) <= 2e-3 * abs(want) + 0.5
+
+
+def test_matches_the_plain_reference():
+    q, k, v, _ = (t.to(DEV) for t in _inputs(2, 4, 2, 50, 60, 64, torch.float32))
+    lens, q_lens = (torch.tensor(x, dtype=torch.int32, device=DEV) for x in ([60, 0], [50, 20]))
+    want, valid = cross_attention_reference(q, k, v, lens, q_lens)
+    got = cross_attention(q, k, v, lens, q_lens)
+    assert (got - want).abs().max() < 1e-4 and not got[~valid.expand_as(got)].any()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_same_bits_from_call_to_call(dtype):
+    q, k, v, d_o = _inputs(4, 8, 2, 200, 1000, 64, dtype)
+    first, second = (_run(q, k, v, d_o, _lens([1000, 5, 600, 999]), None) for _ in range(2))
+    for name in first:
+        assert torch.equal(first[name], second[name]), name
+
+
+@pytest.mark.parametrize("Tq", [1, 100])
+def test_backward_without_the_log_sum_exp(Tq):
+    q, k, v, d_o = (t.to(DEV) for t in _inputs(2, 4, 2, Tq, 70, 64, torch.bfloat16))
+    op = torch.ops.alexdremov_cross_attention
+    o, lse = op.forward(q, k, v, None, None, 0.125, True)
+    _, none = op.forward(q, k, v, None, None, 0.125, False)
+    assert none.numel() == 0
+    for a, b in zip(op.backward(q, k, v, None, None, o, lse, d_o, 0.125), op.backward(q, k, v, None, None, o, none, d_o.float(), 0.125)):
+        assert torch.equal(a, b)
+
+
+def test_graph_replays():
+    """Forward and backward captured once and replayed on new values, with eager work in between, on two workspaces."""
+    shapes = [_inputs(2, 4, 2, 40, 1500, 64, torch.bfloat16, seed) for seed in (1, 2, 3)]
+    static = [t.to(DEV) for t in shapes[0]]
+    lens = torch.tensor([1500, 700], dtype=torch.int32, device=DEV)
+
+    def step():
+        leaves = [t.detach().requires_grad_() for t in static[:3]]
+        o = cross_attention(*leaves, lens)
+        few = cross_attention(static[0][:, :, :2].detach(), static[1], static[2], lens)
+        return (o.detach(), few, *torch.autograd.grad(o, leaves, static[3]))
+
+    step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for values in shapes + shapes[:1]:
+        for s, x in zip(static, values):
+            s.copy_(x.to(DEV))
+        want = [t.clone() for t in step()]
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(out, want):
+            assert torch.equal(a, b)
+
+
+def test_streams():
+    """Calls on two streams at once, each with workspaces of its own."""
+    sets = [[t.to(DEV) for t in _inputs(2, 4, 2, 40, 3000, 64, torch.float16, seed)] for seed in (1, 2)]
+
+    def both(x):
+        leaves = [t.detach().requires_grad_() for t in x[:3]]
+        o = cross_attention(*leaves)
+        return (o.detach(), *torch.autograd.grad(o, leaves, x[3]))
+
+    want = [both(x) for x in sets]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in sets]
+    got = [[], []]
+    for _ in range(5):
+        for i, s in enumerate(streams):
+            s.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(s):
+                got[i].append(both(sets[i]))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for r in got[i]:
+            for a, b in zip(r, want[i]):
+                assert torch.equal(a, b)
+
+
+def test_opcheck():
+    q, k, v, _ = (t.to(DEV) for t in _inputs(2, 4, 2, 40, 70, 64, torch.float32))
+    lens = torch.tensor([70, 20], dtype=torch.int32, device=DEV)
+    leaves = [t.requires_grad_() for t in (q, k, v)]
+    torch.library.opcheck(torch.ops.alexdremov_cross_attention.forward.default, (*leaves, lens, None, 0.125, True))
+    out = torch.compile(cross_attention, backend="aot_eager", fullgraph=True)(*leaves, lens)
+    assert torch.equal(out, cross_attention(*leaves, lens))
+    for a, b in zip(torch.autograd.grad(out.sum(), leaves), torch.autograd.grad(cross_attention(*leaves, lens).sum(), leaves)):
+        assert torch.equal(a, b)
+
+
+def test_long_rows_of_keys():
+    """Strides that the 32-bit offsets of one head do not hold are copied."""
+    T, D = 70, 64
+    g = torch.Generator().manual_seed(4)
+    base = torch.zeros(T, (1 << 31) // 70 // 8 * 8, dtype=torch.float16, device=DEV)   # 4 GiB
+    k = torch.randn(T, D, generator=g).half()
+    base[:, :D] = k.to(DEV)
+    strided = base[:, :D][None, None]
+    q = torch.randn(1, 1, 40, D, generator=g).half().to(DEV)
+    assert (T + 1024) * strided.stride(2) * 2 >= 1 << 32
+    plain = k.to(DEV)[None, None]
+    assert torch.equal(cross_attention(q, strided, strided), cross_attention(q, plain, plain))
