@@ -6,6 +6,7 @@
 // sum over workgroups (few rows and many keys, or the reverse) goes through float32 parts that are added up in order.
 #pragma once
 #include "sa_bwd.h"
+#include "sa_bwd_split.h"
 #include "kv_fwd.h"
 
 namespace kv {
@@ -43,11 +44,13 @@ template <typename T> SA_DEV float dot(typename Elem<T>::Frag a, typename Elem<T
   }
 }
 
+template <typename T, int D> constexpr int dq_tile() { return Elem<T>::HALF ? 64 : fwd_tile<T, D>(); }
+
 template <typename T, int D, int NW>
 __global__ __launch_bounds__(NW * 64) void cross_dq_kernel(const BwdParams p) {
   using G = Geom<T, D>;
   using Frag = typename Elem<T>::Frag;
-  constexpr int TK = fwd_tile<T, D>(), TQ = NW * 32, NT = NW * 64, NF = G::NF, DB = G::DB, STAGE = 2 * TK * D;
+  constexpr int TK = dq_tile<T, D>(), TQ = NW * 32, NT = NW * 64, NF = G::NF, DB = G::DB, STAGE = 2 * TK * D;
   extern __shared__ __attribute__((aligned(16))) char smem_raw[];
   T* smem = reinterpret_cast<T*>(smem_raw);   // [stage][K | V][TK][D]
 
@@ -110,12 +113,21 @@ __global__ __launch_bounds__(NW * 64) void cross_dq_kernel(const BwdParams p) {
 #pragma unroll
   for (int i = 0; i < 16; ++i) dinit[i] = delta;
   const sa::WaveWindow win{0, L, 0, L, 0, L};
-  for (int t = t0; t < t1; ++t) {
+  auto next_tile = [&](int t) {   // waits for tile t, sends for the one after it
     sa::wait_loads<0>();
     __syncthreads();
     if (t + 1 < t1) tiles.issue(smem + ((t + 1 - t0) & 1) * STAGE, t + 1, wave);
+    return smem + ((t - t0) & 1) * STAGE;
+  };
+  int t = t0;
+  if constexpr (Elem<T>::HALF && D == 256)   // a loop of their own: where two paths meet the compiler copies 128 accumulators
+    for (; t < t1 && wr0 < live && (t + 1) * TK <= L; ++t) {
+      const T* keys = next_tile(t);
+      sa::dq2_tile_inside<T, D>(acc, keys, keys + TK * D, qf, gf, sl2e, lse, dinit, lane);
+    }
+  for (; t < t1; ++t) {
+    const T* keys = next_tile(t);
     if (wr0 >= live) continue;
-    const T* keys = smem + ((t - t0) & 1) * STAGE;
     if constexpr (!Elem<T>::HALF)
       dq_tile_f32<T, D, TK>(acc, keys, keys + TK * D, t * TK, L, qf, gf, sl2e, lse, delta, lane);
     else
@@ -131,10 +143,10 @@ __global__ __launch_bounds__(NW * 64) void cross_dq_kernel(const BwdParams p) {
   store_rows<T, D, DB>(out, p.map, bh, wr0, smem + wave * sa::RowPatch<T, D>::ELEMS, acc, -p.scale, lane);
 }
 
-// dV^T += dO^T P and dK^T += Q^T dS, negated, for the TQ rows from r0 on, or one of them (16-bit elements up to head dimension 128:
-// sa::dkdv2_tile).  v holds -V.
+// dV^T += dO^T P and dK^T += Q^T dS, negated, for the TQ rows from r0 on, or one of them: float32 (16-bit elements: sa::dkdv2_tile).
+// v holds -V.
 template <typename T, int D, int TQ, bool WITH_DK, bool WITH_DV, int NF, int NV, int DK, int DV>
-SA_DEV void dkdv_rows(f32x16 (&dk)[DK], f32x16 (&dv)[DV], const T* qt, const T* gt, int r0, int live,
+SA_DEV void dkdv_tile_f32(f32x16 (&dk)[DK], f32x16 (&dv)[DV], const T* qt, const T* gt, int r0, int live,
                           const typename Elem<T>::Frag (&k)[NF], const typename Elem<T>::Frag (&v)[NV], float scale_log2e,
                           const float* stats, int lane) {   // stats: {lse, delta} of RPW rows after one another
   constexpr int RPW = TQ / 4;
@@ -173,8 +185,8 @@ template <typename T, int D> constexpr int dkdv_tile() { return D * (int)sizeof(
 // Bytes of a stage: Q and dO tiles, and lse and delta of their rows.
 template <typename T, int D> constexpr int dkdv_stage() { return 2 * dkdv_tile<T, D>() * (D * (int)sizeof(T) + (int)sizeof(float)); }
 
-// PASS: 0 both gradients, 1 dV, 2 dK.  Head dimension 256 takes a launch for each: two accumulators of 32 x 256 are 256 registers of a
-// lane, the rows of K and V another 128 (float32: 256) of its 512, and in one launch 444 values were spilled.
+// PASS: 0 both gradients, 1 dV, 2 dK.  float32 at head dimension 256 takes a launch for each: two accumulators of 32 x 256 and the rows
+// of K and V are all 512 registers of a lane.
 template <typename T, int D, int NW, int PASS>
 __global__ __launch_bounds__(NW * 64, (sizeof(T) == 2 && D == 64 ? 3 : 1)) void cross_dkdv_kernel(const BwdParams p) {
   using G = Geom<T, D>;
@@ -260,7 +272,7 @@ __global__ __launch_bounds__(NW * 64, (sizeof(T) == 2 && D == 64 ? 3 : 1)) void 
 #pragma unroll
       for (int i = 0; i < NF; ++i) vf[i] = sa::negate<T>(vf[i]);
     }
-    if constexpr (Elem<T>::HALF && PASS == 0)
+    if constexpr (Elem<T>::HALF)
 #pragma unroll
       for (int i = 0; i < NF; ++i) kf[i] = sa::dkdv2_keys<T, D>(kf[i], p.scale_log2e);
   }
@@ -277,7 +289,7 @@ __global__ __launch_bounds__(NW * 64, (sizeof(T) == 2 && D == 64 ? 3 : 1)) void 
     const T* const qt = reinterpret_cast<const T*>(stage);
     const float* const stats = reinterpret_cast<const float*>(stage + 2 * TILE * sizeof(T));
     if (!win.seen(t * TQ, TQ)) continue;
-    if constexpr (Elem<T>::HALF && PASS == 0) {
+    if constexpr (Elem<T>::HALF) {
       sa::dkdv2_tile<T, D, TQ, (D == 64 ? 2 : 4)>(dk, dv, qt, qt + TILE, t * TQ, win, kf, vf, p.scale_log2e,
                                                    [&](int r, f32x4& l4, f32x4& d4) {
         const float* chunk = stats + (r / RPW) * 2 * RPW + r % RPW;
@@ -285,7 +297,7 @@ __global__ __launch_bounds__(NW * 64, (sizeof(T) == 2 && D == 64 ? 3 : 1)) void 
         d4 = *reinterpret_cast<const f32x4*>(chunk + RPW);
       }, lane);
     } else {
-      dkdv_rows<T, D, TQ, WITH_DK, WITH_DV>(dk, dv, qt, qt + TILE, t * TQ, live, kf, vf, p.scale_log2e, stats, lane);
+      dkdv_tile_f32<T, D, TQ, WITH_DK, WITH_DV>(dk, dv, qt, qt + TILE, t * TQ, live, kf, vf, p.scale_log2e, stats, lane);
     }
   }
   if (p.splits > 1) {
@@ -302,6 +314,193 @@ __global__ __launch_bounds__(NW * 64, (sizeof(T) == 2 && D == 64 ? 3 : 1)) void 
   T* patch = reinterpret_cast<T*>(smem_raw) + wave * sa::RowPatch<T, D>::ELEMS;
   if constexpr (WITH_DK) store_rows<T, D, DB>(dk_out, keys, bh, wk0, patch, dk, -p.scale, lane);
   if constexpr (WITH_DV) store_rows<T, D, DB>(dv_out, keys, bh, wk0, patch, dv, 1.0f, lane);
+}
+
+// dK and dV at head dimension 256, 16-bit elements: the four products of 32 keys divided between two waves of one SIMD, as in
+// sa::dkdv_split_wide_kernel.  The score role holds K and dV and forms S, P and dV; the grad role holds V and dK and
+// forms dP, and a step later, with the P that the other has left in LDS in float32, dS and dK.  Steps of 32 rows; a Q tile is read in two
+// steps, a dO tile in one: rings of four and of three, two tiles ahead of the compute.
+template <typename T, int D>
+__global__ __launch_bounds__(512) void cross_dkdv_wide_kernel(const BwdParams p) {
+  using E = Elem<T>;
+  using G = Geom<T, D>;
+  using Frag = typename E::Frag;
+  using S = sa::DkdvSplitWide<T, D>;
+  static_assert(E::HALF && D == 256, "16-bit elements, head dimension 256");
+  constexpr int NP = S::NP, NW = 2 * NP, TQ = S::TQ, TKB = S::TKB, NT = NW * 64;
+  constexpr int NF = G::NF, DB = G::DB, TILE = TQ * D, NQ = S::NQ, NG = S::NG;
+  constexpr int RPW = TQ / NW;   // rows of lse / delta each wave stages
+  static_assert(RPW % 4 == 0 && NQ == 4 && NG == 3, "two tiles ahead: see issue_tile");
+  using Loader = sa::AsyncTile<T, D, TQ, NW, true>;
+  using Gather = RowGather<T, D, TQ, NW>;
+  static_assert(Gather::PER_WAVE == Loader::PER_WAVE, "the same number of copies either way");
+  constexpr int LPT = 2 * Loader::PER_WAVE + 1;   // copies of a wave per tile
+
+  extern __shared__ __attribute__((aligned(16))) char smem_raw[];
+  T* const q_ring = reinterpret_cast<T*>(smem_raw);
+  T* const g_ring = q_ring + NQ * TILE;
+  float* const row_ring = reinterpret_cast<float*>(g_ring + NG * TILE);   // [NQ][NW chunks of {lse[RPW], delta[RPW]}]
+
+  const int tid = threadIdx.x, lane = tid & 63, c = lane & 31, h = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int pair = wave & (NP - 1);   // waves w and w + 4 run on the same SIMD
+  const bool grad_role = wave >= NP;
+  float* const xbuf = row_ring + NQ * 2 * TQ + pair * 2 * S::XSLOT + lane * 4;   // two slots of 16 values per lane
+
+  int bh, tile;
+  sa::tile_coords(blockIdx.x, gridDim.x, p.tiles, bh, tile);
+  int split = 0;
+  if (p.splits > 1) {
+    const int t = div_by(tile, p.by_splits);
+    split = tile - t * p.splits, tile = t;
+  }
+  const int b = div_by(bh, p.tiles.by_heads), hk = bh - b * p.map.Hkv;
+  const int L = clamped_length(p.lens, p.lens_stride, b, p.Tk);
+  const int rows = p.map.rows(), live = clamped_length(p.q_lens, p.q_lens_stride, b, p.map.T) * p.map.G;
+  const int k0 = tile * TKB, wk0 = k0 + pair * 32, key = wk0 + c;
+  const RowMap keys{1, 1, p.Tk, chunk_div(1)};
+  T* const out = reinterpret_cast<T*>(grad_role ? p.dk : p.dv);
+  if (k0 >= L || live == 0) {
+    if (p.splits == 1) {
+      const int k1 = k0 + TKB < p.Tk ? k0 + TKB : p.Tk;
+      zero_rows<T, D, NT / 2>(out, keys, bh, k0, k1, tid % (NT / 2));
+    }
+    return;
+  }
+  int t0, t1;
+  share((live + TQ - 1) / TQ, p.splits, split, t0, t1);
+  const int n = t1 - t0;
+  const bool seen = wk0 < L;   // of the pair's keys
+
+  const T* const q = reinterpret_cast<const T*>(p.q) + b * p.q_sb + (int64_t)hk * p.map.G * p.q_sh;
+  const T* const g = reinterpret_cast<const T*>(p.d_o) + b * p.g_sb + (int64_t)hk * p.map.G * p.g_sh;
+  const float* const row_src = (lane < RPW ? p.row_lse : p.row_delta) + (int64_t)bh * rows;
+  const bool one_head = p.map.G == 1;
+  Loader ldq, ldg;   // of one head
+  ldq.init(q, p.q_st, t0 * TQ, live - 1, wave, lane);
+  ldg.init(g, p.g_st, t0 * TQ, live - 1, wave, lane);
+  // The tile of step `it` goes where those of steps it - 4 (Q, lse, delta) and it - 3 (dO) were: sent for at the beginning of
+  // step it - 2, when every wave has finished step it - 3, the last that reads either.
+  auto issue_tile = [&](int it, int gs) {
+    const int qs = it & (NQ - 1), row0 = (t0 + it) * TQ;
+    if (lane < 2 * RPW) {
+      const int r = row0 + wave * RPW + lane % RPW;
+      sa::async_copy_f32<true>(row_src + (r < live ? r : live - 1), row_ring + (qs * NW + wave) * 2 * RPW);
+    }
+    if (one_head) {
+      ldq.at(it).issue(q_ring + qs * TILE, wave);
+      ldg.at(it).issue(g_ring + gs * TILE, wave);
+    } else {
+      Gather::issue(q, p.q_sh, p.q_st, p.map, row0, live, q_ring + qs * TILE, wave, lane);
+      Gather::issue(g, p.g_sh, p.g_st, p.map, row0, live, g_ring + gs * TILE, wave, lane);
+    }
+  };
+  // this wave's rows first, over the rings
+  using Rows = sa::OwnRows<T, D>;
+  static_assert(NW * Rows::ELEMS * sizeof(T) <= S::lds, "rows of all waves");
+  T* const area = q_ring + wave * Rows::ELEMS;
+  if (grad_role) Rows::send(reinterpret_cast<const T*>(p.v) + b * p.v_sb + hk * p.v_sh, p.v_st, wk0, L - 1, area, lane);
+  else Rows::send(reinterpret_cast<const T*>(p.k) + b * p.k_sb + hk * p.k_sh, p.k_st, wk0, L - 1, area, lane);
+  sa::landed();
+  // resident fragments: K * (-scale * log2 e), rounded, for the score role, -V for the grad role
+  Frag rf[1][NF];
+  {
+    const float mul = grad_role ? -1.0f : -p.scale_log2e;
+#pragma unroll
+    for (int i = 0; i < NF; ++i) {
+      rf[0][i] = Rows::read(area, i, lane);
+#pragma unroll
+      for (int e = 0; e < E::VEC; ++e) rf[0][i][e] = (T)((float)rf[0][i][e] * mul);
+    }
+  }
+  __syncthreads();
+  if (n > 0) issue_tile(0, 0);
+  if (n > 1) issue_tile(1, 1);
+  f32x16 acc[1][DB];   // dV^T[d][key] (score role) or -dK^T[d][key] (grad role)
+  clear(acc[0]);
+
+  // lse (which = 0) or delta (which = 1) of the 16 rows of step it's tile that this lane holds in a C fragment
+  auto rows16 = [&](int it, int which, f32x16& x) {
+    const float* src = row_ring + (it & (NQ - 1)) * 2 * TQ + which * RPW;
+#pragma unroll
+    for (int g4 = 0; g4 < 4; ++g4) {
+      const int r = 8 * g4 + 4 * h;
+      const f32x4 v4 = *reinterpret_cast<const f32x4*>(src + (r / RPW) * 2 * RPW + r % RPW);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[4 * g4 + e] = v4[e];
+    }
+  };
+  auto masked = [&](int it, f32x16& x) {   // the rows of the last tile that are not there
+    const int row0 = (t0 + it) * TQ;
+    if (row0 + TQ <= live) return;
+    asm volatile("");   // a real branch, not selects
+    const uint32_t mask = sa::row_mask(0, live - row0, h);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) x[i] = sa::keep_or_zero(x[i], sa::keep_bits(mask, i));
+  };
+  int gs = 0;   // stage of the current dO tile
+  auto begin_step = [&](int it) {
+    if (it + 1 < n) sa::wait_loads<LPT>();
+    else sa::wait_loads<0>();
+    __syncthreads();
+    if (it + 2 < n) issue_tile(it + 2, gs == 0 ? 2 : gs - 1);
+  };
+  if (!grad_role) {
+    for (int it = 0; it < n; ++it, gs = gs == NG - 1 ? 0 : gs + 1) {
+      begin_step(it);
+      if (!seen) continue;
+      f32x16 s[1][1];
+      rows16(it, 0, s[0][0]);
+      sa::mma_rows_n<T, D>(s, q_ring + (it & (NQ - 1)) * TILE, 0, rf, lane);          // lse - S[row][key]
+#pragma unroll
+      for (int i = 0; i < 16; ++i) s[0][0][i] = sa::fast_exp2(-s[0][0][i]);
+      masked(it, s[0][0]);
+      float* slot = xbuf + (it & 1) * S::XSLOT;
+#pragma unroll
+      for (int g4 = 0; g4 < 4; ++g4)
+        *reinterpret_cast<f32x4*>(slot + g4 * 256) = f32x4{s[0][0][4 * g4], s[0][0][4 * g4 + 1], s[0][0][4 * g4 + 2], s[0][0][4 * g4 + 3]};
+      Frag pf[1][2];
+      sa::pack_c<T>(pf[0], s[0][0]);
+      sa::mma_tr_n<T, D>(acc, g_ring + gs * TILE, 0, pf, lane);                        // dV^T[d][key] += dO^T P
+    }
+    __syncthreads();   // the grad role's last step
+  } else {
+    f32x16 dp[1][1];   // delta - dP of the step before
+    clear(dp[0]);
+    for (int it = 0;; ++it, gs = gs == NG - 1 ? 0 : gs + 1) {
+      if (it < n) begin_step(it);
+      else __syncthreads();
+      const bool prev = it > 0 && seen;
+      Frag df[1][2];
+      if (prev) {
+        const float* slot = xbuf + ((it - 1) & 1) * S::XSLOT;
+#pragma unroll
+        for (int g4 = 0; g4 < 4; ++g4) {
+          const f32x4 p4 = *reinterpret_cast<const f32x4*>(slot + g4 * 256);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) dp[0][0][4 * g4 + e] *= p4[e];   // = -dS
+        }
+        masked(it - 1, dp[0][0]);
+        sa::pack_c<T>(df[0], dp[0][0]);
+      }
+      if (it < n && seen) {
+        rows16(it, 1, dp[0][0]);
+        sa::mma_rows_n<T, D>(dp, g_ring + gs * TILE, 0, rf, lane);                      // delta - dP[row][key]
+      }
+      if (prev) sa::mma_tr_n<T, D>(acc, q_ring + ((it - 1) & (NQ - 1)) * TILE, 0, df, lane);   // -dK^T += Q^T (-dS)
+      if (it == n) break;
+    }
+  }
+  const float mul = grad_role ? -p.scale : 1.0f;
+  if (p.splits > 1) {
+    const int64_t each = (int64_t)p.B * p.map.Hkv * p.Tk;
+    if (key < L)
+      sa::store_acc_T<float, D, DB>(p.part + ((int64_t)(split * 2 + (grad_role ? 0 : 1)) * each + (int64_t)bh * p.Tk + key) * D, acc[0], mul, h);
+    return;
+  }
+  if (key >= L) clear(acc[0]);
+  __syncthreads();   // the row patches lie over the rings
+  store_rows<T, D, DB>(out, keys, bh, wk0, q_ring + wave * sa::RowPatch<T, D>::ELEMS, acc[0], mul, lane);
 }
 
 }  // namespace kv

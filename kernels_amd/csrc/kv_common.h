@@ -176,6 +176,22 @@ SA_DEV int clamped_length(const int32_t* lens, int64_t stride, int b, int most) 
   return n < 0 ? 0 : (n > most ? most : n);
 }
 
+// Tiles of ROWS consecutive rows at addresses of their own (several heads to a key head), by NW waves; the last valid row again in place
+// of those past it.  As assembly, for rings of more than two stages.
+template <typename T, int D, int ROWS, int NW> struct RowGather {
+  using G = Geom<T, D>;
+  static constexpr int PER_WAVE = ROWS / G::RPI / NW;
+  static_assert(ROWS % (G::RPI * NW) == 0, "the tile must split evenly over the waves");
+  SA_DEV static void issue(const T* base, int64_t sh, int64_t st, const RowMap& map, int row0, int live, T* tile, int wave, int lane) {
+#pragma unroll
+    for (int i = 0; i < PER_WAVE; ++i) {
+      const int first = (i * NW + wave) * G::RPI, in_tile = first + lane / G::CPR;
+      const int r = row0 + in_tile < live ? row0 + in_tile : live - 1;
+      copy_gather_asm(base + (map.at(r, sh, st) + ((lane % G::CPR) ^ G::swz(in_tile)) * G::VEC), lds_address(tile + first * D));
+    }
+  }
+};
+
 // Fragments of row `row` (a pointer to its first element), or zeros.
 template <typename T, int D, int NF>
 SA_DEV void load_row(typename Elem<T>::Frag (&f)[NF], const T* row, bool valid, int lane) {

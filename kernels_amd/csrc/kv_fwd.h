@@ -28,6 +28,9 @@ template <int DB> struct RowState {
 template <typename T, int D, int NB, int DB>
 SA_DEV void softmax_step(RowState<DB>& st, f32x16 (&s)[NB], float sl2e, const T* values, int lane) {
   using Frag = typename Elem<T>::Frag;
+  // not where registers are short (guessed probabilities stand beside the scores: 64 values spilled at head dimension 256), nor for
+  // float32, whose matrix instructions leave the time for the search
+  constexpr bool GUESS = Elem<T>::HALF && DB < 8;
   f32x16 p[NB];
   Frag pb[NB][1][2];
   float sum[2];
@@ -44,8 +47,8 @@ SA_DEV void softmax_step(RowState<DB>& st, f32x16 (&s)[NB], float sl2e, const T*
     }
   };
   const bool fresh = __builtin_amdgcn_ballot_w64(st.m != -INFINITY) == 0;
-  bool search = fresh;
-  if (!fresh) {
+  bool search = fresh || !GUESS;
+  if (!search) {
     probabilities();
     const bool behind = !(sum[0] + sum[1] <= kSumLimit) || st.m == -INFINITY;   // true for NaN too
     search = __builtin_amdgcn_ballot_w64(behind) != 0;

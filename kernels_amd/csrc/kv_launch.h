@@ -23,10 +23,11 @@ constexpr int TILE_ROWS = 128;   // rows (or keys) of a workgroup of the tile ke
 constexpr int CUS = 256;
 
 // The tile kernels: with fewer workgroups than CUs the keys (or rows) that each goes through are divided, into shares of at least
-// four tiles, so that there are two workgroups per CU.
+// two tiles, as long as there is a CU for each.  (Two for every CU: 264 -> 274 us for 4 x 8 x 500 rows over up to 2048 keys at D = 256,
+// 126 -> 134 for 2 x 16 x 300 over 4000, 4 key heads, D = 128, forward and backward.)
 inline int tile_splits(int64_t workgroups, int64_t tiles) {
   if (workgroups >= CUS || workgroups == 0) return 1;
-  return (int)std::max<int64_t>(1, std::min<int64_t>(2 * CUS / workgroups, tiles / 4));
+  return (int)std::max<int64_t>(1, std::min<int64_t>(CUS / workgroups, tiles / 2));
 }
 
 // The rows kernel serves up to 32 rows of a key head.  Its keys are divided into shares of a fixed length, not by the number of workgroups: a
