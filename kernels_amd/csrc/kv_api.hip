@@ -45,14 +45,18 @@ template <typename F> int by_dtype(int dtype, F&& f) {
   })
 
 RowMap row_map(int Hkv, int G, int T) { return RowMap{Hkv, G, T, chunk_div(G)}; }
-TileMap tile_map(int64_t nbh, int64_t n_tiles, int heads) {
-  TileMap m{};
-  m.n_tiles = (int)n_tiles;
+Work work_map(int64_t nbh, int64_t n_tiles, int splits, int heads, bool tiles_first) {
+  Work w{};
+  TileMap& m = w.map;
+  m.n_tiles = (int)n_tiles * splits;
   m.nbh = (int)nbh;
-  m.by_tiles = m.by_lead = chunk_div((int)n_tiles);
-  m.by_pairs = chunk_div(nbh >= 16 ? (int)(nbh >> 3) : 1);
+  m.by_tiles = m.by_lead = chunk_div(m.n_tiles);
   m.by_heads = chunk_div(heads);
-  return m;
+  w.splits = splits;
+  w.by_splits = chunk_div(splits);
+  w.tiles_first = tiles_first;
+  w.by_pairs = m.by_pairs = chunk_div(nbh % 8 == 0 ? (int)(nbh >> 3) : (int)nbh);
+  return w;
 }
 
 // How a cross attention is divided: rows kernel, or tiles of rows (and, for dK and dV, of keys).
@@ -192,8 +196,8 @@ int kv_cross_forward(const void* q, const void* k, const void* v, const int32_t*
       p.v_sb = vs[0]; p.v_sh = vs[1]; p.v_st = vs[2];
     }
     p.map = map; p.B = B; p.Tk = Tk; p.scale_log2e = sm_scale * kLog2e;
-    p.splits = c.fwd_splits; p.by_splits = chunk_div(c.fwd_splits);
-    p.tiles = tile_map(c.nbh, ceil_div(c.rows, TILE_ROWS) * c.fwd_splits, Hkv);
+    const int64_t tiles = ceil_div(c.rows, TILE_ROWS);
+    p.work = work_map(c.nbh, tiles, c.fwd_splits, Hkv, tiles_first(tiles));
     p.part_o = part_o; p.part_ml = part_ml;
     if (int rc = KV_LAUNCH(launch_cross_fwd, p)) return rc;
   }
@@ -250,24 +254,23 @@ int kv_cross_backward(const void* q, const void* k, const void* v, const int32_t
   p.part = (float*)((char*)workspace + 2 * c.stats_bytes);
 
   if (Tq > 0) {
-    p.splits = c.dq_splits; p.by_splits = chunk_div(p.splits);
-    p.tiles = tile_map(c.nbh, ceil_div(c.rows, TILE_ROWS) * p.splits, Hkv);
+    const int64_t tiles = ceil_div(c.rows, TILE_ROWS);
+    p.work = work_map(c.nbh, tiles, c.dq_splits, Hkv, tiles_first(tiles));
     if (int rc = KV_LAUNCH(launch_cross_dq, p)) return rc;
   }
   SumParams s{};
   s.part = p.part; s.lens = lens; s.q_lens = q_lens; s.lens_stride = lens_stride; s.q_lens_stride = q_lens_stride;
   s.B = B; s.Tk = Tk; s.Tq = Tq; s.by_heads = chunk_div(Hkv);
-  if (p.splits > 1) {
-    s.map = p.map; s.out = dq; s.splits = p.splits; s.step = c.nbh * c.rows * D; s.keys = false;
+  if (c.dq_splits > 1) {
+    s.map = p.map; s.out = dq; s.splits = c.dq_splits; s.step = c.nbh * c.rows * D; s.keys = false;
     s.by_rows = chunk_div((int)c.rows);
     if (int rc = KV_LAUNCH(launch_sum, s)) return rc;
   }
   if (Tk == 0) return KV_OK;
-  p.splits = c.dkdv_splits; p.by_splits = chunk_div(p.splits);
-  p.tiles = tile_map(c.nbh, ceil_div(Tk, TILE_ROWS) * p.splits, Hkv);
+  p.work = work_map(c.nbh, ceil_div(Tk, TILE_ROWS), c.dkdv_splits, Hkv, false);
   if (int rc = KV_LAUNCH(launch_cross_dkdv, p)) return rc;
-  if (p.splits > 1) {
-    s.map = row_map(Hkv, 1, Tk); s.splits = p.splits; s.step = 2 * c.nbh * Tk * D; s.keys = true;
+  if (c.dkdv_splits > 1) {
+    s.map = row_map(Hkv, 1, Tk); s.splits = c.dkdv_splits; s.step = 2 * c.nbh * Tk * D; s.keys = true;
     s.by_rows = chunk_div(Tk);
     s.out = dk;
     if (int rc = KV_LAUNCH(launch_sum, s)) return rc;

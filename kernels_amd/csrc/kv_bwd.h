@@ -44,6 +44,7 @@ template <typename T> SA_DEV float dot(typename Elem<T>::Frag a, typename Elem<T
   }
 }
 
+template <typename T, int D> constexpr int dq_stages() { return 2; }
 template <typename T, int D> constexpr int dq_tile() { return Elem<T>::HALF ? 64 : fwd_tile<T, D>(); }
 
 template <typename T, int D, int NW>
@@ -56,30 +57,26 @@ __global__ __launch_bounds__(NW * 64) void cross_dq_kernel(const BwdParams p) {
 
   const int tid = threadIdx.x, lane = tid & 63, c = lane & 31, h = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  int bh, tile;
-  sa::tile_coords(blockIdx.x, gridDim.x, p.tiles, bh, tile);
-  int split = 0;
-  if (p.splits > 1) {
-    const int t = div_by(tile, p.by_splits);
-    split = tile - t * p.splits, tile = t;
-  }
-  const int b = div_by(bh, p.tiles.by_heads), hk = bh - b * p.map.Hkv;
-  const int L = clamped_length(p.lens, p.lens_stride, b, p.Tk);
-  const int rows = p.map.rows(), live = clamped_length(p.q_lens, p.q_lens_stride, b, p.map.T) * p.map.G;
+  int bh, tile, split;
+  work_of(p.work, blockIdx.x, gridDim.x, bh, tile, split);
+  const int b = div_by(bh, p.work.map.by_heads), hk = bh - b * p.map.Hkv;
+  const int L = wave_length(p.lens, p.lens_stride, b, p.Tk);
+  const int rows = p.map.rows(), live = wave_length(p.q_lens, p.q_lens_stride, b, p.map.T) * p.map.G;
   const int r0 = tile * TQ, wr0 = r0 + wave * 32, row = wr0 + c;
   T* const out = reinterpret_cast<T*>(p.dq);
   if (r0 >= live) {
-    if (p.splits == 1) zero_rows<T, D, NT>(out, p.map, bh, r0, r0 + TQ < rows ? r0 + TQ : rows, tid);
+    if (p.work.splits == 1) zero_rows<T, D, NT>(out, p.map, bh, r0, r0 + TQ < rows ? r0 + TQ : rows, tid);
     return;
   }
   int t0, t1;
-  share((L + TK - 1) / TK, p.splits, split, t0, t1);
-  PairCopy<T, D, TK, NW> tiles;
-  if (t0 < t1) {
-    tiles.init(reinterpret_cast<const T*>(p.k) + b * p.k_sb + hk * p.k_sh, p.k_st,
-               reinterpret_cast<const T*>(p.v) + b * p.v_sb + hk * p.v_sh, p.v_st, L - 1, wave, lane);
-    tiles.issue(smem, t0, wave);
-  }
+  share((L + TK - 1) / TK, p.work.splits, split, t0, t1);
+  constexpr int NST = dq_stages<T, D>();
+  PairCopy<T, D, TK, NW, (NST > 2)> tiles;
+  tiles.init(reinterpret_cast<const T*>(p.k) + b * p.k_sb + hk * p.k_sh, p.k_st,
+             reinterpret_cast<const T*>(p.v) + b * p.v_sb + hk * p.v_sh, p.v_st, L - 1, wave, lane);
+#pragma unroll
+  for (int i = 0; i < NST - 1; ++i)
+    if (t0 + i < t1) tiles.issue(smem + i * STAGE, t0 + i, wave);
 
   const float sl2e = fabsf(p.scale_log2e);
   Frag qf[NF], gf[NF];
@@ -113,11 +110,15 @@ __global__ __launch_bounds__(NW * 64) void cross_dq_kernel(const BwdParams p) {
 #pragma unroll
   for (int i = 0; i < 16; ++i) dinit[i] = delta;
   const sa::WaveWindow win{0, L, 0, L, 0, L};
-  auto next_tile = [&](int t) {   // waits for tile t, sends for the one after it
-    sa::wait_loads<0>();
+  int stage = -1;
+  auto next_tile = [&](int t) {   // waits for tile t, sends for the one NST - 1 after it
+    if (t + NST - 2 < t1) arrived_but<(NST - 2) * PairCopy<T, D, TK, NW>::PER_WAVE>();
+    else arrived_but<0>();
     __syncthreads();
-    if (t + 1 < t1) tiles.issue(smem + ((t + 1 - t0) & 1) * STAGE, t + 1, wave);
-    return smem + ((t - t0) & 1) * STAGE;
+    const int before = stage < 0 ? NST - 1 : stage;
+    stage = stage + 1 == NST ? 0 : stage + 1;
+    if (t + NST - 1 < t1) tiles.issue(smem + before * STAGE, t + NST - 1, wave);
+    return smem + stage * STAGE;
   };
   int t = t0;
   if constexpr (Elem<T>::HALF && D == 256)   // a loop of their own: where two paths meet the compiler copies 128 accumulators
@@ -133,7 +134,7 @@ __global__ __launch_bounds__(NW * 64) void cross_dq_kernel(const BwdParams p) {
     else
       sa::dq2_tile<T, D, TK>(acc, keys, keys + TK * D, t * TK, win, qf, gf, sl2e, lse, dinit, lane);
   }
-  if (p.splits > 1) {
+  if (p.work.splits > 1) {
     if (row < live)
       sa::store_acc_T<float, D, DB>(p.part + ((int64_t)split * p.B * p.map.Hkv * rows + (int64_t)bh * rows + row) * D, acc, -p.scale, h);
     return;
@@ -198,22 +199,17 @@ __global__ __launch_bounds__(NW * 64, (sizeof(T) == 2 && D == 64 ? 3 : 1)) void 
 
   const int tid = threadIdx.x, lane = tid & 63, c = lane & 31, h = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  int bh, tile;
-  sa::tile_coords(blockIdx.x, gridDim.x, p.tiles, bh, tile);
-  int split = 0;
-  if (p.splits > 1) {
-    const int t = div_by(tile, p.by_splits);
-    split = tile - t * p.splits, tile = t;
-  }
-  const int b = div_by(bh, p.tiles.by_heads), hk = bh - b * p.map.Hkv;
-  const int L = clamped_length(p.lens, p.lens_stride, b, p.Tk);
-  const int rows = p.map.rows(), live = clamped_length(p.q_lens, p.q_lens_stride, b, p.map.T) * p.map.G;
+  int bh, tile, split;
+  work_of(p.work, blockIdx.x, gridDim.x, bh, tile, split);
+  const int b = div_by(bh, p.work.map.by_heads), hk = bh - b * p.map.Hkv;
+  const int L = wave_length(p.lens, p.lens_stride, b, p.Tk);
+  const int rows = p.map.rows(), live = wave_length(p.q_lens, p.q_lens_stride, b, p.map.T) * p.map.G;
   const int k0 = tile * TKB, wk0 = k0 + wave * 32, key = wk0 + c;
   const RowMap keys{1, 1, p.Tk, chunk_div(1)};   // K's gradients are rows of one head each
   T* const dk_out = reinterpret_cast<T*>(p.dk);
   T* const dv_out = reinterpret_cast<T*>(p.dv);
   if (k0 >= L || live == 0) {
-    if (p.splits == 1) {
+    if (p.work.splits == 1) {
       const int k1 = k0 + TKB < p.Tk ? k0 + TKB : p.Tk;
       if constexpr (WITH_DK) zero_rows<T, D, NT>(dk_out, keys, bh, k0, k1, tid);
       if constexpr (WITH_DV) zero_rows<T, D, NT>(dv_out, keys, bh, k0, k1, tid);
@@ -221,7 +217,7 @@ __global__ __launch_bounds__(NW * 64, (sizeof(T) == 2 && D == 64 ? 3 : 1)) void 
     return;
   }
   int t0, t1;
-  share((live + TQ - 1) / TQ, p.splits, split, t0, t1);
+  share((live + TQ - 1) / TQ, p.work.splits, split, t0, t1);
 
   const T* const q = reinterpret_cast<const T*>(p.q) + b * p.q_sb + (int64_t)hk * p.map.G * p.q_sh;
   const T* const g = reinterpret_cast<const T*>(p.d_o) + b * p.g_sb + (int64_t)hk * p.map.G * p.g_sh;
@@ -300,7 +296,7 @@ __global__ __launch_bounds__(NW * 64, (sizeof(T) == 2 && D == 64 ? 3 : 1)) void 
       dkdv_tile_f32<T, D, TQ, WITH_DK, WITH_DV>(dk, dv, qt, qt + TILE, t * TQ, live, kf, vf, p.scale_log2e, stats, lane);
     }
   }
-  if (p.splits > 1) {
+  if (p.work.splits > 1) {
     const int64_t each = (int64_t)p.B * p.map.Hkv * p.Tk;
     if (key < L) {
       float* part = p.part + ((int64_t)split * 2 * each + (int64_t)bh * p.Tk + key) * D;
@@ -347,28 +343,23 @@ __global__ __launch_bounds__(512) void cross_dkdv_wide_kernel(const BwdParams p)
   const bool grad_role = wave >= NP;
   float* const xbuf = row_ring + NQ * 2 * TQ + pair * 2 * S::XSLOT + lane * 4;   // two slots of 16 values per lane
 
-  int bh, tile;
-  sa::tile_coords(blockIdx.x, gridDim.x, p.tiles, bh, tile);
-  int split = 0;
-  if (p.splits > 1) {
-    const int t = div_by(tile, p.by_splits);
-    split = tile - t * p.splits, tile = t;
-  }
-  const int b = div_by(bh, p.tiles.by_heads), hk = bh - b * p.map.Hkv;
-  const int L = clamped_length(p.lens, p.lens_stride, b, p.Tk);
-  const int rows = p.map.rows(), live = clamped_length(p.q_lens, p.q_lens_stride, b, p.map.T) * p.map.G;
+  int bh, tile, split;
+  work_of(p.work, blockIdx.x, gridDim.x, bh, tile, split);
+  const int b = div_by(bh, p.work.map.by_heads), hk = bh - b * p.map.Hkv;
+  const int L = wave_length(p.lens, p.lens_stride, b, p.Tk);
+  const int rows = p.map.rows(), live = wave_length(p.q_lens, p.q_lens_stride, b, p.map.T) * p.map.G;
   const int k0 = tile * TKB, wk0 = k0 + pair * 32, key = wk0 + c;
   const RowMap keys{1, 1, p.Tk, chunk_div(1)};
   T* const out = reinterpret_cast<T*>(grad_role ? p.dk : p.dv);
   if (k0 >= L || live == 0) {
-    if (p.splits == 1) {
+    if (p.work.splits == 1) {
       const int k1 = k0 + TKB < p.Tk ? k0 + TKB : p.Tk;
       zero_rows<T, D, NT / 2>(out, keys, bh, k0, k1, tid % (NT / 2));
     }
     return;
   }
   int t0, t1;
-  share((live + TQ - 1) / TQ, p.splits, split, t0, t1);
+  share((live + TQ - 1) / TQ, p.work.splits, split, t0, t1);
   const int n = t1 - t0;
   const bool seen = wk0 < L;   // of the pair's keys
 
@@ -492,7 +483,7 @@ __global__ __launch_bounds__(512) void cross_dkdv_wide_kernel(const BwdParams p)
     }
   }
   const float mul = grad_role ? -p.scale : 1.0f;
-  if (p.splits > 1) {
+  if (p.work.splits > 1) {
     const int64_t each = (int64_t)p.B * p.map.Hkv * p.Tk;
     if (key < L)
       sa::store_acc_T<float, D, DB>(p.part + ((int64_t)(split * 2 + (grad_role ? 0 : 1)) * each + (int64_t)bh * p.Tk + key) * D, acc[0], mul, h);

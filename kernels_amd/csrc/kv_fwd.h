@@ -88,6 +88,8 @@ SA_DEV void softmax_step(RowState<DB>& st, f32x16 (&s)[NB], float sl2e, const T*
 
 template <typename T, int D> constexpr int fwd_tile() { return D * (int)sizeof(T) <= 256 ? 64 : 32; }
 
+template <typename T, int D> constexpr int fwd_stages() { return 2; }
+
 template <typename T, int D, int NW>
 __global__ __launch_bounds__(NW * 64, (D * sizeof(T) == 512 ? (sizeof(T) == 2 ? 2 : 1) : 1)) void cross_fwd_kernel(const FwdParams p) {
   using G = Geom<T, D>;
@@ -98,21 +100,16 @@ __global__ __launch_bounds__(NW * 64, (D * sizeof(T) == 512 ? (sizeof(T) == 2 ? 
 
   const int tid = threadIdx.x, lane = tid & 63, c = lane & 31, h = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  int bh, tile;
-  sa::tile_coords(blockIdx.x, gridDim.x, p.tiles, bh, tile);
-  int split = 0;
-  if (p.splits > 1) {
-    const int t = div_by(tile, p.by_splits);
-    split = tile - t * p.splits, tile = t;
-  }
-  const int b = div_by(bh, p.tiles.by_heads), hk = bh - b * p.map.Hkv;
-  const int L = clamped_length(p.lens, p.lens_stride, b, p.Tk);
-  const int rows = p.map.rows(), live = clamped_length(p.q_lens, p.q_lens_stride, b, p.map.T) * p.map.G;
+  int bh, tile, split;
+  work_of(p.work, blockIdx.x, gridDim.x, bh, tile, split);
+  const int b = div_by(bh, p.work.map.by_heads), hk = bh - b * p.map.Hkv;
+  const int L = wave_length(p.lens, p.lens_stride, b, p.Tk);
+  const int rows = p.map.rows(), live = wave_length(p.q_lens, p.q_lens_stride, b, p.map.T) * p.map.G;
   const int r0 = tile * TQ, wr0 = r0 + wave * 32, row = wr0 + c;
   T* const out = reinterpret_cast<T*>(p.o);
   const int64_t part_row = (int64_t)split * p.B * p.map.Hkv * rows + (int64_t)bh * rows + row;
   if (r0 >= live) {   // padding: zeros (with several splits the joining kernel writes them)
-    if (p.splits > 1) return;
+    if (p.work.splits > 1) return;
     const int r1 = r0 + TQ < rows ? r0 + TQ : rows;
     zero_rows<T, D, NT>(out, p.map, bh, r0, r1, tid);
     if (p.lse)
@@ -133,19 +130,24 @@ __global__ __launch_bounds__(NW * 64, (D * sizeof(T) == 512 ? (sizeof(T) == 2 ? 
   RowState<DB> st;
   st.init();
   int t0, t1;
-  share((L + TK - 1) / TK, p.splits, split, t0, t1);
+  share((L + TK - 1) / TK, p.work.splits, split, t0, t1);
   if (t0 < t1) {
-    PairCopy<T, D, TK, NW> tiles;
+    constexpr int NST = fwd_stages<T, D>();
+    PairCopy<T, D, TK, NW, (NST > 2)> tiles;
     tiles.init(reinterpret_cast<const T*>(p.k) + b * p.k_sb + hk * p.k_sh, p.k_st,
                reinterpret_cast<const T*>(p.v) + b * p.v_sb + hk * p.v_sh, p.v_st, L - 1, wave, lane);
-    tiles.issue(smem, t0, wave);
-    sa::wait_all_loads();   // the row's fragments (and, as loads complete in order, not more)
-    for (int t = t0; t < t1; ++t) {
-      sa::wait_loads<0>();
-      __syncthreads();   // every wave's share of tile t has arrived; the other stage is free
-      if (t + 1 < t1) tiles.issue(smem + ((t + 1 - t0) & 1) * STAGE, t + 1, wave);
+    sa::wait_all_loads();   // the row's fragments
+#pragma unroll
+    for (int i = 0; i < NST - 1; ++i)
+      if (t0 + i < t1) tiles.issue(smem + i * STAGE, t0 + i, wave);
+    int stage = 0;
+    for (int t = t0; t < t1; ++t, stage = stage + 1 == NST ? 0 : stage + 1) {
+      if (t + NST - 2 < t1) arrived_but<(NST - 2) * PairCopy<T, D, TK, NW>::PER_WAVE>();
+      else arrived_but<0>();
+      __syncthreads();   // every wave's share of tile t has arrived; the stage of the tile before is free
+      if (t + NST - 1 < t1) tiles.issue(smem + (stage == 0 ? NST - 1 : stage - 1) * STAGE, t + NST - 1, wave);
       if (wr0 >= live) continue;
-      const T* keys = smem + ((t - t0) & 1) * STAGE;
+      const T* keys = smem + stage * STAGE;
       f32x16 s[NB];
       clear(s);
       mul_rows<T, D>(s, keys, 0, qf, lane);
@@ -160,7 +162,7 @@ __global__ __launch_bounds__(NW * 64, (D * sizeof(T) == 512 ? (sizeof(T) == 2 ? 
     }
   }
   const float l = sa::half_sum(st.l);
-  if (p.splits > 1) {
+  if (p.work.splits > 1) {
     if (row < live) {
       sa::store_acc_T<float, D, DB>(p.part_o + part_row * D, st.o, 1.0f, h);
       if (h == 0) p.part_ml[part_row * 2] = st.m, p.part_ml[part_row * 2 + 1] = l;

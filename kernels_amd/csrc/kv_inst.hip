@@ -65,8 +65,8 @@ template <> int launch_cross_fwd<ElemT, KV_DGROUP>(const FwdParams& p, int D, hi
   return by_head_dim(D, [&](auto d) {
     constexpr int DD = decltype(d)::value;
     static LdsLimit state;
-    const size_t lds = with_patches<ElemT, DD>(2 * 2 * fwd_tile<ElemT, DD>() * DD * sizeof(ElemT), 4);
-    return launch(cross_fwd_kernel<ElemT, DD, 4>, (int64_t)p.tiles.nbh * p.tiles.n_tiles, 256, lds, state, p, st);
+    const size_t lds = with_patches<ElemT, DD>(fwd_stages<ElemT, DD>() * 2 * fwd_tile<ElemT, DD>() * DD * sizeof(ElemT), 4);
+    return launch(cross_fwd_kernel<ElemT, DD, 4>, (int64_t)p.work.map.nbh * p.work.map.n_tiles, 256, lds, state, p, st);
   });
 }
 #elif KV_KIND == 1
@@ -74,22 +74,22 @@ template <> int launch_cross_dq<ElemT, KV_DGROUP>(const BwdParams& p, int D, hip
   return by_head_dim(D, [&](auto d) {
     constexpr int DD = decltype(d)::value;
     static LdsLimit state;
-    const size_t lds = with_patches<ElemT, DD>(2 * 2 * dq_tile<ElemT, DD>() * DD * sizeof(ElemT), 4);
-    return launch(cross_dq_kernel<ElemT, DD, 4>, (int64_t)p.tiles.nbh * p.tiles.n_tiles, 256, lds, state, p, st);
+    const size_t lds = with_patches<ElemT, DD>(dq_stages<ElemT, DD>() * 2 * dq_tile<ElemT, DD>() * DD * sizeof(ElemT), 4);
+    return launch(cross_dq_kernel<ElemT, DD, 4>, (int64_t)p.work.map.nbh * p.work.map.n_tiles, 256, lds, state, p, st);
   });
 }
 #elif KV_KIND == 2
 template <int D, int PASS> static int launch_dkdv_pass(const BwdParams& p, hipStream_t st) {
   static LdsLimit state;
   const size_t lds = with_patches<ElemT, D>(2 * dkdv_stage<ElemT, D>(), 4);
-  return launch(cross_dkdv_kernel<ElemT, D, 4, PASS>, (int64_t)p.tiles.nbh * p.tiles.n_tiles, 256, lds, state, p, st);
+  return launch(cross_dkdv_kernel<ElemT, D, 4, PASS>, (int64_t)p.work.map.nbh * p.work.map.n_tiles, 256, lds, state, p, st);
 }
 template <> int launch_cross_dkdv<ElemT, KV_DGROUP>(const BwdParams& p, int D, hipStream_t st) {
   return by_head_dim(D, [&](auto d) {
     constexpr int DD = decltype(d)::value;
     if constexpr (sizeof(ElemT) == 2 && DD == 256) {
       static LdsLimit state;
-      return launch(cross_dkdv_wide_kernel<ElemT, DD>, (int64_t)p.tiles.nbh * p.tiles.n_tiles, 512, sa::DkdvSplitWide<ElemT, DD>::lds, state, p, st);
+      return launch(cross_dkdv_wide_kernel<ElemT, DD>, (int64_t)p.work.map.nbh * p.work.map.n_tiles, 512, sa::DkdvSplitWide<ElemT, DD>::lds, state, p, st);
     } else if constexpr (DD == 256) {
       if (int rc = launch_dkdv_pass<DD, 1>(p, st)) return rc;
       return launch_dkdv_pass<DD, 2>(p, st);

@@ -30,6 +30,9 @@ inline int tile_splits(int64_t workgroups, int64_t tiles) {
   return (int)std::max<int64_t>(1, std::min<int64_t>(CUS / workgroups, tiles / 2));
 }
 
+// Few tiles to a pair: tile by tile.
+inline bool tiles_first(int64_t tiles) { return tiles <= 4; }
+
 // The rows kernel serves up to 32 rows of a key head.  Its keys are divided into shares of a fixed length, not by the number of workgroups: a
 // sequence has the same bits alone and in any batch.
 inline bool few_rows(int64_t rows) { return rows <= 32; }

@@ -67,8 +67,8 @@ __global__ __launch_bounds__((RowsShape<T, D>::NW * 64)) void rows_kernel(const 
   const int nbh = p.B * p.map.Hkv, x = div_by(blockIdx.x, p.by_pairs), bh = blockIdx.x - x * nbh;
   const int split = div_by(x, p.by_row_tiles), r0 = (x - split * p.row_tiles) * 32;
   const int b = div_by(bh, p.by_heads), hk = bh - b * p.map.Hkv;
-  const int L = clamped_length(p.lens, p.lens_stride, b, p.max_len);
-  const int tokens = clamped_length(p.q_lens, p.q_lens_stride, b, p.map.T), live = tokens * p.map.G, rows = p.map.rows();
+  const int L = wave_length(p.lens, p.lens_stride, b, p.max_len);
+  const int tokens = wave_length(p.q_lens, p.q_lens_stride, b, p.map.T), live = tokens * p.map.G, rows = p.map.rows();
   const int used = live - r0 < 32 ? live - r0 : 32;   // rows of this workgroup that are not padding
   T* const out = reinterpret_cast<T*>(p.o);
   if (p.splits == 1) {   // (with several splits the joining kernel writes the padding)
