@@ -33,9 +33,10 @@ inline int tile_splits(int64_t workgroups, int64_t tiles) {
 // Few tiles to a pair: tile by tile.
 inline bool tiles_first(int64_t tiles) { return tiles <= 4; }
 
-// The rows kernel serves up to 32 rows of a key head.  Its keys are divided into shares of a fixed length, not by the number of workgroups: a
-// sequence has the same bits alone and in any batch.
+// The rows kernel serves up to 32 rows of a key head.  Its keys are divided into shares whose length follows from the longest that the call may hold,
+// not from the number of workgroups: a sequence has the same bits alone and in any batch.  In us, shares of 16 tiles of 32 keys -> of 32:
+// 8 sequences of up to 4096, 8 key heads, D = 128 24.9 -> 32.4; 64 of 2048 106 -> 101; 64 of up to 8192 112 -> 109.  At most 64 shares.
 inline bool few_rows(int64_t rows) { return rows <= 32; }
-inline int rows_share(int64_t tiles) { return (int)std::max<int64_t>(16, ceil_div(tiles, 64)); }
+inline int rows_share(int64_t tiles) { return (int)std::max<int64_t>(tiles <= 128 ? 16 : 32, ceil_div(tiles, 64)); }
 
 }  // namespace kv

@@ -39,7 +39,10 @@ struct RowsParams {
 
 template <typename T, int D> struct RowsShape {
   static constexpr int ROW = D * (int)sizeof(T);                       // bytes of a row
-  static constexpr int NW = ROW <= 256 ? 4 : ROW <= 512 ? 2 : 1;       // waves
+  // Waves.  The rings take the LDS; two workgroups of two waves, one of which begins while the other one is in its run, read faster than
+  // one of four (64 sequences of up to 8192, 8 key heads, D = 128: 118 -> 109 us), but two waves of each of them may share a SIMD, which
+  // float32 shows (16 x 8 x 2000 keys, D = 64: 38 -> 54), and short sequences want four (300 keys, D = 64: 6.0, 7.3 in two).
+  static constexpr int NW = ROW <= 128 || (ROW == 256 && sizeof(T) == 4) ? 4 : ROW <= 512 ? 2 : 1;
   static constexpr int ST = 2;                                         // tiles on their way
   static constexpr int TILE = 32 * D;                                  // elements
   static constexpr int ENTRIES = 2 * ST * 64 * 4, OFFSETS = 64 * 8;    // bytes per wave, pages only
@@ -114,9 +117,10 @@ __global__ __launch_bounds__((RowsShape<T, D>::NW * 64)) void rows_kernel(const 
   const int count = last - first - wave > 0 ? (last - first - wave + NW - 1) / NW : 0;   // of this wave's tiles
   auto tile_key = [&](int i) { return (first + wave + i * NW) * 32; };
   auto valid_key = [&](int k) { return k < L ? k : L - 1; };   // (a wave with a tile has L > 0)
+  auto table_key = [&](int k) { return k < p.max_len ? k : p.max_len - 1; };
   auto fetch_entries = [&](int i) {   // of this wave's i-th tile
     if constexpr (PAGED) {
-      const int k = valid_key(tile_key(i) + c);
+      const int k = table_key(tile_key(i) + c);
       copy_gather_word_asm(p.table + b * p.table_sb + div_by(k, p.by_page), lds_address(entries + i % (2 * ST) * 64));
     }
   };
@@ -125,7 +129,7 @@ __global__ __launch_bounds__((RowsShape<T, D>::NW * 64)) void rows_kernel(const 
     T* const dst = ring + (i % ST) * 2 * S::TILE;
     const int k0 = tile_key(i);
     if constexpr (PAGED) {   // lanes of the lower half form the rows' places in K, the others in V
-      const int k = valid_key(k0 + c), in_page = k - div_by(k, p.by_page) * p.page;
+      const int k = table_key(k0 + c), in_page = k - div_by(k, p.by_page) * p.page;
       const int32_t e = entries[i % (2 * ST) * 64 + c];
       const int64_t page = present(e) ? e : 0;   // a page that is not there: any that is, its values are replaced below
       offsets[lane] = h == 0 ? page * p.k_sp + in_page * p.k_st : page * p.v_sp + in_page * p.v_st;

@@ -108,11 +108,12 @@ def _paged_append_abstract(k, v, k_pages, v_pages, page_table, lens, new_lens):
     return None
 
 
-_plain_types = (torch.Tensor, type(None))
 _torch_function_modes = torch._C._len_torch_function_stack
+_is_compiling = torch.compiler.is_compiling
+_PLAIN = {torch.Tensor, type(None)}
 
 
 def takes_native_call(*tensors) -> bool:
     """Plain tensors with no torch-function mode around go from Python to the dispatcher in one native call; subclasses,
     proxies and modes need the Python op call, which they can intercept."""
-    return not torch.compiler.is_compiling() and all(type(t) in _plain_types for t in tensors) and not _torch_function_modes()
+    return not _is_compiling() and _PLAIN.issuperset(map(type, tensors)) and not _torch_function_modes()

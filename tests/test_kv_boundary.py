@@ -126,8 +126,8 @@ def test_shares_cover_every_window(lib, B, T, G, page, width, C, R):
             lo = max(at[0] // C - R, 0) * C
             hi = min((at[1] // C + 1) * C, L)
             tiles = max(tiles, -(-hi // 32) - lo // 32)
-    share = max(16, -(-min(-(-most // 32), -(-min(most, (R + -(-(tokens - 1) // C) + 1) * C) // 32) + 1) // 64))
-    assert tiles <= splits * share
+    count = min(-(-most // 32), -(-min(most, (R + -(-(tokens - 1) // C) + 1) * C) // 32) + 1)
+    assert tiles <= splits * max(16 if count <= 128 else 32, -(-count // 64))
 
 
 def _cross(dtype=torch.float32, **kw):
