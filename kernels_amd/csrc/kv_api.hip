@@ -45,15 +45,16 @@ template <typename F> int by_dtype(int dtype, F&& f) {
   })
 
 RowMap row_map(int Hkv, int G, int T) { return RowMap{Hkv, G, T, chunk_div(G)}; }
-Work work_map(int64_t nbh, int64_t n_tiles, int splits, int heads, bool tiles_first) {
+Work work_map(int64_t nbh, int64_t n_tiles, const Shares& sh, int heads, bool tiles_first) {
   Work w{};
   TileMap& m = w.map;
-  m.n_tiles = (int)n_tiles * splits;
+  m.n_tiles = (int)n_tiles * sh.splits;
   m.nbh = (int)nbh;
   m.by_tiles = m.by_lead = chunk_div(m.n_tiles);
   m.by_heads = chunk_div(heads);
-  w.splits = splits;
-  w.by_splits = chunk_div(splits);
+  w.splits = sh.splits;
+  w.share = sh.share;
+  w.by_splits = chunk_div(sh.splits);
   w.tiles_first = tiles_first;
   w.by_pairs = m.by_pairs = chunk_div(nbh % 8 == 0 ? (int)(nbh >> 3) : (int)nbh);
   return w;
@@ -62,7 +63,8 @@ Work work_map(int64_t nbh, int64_t n_tiles, int splits, int heads, bool tiles_fi
 // How a cross attention is divided: rows kernel, or tiles of rows (and, for dK and dV, of keys).
 struct CrossPlan {
   int64_t nbh, rows;
-  int fwd_splits, dq_splits, dkdv_splits, rows_share;
+  Shares fwd, dq, dkdv;
+  int key_tile, dq_key_tile, row_tile;   // of the forward, dQ, dK and dV
   bool few;
   int64_t fwd_bytes, stats_bytes, bwd_bytes;
 };
@@ -75,29 +77,29 @@ int plan_cross(CrossPlan& c, int B, int Hq, int Hkv, int Tq, int Tk, int D, int 
   c.nbh = (int64_t)B * Hkv;
   c.rows = (int64_t)(Hq / Hkv) * Tq;
   if (c.nbh > kMostBlocks || c.rows > kMostBlocks - 1024 || Tk > kMostBlocks - 1024) return KV_ERR_TOO_LARGE;
-  if (Tq == 0) {   // nothing but zeros for dK and dV
-    c.dkdv_splits = 1;
+  c.fwd = c.dq = c.dkdv = Shares{1, 1};
+  if (Tq == 0)   // nothing but zeros for dK and dV
     return c.nbh * ceil_div(Tk, TILE_ROWS) > kMostBlocks ? KV_ERR_TOO_LARGE : KV_OK;
-  }
-  const int tk = D * elem_size(dtype) <= 256 ? 64 : 32;
+  c.key_tile = c.row_tile = D * elem_size(dtype) <= 256 ? 64 : 32;
+  c.dq_key_tile = elem_size(dtype) == 2 ? 64 : c.key_tile;
   const int64_t row_tiles = ceil_div(c.rows, TILE_ROWS), key_tiles = ceil_div(Tk, TILE_ROWS);
   c.few = few_rows(c.rows);
   if (c.few) {
     const int64_t tiles = ceil_div(Tk, 32);
-    c.rows_share = rows_share(tiles);
-    c.fwd_splits = (int)std::max<int64_t>(1, ceil_div(tiles, c.rows_share));
+    c.fwd.share = rows_share(tiles);
+    c.fwd.splits = (int)std::max<int64_t>(1, ceil_div(tiles, c.fwd.share));
   } else {
-    c.fwd_splits = tile_splits(c.nbh * row_tiles, ceil_div(Tk, tk));
+    c.fwd = tile_shares(c.nbh * row_tiles, ceil_div(Tk, c.key_tile));
   }
-  c.dq_splits = tile_splits(c.nbh * row_tiles, ceil_div(Tk, tk));
-  c.dkdv_splits = tile_splits(c.nbh * key_tiles, ceil_div(c.rows, tk));
-  if (c.nbh * std::max(row_tiles * std::max(c.fwd_splits, c.dq_splits), key_tiles * c.dkdv_splits) > kMostBlocks) return KV_ERR_TOO_LARGE;
-  if (std::max(c.fwd_splits, c.dq_splits) > 1 && c.nbh * c.rows > kMostBlocks) return KV_ERR_TOO_LARGE;
-  if (c.dkdv_splits > 1 && c.nbh * Tk > kMostBlocks) return KV_ERR_TOO_LARGE;
-  if (c.fwd_splits > 1) c.fwd_bytes = c.fwd_splits * c.nbh * c.rows * (D + 2) * 4;
+  c.dq = tile_shares(c.nbh * row_tiles, ceil_div(Tk, c.dq_key_tile));
+  c.dkdv = tile_shares(c.nbh * key_tiles, ceil_div(c.rows, c.row_tile));
+  if (c.nbh * std::max(row_tiles * std::max(c.fwd.splits, c.dq.splits), key_tiles * c.dkdv.splits) > kMostBlocks) return KV_ERR_TOO_LARGE;
+  if (std::max(c.fwd.splits, c.dq.splits) > 1 && c.nbh * c.rows > kMostBlocks) return KV_ERR_TOO_LARGE;
+  if (c.dkdv.splits > 1 && c.nbh * Tk > kMostBlocks) return KV_ERR_TOO_LARGE;
+  if (c.fwd.splits > 1) c.fwd_bytes = c.fwd.splits * c.nbh * c.rows * (D + 2) * 4;
   c.stats_bytes = ceil_div(c.nbh * c.rows * 4, 256) * 256;
-  const int64_t dq = c.dq_splits > 1 ? c.dq_splits * c.nbh * c.rows * D * 4 : 0;
-  const int64_t dkdv = c.dkdv_splits > 1 ? (int64_t)c.dkdv_splits * 2 * c.nbh * Tk * D * 4 : 0;
+  const int64_t dq = c.dq.splits > 1 ? c.dq.splits * c.nbh * c.rows * D * 4 : 0;
+  const int64_t dkdv = c.dkdv.splits > 1 ? (int64_t)c.dkdv.splits * 2 * c.nbh * Tk * D * 4 : 0;
   c.bwd_bytes = 2 * c.stats_bytes + std::max(dq, dkdv);
   return KV_OK;
 }
@@ -171,7 +173,7 @@ int kv_cross_forward(const void* q, const void* k, const void* v, const int32_t*
   if (int rc = check_workspace(workspace, workspace_bytes, c.fwd_bytes)) return rc;
   const RowMap map = row_map(Hkv, Hq / Hkv, Tq);
   float* const part_o = (float*)workspace;
-  float* const part_ml = part_o + c.fwd_splits * c.nbh * c.rows * D;
+  float* const part_ml = part_o + c.fwd.splits * c.nbh * c.rows * D;
   if (c.few) {
     RowsParams p{};
     p.q = q; p.k = k; p.v = v; p.o = o; p.lse = lse;
@@ -182,7 +184,7 @@ int kv_cross_forward(const void* q, const void* k, const void* v, const int32_t*
       p.v_sp = vs[0]; p.v_sh = vs[1]; p.v_st = vs[2];
     }
     p.map = map; p.B = B; p.max_len = Tk; p.scale_log2e = sm_scale * kLog2e;
-    p.splits = c.fwd_splits; p.share = c.rows_share; p.row_tiles = 1;
+    p.splits = c.fwd.splits; p.share = c.fwd.share; p.row_tiles = 1;
     p.by_pairs = chunk_div((int)c.nbh); p.by_row_tiles = chunk_div(1); p.by_heads = chunk_div(Hkv);
     p.part_o = part_o; p.part_ml = part_ml;
     if (int rc = KV_LAUNCH(launch_rows, p)) return rc;
@@ -197,12 +199,12 @@ int kv_cross_forward(const void* q, const void* k, const void* v, const int32_t*
     }
     p.map = map; p.B = B; p.Tk = Tk; p.scale_log2e = sm_scale * kLog2e;
     const int64_t tiles = ceil_div(c.rows, TILE_ROWS);
-    p.work = work_map(c.nbh, tiles, c.fwd_splits, Hkv, tiles_first(tiles));
+    p.work = work_map(c.nbh, tiles, c.fwd, Hkv, tiles_first(tiles));
     p.part_o = part_o; p.part_ml = part_ml;
     if (int rc = KV_LAUNCH(launch_cross_fwd, p)) return rc;
   }
-  if (c.fwd_splits == 1) return KV_OK;
-  const JoinParams j = join_params(part_o, part_ml, o, lse, q_lens, q_lens_stride, map, B, c.fwd_splits);
+  if (c.fwd.splits == 1) return KV_OK;
+  const JoinParams j = join_params(part_o, part_ml, o, lse, q_lens, q_lens_stride, map, B, c.fwd.splits);
   return KV_LAUNCH(launch_join, j);
 }
 
@@ -255,29 +257,24 @@ int kv_cross_backward(const void* q, const void* k, const void* v, const int32_t
 
   if (Tq > 0) {
     const int64_t tiles = ceil_div(c.rows, TILE_ROWS);
-    p.work = work_map(c.nbh, tiles, c.dq_splits, Hkv, tiles_first(tiles));
+    p.work = work_map(c.nbh, tiles, c.dq, Hkv, tiles_first(tiles));
     if (int rc = KV_LAUNCH(launch_cross_dq, p)) return rc;
   }
   SumParams s{};
   s.part = p.part; s.lens = lens; s.q_lens = q_lens; s.lens_stride = lens_stride; s.q_lens_stride = q_lens_stride;
-  s.B = B; s.Tk = Tk; s.Tq = Tq; s.by_heads = chunk_div(Hkv);
-  if (c.dq_splits > 1) {
-    s.map = p.map; s.out = dq; s.splits = c.dq_splits; s.step = c.nbh * c.rows * D; s.keys = false;
-    s.by_rows = chunk_div((int)c.rows);
+  s.B = B; s.Tk = Tk; s.Tq = Tq; s.group = Hq / Hkv; s.by_heads = chunk_div(Hkv);
+  if (c.dq.splits > 1) {
+    s.map = p.map; s.out[0] = dq; s.step = c.nbh * c.rows * D; s.keys = false;
+    s.share = c.dq.share; s.tile = c.dq_key_tile; s.by_rows = chunk_div((int)c.rows);
     if (int rc = KV_LAUNCH(launch_sum, s)) return rc;
   }
   if (Tk == 0) return KV_OK;
-  p.work = work_map(c.nbh, ceil_div(Tk, TILE_ROWS), c.dkdv_splits, Hkv, false);
+  p.work = work_map(c.nbh, ceil_div(Tk, TILE_ROWS), c.dkdv, Hkv, false);
   if (int rc = KV_LAUNCH(launch_cross_dkdv, p)) return rc;
-  if (c.dkdv_splits > 1) {
-    s.map = row_map(Hkv, 1, Tk); s.splits = c.dkdv_splits; s.step = 2 * c.nbh * Tk * D; s.keys = true;
-    s.by_rows = chunk_div(Tk);
-    s.out = dk;
-    if (int rc = KV_LAUNCH(launch_sum, s)) return rc;
-    s.out = dv; s.part = p.part + c.nbh * Tk * D;
-    if (int rc = KV_LAUNCH(launch_sum, s)) return rc;
-  }
-  return KV_OK;
+  if (c.dkdv.splits == 1) return KV_OK;
+  s.map = row_map(Hkv, 1, Tk); s.out[0] = dk; s.out[1] = dv; s.second = c.nbh * Tk * D; s.step = 2 * s.second; s.keys = true;
+  s.share = c.dkdv.share; s.tile = c.row_tile; s.by_rows = chunk_div(Tk);
+  return KV_LAUNCH(launch_sum, s);
 }
 
 int64_t kv_paged_forward_workspace(int B, int Hq, int Hkv, int T, int D, int page_size, int width, int context_size, int back_contexts,

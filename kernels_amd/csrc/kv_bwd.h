@@ -69,7 +69,8 @@ __global__ __launch_bounds__(NW * 64) void cross_dq_kernel(const BwdParams p) {
     return;
   }
   int t0, t1;
-  share((L + TK - 1) / TK, p.work.splits, split, t0, t1);
+  part_of(p.work, (L + TK - 1) / TK, split, t0, t1);
+  if (t0 >= t1 && split > 0) return;   // (the first one leaves delta)
   constexpr int NST = dq_stages<T, D>();
   PairCopy<T, D, TK, NW, (NST > 2)> tiles;
   tiles.init(reinterpret_cast<const T*>(p.k) + b * p.k_sb + hk * p.k_sh, p.k_st,
@@ -217,7 +218,8 @@ __global__ __launch_bounds__(NW * 64, (sizeof(T) == 2 && D == 64 ? 3 : 1)) void 
     return;
   }
   int t0, t1;
-  share((live + TQ - 1) / TQ, p.work.splits, split, t0, t1);
+  part_of(p.work, (live + TQ - 1) / TQ, split, t0, t1);
+  if (t0 >= t1) return;
 
   const T* const q = reinterpret_cast<const T*>(p.q) + b * p.q_sb + (int64_t)hk * p.map.G * p.q_sh;
   const T* const g = reinterpret_cast<const T*>(p.d_o) + b * p.g_sb + (int64_t)hk * p.map.G * p.g_sh;
@@ -359,7 +361,8 @@ __global__ __launch_bounds__(512) void cross_dkdv_wide_kernel(const BwdParams p)
     return;
   }
   int t0, t1;
-  share((live + TQ - 1) / TQ, p.work.splits, split, t0, t1);
+  part_of(p.work, (live + TQ - 1) / TQ, split, t0, t1);
+  if (t0 >= t1) return;
   const int n = t1 - t0;
   const bool seen = wk0 < L;   // of the pair's keys
 

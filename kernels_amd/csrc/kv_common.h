@@ -255,18 +255,17 @@ template <typename T, int D, int NT> SA_DEV void zero_rows(T* out, const RowMap&
 }
 
 // ---- split work -----------------------------------------------------------------------------------------------------
-// Where the keys (or, for dK and dV, the rows) are divided over `splits` workgroups, each leaves float32 sums and, in the forward, the
-// reference point and the sum of its probabilities; a second kernel adds them up in the order of the splits.
-SA_DEV void share(int n, int splits, int s, int& first, int& last) {   // of n tiles
-  first = (int)((int64_t)n * s / splits);
-  last = (int)((int64_t)n * (s + 1) / splits);
-}
+// Where the keys (or, for dK and dV, the rows) are divided over several workgroups, each leaves float32 sums and, in the forward, the
+// reference point and the sum of its probabilities; a second kernel adds them up in the order of the splits.  A run of n tiles is divided
+// into as many even parts as shares of `share` tiles would be, so that a long sequence takes more workgroups than a short one.
+SA_BOTH int parts_of(int n, int share) { return (n + share - 1) / share; }
 
 // A workgroup's (batch entry, key head), tile and split.  Pairs are dealt over the XCDs as in sa::tile_coords, with the tiles of a pair
 // side by side; or, tiles_first, tile by tile over all pairs, the first tiles, which are never cut short by a length, at the beginning.
 struct Work {
   TileMap map;           // tiles include the splits
-  int splits, tiles_first;
+  int splits;            // the most that a run of tiles is divided into
+  int share, tiles_first;
   ChunkDiv by_splits, by_pairs;   // by_pairs: the pairs of an XCD, or all
 };
 SA_BOTH void work_of(const Work& w, int bid, int n_blocks, int& bh, int& tile, int& split) {
@@ -283,6 +282,16 @@ SA_BOTH void work_of(const Work& w, int bid, int n_blocks, int& bh, int& tile, i
   if (w.splits > 1) {
     const int t = div_by(tile, w.by_splits);
     split = tile - t * w.splits, tile = t;
+  }
+}
+
+// The part [first, last) of n tiles that split has to do; nothing for the splits that the run is too short for.
+SA_BOTH void part_of(const Work& w, int n, int split, int& first, int& last) {
+  first = 0, last = n;
+  if (w.splits > 1) {
+    const int parts = parts_of(n, w.share);
+    first = split < parts ? (int)((int64_t)n * split / parts) : 0;
+    last = split < parts ? (int)((int64_t)n * (split + 1) / parts) : 0;
   }
 }
 

@@ -22,19 +22,44 @@ template <int DB> struct RowState {
   }
 };
 
-// One step on NB blocks of 32 keys: s holds their raw scores, masked ones -inf.  seen_before: some lane has a reference point.
-// The reference point is looked for only where the probabilities relative to the present one show that it has been left
-// behind; the result does not depend on which point it is, as long as the probabilities stay below 2^8 or so.
+// The maximum of a lane's scores, over both halves of its row.
+template <int NB> SA_DEV float row_max(const f32x16 (&s)[NB]) {
+  float mx = -INFINITY, mk[NB];   // one chain per block, so that consecutive instructions are independent
+#pragma unroll
+  for (int n = 0; n < NB; ++n) mk[n] = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < 16; i += 2)
+#pragma unroll
+    for (int n = 0; n < NB; ++n) mk[n] = sa::fast_max3(mk[n], s[n][i], s[n][i + 1]);
+#pragma unroll
+  for (int n = 0; n < NB; ++n) mx = sa::fast_max(mx, mk[n]);
+  return sa::half_max(mx);
+}
+// Moves the reference point to a maximum that exceeds it by more than kRescaleGap.
+template <int DB> SA_DEV void move_reference(RowState<DB>& st, float mx) {
+  const bool move = mx > st.m + kRescaleGap;   // false for -inf and NaN
+  if (__builtin_amdgcn_ballot_w64(move) != 0) {
+    const float alpha = move ? sa::fast_exp2(st.m - mx) : 1.0f;   // (0 where there was none)
+    st.m = move ? mx : st.m;
+    st.l *= alpha;
+#pragma unroll
+    for (int m = 0; m < DB; ++m)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) st.o[m][i] *= alpha;
+  }
+}
+
+// One step on NB blocks of 32 keys: s holds their raw scores, masked ones -inf.  The maximum is looked for only where the probabilities
+// relative to the present reference point show that it has been left behind; the result does not depend on which point it is, as
+// long as the probabilities stay below 2^8 or so.  Where registers are short (the guessed probabilities stand beside the scores; head
+// dimension 256), and in float32, whose matrix instructions leave the time, it is looked for every time.
 template <typename T, int D, int NB, int DB>
 SA_DEV void softmax_step(RowState<DB>& st, f32x16 (&s)[NB], float sl2e, const T* values, int lane) {
   using Frag = typename Elem<T>::Frag;
-  // not where registers are short (guessed probabilities stand beside the scores: 64 values spilled at head dimension 256), nor for
-  // float32, whose matrix instructions leave the time for the search
   constexpr bool GUESS = Elem<T>::HALF && DB < 8;
-  f32x16 p[NB];
   Frag pb[NB][1][2];
   float sum[2];
-  auto probabilities = [&] {
+  auto probabilities = [&](f32x16 (&p)[NB]) {
     const float m_use = st.m == -INFINITY ? 0.0f : st.m;
     sum[0] = sum[1] = 0.0f;
 #pragma unroll
@@ -46,43 +71,27 @@ SA_DEV void softmax_step(RowState<DB>& st, f32x16 (&s)[NB], float sl2e, const T*
       for (int i = 0; i < 16; i += 2) sum[0] += p[n][i], sum[1] += p[n][i + 1];
     }
   };
-  const bool fresh = __builtin_amdgcn_ballot_w64(st.m != -INFINITY) == 0;
-  bool search = fresh || !GUESS;
-  if (!search) {
-    probabilities();
-    const bool behind = !(sum[0] + sum[1] <= kSumLimit) || st.m == -INFINITY;   // true for NaN too
-    search = __builtin_amdgcn_ballot_w64(behind) != 0;
-  }
-  if (search) {
-    float mx = -INFINITY, mk[NB];
-#pragma unroll
-    for (int n = 0; n < NB; ++n) mk[n] = -INFINITY;
-#pragma unroll
-    for (int i = 0; i < 16; i += 2)
-#pragma unroll
-      for (int n = 0; n < NB; ++n) mk[n] = sa::fast_max3(mk[n], s[n][i], s[n][i + 1]);
-#pragma unroll
-    for (int n = 0; n < NB; ++n) mx = sa::fast_max(mx, mk[n]);
-    mx = sa::half_max(mx) * sl2e;
-    const bool move = mx > st.m + kRescaleGap;   // false for -inf and NaN
-    if (__builtin_amdgcn_ballot_w64(move) != 0) {
-      const float alpha = move ? sa::fast_exp2(st.m - mx) : 1.0f;
-      st.m = move ? mx : st.m;
-      if (!fresh) {
-        st.l *= alpha;
-#pragma unroll
-        for (int m = 0; m < DB; ++m)
-#pragma unroll
-          for (int i = 0; i < 16; ++i) st.o[m][i] *= alpha;
-      }
+  if constexpr (GUESS) {
+    f32x16 p[NB];
+    bool search = __builtin_amdgcn_ballot_w64(st.m != -INFINITY) == 0;   // no lane has a reference point yet
+    if (!search) {
+      probabilities(p);
+      const bool behind = !(sum[0] + sum[1] <= kSumLimit) || st.m == -INFINITY;   // true for NaN too
+      search = __builtin_amdgcn_ballot_w64(behind) != 0;
     }
-    probabilities();
+    if (search) {
+      move_reference(st, row_max(s) * sl2e);
+      probabilities(p);
+    }
+  } else {
+    move_reference(st, row_max(s) * sl2e);
+    probabilities(s);
   }
   st.l += sum[0] + sum[1];
 #pragma unroll
   for (int n = 0; n < NB; ++n) {
     if constexpr (Elem<T>::HALF) sa::mma_tr_n<T, D>(reinterpret_cast<f32x16(&)[1][DB]>(st.o), values, n, pb[n], lane);
-    else mul_tr<T, D>(st.o, values, n * 32, p[n], lane);
+    else mul_tr<T, D>(st.o, values, n * 32, s[n], lane);
   }
 }
 
@@ -117,6 +126,12 @@ __global__ __launch_bounds__(NW * 64, (D * sizeof(T) == 512 ? (sizeof(T) == 2 ? 
     return;
   }
 
+  int t0, t1;
+  part_of(p.work, (L + TK - 1) / TK, split, t0, t1);
+  if (p.work.splits > 1 && t0 >= t1) {
+    if (row < live && h == 0) p.part_ml[part_row * 2] = -INFINITY, p.part_ml[part_row * 2 + 1] = 0.0f;
+    return;
+  }
   // never exactly 0, so that a masked score of -inf stays -inf after scaling
   const float sl2e = fmaxf(fabsf(p.scale_log2e), 1e-30f);
   Frag qf[NF];
@@ -129,8 +144,6 @@ __global__ __launch_bounds__(NW * 64, (D * sizeof(T) == 512 ? (sizeof(T) == 2 ? 
   }
   RowState<DB> st;
   st.init();
-  int t0, t1;
-  share((L + TK - 1) / TK, p.work.splits, split, t0, t1);
   if (t0 < t1) {
     constexpr int NST = fwd_stages<T, D>();
     PairCopy<T, D, TK, NW, (NST > 2)> tiles;

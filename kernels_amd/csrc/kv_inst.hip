@@ -34,11 +34,11 @@ template <typename K> static int raise_lds(K kernel, size_t bytes, LdsLimit& sta
   return rc;
 }
 template <typename K, typename P>
-static int launch(K kernel, int64_t blocks, int threads, size_t lds, LdsLimit& state, const P& p, hipStream_t st) {
+static int launch(K kernel, int64_t blocks, int threads, size_t lds, LdsLimit& state, const P& p, hipStream_t st, int layers = 1) {
   if (blocks > kMostBlocks) return KV_ERR_TOO_LARGE;
   if (blocks == 0) return KV_OK;
   if (int rc = raise_lds(kernel, lds, state)) return rc;
-  kernel<<<dim3((unsigned)blocks), dim3(threads), lds, st>>>(p);
+  kernel<<<dim3((unsigned)blocks, layers), dim3(threads), lds, st>>>(p);
   return (int)hipGetLastError();
 }
 template <typename F> static int by_head_dim(int D, F&& f) {
@@ -123,7 +123,8 @@ template <> int launch_sum<ElemT, KV_DGROUP>(const SumParams& p, int D, hipStrea
   return by_head_dim(D, [&](auto d) {
     constexpr int DD = decltype(d)::value;
     static LdsLimit none;
-    return launch(sum_kernel<ElemT, DD>, ceil_div((int64_t)p.B * p.map.Hkv * p.map.rows(), 256 / (DD / 4)), 256, 0, none, p, st);
+    return launch(sum_kernel<ElemT, DD>, ceil_div((int64_t)p.B * p.map.Hkv * p.map.rows(), 256 / (DD / 4)), 256, 0, none, p, st,
+                  p.keys ? 2 : 1);
   });
 }
 #endif

@@ -22,12 +22,16 @@ inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 constexpr int TILE_ROWS = 128;   // rows (or keys) of a workgroup of the tile kernels: four waves of 32
 constexpr int CUS = 256;
 
-// The tile kernels: with fewer workgroups than CUs the keys (or rows) that each goes through are divided, into shares of at least
-// two tiles, as long as there is a CU for each.  (Two for every CU: 264 -> 274 us for 4 x 8 x 500 rows over up to 2048 keys at D = 256,
-// 126 -> 134 for 2 x 16 x 300 over 4000, 4 key heads, D = 128, forward and backward.)
-inline int tile_splits(int64_t workgroups, int64_t tiles) {
-  if (workgroups >= CUS || workgroups == 0) return 1;
-  return (int)std::max<int64_t>(1, std::min<int64_t>(CUS / workgroups, tiles / 2));
+// The tile kernels: with fewer workgroups than CUs the run of tiles that each goes through is divided, into shares of at least two
+// tiles, as long as there is a CU for each share.  Two for every CU, forward and backward in us: 4 x 8 x 500 rows over up to 2048 keys
+// at D = 256 264 -> 274 (173 -> 190 since), 2 x 16 x 300 over 4000, 4 key heads, D = 128 126 -> 134.
+struct Shares {
+  int splits, share;
+};
+inline Shares tile_shares(int64_t workgroups, int64_t tiles) {
+  if (workgroups > CUS / 2 || workgroups == 0 || tiles < 4) return {1, 1};
+  const int share = (int)std::max<int64_t>(2, ceil_div(tiles, CUS / workgroups));
+  return {(int)ceil_div(tiles, share), share};
 }
 
 // Few tiles to a pair: tile by tile.

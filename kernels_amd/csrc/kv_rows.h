@@ -308,12 +308,14 @@ __global__ __launch_bounds__((SLOTS * D / 4 > 256 ? SLOTS * D / 4 : 256)) void j
 // Gradients whose sums were split: parts [splits, B * Hkv, n, D] added up in order, rows from `limit` on zero.
 struct SumParams {
   const float* part;
-  int64_t step;           // floats between the parts of consecutive splits
-  void* out;
+  int64_t step, second;   // floats between the parts of consecutive splits, and from dK's to dV's
+  void* out[2];           // dQ; or dK and dV, one for each y of the grid
   const int32_t *lens, *q_lens;
   int64_t lens_stride, q_lens_stride;
   RowMap map;             // of the rows of `out`
-  int B, splits, Tk, Tq;
+  int B, Tk, Tq;
+  int share, tile;        // as the parts were made (Work): runs of tiles of `tile` keys (dQ) or rows (dK, dV)
+  int group;              // query heads of a key head
   bool keys;              // rows are keys (dK, dV) instead of queries (dQ)
   ChunkDiv by_rows, by_heads;
 };
@@ -323,17 +325,19 @@ template <typename T, int D> __global__ __launch_bounds__(256) void sum_kernel(c
   const int64_t id = (int64_t)blockIdx.x * RPB + threadIdx.x / Q4;
   if (id >= (int64_t)p.B * p.map.Hkv * rows) return;
   const int bh = div_by((int)id, p.by_rows), row = (int)id - bh * rows, b = div_by(bh, p.by_heads);
-  int limit = clamped_length(p.q_lens, p.q_lens_stride, b, p.Tq) * (p.keys ? 1 : p.map.G);
-  if (p.keys) limit = limit == 0 ? 0 : clamped_length(p.lens, p.lens_stride, b, p.Tk);
+  const int rows_live = clamped_length(p.q_lens, p.q_lens_stride, b, p.Tq) * p.group, L = clamped_length(p.lens, p.lens_stride, b, p.Tk);
+  const int limit = p.keys ? L : rows_live, run = p.keys ? rows_live : L;
+  const int parts = parts_of((run + p.tile - 1) / p.tile, p.share);
+  const float* const part = p.part + (blockIdx.y ? p.second : 0);
   f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
   if (row < limit)
 #pragma unroll 4
-    for (int s = 0; s < p.splits; ++s) {
-      const f32x4 x = *reinterpret_cast<const f32x4*>(p.part + s * p.step + id * D + d);
+    for (int s = 0; s < parts; ++s) {
+      const f32x4 x = *reinterpret_cast<const f32x4*>(part + s * p.step + id * D + d);
 #pragma unroll
       for (int e = 0; e < 4; ++e) sum[e] += x[e];
     }
-  sa::store4<T>(reinterpret_cast<T*>(p.out) + p.map.flat(bh, row) * D + d, sum[0], sum[1], sum[2], sum[3]);
+  sa::store4<T>(reinterpret_cast<T*>(blockIdx.y ? p.out[1] : p.out[0]) + p.map.flat(bh, row) * D + d, sum[0], sum[1], sum[2], sum[3]);
 }
 
 }  // namespace kv
