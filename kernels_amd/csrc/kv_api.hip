@@ -86,7 +86,7 @@ int plan_cross(CrossPlan& c, int B, int Hq, int Hkv, int Tq, int Tk, int D, int 
   c.few = few_rows(c.rows);
   if (c.few) {
     const int64_t tiles = ceil_div(Tk, 32);
-    c.fwd.share = rows_share(tiles);
+    c.fwd.share = rows_share(c.nbh, tiles, D * elem_size(dtype), dtype == 0);
     c.fwd.splits = (int)std::max<int64_t>(1, ceil_div(tiles, c.fwd.share));
   } else {
     c.fwd = tile_shares(c.nbh * row_tiles, ceil_div(Tk, c.key_tile));
@@ -130,7 +130,7 @@ int plan_paged(PagedPlan& c, int B, int Hq, int Hkv, int T, int D, int page, int
   const int64_t tokens = std::min<int64_t>(T, 31 / G + 2), chunks = ceil_div(tokens - 1, C) + 1;
   const int64_t span = R > most || C > most ? most : std::min<int64_t>(most, (R + chunks) * C);
   const int64_t tiles = std::min(ceil_div(most, 32), ceil_div(span, 32) + 1);
-  c.share = rows_share(tiles);
+  c.share = rows_share(c.nbh * c.row_tiles, tiles, D * elem_size(dtype), dtype == 0);
   c.splits = (int)std::max<int64_t>(1, ceil_div(tiles, c.share));
   if (c.nbh * c.row_tiles * c.splits > kMostBlocks || (c.splits > 1 && c.nbh * c.rows > kMostBlocks)) return KV_ERR_TOO_LARGE;
   if (c.splits > 1) c.bytes = c.splits * c.nbh * c.rows * (D + 2) * 4;
@@ -357,7 +357,8 @@ int kv_paged_append(const void* k, const void* v, void* k_pages, void* v_pages, 
   if ((int64_t)B * H > kMostBlocks || (int64_t)B * H * T > kMostBlocks / p.chunks) return KV_ERR_TOO_LARGE;
   p.total = (int64_t)B * H * T * p.chunks;
   p.by_chunks = chunk_div(p.chunks); p.by_tokens = chunk_div(T); p.by_heads = chunk_div(H); p.by_page = chunk_div(page_size);
-  append_kernel<<<dim3((unsigned)ceil_div(p.total, 256)), dim3(256), 0, (hipStream_t)stream>>>(p);
+  const bool streaming = p.total * 32 > (int64_t(32) << 20);   // more than the L2s of all XCDs hold
+  (streaming ? append_kernel<true> : append_kernel<false>)<<<dim3((unsigned)ceil_div(p.total, 256)), dim3(256), 0, (hipStream_t)stream>>>(p);
   return (int)hipGetLastError();
 }
 

@@ -5,7 +5,10 @@
 namespace kv {
 
 // Token i of n = new_lens[b] of sequence b goes to position lens[b] - n + i.  Positions below 0 or past the table, and pages that are not there, are
-// left out.  Bytes only: one thread moves sixteen of K and sixteen of V; consecutive threads go through the chunks of a row, then the heads or tokens.
+// left out.  Bytes only: one thread moves sixteen of K and sixteen of V; consecutive threads go through the chunks of a row, then the tokens of
+// a head.  Bound by memory: prompts of up to 2048 tokens for 8 sequences of 8 heads, D = 128, bfloat16 (67 MB read and written) 12.9 us,
+// 5.2 TB/s, with stores past the caches; 16.1 with plain ones, which a call keeps whose rows stay in the L2 for the attention that
+// follows.  Two or four pieces to a thread took 19 and 27.
 struct AppendParams {
   const char *k, *v;
   char *k_pages, *v_pages;
@@ -18,7 +21,7 @@ struct AppendParams {
   ChunkDiv by_chunks, by_tokens, by_heads, by_page;
   int chunks;
 };
-__global__ __launch_bounds__(256) void append_kernel(const AppendParams p) {
+template <bool STREAMING> __global__ __launch_bounds__(256) void append_kernel(const AppendParams p) {
   const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (id >= p.total) return;
   const int x = div_by((int)id, p.by_chunks), chunk = (int)id - x * p.chunks;
@@ -33,8 +36,15 @@ __global__ __launch_bounds__(256) void append_kernel(const AppendParams p) {
   const int slot = (int)at - entry * p.page;
   const u32x4 kx = *reinterpret_cast<const u32x4*>(p.k + b * p.k_sb + hd * p.k_sh + t * p.k_st + chunk * 16);
   const u32x4 vx = *reinterpret_cast<const u32x4*>(p.v + b * p.v_sb + hd * p.v_sh + t * p.v_st + chunk * 16);
-  *reinterpret_cast<u32x4*>(p.k_pages + to * p.kp_sp + hd * p.kp_sh + slot * p.kp_st + chunk * 16) = kx;
-  *reinterpret_cast<u32x4*>(p.v_pages + to * p.vp_sp + hd * p.vp_sh + slot * p.vp_st + chunk * 16) = vx;
+  char* const kp = p.k_pages + to * p.kp_sp + hd * p.kp_sh + slot * p.kp_st + chunk * 16;
+  char* const vp = p.v_pages + to * p.vp_sp + hd * p.vp_sh + slot * p.vp_st + chunk * 16;
+  if constexpr (STREAMING) {
+    sa::store_streaming(kp, kx);
+    sa::store_streaming(vp, vx);
+  } else {
+    *reinterpret_cast<u32x4*>(kp) = kx;
+    *reinterpret_cast<u32x4*>(vp) = vx;
+  }
 }
 
 }  // namespace kv

@@ -99,12 +99,20 @@ template <> int launch_cross_dkdv<ElemT, KV_DGROUP>(const BwdParams& p, int D, h
   });
 }
 #elif KV_KIND == 3
+template <int D, int NW, bool PAGED> static int launch_rows_shape(const RowsParams& p, int64_t blocks, hipStream_t st) {
+  static LdsLimit state;
+  return launch(rows_kernel<ElemT, D, NW, PAGED>, blocks, NW * 64, RowsShape<ElemT, D, NW>::bytes(PAGED), state, p, st);
+}
 template <bool PAGED> static int launch_rows_any(const RowsParams& p, int D, hipStream_t st) {
   return by_head_dim(D, [&](auto d) {
-    constexpr int DD = decltype(d)::value;
-    static LdsLimit state;
-    using S = RowsShape<ElemT, DD>;
-    return launch(rows_kernel<ElemT, DD, PAGED>, (int64_t)p.B * p.map.Hkv * p.row_tiles * p.splits, S::NW * 64, S::bytes(PAGED), state, p, st);
+    constexpr int DD = decltype(d)::value, ROW = DD * (int)sizeof(ElemT);
+    const int64_t blocks = (int64_t)p.B * p.map.Hkv * p.row_tiles * p.splits;
+    const int waves = rows_waves(ROW, sizeof(ElemT) == 4, blocks, p.share);
+    if constexpr (ROW == 128)
+      if (waves == 8) return launch_rows_shape<DD, 8, PAGED>(p, blocks, st);
+    if constexpr (ROW == 256 && sizeof(ElemT) == 2)
+      if (waves == 2) return launch_rows_shape<DD, 2, PAGED>(p, blocks, st);
+    return launch_rows_shape<DD, ROW <= 256 ? 4 : ROW == 512 ? 2 : 1, PAGED>(p, blocks, st);
   });
 }
 template <> int launch_rows<ElemT, KV_DGROUP>(const RowsParams& p, int D, hipStream_t st) { return launch_rows_any<false>(p, D, st); }
@@ -114,7 +122,7 @@ template <> int launch_join<ElemT, KV_DGROUP>(const JoinParams& p, int D, hipStr
     constexpr int DD = decltype(d)::value;
     static LdsLimit none;
     const int64_t rows = (int64_t)p.B * p.map.Hkv * p.map.rows();
-    if (p.splits <= 4) return launch(join_kernel<ElemT, DD, 1>, ceil_div(rows, 256 / (DD / 4)), 256, 0, none, p, st);
+    if (p.splits <= 8) return launch(join_kernel<ElemT, DD, 1>, ceil_div(rows, 256 / (DD / 4)), 256, 0, none, p, st);
     constexpr int NT = 8 * DD / 4 > 256 ? 8 * DD / 4 : 256;
     return launch(join_kernel<ElemT, DD, 8>, ceil_div(rows, NT / (8 * DD / 4)), NT, 0, none, p, st);
   });

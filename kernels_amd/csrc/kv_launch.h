@@ -37,10 +37,34 @@ inline Shares tile_shares(int64_t workgroups, int64_t tiles) {
 // Few tiles to a pair: tile by tile.
 inline bool tiles_first(int64_t tiles) { return tiles <= 4; }
 
-// The rows kernel serves up to 32 rows of a key head.  Its keys are divided into shares whose length follows from the longest that the call may hold,
-// not from the number of workgroups: a sequence has the same bits alone and in any batch.  In us, shares of 16 tiles of 32 keys -> of 32:
-// 8 sequences of up to 4096, 8 key heads, D = 128 24.9 -> 32.4; 64 of 2048 106 -> 101; 64 of up to 8192 112 -> 109.  At most 64 shares.
+// The rows kernel serves up to 32 rows of a key head.
 inline bool few_rows(int64_t rows) { return rows <= 32; }
-inline int rows_share(int64_t tiles) { return (int)std::max<int64_t>(tiles <= 128 ? 16 : 32, ceil_div(tiles, 64)); }
+// How its keys are divided, from the sizes of the call: at most n tiles of 32 keys for each of `units` workgroups.  A share is
+// what leaves one workgroup for each CU, from four tiles on; short runs are not divided (the joining kernel takes about 4 us), and shares of
+// many workgroups stay short, so that long sequences of a batch spread over the CUs that short ones have left.  float32 is bound by its matrix
+// instructions and gains by every division (128 units of 63 tiles, D = 64: 55 us in one share, 37 in two).
+// One token per sequence, in us for shares of 4, 8, 16, 32, 64, 128 tiles (* chosen), 16-bit elements, D = 128, four waves: 8 units of 63
+// tiles 9.5*, 9.7, 12.0, 15.9, 22.3; of 1000 60.9, 45.9, 34.9, 28.0*, 32.2, 49.7; 32 units of 63 16.2, 12.6*, 14.2, 18.1, 25.1; of 250 49.7, 36.7, 29.6,
+// 26.7*, 32.2, 50.2; 128 units of 16 16.3, 13.1, 11.0*; of 63 45.2, 35.7, 29.8, 26.9*, 28.9; two waves: 512 units of 16 33.4, 29.9, 23.8*; of
+// 63 121, 111, 105, 99.7, 94.5*; of up to 256, ragged: shares of 32 109*, 64 118.  D = 64, four waves: 8 units of 63 8.3*, 8.3, 9.9, 12.7, 16.5; 32 of 63
+// 9.9, 9.0*, 10.7, 13.6, 17.4; 512 units of 63 78.3, 63.3, 57.5, 54.4, 49.2*; eight waves: 128 units of 63 35.3, 24.4, 20.6, 16.9, 15.3* (four: 19.7).
+inline int rows_share(int64_t units, int64_t n, int row_bytes, bool f32) {
+  if (n <= (row_bytes <= 128 ? 32 : 16)) return (int)std::max<int64_t>(n, 1);
+  int64_t share = std::max<int64_t>(4, ceil_div(units * n, CUS));
+  if (2 * share >= n && n <= 64 && !f32) return (int)n;
+  if (share > 32 && units * ceil_div(n, 32) >= 4 * CUS) share = 32;
+  share = std::min<int64_t>(share, 128);
+  return (int)std::max(share, ceil_div(n, 256));   // at most 256 parts to add up
+}
+// Waves of its workgroups, whose rings take most of the LDS.  Rows of 128 bytes: eight, one workgroup to a CU, where there are few workgroups with long
+// shares, else four.  256 bytes: two where there is more than one workgroup for each place, so that one begins while the other one is in its
+// run (512 units of 16 tiles 27.1 -> 23.8 us), else four; float32, whose matrix instructions take their time, always four: two waves of two
+// workgroups may share a SIMD (128 units of 63 tiles 38 -> 54).
+inline int rows_waves(int row_bytes, bool f32, int64_t workgroups, int share) {
+  const bool many = workgroups >= 2 * CUS;
+  if (row_bytes == 128) return !many && share >= 24 ? 8 : 4;
+  if (row_bytes == 256) return many && !f32 ? 2 : 4;
+  return row_bytes < 128 ? 4 : row_bytes == 512 ? 2 : 1;
+}
 
 }  // namespace kv

@@ -37,13 +37,9 @@ struct RowsParams {
   float* part_ml;        // [splits, B * Hkv, rows, 2]
 };
 
-template <typename T, int D> struct RowsShape {
-  static constexpr int ROW = D * (int)sizeof(T);                       // bytes of a row
-  // Waves.  The rings take the LDS; two workgroups of two waves, one of which begins while the other one is in its run, read faster than
-  // one of four (64 sequences of up to 8192, 8 key heads, D = 128: 118 -> 109 us), but two waves of each of them may share a SIMD, which
-  // float32 shows (16 x 8 x 2000 keys, D = 64: 38 -> 54), and short sequences want four (300 keys, D = 64: 6.0, 7.3 in two).
-  static constexpr int NW = ROW <= 128 || (ROW == 256 && sizeof(T) == 4) ? 4 : ROW <= 512 ? 2 : 1;
-  static constexpr int ST = 2;                                         // tiles on their way
+// A wave's rings take 16 KiB at rows of 128 bytes; a workgroup has NW waves (rows_waves in kv_launch.h).
+template <typename T, int D, int NW> struct RowsShape {
+  static constexpr int ST = 2;                                         // tiles on their way; three leave room for one workgroup and are slower
   static constexpr int TILE = 32 * D;                                  // elements
   static constexpr int ENTRIES = 2 * ST * 64 * 4, OFFSETS = 64 * 8;    // bytes per wave, pages only
   static constexpr int OP = D + 4;                                     // floats per row of a wave's result
@@ -54,12 +50,12 @@ template <typename T, int D> struct RowsShape {
   }
 };
 
-template <typename T, int D, bool PAGED>
-__global__ __launch_bounds__((RowsShape<T, D>::NW * 64)) void rows_kernel(const RowsParams p) {
+template <typename T, int D, int NW, bool PAGED>
+__global__ __launch_bounds__(NW * 64) void rows_kernel(const RowsParams p) {
   using G = Geom<T, D>;
-  using S = RowsShape<T, D>;
+  using S = RowsShape<T, D, NW>;
   using Frag = typename Elem<T>::Frag;
-  constexpr int NW = S::NW, ST = S::ST, NF = G::NF, DB = G::DB, RPI = G::RPI, NI = 32 / RPI, NT = NW * 64;
+  constexpr int ST = S::ST, NF = G::NF, DB = G::DB, RPI = G::RPI, NI = 32 / RPI, NT = NW * 64;
   constexpr int IN_FLIGHT = (ST - 1) * 2 * NI < 63 ? (ST - 1) * 2 * NI : 63;
   static_assert(ST == 2, "the waits of the last tiles are written for two");
   extern __shared__ __attribute__((aligned(16))) char smem_raw[];
@@ -264,18 +260,35 @@ __global__ __launch_bounds__((SLOTS * D / 4 > 256 ? SLOTS * D / 4 : 256)) void j
   float m = -INFINITY, l = 0.0f;
   f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
   if (row < live) {
+    // a few splits at a time, whose loads are on their way together; a split that has seen nothing has left no O
+    constexpr int U = 4;
     const float* ml = p.part_ml + id * 2;
-#pragma unroll 4
-    for (int s = slot; s < p.splits; s += SLOTS) m = fmaxf(m, ml[s * all * 2]);
-#pragma unroll 4
-    for (int s = slot; s < p.splits; s += SLOTS) {
-      const float ms = ml[s * all * 2], ls = ml[s * all * 2 + 1];
-      if (ls == 0.0f) continue;   // nothing seen: its O was not written
-      const float f = ms == -INFINITY ? 1.0f : sa::fast_exp2(ms - m);
-      const f32x4 os = *reinterpret_cast<const f32x4*>(p.part_o + (s * all + id) * D + d);
-      l += f * ls;
+    for (int s0 = slot; s0 < p.splits; s0 += SLOTS * U) {
+      float ms[U], ls[U], top = m;
+      f32x4 os[U];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) o[e] += f * os[e];
+      for (int u = 0; u < U; ++u) {
+        const bool there = s0 + u * SLOTS < p.splits;
+        const int64_t s = there ? s0 + u * SLOTS : s0;   // (no branch around the loads)
+        ms[u] = ml[s * all * 2];
+        ls[u] = there ? ml[s * all * 2 + 1] : 0.0f;
+        os[u] = *reinterpret_cast<const f32x4*>(p.part_o + (s * all + id) * D + d);
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) top = ls[u] == 0.0f ? top : fmaxf(top, ms[u]);
+      const float alpha = m == top ? 1.0f : sa::fast_exp2(m - top);
+      m = top;
+      l *= alpha;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[e] *= alpha;
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (ls[u] == 0.0f) continue;
+        const float f = ms[u] == -INFINITY ? 1.0f : sa::fast_exp2(ms[u] - m);   // (-inf: values that are not numbers)
+        l += f * ls[u];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] += f * os[u][e];
+      }
     }
   }
   if constexpr (SLOTS > 1) {

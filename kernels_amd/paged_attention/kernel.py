@@ -73,7 +73,8 @@ def paged_attention(
 
     Tokens beyond ``new_lens[b]`` give 0 and log-sum-exp 0; a token that sees no position gives 0 and log-sum-exp -inf.  What the cache holds
     where no token sees it does not matter.  (A value that is not finite, seen by one of several new tokens, reaches the others of
-    its sequence.)  A sequence has the same bits alone and in any batch, for one width of the page table.  Forward only.
+    its sequence.)  The bits of a sequence's result depend on the sizes of the call, not on the lengths or values of other sequences.
+    Forward only.
     """
     if back_contexts is None:
         back_contexts = _NO_LIMIT

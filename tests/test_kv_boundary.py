@@ -108,7 +108,7 @@ def test_paged_codes(lib):
     assert append(N=0) == 0 and append(W=0) == 0
     need = lib.kv_paged_forward_workspace(1, 2, 1, 1, 64, 8, 1000, 1, 2 ** 31 - 1, 1)
     assert need > 0 and forward(W=1000, R=2 ** 31 - 1, ws=p, bytes=need - 1) == -6
-    assert lib.kv_paged_forward_workspace(1, 2, 1, 1, 64, 8, 1000, 1, 100, 1) == 0       # a window within one share
+    assert lib.kv_paged_forward_workspace(1, 2, 1, 1, 64, 8, 1000, 1, 100, 1) == 0       # a short window is not divided
 
 
 @pytest.mark.parametrize("B,T,G,page,width,C,R", [(2, 1, 1, 16, 4000, 1, 2 ** 31 - 1), (1, 40, 3, 7, 900, 13, 60), (3, 5, 40, 1, 3000, 1, 900),
@@ -126,8 +126,14 @@ def test_shares_cover_every_window(lib, B, T, G, page, width, C, R):
             lo = max(at[0] // C - R, 0) * C
             hi = min((at[1] // C + 1) * C, L)
             tiles = max(tiles, -(-hi // 32) - lo // 32)
-    count = min(-(-most // 32), -(-min(most, (R + -(-(tokens - 1) // C) + 1) * C) // 32) + 1)
-    assert tiles <= splits * max(16 if count <= 128 else 32, -(-count // 64))
+    n = min(-(-most // 32), -(-min(most, (R + -(-(tokens - 1) // C) + 1) * C) // 32) + 1)
+    units = B * 2 * -(-G * T // 32)
+    share = max(4, -(-units * n // 256))
+    if n <= 32 or (2 * share >= n and n <= 64):   # (float16 at head dimension 64)
+        share = n
+    else:
+        share = max(min(32 if share > 32 and units * -(-n // 32) >= 1024 else share, 128), -(-n // 256))
+    assert splits == -(-n // share) and tiles <= splits * share
 
 
 def _cross(dtype=torch.float32, **kw):

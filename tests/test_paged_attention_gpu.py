@@ -206,16 +206,35 @@ def test_long_cache_offsets():
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-def test_same_bits_alone_and_in_a_batch(dtype):
-    lens = [900, 2000, 17, 1300, 64]
+@pytest.mark.parametrize("B", [5, 150])
+def test_same_bits_whatever_the_other_sequences(dtype, B):
+    lens = [900, 2000, 17, 1300, 64] + [40] * (B - 5)
     k, v, table = _cache(lens, 2, 64, 16, dtype)
-    q = _q(5, 8, 2, 64, dtype)
-    q, k, v, table, lens = _gpu(q, k, v, table, _i32(lens))
+    q, k, v, table, lens = _gpu(_q(B, 8, 2, 64, dtype), k, v, table, _i32(lens))
     whole = paged_attention(q, k, v, table, lens)
-    for b in range(5):
-        one = slice(b, b + 1)
-        assert torch.equal(paged_attention(q[one], k, v, table[one], lens[one]), whole[one])
     assert torch.equal(paged_attention(q, k, v, table, lens), whole)
+    for b in range(5):
+        others = torch.where(torch.arange(B, device=DEV) == b, lens, lens // 3)
+        moved = q.roll(1, 0)
+        moved[b] = q[b]
+        assert torch.equal(paged_attention(moved, k, v, table, others)[b], whole[b])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("D", [16, 32, 64, 128, 256])
+@pytest.mark.parametrize("B,T", [(1, 3000), (40, 1500), (300, 700), (300, 100)])
+def test_every_division_of_the_work(dtype, D, B, T):
+    """Few and many workgroups, short and long shares: every number of waves."""
+    lens = [T - 37 * (b % 7) for b in range(B)]
+    g = torch.Generator().manual_seed(3)
+    pages = (T + 15) // 16
+    k, v = (torch.randn(pages, 2, 16, D, generator=g).to(dtype) for _ in range(2))
+    table = torch.stack([torch.arange(pages).roll(b) for b in range(B)]).to(torch.int32)   # all share the pages
+    q = _q(B, 4, 1, D, dtype)
+    got = paged_attention(*_gpu(q, k, v, table, _i32(lens)))
+    some = sorted({0, B // 2, B - 1})
+    want = kv_oracle.paged(q[some], k, v, table[some], _i32([lens[b] for b in some]))
+    kv_oracle.assert_within("o", got[some], want["o"])
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
