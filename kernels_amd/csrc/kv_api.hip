@@ -65,7 +65,7 @@ struct CrossPlan {
   int64_t nbh, rows;
   Shares fwd, dq, dkdv;
   int key_tile, dq_key_tile, row_tile;   // of the forward, dQ, dK and dV
-  bool few;
+  bool few, long_rows, long_keys;        // the rows kernel; the hand-scheduled forward and dQ; dK and dV
   int64_t fwd_bytes, stats_bytes, bwd_bytes;
 };
 // KV_ERR_TOO_LARGE where a count of the kernels would pass 31 bits
@@ -84,6 +84,9 @@ int plan_cross(CrossPlan& c, int B, int Hq, int Hkv, int Tq, int Tk, int D, int 
   c.dq_key_tile = elem_size(dtype) == 2 ? 64 : c.key_tile;
   const int64_t row_tiles = ceil_div(c.rows, TILE_ROWS), key_tiles = ceil_div(Tk, TILE_ROWS);
   c.few = few_rows(c.rows);
+  const bool hand_scheduled = D == 128 && dtype != 0;
+  c.long_rows = hand_scheduled && long_rows((int64_t)B * Hq, Tq, Tk);
+  c.long_keys = hand_scheduled && long_keys(c.nbh, c.rows, Tk);
   if (c.few) {
     const int64_t tiles = ceil_div(Tk, 32);
     c.fwd.share = rows_share(c.nbh, tiles, D * elem_size(dtype), dtype == 0);
@@ -103,10 +106,23 @@ int plan_cross(CrossPlan& c, int B, int Hq, int Hkv, int Tq, int Tk, int D, int 
   c.bwd_bytes = 2 * c.stats_bytes + std::max(dq, dkdv);
   return KV_OK;
 }
+// The rows of one head within 32-bit byte offsets: what the hand-scheduled kernels need of q and d_o.
+bool rows_fit(const int64_t* s, int64_t n, int dtype) { return s[2] <= ((int64_t(1) << 32) - 1) / elem_size(dtype) / (n + 1024); }
 int check_workspace(void* workspace, int64_t have, int64_t need) {
   if (need == 0) return KV_OK;
   if (!workspace || have < need) return KV_ERR_WORKSPACE;
   return (reinterpret_cast<uintptr_t>(workspace) & 15u) ? KV_ERR_LAYOUT : KV_OK;
+}
+
+// The hand-scheduled forward and dQ: a workgroup owns LONG_ROWS queries of one head; the heads of a key head follow each other.
+template <typename P> void long_sides(P& p, int B, int Hq, int Hkv, int Tq, int Tk) {
+  p.B = B; p.H = Hq; p.T = Tq; p.C = 1; p.R = 0;
+  p.cdiv = chunk_div(1);
+  p.other_T = Tk;
+  p.group = Hq / Hkv;
+  p.q_tiles = (int)ceil_div(Tq, LONG_ROWS);
+  p.by_q_tiles = chunk_div(p.q_tiles);
+  p.tiles = work_map((int64_t)B * Hkv, (int64_t)p.group * p.q_tiles, Shares{1, 1}, Hkv, false).map;
 }
 
 // How the rows kernel goes through the pages.
@@ -188,6 +204,16 @@ int kv_cross_forward(const void* q, const void* k, const void* v, const int32_t*
     p.by_pairs = chunk_div((int)c.nbh); p.by_row_tiles = chunk_div(1); p.by_heads = chunk_div(Hkv);
     p.part_o = part_o; p.part_ml = part_ml;
     if (int rc = KV_LAUNCH(launch_rows, p)) return rc;
+  } else if (c.long_rows && Tk > 0 && rows_fit(qs, Tq, dtype)) {
+    LongFwd p{};
+    p.q = q; p.k = k; p.v = v; p.o = o; p.lse = lse;
+    p.lens = q_lens; p.lens_stride = q_lens_stride; p.other_lens = lens; p.other_lens_stride = lens_stride;
+    p.q_sb = qs[0]; p.q_sh = qs[1]; p.q_st = qs[2];
+    p.k_sb = ks[0]; p.k_sh = ks[1]; p.k_st = ks[2];
+    p.v_sb = vs[0]; p.v_sh = vs[1]; p.v_st = vs[2];
+    p.scale_log2e = sm_scale * kLog2e;
+    long_sides(p, B, Hq, Hkv, Tq, Tk);
+    return dtype == 1 ? launch_long_fwd<_Float16>(p, (hipStream_t)stream) : launch_long_fwd<__bf16>(p, (hipStream_t)stream);
   } else {
     FwdParams p{};
     p.q = q; p.k = k; p.v = v; p.o = o; p.lse = lse;
@@ -255,8 +281,34 @@ int kv_cross_backward(const void* q, const void* k, const void* v, const int32_t
   p.row_delta = (float*)((char*)workspace + c.stats_bytes);
   p.part = (float*)((char*)workspace + 2 * c.stats_bytes);
 
-  if (Tq > 0) {
+  const int G = Hq / Hkv;
+  // The hand-scheduled dK/dV kernel goes through the rows of all heads at one stride: one head, or heads that follow each other without
+  // padding inside them.
+  const bool one_run = Tq > 0 && rows_fit(qs, c.rows, dtype) && rows_fit(gs, c.rows, dtype) &&
+                       (G == 1 || (!q_lens && qs[1] == Tq * qs[2] && gs[1] == Tq * gs[2]));
+  const bool keys_by_hand = c.long_keys && one_run;
+  LongBwd r{};
+  if ((c.long_rows || c.long_keys) && Tq > 0 && Tk > 0) {
+    r.q = q; r.k = k; r.v = v; r.d_o = d_o;
+    r.scale = p.scale; r.scale_log2e = p.scale_log2e;
+    r.q_sb = qs[0]; r.q_sh = qs[1]; r.q_st = qs[2];
+    r.k_sb = ks[0]; r.k_sh = ks[1]; r.k_st = ks[2];
+    r.v_sb = vs[0]; r.v_sh = vs[1]; r.v_st = vs[2];
+    r.do_sb = gs[0]; r.do_sh = gs[1]; r.do_st = gs[2];
+  }
+  if (c.long_rows && Tk > 0 && rows_fit(qs, Tq, dtype) && rows_fit(gs, Tq, dtype)) {
+    LongBwd d = r;
+    d.lse = lse; d.dq = dq; d.o = o;
+    d.o_sb = os[0]; d.o_sh = os[1]; d.o_st = os[2];
+    d.lens = q_lens; d.lens_stride = q_lens_stride; d.other_lens = lens; d.other_lens_stride = lens_stride;
+    d.delta_out = p.row_delta; d.lse_out = p.row_lse;
+    d.token_major = !keys_by_hand;
+    long_sides(d, B, Hq, Hkv, Tq, Tk);
+    if (int rc = dtype == 1 ? launch_long_dq<_Float16>(d, (hipStream_t)stream) : launch_long_dq<__bf16>(d, (hipStream_t)stream)) return rc;
+    c.dq.splits = 1;
+  } else if (Tq > 0) {
     const int64_t tiles = ceil_div(c.rows, TILE_ROWS);
+    p.head_major = keys_by_hand;
     p.work = work_map(c.nbh, tiles, c.dq, Hkv, tiles_first(tiles));
     if (int rc = KV_LAUNCH(launch_cross_dq, p)) return rc;
   }
@@ -269,6 +321,16 @@ int kv_cross_backward(const void* q, const void* k, const void* v, const int32_t
     if (int rc = KV_LAUNCH(launch_sum, s)) return rc;
   }
   if (Tk == 0) return KV_OK;
+  if (keys_by_hand) {
+    r.lse = p.row_lse; r.delta = p.row_delta; r.dk = dk; r.dv = dv;
+    r.lens = lens; r.lens_stride = lens_stride; r.other_lens = q_lens; r.other_lens_stride = q_lens_stride;
+    r.B = B; r.H = Hkv; r.T = Tk; r.C = 1; r.R = 0;
+    r.cdiv = chunk_div(1);
+    r.other_T = (int)c.rows;
+    r.group = G;
+    r.tiles = work_map(c.nbh, ceil_div(Tk, TILE_ROWS), Shares{1, 1}, Hkv, false).map;
+    return dtype == 1 ? launch_long_dkdv<_Float16>(r, (hipStream_t)stream) : launch_long_dkdv<__bf16>(r, (hipStream_t)stream);
+  }
   p.work = work_map(c.nbh, ceil_div(Tk, TILE_ROWS), c.dkdv, Hkv, false);
   if (int rc = KV_LAUNCH(launch_cross_dkdv, p)) return rc;
   if (c.dkdv.splits == 1) return KV_OK;

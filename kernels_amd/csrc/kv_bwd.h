@@ -97,8 +97,9 @@ __global__ __launch_bounds__(NW * 64) void cross_dq_kernel(const BwdParams p) {
     lse = p.lse[p.map.flat(bh, r)];
     if (lse == -INFINITY || row >= live) lse = INFINITY;   // P = exp2(-inf) = 0: no key is seen, or padding
     if (split == 0 && h == 0 && row < live) {
-      p.row_lse[(int64_t)bh * rows + row] = lse;
-      p.row_delta[(int64_t)bh * rows + row] = delta;
+      const int64_t at = p.head_major ? p.map.flat(bh, row) : (int64_t)bh * rows + row;
+      p.row_lse[at] = lse;
+      p.row_delta[at] = delta;
     }
 #pragma unroll
     for (int i = 0; i < NF; ++i) {

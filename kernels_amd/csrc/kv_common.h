@@ -322,6 +322,7 @@ struct BwdParams {
   float scale, scale_log2e;
   Work work;
   float *row_lse, *row_delta;   // [B * Hkv, rows]: written with dQ, read with dK and dV
+  bool head_major;     // those in the order (head, token) instead of that of the rows
   float* part;         // dQ: [splits, B * Hkv, rows, D]; dK and dV: [splits, 2, B * Hkv, Tk, D]
 };
 

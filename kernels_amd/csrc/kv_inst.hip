@@ -135,6 +135,22 @@ template <> int launch_sum<ElemT, KV_DGROUP>(const SumParams& p, int D, hipStrea
                   p.keys ? 2 : 1);
   });
 }
+#elif KV_KIND == 4
+constexpr size_t long_stages(int n, size_t tile_rows) { return n * 2 * tile_rows * 128 * sizeof(ElemT); }
+static int64_t long_blocks(const sa::TileMap& m) { return (int64_t)m.nbh * m.n_tiles; }
+template <> int launch_long_fwd<ElemT>(const LongFwd& p, hipStream_t st) {
+  static LdsLimit state;
+  return launch(sa::fwd3_kernel<ElemT, 128, 4, LongFwd>, long_blocks(p.tiles), 256, long_stages(4, 64), state, p, st);
+}
+template <> int launch_long_dq<ElemT>(const LongBwd& p, hipStream_t st) {
+  static LdsLimit state;   // (a fifth stage for half of the dO rows)
+  return launch(sa::dq3_kernel<ElemT, 128, 4, LongBwd>, long_blocks(p.tiles), 256, long_stages(5, 64), state, p, st);
+}
+template <> int launch_long_dkdv<ElemT>(const LongBwd& p, hipStream_t st) {
+  static LdsLimit state;   // three stages with lse and delta, and the workgroup's V rows
+  const size_t lds = long_stages(3, 64) + 3 * 2 * 64 * sizeof(float) + 128 * 128 * sizeof(ElemT);
+  return launch(sa::dkdv3_kernel<ElemT, 128, 3, LongBwd>, long_blocks(p.tiles), 256, lds, state, p, st);
+}
 #endif
 
 }  // namespace kv

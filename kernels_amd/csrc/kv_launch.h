@@ -5,6 +5,9 @@
 #include "../../include/kv_attention.h"
 #include "kv_bwd.h"
 #include "kv_rows.h"
+#include "sa_bwd3.h"
+#include "sa_bwd4.h"
+#include "sa_fwd3.h"
 
 namespace kv {
 
@@ -15,6 +18,13 @@ template <typename T, int DGROUP> int launch_rows(const RowsParams& p, int D, hi
 template <typename T, int DGROUP> int launch_rows_paged(const RowsParams& p, int D, hipStream_t st);
 template <typename T, int DGROUP> int launch_join(const JoinParams& p, int D, hipStream_t st);
 template <typename T, int DGROUP> int launch_sum(const SumParams& p, int D, hipStream_t st);
+
+// The hand-scheduled kernels of streaming attention on another sequence's keys: 16-bit elements, head dimension 128.
+using LongFwd = sa::CrossOf<sa::FwdParams>;
+using LongBwd = sa::CrossOf<sa::BwdParams>;
+template <typename T> int launch_long_fwd(const LongFwd& p, hipStream_t st);
+template <typename T> int launch_long_dq(const LongBwd& p, hipStream_t st);
+template <typename T> int launch_long_dkdv(const LongBwd& p, hipStream_t st);
 
 constexpr int64_t kMostBlocks = 0x7fffffff;
 inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
@@ -36,6 +46,20 @@ inline Shares tile_shares(int64_t workgroups, int64_t tiles) {
 
 // Few tiles to a pair: tile by tile.
 inline bool tiles_first(int64_t tiles) { return tiles <= 4; }
+
+// Where the hand-scheduled kernels are taken.  Forward and dQ: a workgroup owns 256 queries of one head and a CU; from 512 keys on, where there is
+// one for every CU and its rows are filled.  Forward, dQ in us, tile kernels -> these, bfloat16 and float16: 2 x 32 x 4096 queries over
+// 8192 keys, 8 key heads 1000, 1354 -> 957, 1248; 32 x 16 x 200 over up to 1000 61.9, 74.6 -> 62.3, 78.6, and with
+// a pass among others 273 -> 257 for all; 16 x 16 x 256 over 1500 57.6, 77.9 -> 55.0, 76.0;
+// on the other side 8 x 16 x 1000 over 300 27.3, 38.5 -> 33.5, 43.6; 300 rows over 3000, ragged 71, 88 -> 76, 91; 4000 over 128 38.6, 62.8 -> 53.7,
+// 77.3.  dK and dV: from 384 rows of a key head on, where there is a workgroup of 128 keys for every CU: the first 2308 -> 1760; 8 heads
+// of 8000 over 8000 562 -> 430; 400 rows over up to 1000 123 -> 111; 1024 over 1500 133 -> 108; 300 over 3000, ragged 106 -> 107.
+constexpr int LONG_ROWS = 256;
+inline bool long_rows(int64_t heads, int64_t Tq, int64_t Tk) {
+  const int64_t tiles = ceil_div(Tq, LONG_ROWS);
+  return Tk >= 512 && 4 * Tq >= 3 * tiles * LONG_ROWS && heads * tiles >= CUS;
+}
+inline bool long_keys(int64_t key_heads, int64_t rows, int64_t Tk) { return rows >= 384 && key_heads * ceil_div(Tk, TILE_ROWS) >= CUS; }
 
 // The rows kernel serves up to 32 rows of a key head.
 inline bool few_rows(int64_t rows) { return rows <= 32; }

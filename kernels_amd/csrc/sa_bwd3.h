@@ -66,8 +66,9 @@ typedef uint32_t u32x8 __attribute__((ext_vector_type(8)));
     "s54", "s55", "s56", "s57", "s58", "s59", "s60", "s61", "s62", "s63", "s64", "s65", "s66", "s67",  \
     "s68", "s69", "vcc", "scc", "m0", "memory"
 
-template <typename T, int D, int NST>
-__global__ __launch_bounds__(256) void dkdv3_kernel(const BwdParams p) {
+template <typename T, int D, int NST, typename P = BwdParams>
+__global__ __launch_bounds__(256) void dkdv3_kernel(const P p) {
+  constexpr bool CROSS = IsCross<P>::value;
   using E = Elem<T>;
   using G = TileGeom<T, D>;
   using Frag = typename E::Frag;
@@ -93,21 +94,27 @@ __global__ __launch_bounds__(256) void dkdv3_kernel(const BwdParams p) {
   int bh, kt, L;
   key_tile_coords(blockIdx.x, gridDim.x, p.tiles, TKB, p.T, p.lens, p.lens_stride, bh, kt, L);
   const int b = div_by(bh, p.tiles.by_heads), hd = bh - b * p.H;
+  int LQ = L, hq = hd, rows = p.T;   // queries, their first head, and how many a head of lse and delta has
+  if constexpr (CROSS) {
+    LQ = other_length(p, b), hq = hd * p.group, rows = p.other_T;
+    L = __builtin_amdgcn_readfirstlane(L);
+  }
   const int T_ = p.T, C = p.C, R = p.R;
   auto cdiv = [&](int x) { return div_by(x, p.cdiv); };   // x / C
   const int k0 = kt * TKB;
   T* dk_base = reinterpret_cast<T*>(p.dk) + (int64_t)bh * T_ * D;
   T* dv_base = reinterpret_cast<T*>(p.dv) + (int64_t)bh * T_ * D;
   const int k_end = k0 + TKB < T_ ? k0 + TKB : T_;
-  if (k0 >= L) {
+  if (k0 >= L || (CROSS && LQ == 0)) {
     zero_rows<T, D, NT>(dk_base, k0, k_end, tid);
     zero_rows<T, D, NT>(dv_base, k0, k_end, tid);
     return;
   }
 
   // ---- windows ---------------------------------------------------------------------------
-  auto win_lo = [&](int key) { return (cdiv(key)) * C; };
+  auto win_lo = [&](int key) { return CROSS ? 0 : (cdiv(key)) * C; };
   auto win_hi = [&](int key) {
+    if (CROSS) return LQ;
     const int64_t e = ((int64_t)(cdiv(key)) + R + 1) * (int64_t)C;
     return e < (int64_t)L ? (int)e : L;
   };
@@ -121,21 +128,21 @@ __global__ __launch_bounds__(256) void dkdv3_kernel(const BwdParams p) {
   const int qt0 = win_lo(k0) / TQ, qt1 = (win_hi(gk_last) + TQ - 1) / TQ;
 
   // ---- asynchronous tile loads ---------------------------------------------------------
-  const T* qbase = reinterpret_cast<const T*>(p.q) + (int64_t)b * p.q_sb + (int64_t)hd * p.q_sh;
-  const T* gbase = reinterpret_cast<const T*>(p.d_o) + (int64_t)b * p.do_sb + (int64_t)hd * p.do_sh;
-  const float* lse_base = p.lse + (int64_t)bh * T_;
-  const float* delta_base = p.delta + (int64_t)bh * T_;
+  const T* qbase = reinterpret_cast<const T*>(p.q) + (int64_t)b * p.q_sb + (int64_t)hq * p.q_sh;
+  const T* gbase = reinterpret_cast<const T*>(p.d_o) + (int64_t)b * p.do_sb + (int64_t)hq * p.do_sh;
+  const float* lse_base = p.lse + (int64_t)bh * rows;
+  const float* delta_base = p.delta + (int64_t)bh * rows;
   auto stage_off = [&](int t) { return (uint32_t)(((t - qt0 + NST) % NST) * STAGE_B); };   // t >= qt0 - 1
   Loader ldq, ldg;
-  ldq.init(qbase, p.q_st, qt0 * TQ, L - 1, wave, lane);
-  ldg.init(gbase, p.do_st, qt0 * TQ, L - 1, wave, lane);
+  ldq.init(qbase, p.q_st, qt0 * TQ, LQ - 1, wave, lane);
+  ldg.init(gbase, p.do_st, qt0 * TQ, LQ - 1, wave, lane);
   auto issue_tile = [&](int t) {   // tiles are issued in ascending order
     char* sp = smem_raw + stage_off(t);
     T* st = reinterpret_cast<T*>(sp);
     // lanes [0, RPW) fetch lse, lanes [RPW, 2*RPW) fetch delta of this wave's RPW rows
     if (lane < 2 * RPW) {
       int r = t * TQ + wave * RPW + (lane % RPW);
-      r = r < L ? r : L - 1;
+      r = r < LQ ? r : LQ - 1;
       const float* src = (lane < RPW ? lse_base : delta_base) + r;
       float* dst = reinterpret_cast<float*>(sp + 2 * TILE_B) + wave * 2 * RPW;
       async_copy_f32(src, dst);
@@ -221,7 +228,7 @@ __global__ __launch_bounds__(256) void dkdv3_kernel(const BwdParams p) {
     r_scal[SA_DKDV3_SC_ST2] = lds0 + stage_off(t0 + 2);
     r_scal[SA_DKDV3_SC_WAVE_TILE] = (uint32_t)(wave * Loader::RPI * ROWB);
     r_scal[SA_DKDV3_SC_WAVE_ROWS] = (uint32_t)(2 * TILE_B + wave * 2 * RPW * (int)sizeof(float));
-    r_scal[SA_DKDV3_SC_LAST_ROW] = (uint32_t)(L - 1);
+    r_scal[SA_DKDV3_SC_LAST_ROW] = (uint32_t)(LQ - 1);
     r_scal[SA_DKDV3_SC_QLO_MAX] = (uint32_t)qlo_max;
     r_scal[SA_DKDV3_SC_QHI_MIN] = (uint32_t)qhi_min;
     // buffer resources as Loader::init builds them: base, no stride, extent up to the last valid
@@ -230,11 +237,11 @@ __global__ __launch_bounds__(256) void dkdv3_kernel(const BwdParams p) {
     const uint32_t es = (uint32_t)sizeof(T);
     r_scal[SA_DKDV3_SC_RQ0] = (uint32_t)qa;
     r_scal[SA_DKDV3_SC_RQ1] = (uint32_t)(qa >> 32) & 0xffffu;
-    r_scal[SA_DKDV3_SC_RQ2] = ((uint32_t)(L - 1) * (uint32_t)p.q_st + (uint32_t)D) * es;
+    r_scal[SA_DKDV3_SC_RQ2] = ((uint32_t)(LQ - 1) * (uint32_t)p.q_st + (uint32_t)D) * es;
     r_scal[SA_DKDV3_SC_RQ3] = 0x00020000u;
     r_scal[SA_DKDV3_SC_RG0] = (uint32_t)ga;
     r_scal[SA_DKDV3_SC_RG1] = (uint32_t)(ga >> 32) & 0xffffu;
-    r_scal[SA_DKDV3_SC_RG2] = ((uint32_t)(L - 1) * (uint32_t)p.do_st + (uint32_t)D) * es;
+    r_scal[SA_DKDV3_SC_RG2] = ((uint32_t)(LQ - 1) * (uint32_t)p.do_st + (uint32_t)D) * es;
     r_scal[SA_DKDV3_SC_RG3] = 0x00020000u;
     r_scal[SA_DKDV3_SC_SOFF_Q] = ldq.soff;
     r_scal[SA_DKDV3_SC_SOFF_G] = ldg.soff;

@@ -43,8 +43,9 @@ typedef uint32_t u32x16_d3 __attribute__((ext_vector_type(16)));
     "s54", "s55", "s56", "s57", "s58", "s59", "s60", "s61", "s62", "s63", "s64", "s65", "s66", "s67",   \
     "s68", "s69", "s70", "s71", "vcc", "scc", "m0", "memory"
 
-template <typename T, int D, int NST>
-__global__ __launch_bounds__(256) void dq3_kernel(const BwdParams p) {
+template <typename T, int D, int NST, typename P = BwdParams>
+__global__ __launch_bounds__(256) void dq3_kernel(const P p) {
+  constexpr bool CROSS = IsCross<P>::value;
   using E = Elem<T>;
   using G = TileGeom<T, D>;
   using Frag = typename E::Frag;
@@ -67,7 +68,15 @@ __global__ __launch_bounds__(256) void dq3_kernel(const BwdParams p) {
 
   int bh, qt;
   tile_coords(blockIdx.x, gridDim.x, p.tiles, bh, qt);
-  const int b = div_by(bh, p.tiles.by_heads), hd = bh - b * p.H;
+  int b, hd, hk;   // hk: head of k and v
+  if constexpr (CROSS) {
+    const int g = div_by(qt, p.by_q_tiles);
+    qt -= g * p.q_tiles;
+    b = div_by(bh, p.tiles.by_heads), hk = bh - b * (p.H / p.group);
+    hd = hk * p.group + g, bh = b * p.H + hd;
+  } else {
+    b = div_by(bh, p.tiles.by_heads), hd = bh - b * p.H, hk = hd;
+  }
   const int T_ = p.T, C = p.C, R = p.R;
   auto cdiv = [&](int x) { return div_by(x, p.cdiv); };   // x / C
 
@@ -79,16 +88,18 @@ __global__ __launch_bounds__(256) void dq3_kernel(const BwdParams p) {
   const int q0 = qt * TQ;
   T* dq_base = reinterpret_cast<T*>(p.dq) + (int64_t)bh * T_ * D;
   const int q_end = q0 + TQ < T_ ? q0 + TQ : T_;
-  if (q0 >= L) {
+  int LK = L;   // keys
+  if constexpr (CROSS) LK = other_length(p, b);
+  if (q0 >= L || (CROSS && LK == 0)) {   // (without a key nobody reads delta)
     zero_rows<T, D, NT>(dq_base, q0, q_end, tid);
-    if (p.delta_out)
+    if (!CROSS && p.delta_out)
       for (int r = q0 + tid; r < q_end; r += NT) p.delta_out[(int64_t)bh * T_ + r] = 0.0f;
     return;
   }
 
   // ---- windows: this lane's two queries, the wave's 64, the workgroup's 256 ----------------
-  auto win_lo = [&](int q) { return (cdiv(q) > R ? cdiv(q) - R : 0) * C; };
-  auto win_hi = [&](int q) { return (cdiv(q) + 1) * C < L ? (cdiv(q) + 1) * C : L; };
+  auto win_lo = [&](int q) { return CROSS ? 0 : (cdiv(q) > R ? cdiv(q) - R : 0) * C; };
+  auto win_hi = [&](int q) { return CROSS ? LK : (cdiv(q) + 1) * C < L ? (cdiv(q) + 1) * C : L; };
   int qrow[2], qe[2];
 #pragma unroll
   for (int qb = 0; qb < 2; ++qb) {
@@ -107,12 +118,12 @@ __global__ __launch_bounds__(256) void dq3_kernel(const BwdParams p) {
   wt1 = wt1 < kt1 ? wt1 : kt1;
 
   // ---- asynchronous tile loads ---------------------------------------------------------
-  const T* kbase = reinterpret_cast<const T*>(p.k) + (int64_t)b * p.k_sb + (int64_t)hd * p.k_sh;
-  const T* vbase = reinterpret_cast<const T*>(p.v) + (int64_t)b * p.v_sb + (int64_t)hd * p.v_sh;
+  const T* kbase = reinterpret_cast<const T*>(p.k) + (int64_t)b * p.k_sb + (int64_t)hk * p.k_sh;
+  const T* vbase = reinterpret_cast<const T*>(p.v) + (int64_t)b * p.v_sb + (int64_t)hk * p.v_sh;
   auto stage_off = [&](int t) { return (uint32_t)(((t - kt0 + NST) % NST) * STAGE_B); };   // t >= kt0 - 1
   Loader ldk, ldv;
-  ldk.init(kbase, p.k_st, kt0 * TK, L - 1, wave, lane);
-  ldv.init(vbase, p.v_st, kt0 * TK, L - 1, wave, lane);
+  ldk.init(kbase, p.k_st, kt0 * TK, LK - 1, wave, lane);
+  ldv.init(vbase, p.v_st, kt0 * TK, LK - 1, wave, lane);
   auto issue_tile = [&](int t) {   // tiles are issued in ascending order
     T* st = reinterpret_cast<T*>(smem_raw + stage_off(t));
     ldk.issue(st, wave);
@@ -163,6 +174,7 @@ __global__ __launch_bounds__(256) void dq3_kernel(const BwdParams p) {
                     p.delta_out ? p.o_st : p.do_st, q0 + wave * WQ + qb * 32, L - 1, lane);
       // rows past L: P = exp2(S c - inf) = 0
       lse_q2[qb] = qrow[qb] < L ? p.lse[(int64_t)bh * T_ + qe[qb]] : INFINITY;
+      if constexpr (CROSS) lse_q2[qb] = lse_q2[qb] == -INFINITY ? INFINITY : lse_q2[qb];   // a row that sees nothing
     }
     landed();
 #pragma unroll
@@ -186,7 +198,15 @@ __global__ __launch_bounds__(256) void dq3_kernel(const BwdParams p) {
     for (int qb = 0; qb < 2; ++qb) {
       const float lse_q = lse_q2[qb];
       float delta_q;
-      if (p.delta_out) {
+      if constexpr (CROSS) {
+        delta_q = RowDots<T, D>::total(reinterpret_cast<const float*>(q_area(qb)), lane);
+        if (h == 0 && qrow[qb] < L) {
+          const int64_t at = p.token_major ? ((int64_t)(bh - (hd - hk * p.group)) * T_ + (int64_t)qrow[qb] * p.group + (hd - hk * p.group))
+                                           : (int64_t)bh * T_ + qrow[qb];
+          p.delta_out[at] = delta_q;
+          p.lse_out[at] = lse_q;
+        }
+      } else if (p.delta_out) {
         delta_q = RowDots<T, D>::total(reinterpret_cast<const float*>(q_area(qb)), lane);
         if (h == 0 && qrow[qb] < T_) p.delta_out[(int64_t)bh * T_ + qrow[qb]] = qrow[qb] < L ? delta_q : 0.0f;
       } else {
@@ -241,11 +261,11 @@ __global__ __launch_bounds__(256) void dq3_kernel(const BwdParams p) {
     const uint32_t es = (uint32_t)sizeof(T);
     r_scal[SA_DQ3_SC_RK0] = (uint32_t)ka;
     r_scal[SA_DQ3_SC_RK1] = (uint32_t)(ka >> 32) & 0xffffu;
-    r_scal[SA_DQ3_SC_RK2] = ((uint32_t)(L - 1) * (uint32_t)p.k_st + (uint32_t)D) * es;
+    r_scal[SA_DQ3_SC_RK2] = ((uint32_t)(LK - 1) * (uint32_t)p.k_st + (uint32_t)D) * es;
     r_scal[SA_DQ3_SC_RK3] = 0x00020000u;
     r_scal[SA_DQ3_SC_RV0] = (uint32_t)va;
     r_scal[SA_DQ3_SC_RV1] = (uint32_t)(va >> 32) & 0xffffu;
-    r_scal[SA_DQ3_SC_RV2] = ((uint32_t)(L - 1) * (uint32_t)p.v_st + (uint32_t)D) * es;
+    r_scal[SA_DQ3_SC_RV2] = ((uint32_t)(LK - 1) * (uint32_t)p.v_st + (uint32_t)D) * es;
     r_scal[SA_DQ3_SC_RV3] = 0x00020000u;
     r_scal[SA_DQ3_SC_SOFF_K] = ldk.soff + ldk.tstep;   // of tile kt0 + 2
     r_scal[SA_DQ3_SC_SOFF_V] = ldv.soff + ldv.tstep;

@@ -1015,6 +1015,29 @@ struct BwdParams {
   int fused_rows;     // one-launch backward only: query rows whose lse and delta a workgroup keeps
 };
 
+// Cross attention in the hand-scheduled kernels: FwdParams and BwdParams describe the side that a workgroup owns (T, lens, and H heads of q;
+// in the dK/dV kernel T keys, their lens and the key heads), this the side that goes by.  No windows: all of it is seen.
+template <typename Base> struct CrossOf : Base {
+  int other_T;                  // keys; in the dK/dV kernel the rows of all query heads of a key head, at one stride
+  const int32_t* other_lens;    // or null
+  int64_t other_lens_stride;
+  int group;                    // query heads of a key head
+  int q_tiles;                  // query tiles of a head: the map has group * q_tiles tiles for each key head
+  ChunkDiv by_q_tiles;
+  float* lse_out;               // dQ kernel: log-sum-exp of the rows beside delta_out, +inf where a row sees nothing
+  bool token_major;             // dQ kernel: those in the order (token, head) of a key head instead of (head, token)
+};
+template <typename P> struct IsCross { static constexpr bool value = false; };
+template <typename B> struct IsCross<CrossOf<B>> { static constexpr bool value = true; };
+template <typename P> SA_DEV int other_length(const P& p, int b) {
+  int n = p.other_T;
+  if (p.other_lens) {
+    n = p.other_lens[(int64_t)b * p.other_lens_stride];
+    n = n < 0 ? 0 : (n > p.other_T ? p.other_T : n);
+  }
+  return __builtin_amdgcn_readfirstlane(n);
+}
+
 struct DeltaParams {
   const void *o, *d_o;
   float* delta;

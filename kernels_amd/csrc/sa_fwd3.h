@@ -48,8 +48,9 @@ typedef uint32_t u32x8_f3 __attribute__((ext_vector_type(8)));
     "s54", "s55", "s56", "s57", "s58", "s59", "s60", "s61", "s62", "s63", "s64", "s65", "s66", "s67",   \
     "s68", "s69", "s70", "s71", "s72", "s73", "s74", "s75", "s76", "s77", "s78", "vcc", "scc", "m0", "memory"
 
-template <typename T, int D, int NST>
-__global__ __launch_bounds__(256) void fwd3_kernel(const FwdParams p) {
+template <typename T, int D, int NST, typename P = FwdParams>
+__global__ __launch_bounds__(256) void fwd3_kernel(const P p) {
+  constexpr bool CROSS = IsCross<P>::value;
   using E = Elem<T>;
   using G = TileGeom<T, D>;
   using Frag = typename E::Frag;
@@ -116,7 +117,15 @@ __global__ __launch_bounds__(256) void fwd3_kernel(const FwdParams p) {
     const int lane = lane_id(), c = lane & 31, h = lane >> 5;
     int bh, qt;
     tile_coords(bid, gridDim.x, p.tiles, bh, qt);
-    const int b = div_by(bh, p.tiles.by_heads), hd = bh - b * p.H;
+    int b, hd, hk;   // hk: head of k and v
+    if constexpr (CROSS) {
+      const int g = div_by(qt, p.by_q_tiles);
+      qt -= g * p.q_tiles;
+      b = div_by(bh, p.tiles.by_heads), hk = bh - b * (p.H / p.group);
+      hd = hk * p.group + g, bh = b * p.H + hd;
+    } else {
+      b = div_by(bh, p.tiles.by_heads), hd = bh - b * p.H, hk = hd;
+    }
     int L = T_;
     if (p.lens) {
       // a scalar load: the lengths are read-only for the whole launch
@@ -134,14 +143,25 @@ __global__ __launch_bounds__(256) void fwd3_kernel(const FwdParams p) {
         for (int r = q0 + tid; r < q_end; r += NT) lse_base[r] = 0.0f;
       return false;
     }
+    int LK = L;   // keys
+    if constexpr (CROSS) {
+      LK = other_length(p, b);
+      if (LK == 0) {
+        const int q_end = q0 + TQ < T_ ? q0 + TQ : T_;
+        zero_rows<T, D, NT>(o_base, q0, q_end, tid);
+        if (lse_base)
+          for (int r = q0 + tid; r < q_end; r += NT) lse_base[r] = r < L ? -INFINITY : 0.0f;
+        return false;
+      }
+    }
     cu.o_base = o_base;
     cu.lse_base = lse_base;
     cu.q0 = q0;
     cu.L = L;
 
     // windows: this lane's two queries, the wave's 64, the workgroup's 256
-    auto win_lo = [&](int q) { return (cdiv(q) > R ? cdiv(q) - R : 0) * C; };
-    auto win_hi = [&](int q) { return (cdiv(q) + 1) * C < L ? (cdiv(q) + 1) * C : L; };
+    auto win_lo = [&](int q) { return CROSS ? 0 : (cdiv(q) > R ? cdiv(q) - R : 0) * C; };
+    auto win_hi = [&](int q) { return CROSS ? LK : (cdiv(q) + 1) * C < L ? (cdiv(q) + 1) * C : L; };
     int qe[2];
 #pragma unroll
     for (int qb = 0; qb < 2; ++qb) {
@@ -160,12 +180,12 @@ __global__ __launch_bounds__(256) void fwd3_kernel(const FwdParams p) {
     wt1 = wt1 < kt1 ? wt1 : kt1;
 
     // asynchronous tile loads
-    const T* kbase = reinterpret_cast<const T*>(p.k) + (int64_t)b * p.k_sb + (int64_t)hd * p.k_sh;
-    const T* vbase = reinterpret_cast<const T*>(p.v) + (int64_t)b * p.v_sb + (int64_t)hd * p.v_sh;
+    const T* kbase = reinterpret_cast<const T*>(p.k) + (int64_t)b * p.k_sb + (int64_t)hk * p.k_sh;
+    const T* vbase = reinterpret_cast<const T*>(p.v) + (int64_t)b * p.v_sb + (int64_t)hk * p.v_sh;
     auto stage_off = [&](int t) { return (uint32_t)(((t - kt0 + NST) % NST) * STAGE_B); };   // t >= kt0 - 1
     Loader ldk, ldv;
-    ldk.init(kbase, p.k_st, kt0 * TK, L - 1, wave, lane);
-    ldv.init(vbase, p.v_st, kt0 * TK, L - 1, wave, lane);
+    ldk.init(kbase, p.k_st, kt0 * TK, LK - 1, wave, lane);
+    ldv.init(vbase, p.v_st, kt0 * TK, LK - 1, wave, lane);
     auto issue_tile = [&](int t) {   // tiles are issued in ascending order
       T* st = reinterpret_cast<T*>(smem_raw + stage_off(t));
       ldk.issue(st, wave);
@@ -225,11 +245,11 @@ __global__ __launch_bounds__(256) void fwd3_kernel(const FwdParams p) {
     const uint32_t es = (uint32_t)sizeof(T);
     r_scal[SA_FWD3_SC_RK0] = (uint32_t)ka;
     r_scal[SA_FWD3_SC_RK1] = (uint32_t)(ka >> 32) & 0xffffu;
-    r_scal[SA_FWD3_SC_RK2] = ((uint32_t)(L - 1) * (uint32_t)p.k_st + (uint32_t)D) * es;
+    r_scal[SA_FWD3_SC_RK2] = ((uint32_t)(LK - 1) * (uint32_t)p.k_st + (uint32_t)D) * es;
     r_scal[SA_FWD3_SC_RK3] = 0x00020000u;
     r_scal[SA_FWD3_SC_RV0] = (uint32_t)va;
     r_scal[SA_FWD3_SC_RV1] = (uint32_t)(va >> 32) & 0xffffu;
-    r_scal[SA_FWD3_SC_RV2] = ((uint32_t)(L - 1) * (uint32_t)p.v_st + (uint32_t)D) * es;
+    r_scal[SA_FWD3_SC_RV2] = ((uint32_t)(LK - 1) * (uint32_t)p.v_st + (uint32_t)D) * es;
     r_scal[SA_FWD3_SC_RV3] = 0x00020000u;
     r_scal[SA_FWD3_SC_SOFF_K] = ldk.soff;
     r_scal[SA_FWD3_SC_SOFF_V] = ldv.soff;
@@ -255,9 +275,9 @@ __global__ __launch_bounds__(256) void fwd3_kernel(const FwdParams p) {
       const float m_run = qb == 0 ? r_m0 : r_m1;
       const float l_tot = half_sum(qb == 0 ? r_l0 : r_l1);
       const int qrow = cu.q0 + wave * WQ + qb * 32 + c;
-      const bool valid = qrow < cu.L;
-      const float inv = valid ? 1.0f / l_tot : 0.0f;
-      if (!valid) {
+      const bool valid = qrow < cu.L, some = !CROSS || !(l_tot == 0.0f);   // (some: a score above -inf)
+      const float inv = valid && some ? 1.0f / l_tot : 0.0f;
+      if (!valid || !some) {
 #pragma unroll
         for (int m = 0; m < DB; ++m)
 #pragma unroll
@@ -268,7 +288,7 @@ __global__ __launch_bounds__(256) void fwd3_kernel(const FwdParams p) {
       if (row0 < T_)
         store_rows_coalesced<T, D, DB>(patch, cu.o_base + (int64_t)row0 * D, T_ - row0, oacc, inv, lane);
       if (cu.lse_base && h == 0 && qrow < T_)
-        cu.lse_base[qrow] = valid ? m_run + __builtin_amdgcn_logf(l_tot) : 0.0f;
+        cu.lse_base[qrow] = valid ? (some ? m_run + __builtin_amdgcn_logf(l_tot) : -INFINITY) : 0.0f;
     }
   };
 

@@ -72,6 +72,54 @@ def test_split_work(dtype, D, Tq, Tk, lens, q_lens):
     _check(*_inputs(2, 4, 2, Tq, Tk, D, dtype), lens, q_lens)
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("B,Hq,Hkv,Tq,Tk,lens,q_lens,layout", [
+    (8, 16, 16, 500, 520, [520, 64, 0, 1, 519, 300, 128, 65], [500, 1, 500, 0, 257, 256, 64, 333], "plain"),
+    (4, 32, 8, 512, 1100, [1100, 513, 64, 0], None, "plain"),           # heads of a key head as one run of rows
+    (4, 32, 8, 512, 1100, [1100, 513, 64, 0], [512, 500, 3, 512], "plain"),   # padding inside them: dK and dV of the tile kernel
+    (4, 32, 8, 512, 1100, None, None, "tokens"),                        # heads next to each other: likewise
+    (2, 8, 8, 600, 2100, [2100, 1999], [600, 77], "plain"),             # dK and dV by hand, too few workgroups for the others
+    (8, 64, 1, 256, 600, None, None, "plain"),                          # the reverse
+])
+def test_hand_scheduled(dtype, B, Hq, Hkv, Tq, Tk, lens, q_lens, layout):
+    """Head dimension 128 on long runs, against the oracle on some heads and the tile kernels' bounds."""
+    D = 128
+    q, k, v, d_o = _inputs(B, Hq, Hkv, Tq, Tk, D, dtype)
+    lens, q_lens = _lens(lens), _lens(q_lens)
+    on = [t.to(DEV) for t in (q, k, v, d_o)]
+    if layout == "tokens":
+        on = [t.transpose(1, 2).contiguous().transpose(1, 2) for t in on]
+    leaves = [t.requires_grad_() for t in on[:3]]
+    args = [None if x is None else x.to(DEV) for x in (lens, q_lens)]
+    o, lse = cross_attention(*leaves, *args, return_lse=True)
+    dq, dk, dv = torch.autograd.grad(o, leaves, on[3])
+    torch.cuda.synchronize()
+    G = Hq // Hkv
+    for b in range(B):
+        h = b % Hkv
+        heads = slice(h * G, (h + 1) * G)
+        one = [t[b:b + 1] for t in (q[:, heads], k[:, h:h + 1], v[:, h:h + 1], d_o[:, heads])]
+        want = kv_oracle.cross(*one[:3], None if lens is None else lens[b:b + 1], None if q_lens is None else q_lens[b:b + 1], None, one[3])
+        for name, got in (("o", o[b:b + 1, heads]), ("lse", lse[b:b + 1, heads]), ("dq", dq[b:b + 1, heads]),
+                          ("dk", dk[b:b + 1, h:h + 1]), ("dv", dv[b:b + 1, h:h + 1])):
+            kv_oracle.assert_within(f"{name} of {b}", got, want[name])
+
+
+@pytest.mark.parametrize("junk", [float("nan"), float("inf")])
+def test_hand_scheduled_padding_is_never_used(junk):
+    B, H, Tq, Tk = 8, 16, 500, 600
+    q, k, v, d_o = _inputs(B, H, H, Tq, Tk, 128, torch.bfloat16)
+    lens, q_lens = [600, 1, 64, 65, 0, 333, 512, 599], [500, 499, 256, 257, 31, 1, 0, 64]
+    clean = _run(q, k, v, d_o, _lens(lens), _lens(q_lens))
+    for b in range(B):
+        k[b, :, lens[b]:], v[b, :, lens[b]:] = junk, junk
+        q[b, :, q_lens[b]:], d_o[b, :, q_lens[b]:] = junk, junk
+    dirty = _run(q, k, v, d_o, _lens(lens), _lens(q_lens))
+    for name in clean:
+        assert torch.equal(clean[name], dirty[name]), name
+    assert (dirty["lse"][4, :, :31] == -float("inf")).all() and not dirty["o"][4].any()
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("scale", [-0.3, 0.0, 1.7])
 def test_scales(dtype, scale):
