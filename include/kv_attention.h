@@ -18,8 +18,8 @@
  *   - Outputs are fully written.  Rows from q_lens[b] (new_lens[b]) on: O, LSE and dQ are 0, and dO is not read.  A row that sees no key, or
  *     none with a score above -inf: O is 0, LSE -inf, and it passes no gradient on.  Keys that no row sees: dK and dV are 0.
  *   - Softmax statistics and all sums are float32.  The probabilities, and dS, are rounded to the element type as operands of
- *     the second products (float32 stays float32); the 16-bit dK/dV kernel at D >= 32 multiplies K by -sm_scale*log2(e) and
- *     rounds the product to the element type, as sa_bwd_dkdv does.  No atomics: results do not change from call to call.
+ *     the second products (float32 stays float32); the scale is applied to the scores in float32.  No atomics: results do not
+ *     change from call to call.
  *   - Return value: 0 on success, > 0 a hipError_t from a launch, < 0 one of KV_ERR_*; a call that returns KV_ERR_* has enqueued
  *     nothing.
  *   - Re-entrant.  The library's only mutable state is the kernels' LDS limits (hipFuncSetAttribute on the first call of each

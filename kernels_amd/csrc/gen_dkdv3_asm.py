@@ -23,7 +23,7 @@ Register map (the kernel is built for D = 128):
   v[208:239] wave-uniform inputs, copied to s40... at entry (see SCALARS below)
   v240, v241 buffer offsets of this lane for the Q / dO tile loads    v[242:243] lse (lanes 0-15) or delta
   (lanes 16-31) row pointer    v244 row of the next tile this lane fetches lse / delta for    v[245:247] temporaries
-  s40 free  s41 one past the last query tile  s42 query tile of the B side  s43 64*s42  s44 first row of
+  s40 free, or -scale*log2(e) (see v1_ops)  s41 one past the last query tile  s42 query tile of the B side  s43 64*s42  s44 first row of
   the block being masked  s45..s47 LDS address of the stages of tiles s42, s42+1, s42+2  s48 wave offset inside a
   tile for the asynchronous loads  s49 same for lse/delta  s50 last valid row  s[52:55], s[56:59] buffer resources
   of Q and dO  s60, s61 their running byte offsets  s62, s63 bytes between a wave's load instructions
@@ -44,8 +44,8 @@ PF = RING - 1
 
 
 class Gen:
-    def __init__(self, D, dt):
-        self.D, self.dt = D, dt
+    def __init__(self, D, dt, mul=False):
+        self.D, self.dt, self.mul = D, dt, mul
         self.NF, self.DB = D // 16, D // 32
         self.ROWB = D * 2
         self.TILE_B = TQ * self.ROWB
@@ -155,12 +155,17 @@ class Gen:
         """Probabilities of the block whose accumulator S[par] holds lse - score*scale*log2(e):
         P = exp2(-S), rounded per pair.  Returns one list of instructions per element step; a v_exp
         result is never consumed by the very next instruction (transcendental forwarding needs one
-        instruction in between), so a pair is rounded after the exponential of the next element."""
+        instruction in between), so a pair is rounded after the exponential of the next element.
+        With `mul` the K fragments are not scaled, S[par] holds lse/(scale*log2(e)) - score, and one multiplication by s40 comes before,
+        an element ahead of its exponential."""
         def cvt(i):     # pair (i - 1, i)
             return f"{self.cvt} {self.PB(i >> 3, (i & 7) >> 1)}, {self.PR(i - 1)}, {self.PR(i)}"
         steps = []
         for i in range(16):
             ops = [f"v_exp_f32 {self.PR(i)}, -{self.S(par, i)}"]
+            if self.mul:
+                ahead = [0, 1] if i == 0 else [i + 1] if i + 1 < 16 else []
+                ops = [f"v_mul_f32 {self.PR(k)}, s40, {self.S(par, k)}" for k in ahead] + [f"v_exp_f32 {self.PR(i)}, {self.PR(i)}"]
             if i >= 2 and (i & 1) == 0:
                 ops.append(cvt(i - 1))
             if i == 15:
@@ -317,7 +322,7 @@ class Gen:
         return self.out
 
 
-SCALARS = ["spare", "qt1", "t", "q64", "n32", "st0", "st1", "st2", "wave_tile", "wave_rows", "last_row", "qlo_max",
+SCALARS = ["mul", "qt1", "t", "q64", "n32", "st0", "st1", "st2", "wave_tile", "wave_rows", "last_row", "qlo_max",
            "rq0", "rq1", "rq2", "rq3", "rg0", "rg1", "rg2", "rg3", "soff_q", "soff_g", "istep_q", "istep_g",
            "tstep_q", "tstep_g", "tmp0", "tmp1", "tmp2", "qhi_min"]          # v208 + i  ->  s40 + i
 
@@ -350,8 +355,8 @@ def issue_tile(g):
     return out, 2 * per_wave + 1
 
 
-def generate(D, dt):
-    g = Gen(D, dt)
+def generate(D, dt, mul=False):
+    g = Gen(D, dt, mul)
     NS = g.NS
     split = NS - PF
     # steady state: simulate odd, even, odd, even steps and keep the last pair
@@ -364,7 +369,7 @@ def generate(D, dt):
         k += 2
     # prologue: addresses of the first tile, ring entries of the first step's slots 0..PF-1, the first
     # block's accumulator starts; everything has returned when it ends
-    p = Gen(D, dt)
+    p = Gen(D, dt, mul)
     pro = [f"v_readfirstlane_b32 s{40 + i}, v{208 + i}" for i in range(len(SCALARS))]
     p.out = pro + p.prologue()
     for j in range(PF):
@@ -410,7 +415,7 @@ def generate(D, dt):
     text += ["s_branch " + L("Lloop"),
              L("Lend") + ":",
              "s_nop 15", "s_nop 15"]            # the accumulators are read by vector instructions next
-    name = f"SA_DKDV3_{D}_{dt.upper()}"
+    name = f"SA_DKDV3{'_MUL' if mul else ''}_{D}_{dt.upper()}"
     return f"#define {name} \\\n" + " \\\n".join('    "' + ln + '\\n"' for ln in text) + "\n"
 
 
@@ -423,6 +428,7 @@ def main():
     for D in (128,):
         for dt in ("bf16", "f16"):
             print(generate(D, dt))
+            print(generate(D, dt, True))
 
 
 if __name__ == "__main__":

@@ -98,7 +98,7 @@ __global__ __launch_bounds__(NW * 64) void cross_dq_kernel(const BwdParams p) {
     if (lse == -INFINITY || row >= live) lse = INFINITY;   // P = exp2(-inf) = 0: no key is seen, or padding
     if (split == 0 && h == 0 && row < live) {
       const int64_t at = p.head_major ? p.map.flat(bh, row) : (int64_t)bh * rows + row;
-      p.row_lse[at] = lse;
+      p.row_lse[at] = Elem<T>::HALF ? lse / sa::score_scale(p.scale_log2e) : lse;
       p.row_delta[at] = delta;
     }
 #pragma unroll
@@ -146,7 +146,7 @@ __global__ __launch_bounds__(NW * 64) void cross_dq_kernel(const BwdParams p) {
   store_rows<T, D, DB>(out, p.map, bh, wr0, smem + wave * sa::RowPatch<T, D>::ELEMS, acc, -p.scale, lane);
 }
 
-// dV^T += dO^T P and dK^T += Q^T dS, negated, for the TQ rows from r0 on, or one of them: float32 (16-bit elements: sa::dkdv2_tile).
+// dV^T += dO^T P and dK^T += Q^T dS, negated, for the TQ rows from r0 on, or one of them: float32 (16-bit elements: below).
 // v holds -V.
 template <typename T, int D, int TQ, bool WITH_DK, bool WITH_DV, int NF, int NV, int DK, int DV>
 SA_DEV void dkdv_tile_f32(f32x16 (&dk)[DK], f32x16 (&dv)[DV], const T* qt, const T* gt, int r0, int live,
@@ -181,6 +181,45 @@ SA_DEV void dkdv_tile_f32(f32x16 (&dk)[DK], f32x16 (&dv)[DV], const T* qt, const
     }
     if constexpr (WITH_DV) mul_tr<T, D>(dv, gt, n * 32, s[0], lane);
     if constexpr (WITH_DK) mul_tr<T, D>(dk, qt, n * 32, dp[0], lane);
+  }
+}
+
+// The same, both gradients, 16-bit elements.  k holds -K (K for a negative scale), unrounded; the score accumulator starts at
+// lse / score_scale, so that one multiplication by mul = -score_scale gives the exponent.  (K scaled and rounded, as streaming attention has it, saves that
+// and takes dK and dV further from the exact result: relative errors 0.0030 instead of 0.0024 in bfloat16, whose own rounding is 0.0017.)
+// rows(r) gives the four lse and the four delta values of the tile's rows r to r + 3; v holds -V.
+template <typename T, int D, int TQ, int PG, int NF, int DB, typename Rows>
+SA_DEV void dkdv_tile_16(f32x16 (&dk)[DB], f32x16 (&dv)[DB], const T* qt, const T* gt, int r0, int live,
+                         const typename Elem<T>::Frag (&k)[NF], const typename Elem<T>::Frag (&v)[NF], float mul, Rows&& rows,
+                         int lane) {
+  const int h = lane >> 5;
+#pragma unroll
+  for (int n = 0; n < TQ / 32; ++n) {
+    if (r0 + n * 32 >= live) continue;
+    f32x16 s, dp;
+#pragma unroll
+    for (int g4 = 0; g4 < 4; ++g4) {
+      f32x4 l4, d4;
+      rows(n * 32 + 8 * g4 + 4 * h, l4, d4);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s[4 * g4 + e] = l4[e], dp[4 * g4 + e] = d4[e];
+    }
+    sa::mma_rows_pair<T, D, NF, PG>(s, dp, qt, gt, n * 32, k, v, lane);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      s[i] = sa::fast_exp2(s[i] * mul);
+      dp[i] *= s[i];   // = -dS
+    }
+    if (r0 + n * 32 + 32 > live) {
+      const uint32_t mask = sa::row_mask(0, live - r0 - n * 32, h);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const uint32_t keep = sa::keep_bits(mask, i);
+        s[i] = sa::keep_or_zero(s[i], keep);
+        dp[i] = sa::keep_or_zero(dp[i], keep);
+      }
+    }
+    sa::mma_tr_pair<T, D, DB, PG>(dv, dk, gt, qt, n, s, dp, lane);
   }
 }
 
@@ -273,13 +312,13 @@ __global__ __launch_bounds__(NW * 64, (sizeof(T) == 2 && D == 64 ? 3 : 1)) void 
     }
     if constexpr (Elem<T>::HALF)
 #pragma unroll
-      for (int i = 0; i < NF; ++i) kf[i] = sa::dkdv2_keys<T, D>(kf[i], p.scale_log2e);
+      for (int i = 0; i < NF; ++i)
+        if (p.scale_log2e >= 0.0f) kf[i] = sa::negate<T>(kf[i]);
   }
   f32x16 dk[WITH_DK ? DB : 1], dv[WITH_DV ? DB : 1];
   clear(dk);
   clear(dv);
   sa::wait_all_loads();
-  const sa::WaveWindow win{0, live, 0, live, 0, wk0 < L ? live : 0};
   for (int t = t0; t < t1; ++t) {
     sa::wait_loads<0>();
     __syncthreads();
@@ -287,10 +326,10 @@ __global__ __launch_bounds__(NW * 64, (sizeof(T) == 2 && D == 64 ? 3 : 1)) void 
     const char* const stage = smem_raw + ((t - t0) & 1) * STAGE;
     const T* const qt = reinterpret_cast<const T*>(stage);
     const float* const stats = reinterpret_cast<const float*>(stage + 2 * TILE * sizeof(T));
-    if (!win.seen(t * TQ, TQ)) continue;
+    if (wk0 >= L) continue;
     if constexpr (Elem<T>::HALF) {
-      sa::dkdv2_tile<T, D, TQ, (D == 64 ? 2 : 4)>(dk, dv, qt, qt + TILE, t * TQ, win, kf, vf, p.scale_log2e,
-                                                   [&](int r, f32x4& l4, f32x4& d4) {
+      dkdv_tile_16<T, D, TQ, (D == 64 ? 2 : 4)>(dk, dv, qt, qt + TILE, t * TQ, live, kf, vf, -sa::score_scale(p.scale_log2e),
+                                                 [&](int r, f32x4& l4, f32x4& d4) {
         const float* chunk = stats + (r / RPW) * 2 * RPW + r % RPW;
         l4 = *reinterpret_cast<const f32x4*>(chunk);
         d4 = *reinterpret_cast<const f32x4*>(chunk + RPW);
@@ -397,17 +436,18 @@ __global__ __launch_bounds__(512) void cross_dkdv_wide_kernel(const BwdParams p)
   if (grad_role) Rows::send(reinterpret_cast<const T*>(p.v) + b * p.v_sb + hk * p.v_sh, p.v_st, wk0, L - 1, area, lane);
   else Rows::send(reinterpret_cast<const T*>(p.k) + b * p.k_sb + hk * p.k_sh, p.k_st, wk0, L - 1, area, lane);
   sa::landed();
-  // resident fragments: K * (-scale * log2 e), rounded, for the score role, -V for the grad role
+  // resident fragments: -K (K for a negative scale) for the score role, -V for the grad role; the scores as in dkdv_tile_16
   Frag rf[1][NF];
   {
-    const float mul = grad_role ? -1.0f : -p.scale_log2e;
+    uint32_t flip = grad_role || !(p.scale_log2e < 0.0f) ? E::SIGN : 0u;
+    asm("" : "+v"(flip));
 #pragma unroll
     for (int i = 0; i < NF; ++i) {
-      rf[0][i] = Rows::read(area, i, lane);
-#pragma unroll
-      for (int e = 0; e < E::VEC; ++e) rf[0][i][e] = (T)((float)rf[0][i][e] * mul);
+      const Frag f = Rows::read(area, i, lane);
+      rf[0][i] = __builtin_bit_cast(Frag, __builtin_bit_cast(u32x4, f) ^ flip);
     }
   }
+  const float score_mul = -sa::score_scale(p.scale_log2e);
   __syncthreads();
   if (n > 0) issue_tile(0, 0);
   if (n > 1) issue_tile(1, 1);
@@ -446,9 +486,9 @@ __global__ __launch_bounds__(512) void cross_dkdv_wide_kernel(const BwdParams p)
       if (!seen) continue;
       f32x16 s[1][1];
       rows16(it, 0, s[0][0]);
-      sa::mma_rows_n<T, D>(s, q_ring + (it & (NQ - 1)) * TILE, 0, rf, lane);          // lse - S[row][key]
+      sa::mma_rows_n<T, D>(s, q_ring + (it & (NQ - 1)) * TILE, 0, rf, lane);          // lse / score_scale - S[row][key]
 #pragma unroll
-      for (int i = 0; i < 16; ++i) s[0][0][i] = sa::fast_exp2(-s[0][0][i]);
+      for (int i = 0; i < 16; ++i) s[0][0][i] = sa::fast_exp2(s[0][0][i] * score_mul);
       masked(it, s[0][0]);
       float* slot = xbuf + (it & 1) * S::XSLOT;
 #pragma unroll

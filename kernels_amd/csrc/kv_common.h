@@ -92,9 +92,8 @@ SA_DEV void copy_gather_asm(const void* src, uint32_t lds_addr) {
 SA_DEV void copy_gather_word_asm(const void* src, uint32_t lds_addr) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" : : "s"(lds_addr), "v"(src) : "memory", "m0");
 }
-SA_DEV uint32_t lds_address(const void* p) {
-  return (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(uintptr_t)(SA_LDS const void*)p);
-}
+// The low half of a generic address in LDS is the address there (a cast of the pointer would compare it with null first).
+SA_DEV uint32_t lds_address(const void* p) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(uintptr_t)p); }
 // Until at most N of this wave's copies are on their way; no LDS access is moved ahead of it.
 template <int N> SA_DEV void arrived_but() {
   static_assert(N >= 0 && N < 64, "vmcnt is a 6-bit counter");
@@ -321,7 +320,7 @@ struct BwdParams {
   int B, Tk;
   float scale, scale_log2e;
   Work work;
-  float *row_lse, *row_delta;   // [B * Hkv, rows]: written with dQ, read with dK and dV
+  float *row_lse, *row_delta;   // [B * Hkv, rows]: written with dQ, read with dK and dV; 16-bit elements: lse / score_scale
   bool head_major;     // those in the order (head, token) instead of that of the rows
   float* part;         // dQ: [splits, B * Hkv, rows, D]; dK and dV: [splits, 2, B * Hkv, Tk, D]
 };

@@ -179,7 +179,10 @@ __global__ __launch_bounds__(256) void dkdv3_kernel(const P p) {
     // and ends at delta - dP.  K enters multiplied by -scale*log2(e) and rounded to the element
     // type: the score accumulator starts at lse and ends at lse - score*scale*log2(e), whose
     // negated exp2 is the probability, with no vector instruction between MFMA and v_exp.
-    const float kmul = -p.scale_log2e;
+    // CROSS: K enters with its sign turned (twice where the scale is negative), nothing rounded, and the accumulator of
+    // lse / (scale*log2(e)) - score is multiplied once more.  Rounded to bfloat16 the scaled K took dK and dV of long runs 1.7 times
+    // as far from the exact result as a rounding of them does, unscaled 1.4 times.
+    const float kmul = CROSS ? (p.scale_log2e < 0.0f ? 1.0f : -1.0f) : -p.scale_log2e;
     landed();
 #pragma unroll
     for (int g = 0; g < NF; ++g) {
@@ -220,6 +223,7 @@ __global__ __launch_bounds__(256) void dkdv3_kernel(const P p) {
   for (int i = 0; i < 32; ++i) r_scal[i] = 0u;
   {
     const int t0 = qt0 - 1;   // tile of the first step's B side: the phantom block's
+    if constexpr (CROSS) r_scal[SA_DKDV3_SC_MUL] = __float_as_uint(-score_scale(p.scale_log2e));
     r_scal[SA_DKDV3_SC_QT1] = (uint32_t)qt1;
     r_scal[SA_DKDV3_SC_T] = (uint32_t)t0;
     r_scal[SA_DKDV3_SC_Q64] = (uint32_t)(64 * t0);
@@ -259,7 +263,9 @@ __global__ __launch_bounds__(256) void dkdv3_kernel(const P p) {
     r_ptrs[4] = (uint32_t)((qt0 + 2) * TQ + wave * RPW + (lane % RPW));
     r_ptrs[5] = r_ptrs[6] = r_ptrs[7] = 0u;
   }
-  if constexpr (BF16) asm volatile(SA_DKDV3_128_BF16 SA_DKDV3_OPERANDS);
+  if constexpr (CROSS && BF16) asm volatile(SA_DKDV3_MUL_128_BF16 SA_DKDV3_OPERANDS);
+  else if constexpr (CROSS) asm volatile(SA_DKDV3_MUL_128_F16 SA_DKDV3_OPERANDS);
+  else if constexpr (BF16) asm volatile(SA_DKDV3_128_BF16 SA_DKDV3_OPERANDS);
   else asm volatile(SA_DKDV3_128_F16 SA_DKDV3_OPERANDS);
 
   f32x16 dk[DB], dv[DB];

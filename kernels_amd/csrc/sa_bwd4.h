@@ -204,7 +204,7 @@ __global__ __launch_bounds__(256) void dq3_kernel(const P p) {
           const int64_t at = p.token_major ? ((int64_t)(bh - (hd - hk * p.group)) * T_ + (int64_t)qrow[qb] * p.group + (hd - hk * p.group))
                                            : (int64_t)bh * T_ + qrow[qb];
           p.delta_out[at] = delta_q;
-          p.lse_out[at] = lse_q;
+          p.lse_out[at] = lse_q / score_scale(p.scale_log2e);
         }
       } else if (p.delta_out) {
         delta_q = RowDots<T, D>::total(reinterpret_cast<const float*>(q_area(qb)), lane);

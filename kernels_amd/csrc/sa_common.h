@@ -1024,9 +1024,11 @@ template <typename Base> struct CrossOf : Base {
   int group;                    // query heads of a key head
   int q_tiles;                  // query tiles of a head: the map has group * q_tiles tiles for each key head
   ChunkDiv by_q_tiles;
-  float* lse_out;               // dQ kernel: log-sum-exp of the rows beside delta_out, +inf where a row sees nothing
+  float* lse_out;               // dQ kernel: lse / score_scale of the rows beside delta_out, +inf where a row sees nothing
   bool token_major;             // dQ kernel: those in the order (token, head) of a key head instead of (head, token)
 };
+// |scale * log2(e)|, never exactly 0: what is divided by it comes back when it is multiplied.
+SA_DEV float score_scale(float scale_log2e) { return fmaxf(fabsf(scale_log2e), 1e-30f); }
 template <typename P> struct IsCross { static constexpr bool value = false; };
 template <typename B> struct IsCross<CrossOf<B>> { static constexpr bool value = true; };
 template <typename P> SA_DEV int other_length(const P& p, int b) {

@@ -2,7 +2,7 @@
 the kernels' roundings may change, element by element.
 
 The bounds count roundings (u: half a step of the element type, e: 2^-24 of float32) against sums of magnitudes:
-  a score       e * (D + 4) * scale * |q| . |k|; in the 16-bit dK/dV kernel also u * that product (K is scaled and rounded)
+  a score       e * (D + 4) * scale * |q| . |k|
   P             relative: twice the score's error (exp, and the sum it is divided by) + 2^-20 (exp2, log2) + u as an operand
   O             sum P |v| times P's relative error + u * |O| + e * (keys + 64) * sum P |v|
   delta         sum over D of O's error times |dO|
@@ -52,20 +52,18 @@ def _head(q, k, v, seen, scale, dtype, g=None):
     dp = g @ v.T
     delta = (o * g).sum(-1, keepdim=True)
     ds = p * (dp - delta)
-    scaled = u * qk if D >= 32 else 0.0   # dK/dV
     p_rel = rel + u + worst
     delta_err = (o_err * g.abs()).sum(-1, keepdim=True)
     sums = E32 * (D + 4) * (g.abs() @ v.abs().T + (o.abs() * g.abs()).sum(-1, keepdim=True))
     ds_err = ds.abs() * p_rel + p * (delta_err + sums)
-    ds_err_k = ds_err + ds.abs() * scaled * 1.1
     more = E32 * (max(m, n) + 64)
     dv = p.T @ g
     dq = scale * (ds @ k)
     dk = scale * (ds.T @ q)
     s = abs(scale)
-    out["dv"] = (dv, (p * (p_rel + scaled * 1.1 + more) + sub * visible).T @ g.abs() + final * dv.abs() + tiny)
+    out["dv"] = (dv, (p * (p_rel + more) + sub * visible).T @ g.abs() + final * dv.abs() + tiny)
     out["dq"] = (dq, s * ((ds_err + ds.abs() * more + sub * visible) @ k.abs()) + final * dq.abs() + tiny)
-    out["dk"] = (dk, s * ((ds_err_k + ds.abs() * more + sub * visible).T @ q.abs()) + final * dk.abs() + tiny)
+    out["dk"] = (dk, s * ((ds_err + ds.abs() * more + sub * visible).T @ q.abs()) + final * dk.abs() + tiny)
     return out
 
 
