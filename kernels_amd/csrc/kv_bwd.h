@@ -44,7 +44,6 @@ template <typename T> SA_DEV float dot(typename Elem<T>::Frag a, typename Elem<T
   }
 }
 
-template <typename T, int D> constexpr int dq_stages() { return 2; }
 template <typename T, int D> constexpr int dq_tile() { return Elem<T>::HALF ? 64 : fwd_tile<T, D>(); }
 
 template <typename T, int D, int NW>
@@ -71,13 +70,10 @@ __global__ __launch_bounds__(NW * 64) void cross_dq_kernel(const BwdParams p) {
   int t0, t1;
   part_of(p.work, (L + TK - 1) / TK, split, t0, t1);
   if (t0 >= t1 && split > 0) return;   // (the first one leaves delta)
-  constexpr int NST = dq_stages<T, D>();
-  PairCopy<T, D, TK, NW, (NST > 2)> tiles;
+  PairCopy<T, D, TK, NW> tiles;
   tiles.init(reinterpret_cast<const T*>(p.k) + b * p.k_sb + hk * p.k_sh, p.k_st,
              reinterpret_cast<const T*>(p.v) + b * p.v_sb + hk * p.v_sh, p.v_st, L - 1, wave, lane);
-#pragma unroll
-  for (int i = 0; i < NST - 1; ++i)
-    if (t0 + i < t1) tiles.issue(smem + i * STAGE, t0 + i, wave);
+  if (t0 < t1) tiles.issue(smem, t0, wave);
 
   const float sl2e = fabsf(p.scale_log2e);
   Frag qf[NF], gf[NF];
@@ -112,15 +108,11 @@ __global__ __launch_bounds__(NW * 64) void cross_dq_kernel(const BwdParams p) {
 #pragma unroll
   for (int i = 0; i < 16; ++i) dinit[i] = delta;
   const sa::WaveWindow win{0, L, 0, L, 0, L};
-  int stage = -1;
-  auto next_tile = [&](int t) {   // waits for tile t, sends for the one NST - 1 after it
-    if (t + NST - 2 < t1) arrived_but<(NST - 2) * PairCopy<T, D, TK, NW>::PER_WAVE>();
-    else arrived_but<0>();
+  auto next_tile = [&](int t) {   // waits for tile t, sends for the next one
+    sa::wait_loads<0>();
     __syncthreads();
-    const int before = stage < 0 ? NST - 1 : stage;
-    stage = stage + 1 == NST ? 0 : stage + 1;
-    if (t + NST - 1 < t1) tiles.issue(smem + before * STAGE, t + NST - 1, wave);
-    return smem + stage * STAGE;
+    if (t + 1 < t1) tiles.issue(smem + ((t + 1 - t0) & 1) * STAGE, t + 1, wave);
+    return smem + ((t - t0) & 1) * STAGE;
   };
   int t = t0;
   if constexpr (Elem<T>::HALF && D == 256)   // a loop of their own: where two paths meet the compiler copies 128 accumulators

@@ -101,15 +101,13 @@ template <int N> SA_DEV void arrived_but() {
 }
 
 // Rows [first, first + ROWS) of a [*, D] matrix with one row stride, by NW waves.  Rows past the last valid one come as zeros (the
-// buffer's range check).  Offsets inside the matrix are 32-bit: the host checks that (rows + 1024) * stride fits.  ASM: as assembly, for
-// rings of more than two stages (see copy_gather_asm).
-template <typename T, int D, int ROWS, int NW, bool ASM = false> struct RowCopy {
+// buffer's range check).  Offsets inside the matrix are 32-bit: the host checks that (rows + 1024) * stride fits.
+template <typename T, int D, int ROWS, int NW> struct RowCopy {
   using G = Geom<T, D>;
   static constexpr int RPI = G::RPI, NI = ROWS / RPI, PER_WAVE = NI / NW;
   static_assert(ROWS % (RPI * NW) == 0, "the tile must split evenly over the waves");
   static constexpr int NVO = (RPI * NW) % 16 == 0 ? 1 : 16 / (RPI * NW);   // the exchange of chunks repeats every 16 rows
   __amdgpu_buffer_rsrc_t rsrc;
-  u32x4 words;   // the same descriptor for the assembly
   uint32_t voff[NVO], istep, tstep;
 
   SA_DEV void init(const T* base, int64_t row_stride, int last_row, int wave, int lane) {
@@ -117,12 +115,7 @@ template <typename T, int D, int ROWS, int NW, bool ASM = false> struct RowCopy 
     const uint32_t rs = (uint32_t)row_stride;
     const int lrow = lane / G::CPR, ch = lane % G::CPR;
     const uint32_t bytes = ((uint32_t)last_row * rs + (uint32_t)D) * ES;
-    const uint64_t addr = reinterpret_cast<uint64_t>(base);
     rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(base), 0, (int)bytes, 0x00020000);
-    words[0] = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)addr);
-    words[1] = (uint32_t)__builtin_amdgcn_readfirstlane((int)((uint32_t)(addr >> 32) & 0xFFFFu));
-    words[2] = (uint32_t)__builtin_amdgcn_readfirstlane((int)bytes);
-    words[3] = 0x00020000u;
 #pragma unroll
     for (int j = 0; j < NVO; ++j)
       voff[j] = ((uint32_t)(wave * RPI + lrow) * rs + (uint32_t)((ch ^ G::swz((j * NW + wave) * RPI + lrow)) * G::VEC)) * ES;
@@ -131,21 +124,17 @@ template <typename T, int D, int ROWS, int NW, bool ASM = false> struct RowCopy 
   }
   SA_DEV void issue(T* tile, int t, int wave) const {   // rows [t * ROWS, (t + 1) * ROWS)
 #pragma unroll
-    for (int i = 0; i < PER_WAVE; ++i) {
-      T* const dst = tile + (i * NW + wave) * RPI * D;
-      const uint32_t off = (uint32_t)t * tstep + (uint32_t)i * istep;
-      if constexpr (ASM) sa::copy_rows_asm(words, voff[i % NVO], (uint32_t)__builtin_amdgcn_readfirstlane((int)off), lds_address(dst));
-      else __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (SA_LDS void*)dst, 16, (int)voff[i % NVO], (int)off, 0, 0);
-    }
+    for (int i = 0; i < PER_WAVE; ++i)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (SA_LDS void*)(tile + (i * NW + wave) * RPI * D), 16, (int)voff[i % NVO],
+                                               (int)((uint32_t)t * tstep + (uint32_t)i * istep), 0, 0);
   }
 };
 
 // The tiles of two matrices that a step reads together, one behind the other in a stage.
-template <typename T, int D, int ROWS, int NW, bool ASM = false> struct PairCopy {
+template <typename T, int D, int ROWS, int NW> struct PairCopy {
   static constexpr bool SHARED = ROWS / Geom<T, D>::RPI % NW != 0;   // D = 16, 16-bit: half of the waves to a matrix
   static constexpr int EACH = SHARED ? NW / 2 : NW;
-  using Copy = RowCopy<T, D, ROWS, EACH, ASM>;
-  static constexpr int PER_WAVE = (SHARED ? 1 : 2) * Copy::PER_WAVE;   // copies of a wave per step
+  using Copy = RowCopy<T, D, ROWS, EACH>;
   Copy a, b;   // SHARED: a is this wave's
   SA_DEV void init(const T* base_a, int64_t stride_a, const T* base_b, int64_t stride_b, int last_row, int wave, int lane) {
     const bool second = SHARED && wave >= EACH;

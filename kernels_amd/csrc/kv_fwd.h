@@ -97,8 +97,6 @@ SA_DEV void softmax_step(RowState<DB>& st, f32x16 (&s)[NB], float sl2e, const T*
 
 template <typename T, int D> constexpr int fwd_tile() { return D * (int)sizeof(T) <= 256 ? 64 : 32; }
 
-template <typename T, int D> constexpr int fwd_stages() { return 2; }
-
 template <typename T, int D, int NW>
 __global__ __launch_bounds__(NW * 64, (D * sizeof(T) == 512 ? (sizeof(T) == 2 ? 2 : 1) : 1)) void cross_fwd_kernel(const FwdParams p) {
   using G = Geom<T, D>;
@@ -145,22 +143,17 @@ __global__ __launch_bounds__(NW * 64, (D * sizeof(T) == 512 ? (sizeof(T) == 2 ? 
   RowState<DB> st;
   st.init();
   if (t0 < t1) {
-    constexpr int NST = fwd_stages<T, D>();
-    PairCopy<T, D, TK, NW, (NST > 2)> tiles;
+    PairCopy<T, D, TK, NW> tiles;
     tiles.init(reinterpret_cast<const T*>(p.k) + b * p.k_sb + hk * p.k_sh, p.k_st,
                reinterpret_cast<const T*>(p.v) + b * p.v_sb + hk * p.v_sh, p.v_st, L - 1, wave, lane);
     sa::wait_all_loads();   // the row's fragments
-#pragma unroll
-    for (int i = 0; i < NST - 1; ++i)
-      if (t0 + i < t1) tiles.issue(smem + i * STAGE, t0 + i, wave);
-    int stage = 0;
-    for (int t = t0; t < t1; ++t, stage = stage + 1 == NST ? 0 : stage + 1) {
-      if (t + NST - 2 < t1) arrived_but<(NST - 2) * PairCopy<T, D, TK, NW>::PER_WAVE>();
-      else arrived_but<0>();
-      __syncthreads();   // every wave's share of tile t has arrived; the stage of the tile before is free
-      if (t + NST - 1 < t1) tiles.issue(smem + (stage == 0 ? NST - 1 : stage - 1) * STAGE, t + NST - 1, wave);
+    tiles.issue(smem, t0, wave);
+    for (int t = t0; t < t1; ++t) {
+      sa::wait_loads<0>();
+      __syncthreads();   // every wave's share of tile t has arrived; the other stage, that of the tile before, is free
+      if (t + 1 < t1) tiles.issue(smem + ((t + 1 - t0) & 1) * STAGE, t + 1, wave);
       if (wr0 >= live) continue;
-      const T* keys = smem + stage * STAGE;
+      const T* keys = smem + ((t - t0) & 1) * STAGE;
       f32x16 s[NB];
       clear(s);
       mul_rows<T, D>(s, keys, 0, qf, lane);

@@ -65,7 +65,7 @@ template <> int launch_cross_fwd<ElemT, KV_DGROUP>(const FwdParams& p, int D, hi
   return by_head_dim(D, [&](auto d) {
     constexpr int DD = decltype(d)::value;
     static LdsLimit state;
-    const size_t lds = with_patches<ElemT, DD>(fwd_stages<ElemT, DD>() * 2 * fwd_tile<ElemT, DD>() * DD * sizeof(ElemT), 4);
+    const size_t lds = with_patches<ElemT, DD>(2 * 2 * fwd_tile<ElemT, DD>() * DD * sizeof(ElemT), 4);
     return launch(cross_fwd_kernel<ElemT, DD, 4>, (int64_t)p.work.map.nbh * p.work.map.n_tiles, 256, lds, state, p, st);
   });
 }
@@ -74,7 +74,7 @@ template <> int launch_cross_dq<ElemT, KV_DGROUP>(const BwdParams& p, int D, hip
   return by_head_dim(D, [&](auto d) {
     constexpr int DD = decltype(d)::value;
     static LdsLimit state;
-    const size_t lds = with_patches<ElemT, DD>(dq_stages<ElemT, DD>() * 2 * dq_tile<ElemT, DD>() * DD * sizeof(ElemT), 4);
+    const size_t lds = with_patches<ElemT, DD>(2 * 2 * dq_tile<ElemT, DD>() * DD * sizeof(ElemT), 4);
     return launch(cross_dq_kernel<ElemT, DD, 4>, (int64_t)p.work.map.nbh * p.work.map.n_tiles, 256, lds, state, p, st);
   });
 }
