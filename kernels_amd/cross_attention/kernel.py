@@ -51,7 +51,7 @@ def cross_attention(
     key head (a decoding step) run a kernel that divides long runs of keys over the GPU.
 
     Results do not change from call to call.  Forward and backward can be captured into a HIP graph together, after one call
-    with the same type and head dimension outside the capture; as with any PyTorch operator, no graph of autograd that was recorded
+    of the same sizes and type outside the capture; as with any PyTorch operator, no graph of autograd that was recorded
     outside the capture and shares its leaves may be alive then.
     """
     if ops.takes_native_call(q, k, v, lens, q_lens):

@@ -89,7 +89,7 @@ int plan_cross(CrossPlan& c, int B, int Hq, int Hkv, int Tq, int Tk, int D, int 
   c.long_keys = hand_scheduled && long_keys(c.nbh, c.rows, Tk);
   if (c.few) {
     const int64_t tiles = ceil_div(Tk, 32);
-    c.fwd.share = rows_share(c.nbh, tiles, D * elem_size(dtype), dtype == 0);
+    c.fwd.share = rows_share(c.nbh, (int)c.rows, tiles, D * elem_size(dtype), dtype == 0);
     c.fwd.splits = (int)std::max<int64_t>(1, ceil_div(tiles, c.fwd.share));
   } else {
     c.fwd = tile_shares(c.nbh * row_tiles, ceil_div(Tk, c.key_tile));
@@ -146,7 +146,7 @@ int plan_paged(PagedPlan& c, int B, int Hq, int Hkv, int T, int D, int page, int
   const int64_t tokens = std::min<int64_t>(T, 31 / G + 2), chunks = ceil_div(tokens - 1, C) + 1;
   const int64_t span = R > most || C > most ? most : std::min<int64_t>(most, (R + chunks) * C);
   const int64_t tiles = std::min(ceil_div(most, 32), ceil_div(span, 32) + 1);
-  c.share = rows_share(c.nbh * c.row_tiles, tiles, D * elem_size(dtype), dtype == 0);
+  c.share = rows_share(c.nbh * c.row_tiles, (int)std::min<int64_t>(c.rows, 32), tiles, D * elem_size(dtype), dtype == 0);
   c.splits = (int)std::max<int64_t>(1, ceil_div(tiles, c.share));
   if (c.nbh * c.row_tiles * c.splits > kMostBlocks || (c.splits > 1 && c.nbh * c.rows > kMostBlocks)) return KV_ERR_TOO_LARGE;
   if (c.splits > 1) c.bytes = c.splits * c.nbh * c.rows * (D + 2) * 4;
@@ -405,6 +405,8 @@ int kv_paged_append(const void* k, const void* v, void* k_pages, void* v_pages, 
   if (int rc = check_layout(k_pages, kps, dtype, page_size, false)) return rc;
   if (int rc = check_layout(v_pages, vps, dtype, page_size, false)) return rc;
   if (!lens || !page_table) return KV_ERR_ARG;
+  for (const int64_t* s : {kps, vps})   // each place of the cache its own
+    if ((s[0] == 0 && num_pages > 1) || (s[1] == 0 && H > 1)) return KV_ERR_LAYOUT;
   const int64_t es = elem_size(dtype);
   AppendParams p{};
   p.k = (const char*)k; p.v = (const char*)v; p.k_pages = (char*)k_pages; p.v_pages = (char*)v_pages;

@@ -63,7 +63,7 @@ inline bool long_keys(int64_t key_heads, int64_t rows, int64_t Tk) { return rows
 
 // The rows kernel serves up to 32 rows of a key head.
 inline bool few_rows(int64_t rows) { return rows <= 32; }
-// How its keys are divided, from the sizes of the call: at most n tiles of 32 keys for each of `units` workgroups.  A share is
+// How its keys are divided, from the sizes of the call: at most n tiles of 32 keys for each of `units` workgroups of `rows` rows.  A share is
 // what leaves one workgroup for each CU, from four tiles on; short runs are not divided (the joining kernel takes about 4 us), and shares of
 // many workgroups stay short, so that long sequences of a batch spread over the CUs that short ones have left.  float32 is bound by its matrix
 // instructions and gains by every division (128 units of 63 tiles, D = 64: 55 us in one share, 37 in two).
@@ -72,13 +72,16 @@ inline bool few_rows(int64_t rows) { return rows <= 32; }
 // 26.7*, 32.2, 50.2; 128 units of 16 16.3, 13.1, 11.0*; of 63 45.2, 35.7, 29.8, 26.9*, 28.9; two waves: 512 units of 16 33.4, 29.9, 23.8*; of
 // 63 121, 111, 105, 99.7, 94.5*; of up to 256, ragged: shares of 32 109*, 64 118.  D = 64, four waves: 8 units of 63 8.3*, 8.3, 9.9, 12.7, 16.5; 32 of 63
 // 9.9, 9.0*, 10.7, 13.6, 17.4; 512 units of 63 78.3, 63.3, 57.5, 54.4, 49.2*; eight waves: 128 units of 63 35.3, 24.4, 20.6, 16.9, 15.3* (four: 19.7).
-inline int rows_share(int64_t units, int64_t n, int row_bytes, bool f32) {
+inline int rows_share(int64_t units, int rows, int64_t n, int row_bytes, bool f32) {
   if (n <= (row_bytes <= 128 ? 32 : 16)) return (int)std::max<int64_t>(n, 1);
   int64_t share = std::max<int64_t>(4, ceil_div(units * n, CUS));
   if (2 * share >= n && n <= 64 && !f32) return (int)n;
   if (share > 32 && units * ceil_div(n, 32) >= 4 * CUS) share = 32;
   share = std::min<int64_t>(share, 128);
-  return (int)std::max(share, ceil_div(n, 256));   // at most 256 parts to add up
+  // at most 256 parts to add up, and 256 MiB of them (the chunks of many long sequences)
+  const int64_t part = units * rows * (row_bytes / (f32 ? 4 : 2) + 2) * 4;
+  const int64_t most = std::max<int64_t>(1, std::min<int64_t>(256, (256 << 20) / part));
+  return (int)std::max(share, ceil_div(n, most));
 }
 // Waves of its workgroups, whose rings take most of the LDS.  Rows of 128 bytes: eight, one workgroup to a CU, where there are few workgroups with long
 // shares, else four.  256 bytes: two where there is more than one workgroup for each place, so that one begins while the other one is in its

@@ -74,7 +74,8 @@ def paged_attention(
     Tokens beyond ``new_lens[b]`` give 0 and log-sum-exp 0; a token that sees no position gives 0 and log-sum-exp -inf.  What the cache holds
     where no token sees it does not matter.  (A value that is not finite, seen by one of several new tokens, reaches the others of
     its sequence.)  The bits of a sequence's result depend on the sizes of the call, not on the lengths or values of other sequences.
-    Forward only.
+    Forward only.  Can be captured into a HIP graph after one call of the same sizes and type outside the capture.  Meant for few new
+    tokens: a whole prompt runs faster through :func:`streaming_attention.streaming_attention`, beside a :func:`paged_append`.
     """
     if back_contexts is None:
         back_contexts = _NO_LIMIT

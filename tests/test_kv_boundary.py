@@ -106,6 +106,7 @@ def test_paged_codes(lib):
     assert forward(Hq=3, Hkv=2) == -3 and forward(C=0) == -3 and forward(R=-1) == -3 and forward(o=None) == -3
     assert append(B=1 << 15, T=1 << 15) == -5
     assert append(N=0) == 0 and append(W=0) == 0
+    assert append(ks=_strides(512, 0, 64, 1)) == -4 and append(ks=_strides(0, 512, 64, 1)) == -4   # two heads, or two pages, in one place
     need = lib.kv_paged_forward_workspace(1, 2, 1, 1, 64, 8, 1000, 1, 2 ** 31 - 1, 1)
     assert need > 0 and forward(W=1000, R=2 ** 31 - 1, ws=p, bytes=need - 1) == -6
     assert lib.kv_paged_forward_workspace(1, 2, 1, 1, 64, 8, 1000, 1, 100, 1) == 0       # a short window is not divided
@@ -134,6 +135,14 @@ def test_shares_cover_every_window(lib, B, T, G, page, width, C, R):
     else:
         share = max(min(32 if share > 32 and units * -(-n // 32) >= 1024 else share, 128), -(-n // 256))
     assert splits == -(-n // share) and tiles <= splits * share
+    assert bytes_ <= 1 << 28
+
+
+def test_parts_stay_small(lib):
+    """A long chunk of many sequences does not ask for a workspace of gigabytes."""
+    for B, Hq, T in ((8, 64, 2048), (128, 64, 4), (1, 8, 1), (512, 128, 1)):
+        assert 0 <= lib.kv_paged_forward_workspace(B, Hq, 8, T, 128, 16, 4096, 1, 2 ** 31 - 1, 2) <= 1 << 28
+    assert lib.kv_paged_forward_workspace(64, 64, 8, 1, 128, 16, 4096, 1, 2 ** 31 - 1, 2) > 0   # and few rows are still divided
 
 
 def _cross(dtype=torch.float32, **kw):
