@@ -2,7 +2,8 @@
 //   cross_dq_kernel     dQ = scale * dS K               a lane owns a row, the keys go by
 //   cross_dkdv_kernel   dV = P^T dO, dK = scale * dS^T Q  a lane owns a key, the rows of all query heads that share it go by, so
 //                                                       that the sum over the heads is part of the product
-// The first one forms delta and leaves it, beside the log-sum-exp, in the order of the rows for the second.  No atomics: a
+// The first one forms delta (over few keys as rowsum(P * dP), in which O is not rounded: sa::few_keys_delta) and leaves it, beside the
+// log-sum-exp, in the order of the rows for the second.  No atomics: a
 // sum over workgroups (few rows and many keys, or the reverse) goes through float32 parts that are added up in order.
 #pragma once
 #include "sa_bwd.h"
@@ -85,22 +86,27 @@ __global__ __launch_bounds__(NW * 64) void cross_dq_kernel(const BwdParams p) {
     const int64_t head = (int64_t)hk * p.map.G + g;
     load_row<T, D>(qf, reinterpret_cast<const T*>(p.q) + b * p.q_sb + head * p.q_sh + t * p.q_st, true, lane);
     load_row<T, D>(gf, reinterpret_cast<const T*>(p.d_o) + b * p.g_sb + head * p.g_sh + t * p.g_st, true, lane);
-    const T* o = reinterpret_cast<const T*>(p.o) + b * p.o_sb + head * p.o_sh + t * p.o_st;
-#pragma unroll
-    for (int i = 0; i < NF; ++i)
-      delta = dot<T>(gf[i], *reinterpret_cast<const Frag*>(o + (i * 2 + h) * Elem<T>::VEC), delta);
-    delta = sa::half_sum(delta);
     lse = p.lse[p.map.flat(bh, r)];
     if (lse == -INFINITY || row >= live) lse = INFINITY;   // P = exp2(-inf) = 0: no key is seen, or padding
-    if (split == 0 && h == 0 && row < live) {
-      const int64_t at = p.head_major ? p.map.flat(bh, row) : (int64_t)bh * rows + row;
-      p.row_lse[at] = Elem<T>::HALF ? lse / sa::score_scale(p.scale_log2e) : lse;
-      p.row_delta[at] = delta;
-    }
 #pragma unroll
     for (int i = 0; i < NF; ++i) {
       if (p.scale_log2e < 0.0f) qf[i] = sa::negate<T>(qf[i]);
       gf[i] = sa::negate<T>(gf[i]);   // the dP accumulator starts at delta and ends at delta - dP
+    }
+    if (Elem<T>::HALF && L <= sa::FEW_KEYS) {
+      delta = sa::few_keys_delta<T>(reinterpret_cast<const T*>(p.k) + b * p.k_sb + hk * p.k_sh, p.k_st,
+                                    reinterpret_cast<const T*>(p.v) + b * p.v_sb + hk * p.v_sh, p.v_st, L, qf, gf, sl2e, lse, lane);
+    } else {
+      const T* o = reinterpret_cast<const T*>(p.o) + b * p.o_sb + head * p.o_sh + t * p.o_st;
+#pragma unroll
+      for (int i = 0; i < NF; ++i)
+        delta = dot<T>(gf[i], *reinterpret_cast<const Frag*>(o + (i * 2 + h) * Elem<T>::VEC), delta);
+      delta = -sa::half_sum(delta);
+    }
+    if (split == 0 && h == 0 && row < live) {
+      const int64_t at = p.head_major ? p.map.flat(bh, row) : (int64_t)bh * rows + row;
+      p.row_lse[at] = Elem<T>::HALF ? lse / sa::score_scale(p.scale_log2e) : lse;
+      p.row_delta[at] = delta;
     }
   }
   f32x16 acc[DB], dinit;

@@ -200,6 +200,17 @@ __global__ __launch_bounds__(256) void dq3_kernel(const P p) {
       float delta_q;
       if constexpr (CROSS) {
         delta_q = RowDots<T, D>::total(reinterpret_cast<const float*>(q_area(qb)), lane);
+        if (LK <= FEW_KEYS) {
+          Frag qf[NF], gf[NF];
+#pragma unroll
+          for (int g = 0; g < NF; ++g) {
+            u32x4 qu, gu;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) qu[e] = (qb == 0 ? r_q0 : r_q1)[4 * g + e], gu[e] = (qb == 0 ? r_g0 : r_g1)[4 * g + e];
+            qf[g] = __builtin_bit_cast(Frag, qu), gf[g] = __builtin_bit_cast(Frag, gu);
+          }
+          delta_q = few_keys_delta<T>(kbase, p.k_st, vbase, p.v_st, LK, qf, gf, fabsf(p.scale_log2e), lse_q, lane);
+        }
         if (h == 0 && qrow[qb] < L) {
           const int64_t at = p.token_major ? ((int64_t)(bh - (hd - hk * p.group)) * T_ + (int64_t)qrow[qb] * p.group + (hd - hk * p.group))
                                            : (int64_t)bh * T_ + qrow[qb];

@@ -1039,6 +1039,34 @@ template <typename P> SA_DEV int other_length(const P& p, int b) {
   }
   return __builtin_amdgcn_readfirstlane(n);
 }
+// delta of this lane's row as rowsum(P * dP), for rows over up to FEW_KEYS keys, whose K and V are read from memory once more.  It is
+// rowsum(O * dO) but for the rounding of O, which reaches dS whole where few keys share it: relative errors of dQ in float16 over 8 keys
+// 3.6e-4, over 12 3.2e-4, over 34 3.06e-4, where the roundings of dS and of dQ itself are 2.9e-4 together.  One key, whose dS is 0, got
+// that rounding as its dS.  q: the row's fragments, negated for a negative scale; g: -dO.
+constexpr int FEW_KEYS = 64;
+template <typename T, int NF>
+SA_DEV float few_keys_delta(const T* k, int64_t k_st, const T* v, int64_t v_st, int L, const typename Elem<T>::Frag (&q)[NF],
+                            const typename Elem<T>::Frag (&g)[NF], float sl2e, float lse, int lane) {
+  using Frag = typename Elem<T>::Frag;
+  const int c = lane & 31, h = lane >> 5;
+  float sum = 0.0f;
+  for (int k0 = 0; k0 < L; k0 += 32) {
+    const int64_t row = k0 + c < L ? k0 + c : L - 1;
+    f32x16 s, dp;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) s[i] = dp[i] = 0.0f;
+#pragma unroll
+    for (int i = 0; i < NF; ++i) {
+      mma(s, *reinterpret_cast<const Frag*>(k + row * k_st + (i * 2 + h) * Elem<T>::VEC), q[i]);
+      mma(dp, *reinterpret_cast<const Frag*>(v + row * v_st + (i * 2 + h) * Elem<T>::VEC), g[i]);
+    }
+    const uint32_t mask = row_mask(0, L - k0, h);
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+      sum += keep_or_zero(fast_exp2(__builtin_fmaf(s[i], sl2e, -lse)) * dp[i], keep_bits(mask, i));
+  }
+  return -half_sum(sum);
+}
 
 struct DeltaParams {
   const void *o, *d_o;

@@ -120,6 +120,32 @@ def test_hand_scheduled_padding_is_never_used(junk):
     assert (dirty["lse"][4, :, :31] == -float("inf")).all() and not dirty["o"][4].any()
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("scale", [None, -0.2])
+@pytest.mark.parametrize("Hq,Hkv,Tq,Tk,D", [(12, 12, 300, 65, 32), (4, 4, 300, 65, 256), (8, 2, 90, 300, 64), (16, 16, 500, 520, 128)])
+def test_few_keys(dtype, scale, Hq, Hkv, Tq, Tk, D):
+    """Gradients of rows over few keys carry the roundings of dS and of the result only, not that of O.  A rounding is uniform over half a
+    step u to either side: relative to a value with any mantissa its root mean square is u sqrt(mean(1 / m^2) / 3) = 0.425 u, two of them
+    0.60 u.  Over one key dS is 0: P, a sum of which is 1 within 2^-19, leaves that much of dP."""
+    lens = [1, 2, 3, 5, 8, 20, 33, 64]
+    q, k, v, d_o = _inputs(8, Hq, Hkv, Tq, Tk, D, dtype)
+    got = _run(q, k, v, d_o, _lens(lens), None, scale)
+    torch.cuda.synchronize()
+    u = torch.finfo(dtype).eps / 2
+    s = abs(D ** -0.5 if scale is None else scale)
+    for b, n in enumerate(lens):
+        one = [t[b:b + 1].double() for t in (q, k[:, :, :n], v[:, :, :n], d_o)]
+        leaves = [t.requires_grad_() for t in one[:3]]
+        want = torch.autograd.grad(cross_attention_reference(*leaves, sm_scale=scale)[0], leaves, one[3])
+        if n == 1:
+            heads = [t.repeat_interleave(Hq // Hkv, dim=1) for t in one[1:3]]
+            dp = (one[3].abs() @ heads[1].abs().transpose(-1, -2)) * 2.0 ** -18
+            assert (got["dq"][b].cpu().double().abs() <= s * dp[0] * heads[0][0].abs() + 2.0 ** -24).all()
+            continue
+        for name, x, w in (("dq", got["dq"][b], want[0][0]), ("dk", got["dk"][b, :, :n], want[1][0])):
+            assert (x.cpu().double() - w).norm() <= 0.66 * u * w.norm(), (name, n)
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("scale", [-0.3, 0.0, 1.7])
 def test_scales(dtype, scale):
