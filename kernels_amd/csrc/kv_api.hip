@@ -80,7 +80,8 @@ int plan_cross(CrossPlan& c, int B, int Hq, int Hkv, int Tq, int Tk, int D, int 
   c.fwd = c.dq = c.dkdv = Shares{1, 1};
   if (Tq == 0)   // nothing but zeros for dK and dV
     return c.nbh * ceil_div(Tk, TILE_ROWS) > kMostBlocks ? KV_ERR_TOO_LARGE : KV_OK;
-  c.key_tile = c.row_tile = D * elem_size(dtype) <= 256 ? 64 : 32;
+  const int row_bytes = D * elem_size(dtype);
+  c.key_tile = c.row_tile = row_bytes <= 256 ? 64 : 32;
   c.dq_key_tile = elem_size(dtype) == 2 ? 64 : c.key_tile;
   const int64_t row_tiles = ceil_div(c.rows, TILE_ROWS), key_tiles = ceil_div(Tk, TILE_ROWS);
   c.few = few_rows(c.rows);
@@ -89,13 +90,13 @@ int plan_cross(CrossPlan& c, int B, int Hq, int Hkv, int Tq, int Tk, int D, int 
   c.long_keys = hand_scheduled && long_keys(c.nbh, c.rows, Tk);
   if (c.few) {
     const int64_t tiles = ceil_div(Tk, 32);
-    c.fwd.share = rows_share(c.nbh, (int)c.rows, tiles, D * elem_size(dtype), dtype == 0);
+    c.fwd.share = rows_share(c.nbh, (int)c.rows, tiles, row_bytes, dtype == 0);
     c.fwd.splits = (int)std::max<int64_t>(1, ceil_div(tiles, c.fwd.share));
-  } else {
-    c.fwd = tile_shares(c.nbh * row_tiles, ceil_div(Tk, c.key_tile));
+  } else if (!c.long_rows) {
+    c.fwd = tile_shares(c.nbh * row_tiles, ceil_div(Tk, c.key_tile), row_places(row_bytes), false);
   }
-  c.dq = tile_shares(c.nbh * row_tiles, ceil_div(Tk, c.dq_key_tile));
-  c.dkdv = tile_shares(c.nbh * key_tiles, ceil_div(c.rows, c.row_tile));
+  if (!c.long_rows) c.dq = tile_shares(c.nbh * row_tiles, ceil_div(Tk, c.dq_key_tile), row_places(row_bytes), false);
+  c.dkdv = tile_shares(c.nbh * key_tiles, ceil_div(c.rows, c.row_tile), key_places(row_bytes), true);
   if (c.nbh * std::max(row_tiles * std::max(c.fwd.splits, c.dq.splits), key_tiles * c.dkdv.splits) > kMostBlocks) return KV_ERR_TOO_LARGE;
   if (std::max(c.fwd.splits, c.dq.splits) > 1 && c.nbh * c.rows > kMostBlocks) return KV_ERR_TOO_LARGE;
   if (c.dkdv.splits > 1 && c.nbh * Tk > kMostBlocks) return KV_ERR_TOO_LARGE;

@@ -32,17 +32,30 @@ inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 constexpr int TILE_ROWS = 128;   // rows (or keys) of a workgroup of the tile kernels: four waves of 32
 constexpr int CUS = 256;
 
-// The tile kernels: with fewer workgroups than CUs the run of tiles that each goes through is divided, into shares of at least two
-// tiles, as long as there is a CU for each share.  Two for every CU, forward and backward in us: 4 x 8 x 500 rows over up to 2048 keys
-// at D = 256 264 -> 274 (173 -> 190 since), 2 x 16 x 300 over 4000, 4 key heads, D = 128 126 -> 134.
+// How the run of tiles that each workgroup of the tile kernels goes through is divided.
+//   Up to half as many workgroups as CUs: shares of at least two tiles, as long as there is a CU for each.
+//   Up to as many: shares of at least eight, up to 64 of them (adding up more costs what they save), as long as there is a place
+//   for each (`places` workgroups fit a CU).  Forward and backward in us,
+//   without -> with: 4 x 1 x 6105 rows over up to 14047 keys, D = 64 539 -> 388; 2 x 12 x 900 over 8000 303 -> 239; 2 x 4 x 3000 over 3000 162 -> 136;
+//   12 x 8 x 5335 over 4 171 -> 117; D = 128, 2 x 16 x 300 over 4000 167 -> 156.  With more workgroups than CUs, 8 x 12 x 448 over up to
+//   1500, D = 64 101 -> 112; at D = 256 2 x 3 x 4039 over up to 1246 184 -> 195.
+//   Forward and dQ, where the workgroups do not fill the CUs several times over: shares of at most 100 tiles.  3 x 16 x 1424 over 14631,
+//   4 key heads, D = 64 1350 -> 1244, with lengths from 64 on 1332 -> 1222; D = 256, 4 x 8 x 900 over up to 6000 714 -> 650.  Shares of 64: 4 x 12 x
+//   1574 over 5451, lengths from 64 on 319 -> 351.  dK and dV, whose parts are twice as large: 4 x 12 x 5451 over 1574 407 -> 468 with 64.
 struct Shares {
   int splits, share;
 };
-inline Shares tile_shares(int64_t workgroups, int64_t tiles) {
-  if (workgroups > CUS / 2 || workgroups == 0 || tiles < 4) return {1, 1};
-  const int share = (int)std::max<int64_t>(2, ceil_div(tiles, CUS / workgroups));
-  return {(int)ceil_div(tiles, share), share};
+inline Shares tile_shares(int64_t workgroups, int64_t tiles, int places, bool keys) {
+  if (workgroups == 0 || tiles < 4) return {1, 1};
+  int64_t share = tiles;
+  if (workgroups <= CUS / 2) share = std::max<int64_t>(2, ceil_div(tiles, CUS / workgroups));
+  if (workgroups <= CUS) share = std::min(share, std::max<int64_t>(8, ceil_div(tiles, std::min<int64_t>(64, places * CUS / workgroups))));
+  if (!keys && workgroups <= 4 * CUS) share = std::min(share, std::max<int64_t>(100, ceil_div(tiles, 8 * CUS / workgroups)));
+  return {(int)ceil_div(tiles, share), (int)share};
 }
+// Workgroups of the forward and dQ, and of dK and dV, that fit a CU (their registers; head dimension 256 gains nothing from a second one).
+inline int row_places(int row_bytes) { return row_bytes <= 128 ? 3 : row_bytes == 256 ? 2 : 1; }
+inline int key_places(int row_bytes) { return row_bytes <= 128 ? 3 : 1; }
 
 // Few tiles to a pair: tile by tile.
 inline bool tiles_first(int64_t tiles) { return tiles <= 4; }
@@ -66,15 +79,17 @@ inline bool few_rows(int64_t rows) { return rows <= 32; }
 // How its keys are divided, from the sizes of the call: at most n tiles of 32 keys for each of `units` workgroups of `rows` rows.  A share is
 // what leaves one workgroup for each CU, from four tiles on; short runs are not divided (the joining kernel takes about 4 us), and shares of
 // many workgroups stay short, so that long sequences of a batch spread over the CUs that short ones have left.  float32 is bound by its matrix
-// instructions and gains by every division (128 units of 63 tiles, D = 64: 55 us in one share, 37 in two).
+// instructions and gains by every division, down to one tile to a wave (128 units of 63 tiles, D = 64: 55 us in one share, 37 in two; 2 units of
+// 13, D = 128 38 in one, 11.7 in seven; 32 of 10, D = 64 12.1 and 8.8).
 // One token per sequence, in us for shares of 4, 8, 16, 32, 64, 128 tiles (* chosen), 16-bit elements, D = 128, four waves: 8 units of 63
 // tiles 9.5*, 9.7, 12.0, 15.9, 22.3; of 1000 60.9, 45.9, 34.9, 28.0*, 32.2, 49.7; 32 units of 63 16.2, 12.6*, 14.2, 18.1, 25.1; of 250 49.7, 36.7, 29.6,
 // 26.7*, 32.2, 50.2; 128 units of 16 16.3, 13.1, 11.0*; of 63 45.2, 35.7, 29.8, 26.9*, 28.9; two waves: 512 units of 16 33.4, 29.9, 23.8*; of
 // 63 121, 111, 105, 99.7, 94.5*; of up to 256, ragged: shares of 32 109*, 64 118.  D = 64, four waves: 8 units of 63 8.3*, 8.3, 9.9, 12.7, 16.5; 32 of 63
 // 9.9, 9.0*, 10.7, 13.6, 17.4; 512 units of 63 78.3, 63.3, 57.5, 54.4, 49.2*; eight waves: 128 units of 63 35.3, 24.4, 20.6, 16.9, 15.3* (four: 19.7).
 inline int rows_share(int64_t units, int rows, int64_t n, int row_bytes, bool f32) {
-  if (n <= (row_bytes <= 128 ? 32 : 16)) return (int)std::max<int64_t>(n, 1);
-  int64_t share = std::max<int64_t>(4, ceil_div(units * n, CUS));
+  const int64_t least = !f32 || row_bytes <= 256 ? 4 : row_bytes == 512 ? 2 : 1;
+  if (n <= (f32 ? 2 * least : row_bytes <= 128 ? 32 : 16)) return (int)std::max<int64_t>(n, 1);
+  int64_t share = std::max(least, ceil_div(units * n, CUS));
   if (2 * share >= n && n <= 64 && !f32) return (int)n;
   if (share > 32 && units * ceil_div(n, 32) >= 4 * CUS) share = 32;
   share = std::min<int64_t>(share, 128);

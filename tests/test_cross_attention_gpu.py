@@ -72,6 +72,35 @@ def test_split_work(dtype, D, Tq, Tk, lens, q_lens):
     _check(*_inputs(2, 4, 2, Tq, Tk, D, dtype), lens, q_lens)
 
 
+@pytest.mark.parametrize("dtype,B,Hq,Hkv,Tq,Tk,D,lens,q_lens", [
+    (torch.float16, 2, 8, 8, 1300, 1100, 64, [1100, 40], [1300, 3]),      # more workgroups than half of the CUs, a place for each share
+    (torch.bfloat16, 2, 8, 8, 1100, 1300, 128, [1300, 1025], None),
+    (torch.float32, 1, 8, 4, 1200, 1100, 32, None, [1111]),
+    (torch.float16, 5, 2, 1, 3000, 15, 32, [15, 1, 0, 9, 15], [3000, 1, 700, 0, 2999]),
+    (torch.bfloat16, 3, 8, 8, 1400, 6500, 64, [6500, 64, 6401], [1400, 1300, 127]),   # more than CUs, long runs
+    (torch.float16, 2, 8, 2, 512, 3300, 256, [3300, 3201], None),
+])
+def test_divided_runs(dtype, B, Hq, Hkv, Tq, Tk, D, lens, q_lens):
+    """Every rule by which runs are divided, against the oracle on one key head of each batch entry."""
+    from kv_attention import _lib
+
+    q, k, v, d_o = _inputs(B, Hq, Hkv, Tq, Tk, D, dtype)
+    lens, q_lens = _lens(lens), _lens(q_lens)
+    plain = 2 * ((B * Hq * Tq * 4 + 255) // 256 * 256)
+    assert _lib.load().kv_cross_backward_workspace(B, Hq, Hkv, Tq, Tk, D, DTYPES.index(dtype)) > plain
+    got = _run(q, k, v, d_o, lens, q_lens)
+    torch.cuda.synchronize()
+    G = Hq // Hkv
+    for b in range(B):
+        h = b % Hkv
+        heads = slice(h * G, (h + 1) * G)
+        one = [t[b:b + 1] for t in (q[:, heads], k[:, h:h + 1], v[:, h:h + 1], d_o[:, heads])]
+        want = kv_oracle.cross(*one[:3], None if lens is None else lens[b:b + 1], None if q_lens is None else q_lens[b:b + 1], None, one[3])
+        for name in want:
+            of = slice(h, h + 1) if name in ("dk", "dv") else heads
+            kv_oracle.assert_within(f"{name} of {b}", got[name][b:b + 1, of], want[name])
+
+
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
 @pytest.mark.parametrize("B,Hq,Hkv,Tq,Tk,lens,q_lens,layout", [
     (8, 16, 16, 500, 520, [520, 64, 0, 1, 519, 300, 128, 65], [500, 1, 500, 0, 257, 256, 64, 333], "plain"),

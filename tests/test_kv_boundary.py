@@ -145,6 +145,18 @@ def test_parts_stay_small(lib):
     assert lib.kv_paged_forward_workspace(64, 64, 8, 1, 128, 16, 4096, 1, 2 ** 31 - 1, 2) > 0   # and few rows are still divided
 
 
+@pytest.mark.parametrize("dtype,es", [(0, 4), (1, 2)])
+def test_cross_parts_stay_small(lib, dtype, es):
+    """Parts of divided runs: a few times the rows of a GPU full of workgroups, however long the other side is."""
+    for D in (16, 64, 128, 256):
+        for B, Hq, Hkv, Tq, Tk in ((1, 1, 1, 100, 1 << 20), (3, 16, 4, 1424, 14631), (1, 8, 8, 4096, 1 << 20), (1, 1, 1, 1 << 20, 100),
+                                   (64, 16, 16, 40, 9000), (13, 16, 1, 3974, 15)):
+            most = 9 * 256 * 128 * (D + 2) * 4
+            assert 0 <= lib.kv_cross_forward_workspace(B, Hq, Hkv, Tq, Tk, D, dtype) <= most
+            stats = 2 * (B * Hq * Tq * 4 + 256)
+            assert 0 < lib.kv_cross_backward_workspace(B, Hq, Hkv, Tq, Tk, D, dtype) <= stats + most
+
+
 def _cross(dtype=torch.float32, **kw):
     a = dict(q=torch.zeros(2, 4, 5, 64, dtype=dtype), k=torch.zeros(2, 2, 7, 64, dtype=dtype), v=torch.zeros(2, 2, 7, 64, dtype=dtype),
              lens=None, q_lens=None, sm_scale=0.1)
