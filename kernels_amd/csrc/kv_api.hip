@@ -44,6 +44,12 @@ template <typename F> int by_dtype(int dtype, F&& f) {
     return D == 256 ? fn<E, 1>(p, D, (hipStream_t)stream) : fn<E, 0>(p, D, (hipStream_t)stream); \
   })
 
+#ifdef SA_NO_ASM_KERNELS
+#define KV_LAUNCH_LONG(fn, p) KV_ERR_ARG   // (no call comes here)
+#else
+#define KV_LAUNCH_LONG(fn, p) (dtype == 1 ? fn<_Float16>(p, (hipStream_t)stream) : fn<__bf16>(p, (hipStream_t)stream))
+#endif
+
 RowMap row_map(int Hkv, int G, int T) { return RowMap{Hkv, G, T, chunk_div(G)}; }
 Work work_map(int64_t nbh, int64_t n_tiles, const Shares& sh, int heads, bool tiles_first) {
   Work w{};
@@ -85,7 +91,7 @@ int plan_cross(CrossPlan& c, int B, int Hq, int Hkv, int Tq, int Tk, int D, int 
   c.dq_key_tile = elem_size(dtype) == 2 ? 64 : c.key_tile;
   const int64_t row_tiles = ceil_div(c.rows, TILE_ROWS), key_tiles = ceil_div(Tk, TILE_ROWS);
   c.few = few_rows(c.rows);
-  const bool hand_scheduled = D == 128 && dtype != 0;
+  const bool hand_scheduled = HAVE_ASM_KERNELS && D == 128 && dtype != 0;
   c.long_rows = hand_scheduled && long_rows((int64_t)B * Hq, Tq, Tk);
   c.long_keys = hand_scheduled && long_keys(c.nbh, c.rows, Tk);
   if (c.few) {
@@ -214,7 +220,7 @@ int kv_cross_forward(const void* q, const void* k, const void* v, const int32_t*
     p.v_sb = vs[0]; p.v_sh = vs[1]; p.v_st = vs[2];
     p.scale_log2e = sm_scale * kLog2e;
     long_sides(p, B, Hq, Hkv, Tq, Tk);
-    return dtype == 1 ? launch_long_fwd<_Float16>(p, (hipStream_t)stream) : launch_long_fwd<__bf16>(p, (hipStream_t)stream);
+    return KV_LAUNCH_LONG(launch_long_fwd, p);
   } else {
     FwdParams p{};
     p.q = q; p.k = k; p.v = v; p.o = o; p.lse = lse;
@@ -305,7 +311,7 @@ int kv_cross_backward(const void* q, const void* k, const void* v, const int32_t
     d.delta_out = p.row_delta; d.lse_out = p.row_lse;
     d.token_major = !keys_by_hand;
     long_sides(d, B, Hq, Hkv, Tq, Tk);
-    if (int rc = dtype == 1 ? launch_long_dq<_Float16>(d, (hipStream_t)stream) : launch_long_dq<__bf16>(d, (hipStream_t)stream)) return rc;
+    if (int rc = KV_LAUNCH_LONG(launch_long_dq, d)) return rc;
     c.dq.splits = 1;
   } else if (Tq > 0) {
     const int64_t tiles = ceil_div(c.rows, TILE_ROWS);
@@ -330,7 +336,7 @@ int kv_cross_backward(const void* q, const void* k, const void* v, const int32_t
     r.other_T = (int)c.rows;
     r.group = G;
     r.tiles = work_map(c.nbh, ceil_div(Tk, TILE_ROWS), Shares{1, 1}, Hkv, false).map;
-    return dtype == 1 ? launch_long_dkdv<_Float16>(r, (hipStream_t)stream) : launch_long_dkdv<__bf16>(r, (hipStream_t)stream);
+    return KV_LAUNCH_LONG(launch_long_dkdv, r);
   }
   p.work = work_map(c.nbh, ceil_div(Tk, TILE_ROWS), c.dkdv, Hkv, false);
   if (int rc = KV_LAUNCH(launch_cross_dkdv, p)) return rc;

@@ -135,7 +135,7 @@ template <> int launch_sum<ElemT, KV_DGROUP>(const SumParams& p, int D, hipStrea
                   p.keys ? 2 : 1);
   });
 }
-#elif KV_KIND == 4
+#elif KV_KIND == 4 && !defined(SA_NO_ASM_KERNELS)
 constexpr size_t long_stages(int n, size_t tile_rows) { return n * 2 * tile_rows * 128 * sizeof(ElemT); }
 static int64_t long_blocks(const sa::TileMap& m) { return (int64_t)m.nbh * m.n_tiles; }
 template <> int launch_long_fwd<ElemT>(const LongFwd& p, hipStream_t st) {

@@ -5,9 +5,11 @@
 #include "../../include/kv_attention.h"
 #include "kv_bwd.h"
 #include "kv_rows.h"
+#ifndef SA_NO_ASM_KERNELS
 #include "sa_bwd3.h"
 #include "sa_bwd4.h"
 #include "sa_fwd3.h"
+#endif
 
 namespace kv {
 
@@ -19,7 +21,13 @@ template <typename T, int DGROUP> int launch_rows_paged(const RowsParams& p, int
 template <typename T, int DGROUP> int launch_join(const JoinParams& p, int D, hipStream_t st);
 template <typename T, int DGROUP> int launch_sum(const SumParams& p, int D, hipStream_t st);
 
-// The hand-scheduled kernels of streaming attention on another sequence's keys: 16-bit elements, head dimension 128.
+// The hand-scheduled kernels of streaming attention on another sequence's keys: 16-bit elements, head dimension 128.  -DSA_NO_ASM_KERNELS
+// leaves them out, as in sa_launch.h.
+#ifdef SA_NO_ASM_KERNELS
+constexpr bool HAVE_ASM_KERNELS = false;
+#else
+constexpr bool HAVE_ASM_KERNELS = true;
+#endif
 using LongFwd = sa::CrossOf<sa::FwdParams>;
 using LongBwd = sa::CrossOf<sa::BwdParams>;
 template <typename T> int launch_long_fwd(const LongFwd& p, hipStream_t st);
