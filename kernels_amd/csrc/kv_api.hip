@@ -99,10 +99,10 @@ int plan_cross(CrossPlan& c, int B, int Hq, int Hkv, int Tq, int Tk, int D, int 
     c.fwd.share = rows_share(c.nbh, (int)c.rows, tiles, row_bytes, dtype == 0);
     c.fwd.splits = (int)std::max<int64_t>(1, ceil_div(tiles, c.fwd.share));
   } else if (!c.long_rows) {
-    c.fwd = tile_shares(c.nbh * row_tiles, ceil_div(Tk, c.key_tile), row_places(row_bytes), false);
+    c.fwd = tile_shares(c.nbh * row_tiles, ceil_div(Tk, c.key_tile), row_places(row_bytes), false, dtype == 0);
   }
-  if (!c.long_rows) c.dq = tile_shares(c.nbh * row_tiles, ceil_div(Tk, c.dq_key_tile), row_places(row_bytes), false);
-  c.dkdv = tile_shares(c.nbh * key_tiles, ceil_div(c.rows, c.row_tile), key_places(row_bytes), true);
+  if (!c.long_rows) c.dq = tile_shares(c.nbh * row_tiles, ceil_div(Tk, c.dq_key_tile), row_places(row_bytes), false, dtype == 0);
+  c.dkdv = tile_shares(c.nbh * key_tiles, ceil_div(c.rows, c.row_tile), key_places(row_bytes), true, dtype == 0);
   if (c.nbh * std::max(row_tiles * std::max(c.fwd.splits, c.dq.splits), key_tiles * c.dkdv.splits) > kMostBlocks) return KV_ERR_TOO_LARGE;
   if (std::max(c.fwd.splits, c.dq.splits) > 1 && c.nbh * c.rows > kMostBlocks) return KV_ERR_TOO_LARGE;
   if (c.dkdv.splits > 1 && c.nbh * Tk > kMostBlocks) return KV_ERR_TOO_LARGE;

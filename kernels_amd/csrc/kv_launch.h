@@ -41,7 +41,9 @@ constexpr int TILE_ROWS = 128;   // rows (or keys) of a workgroup of the tile ke
 constexpr int CUS = 256;
 
 // How the run of tiles that each workgroup of the tile kernels goes through is divided.
-//   Up to half as many workgroups as CUs: shares of at least two tiles, as long as there is a CU for each.
+//   Up to half as many workgroups as CUs: shares of at least two tiles, as long as there is a CU for each; of one in float32, whose tile takes
+//   3-10 us (kernels of a pass in us, two -> one: 2 x 4 x 50 rows over up to 512, D = 64 55 -> 44; 4 x 8 x 100 over 130 63 -> 52; 4 x 300 over
+//   150, D = 256 214 -> 168; bfloat16, 4 x 8 x 100 over 130, D = 64 23 -> 33).
 //   Up to as many: shares of at least eight, up to 64 of them (adding up more costs what they save), as long as there is a place
 //   for each (`places` workgroups fit a CU).  Forward and backward in us,
 //   without -> with: 4 x 1 x 6105 rows over up to 14047 keys, D = 64 539 -> 388; 2 x 12 x 900 over 8000 303 -> 239; 2 x 4 x 3000 over 3000 162 -> 136;
@@ -53,10 +55,11 @@ constexpr int CUS = 256;
 struct Shares {
   int splits, share;
 };
-inline Shares tile_shares(int64_t workgroups, int64_t tiles, int places, bool keys) {
-  if (workgroups == 0 || tiles < 4) return {1, 1};
+inline Shares tile_shares(int64_t workgroups, int64_t tiles, int places, bool keys, bool f32) {
+  const int least = f32 ? 1 : 2;
+  if (workgroups == 0 || tiles < 2 * least) return {1, 1};
   int64_t share = tiles;
-  if (workgroups <= CUS / 2) share = std::max<int64_t>(2, ceil_div(tiles, CUS / workgroups));
+  if (workgroups <= CUS / 2) share = std::max<int64_t>(least, ceil_div(tiles, CUS / workgroups));
   if (workgroups <= CUS) share = std::min(share, std::max<int64_t>(8, ceil_div(tiles, std::min<int64_t>(64, places * CUS / workgroups))));
   if (!keys && workgroups <= 4 * CUS) share = std::min(share, std::max<int64_t>(100, ceil_div(tiles, 8 * CUS / workgroups)));
   return {(int)ceil_div(tiles, share), (int)share};
