@@ -72,7 +72,7 @@ struct CrossPlan {
   Shares fwd, dq, dkdv;
   int key_tile, dq_key_tile, row_tile;   // of the forward, dQ, dK and dV
   bool few, long_rows, long_keys;        // the rows kernel; the hand-scheduled forward and dQ; dK and dV
-  int64_t fwd_bytes, stats_bytes, bwd_bytes;
+  int64_t fwd_bytes, stats_bytes, dq_bytes, bwd_bytes;
 };
 // KV_ERR_TOO_LARGE where a count of the kernels would pass 31 bits
 int plan_cross(CrossPlan& c, int B, int Hq, int Hkv, int Tq, int Tk, int D, int dtype) {
@@ -110,7 +110,8 @@ int plan_cross(CrossPlan& c, int B, int Hq, int Hkv, int Tq, int Tk, int D, int 
   c.stats_bytes = ceil_div(c.nbh * c.rows * 4, 256) * 256;
   const int64_t dq = c.dq.splits > 1 ? c.dq.splits * c.nbh * c.rows * D * 4 : 0;
   const int64_t dkdv = c.dkdv.splits > 1 ? (int64_t)c.dkdv.splits * 2 * c.nbh * Tk * D * 4 : 0;
-  c.bwd_bytes = 2 * c.stats_bytes + std::max(dq, dkdv);
+  c.dq_bytes = dq;
+  c.bwd_bytes = 2 * c.stats_bytes + dq + dkdv;
   return KV_OK;
 }
 // The rows of one head within 32-bit byte offsets: what the hand-scheduled kernels need of q and d_o.
@@ -320,15 +321,15 @@ int kv_cross_backward(const void* q, const void* k, const void* v, const int32_t
     if (int rc = KV_LAUNCH(launch_cross_dq, p)) return rc;
   }
   SumParams s{};
-  s.part = p.part; s.lens = lens; s.q_lens = q_lens; s.lens_stride = lens_stride; s.q_lens_stride = q_lens_stride;
-  s.B = B; s.Tk = Tk; s.Tq = Tq; s.group = Hq / Hkv; s.by_heads = chunk_div(Hkv);
+  s.lens = lens; s.q_lens = q_lens; s.lens_stride = lens_stride; s.q_lens_stride = q_lens_stride;
+  s.B = B; s.Hkv = Hkv; s.Tk = Tk; s.Tq = Tq; s.group = G; s.by_heads = chunk_div(Hkv);
   if (c.dq.splits > 1) {
-    s.map = p.map; s.out[0] = dq; s.step = c.nbh * c.rows * D; s.keys = false;
-    s.share = c.dq.share; s.tile = c.dq_key_tile; s.by_rows = chunk_div((int)c.rows);
-    if (int rc = KV_LAUNCH(launch_sum, s)) return rc;
+    SumSide& x = s.queries;
+    x.part = p.part; x.map = p.map; x.out[0] = dq; x.step = c.nbh * c.rows * D;
+    x.share = c.dq.share; x.tile = c.dq_key_tile; x.by_rows = chunk_div((int)c.rows);
+    s.first_keys = 1;
   }
-  if (Tk == 0) return KV_OK;
-  if (keys_by_hand) {
+  if (Tk > 0 && keys_by_hand) {
     r.lse = p.row_lse; r.delta = p.row_delta; r.dk = dk; r.dv = dv;
     r.lens = lens; r.lens_stride = lens_stride; r.other_lens = q_lens; r.other_lens_stride = q_lens_stride;
     r.B = B; r.H = Hkv; r.T = Tk; r.C = 1; r.R = 0;
@@ -336,14 +337,19 @@ int kv_cross_backward(const void* q, const void* k, const void* v, const int32_t
     r.other_T = (int)c.rows;
     r.group = G;
     r.tiles = work_map(c.nbh, ceil_div(Tk, TILE_ROWS), Shares{1, 1}, Hkv, false).map;
-    return KV_LAUNCH_LONG(launch_long_dkdv, r);
+    if (int rc = KV_LAUNCH_LONG(launch_long_dkdv, r)) return rc;
+  } else if (Tk > 0) {
+    p.part = (float*)((char*)p.part + c.dq_bytes);
+    p.work = work_map(c.nbh, ceil_div(Tk, TILE_ROWS), c.dkdv, Hkv, false);
+    if (int rc = KV_LAUNCH(launch_cross_dkdv, p)) return rc;
+    if (c.dkdv.splits > 1) {
+      SumSide& x = s.keys;
+      x.part = p.part; x.map = row_map(Hkv, 1, Tk); x.out[0] = dk; x.out[1] = dv;
+      x.second = c.nbh * Tk * D; x.step = 2 * x.second;
+      x.share = c.dkdv.share; x.tile = c.row_tile; x.by_rows = chunk_div(Tk);
+    }
   }
-  p.work = work_map(c.nbh, ceil_div(Tk, TILE_ROWS), c.dkdv, Hkv, false);
-  if (int rc = KV_LAUNCH(launch_cross_dkdv, p)) return rc;
-  if (c.dkdv.splits == 1) return KV_OK;
-  s.map = row_map(Hkv, 1, Tk); s.out[0] = dk; s.out[1] = dv; s.second = c.nbh * Tk * D; s.step = 2 * s.second; s.keys = true;
-  s.share = c.dkdv.share; s.tile = c.row_tile; s.by_rows = chunk_div(Tk);
-  return KV_LAUNCH(launch_sum, s);
+  return s.first_keys > 0 || s.keys.part ? KV_LAUNCH(launch_sum, s) : KV_OK;
 }
 
 int64_t kv_paged_forward_workspace(int B, int Hq, int Hkv, int T, int D, int page_size, int width, int context_size, int back_contexts,

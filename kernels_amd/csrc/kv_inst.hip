@@ -131,8 +131,9 @@ template <> int launch_sum<ElemT, KV_DGROUP>(const SumParams& p, int D, hipStrea
   return by_head_dim(D, [&](auto d) {
     constexpr int DD = decltype(d)::value;
     static LdsLimit none;
-    return launch(sum_kernel<ElemT, DD>, ceil_div((int64_t)p.B * p.map.Hkv * p.map.rows(), 256 / (DD / 4)), 256, 0, none, p, st,
-                  p.keys ? 2 : 1);
+    const bool queries = p.first_keys > 0, keys = p.keys.part != nullptr;
+    const int64_t rows = std::max<int64_t>(queries ? p.queries.map.rows() : 0, keys ? p.keys.map.rows() : 0);
+    return launch(sum_kernel<ElemT, DD>, ceil_div((int64_t)p.B * p.Hkv * rows, 256 / (DD / 4)), 256, 0, none, p, st, queries + 2 * keys);
   });
 }
 #elif KV_KIND == 4 && !defined(SA_NO_ASM_KERNELS)

@@ -318,39 +318,45 @@ __global__ __launch_bounds__((SLOTS * D / 4 > 256 ? SLOTS * D / 4 : 256)) void j
   if (p.lse && d == 0) p.lse[to] = row >= live ? 0.0f : some ? m + __builtin_amdgcn_logf(l) : -INFINITY;
 }
 
-// Gradients whose sums were split: parts [splits, B * Hkv, n, D] added up in order, rows from `limit` on zero.
-struct SumParams {
+// Gradients whose sums were split: parts [splits, B * Hkv, n, D] added up in order, rows from their limit on zero.
+struct SumSide {
   const float* part;
   int64_t step, second;   // floats between the parts of consecutive splits, and from dK's to dV's
-  void* out[2];           // dQ; or dK and dV, one for each y of the grid
+  void* out[2];           // dQ; or dK and dV
+  RowMap map;             // of the rows of `out`
+  int share, tile;        // as the parts were made (Work): runs of tiles of `tile` keys (dQ) or rows (dK, dV)
+  ChunkDiv by_rows;
+};
+struct SumParams {
+  SumSide queries, keys;
+  int first_keys;         // layers of the grid: dQ below this one, dK and dV from it on
   const int32_t *lens, *q_lens;
   int64_t lens_stride, q_lens_stride;
-  RowMap map;             // of the rows of `out`
-  int B, Tk, Tq;
-  int share, tile;        // as the parts were made (Work): runs of tiles of `tile` keys (dQ) or rows (dK, dV)
+  int B, Hkv, Tk, Tq;
   int group;              // query heads of a key head
-  bool keys;              // rows are keys (dK, dV) instead of queries (dQ)
-  ChunkDiv by_rows, by_heads;
+  ChunkDiv by_heads;
 };
 template <typename T, int D> __global__ __launch_bounds__(256) void sum_kernel(const SumParams p) {
   constexpr int Q4 = D / 4, RPB = 256 / Q4;
-  const int d = threadIdx.x % Q4 * 4, rows = p.map.rows();
+  const bool keys = (int)blockIdx.y >= p.first_keys, second = (int)blockIdx.y > p.first_keys;
+  const SumSide side = keys ? p.keys : p.queries;
+  const int d = threadIdx.x % Q4 * 4, rows = side.map.rows();
   const int64_t id = (int64_t)blockIdx.x * RPB + threadIdx.x / Q4;
-  if (id >= (int64_t)p.B * p.map.Hkv * rows) return;
-  const int bh = div_by((int)id, p.by_rows), row = (int)id - bh * rows, b = div_by(bh, p.by_heads);
+  if (id >= (int64_t)p.B * p.Hkv * rows) return;
+  const int bh = div_by((int)id, side.by_rows), row = (int)id - bh * rows, b = div_by(bh, p.by_heads);
   const int rows_live = clamped_length(p.q_lens, p.q_lens_stride, b, p.Tq) * p.group, L = clamped_length(p.lens, p.lens_stride, b, p.Tk);
-  const int limit = p.keys ? L : rows_live, run = p.keys ? rows_live : L;
-  const int parts = parts_of((run + p.tile - 1) / p.tile, p.share);
-  const float* const part = p.part + (blockIdx.y ? p.second : 0);
+  const int limit = keys ? L : rows_live, run = keys ? rows_live : L;
+  const int parts = parts_of((run + side.tile - 1) / side.tile, side.share);
+  const float* const part = side.part + (second ? side.second : 0);
   f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
   if (row < limit)
 #pragma unroll 4
     for (int s = 0; s < parts; ++s) {
-      const f32x4 x = *reinterpret_cast<const f32x4*>(part + s * p.step + id * D + d);
+      const f32x4 x = *reinterpret_cast<const f32x4*>(part + s * side.step + id * D + d);
 #pragma unroll
       for (int e = 0; e < 4; ++e) sum[e] += x[e];
     }
-  sa::store4<T>(reinterpret_cast<T*>(blockIdx.y ? p.out[1] : p.out[0]) + p.map.flat(bh, row) * D + d, sum[0], sum[1], sum[2], sum[3]);
+  sa::store4<T>(reinterpret_cast<T*>(second ? side.out[1] : side.out[0]) + side.map.flat(bh, row) * D + d, sum[0], sum[1], sum[2], sum[3]);
 }
 
 }  // namespace kv
