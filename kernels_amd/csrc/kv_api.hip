@@ -96,7 +96,7 @@ int plan_cross(CrossPlan& c, int B, int Hq, int Hkv, int Tq, int Tk, int D, int 
   c.long_keys = hand_scheduled && long_keys(c.nbh, c.rows, Tk);
   if (c.few) {
     const int64_t tiles = ceil_div(Tk, 32);
-    c.fwd.share = rows_share(c.nbh, (int)c.rows, tiles, row_bytes, dtype == 0);
+    c.fwd.share = rows_share(c.nbh, (int)c.rows, tiles, row_bytes, dtype == 0, by_length(B, 1, row_bytes));
     c.fwd.splits = (int)std::max<int64_t>(1, ceil_div(tiles, c.fwd.share));
   } else if (!c.long_rows) {
     c.fwd = tile_shares(c.nbh * row_tiles, ceil_div(Tk, c.key_tile), row_places(row_bytes), false, dtype == 0);
@@ -154,18 +154,21 @@ int plan_paged(PagedPlan& c, int B, int Hq, int Hkv, int T, int D, int page, int
   const int64_t tokens = std::min<int64_t>(T, 31 / G + 2), chunks = ceil_div(tokens - 1, C) + 1;
   const int64_t span = R > most || C > most ? most : std::min<int64_t>(most, (R + chunks) * C);
   const int64_t tiles = std::min(ceil_div(most, 32), ceil_div(span, 32) + 1);
-  c.share = rows_share(c.nbh * c.row_tiles, (int)std::min<int64_t>(c.rows, 32), tiles, D * elem_size(dtype), dtype == 0);
+  const int row_bytes = D * elem_size(dtype);
+  c.share = rows_share(c.nbh * c.row_tiles, (int)std::min<int64_t>(c.rows, 32), tiles, row_bytes, dtype == 0, by_length(B, c.row_tiles, row_bytes));
   c.splits = (int)std::max<int64_t>(1, ceil_div(tiles, c.share));
   if (c.nbh * c.row_tiles * c.splits > kMostBlocks || (c.splits > 1 && c.nbh * c.rows > kMostBlocks)) return KV_ERR_TOO_LARGE;
   if (c.splits > 1) c.bytes = c.splits * c.nbh * c.rows * (D + 2) * 4;
   return KV_OK;
 }
 
-JoinParams join_params(const float* part_o, const float* part_ml, void* o, float* lse, const int32_t* q_lens, int64_t q_lens_stride,
-                       const RowMap& map, int B, int splits) {
+// P: the parameters of the kernel that leaves the parts, runs of up to `share` tiles of `tile` keys
+template <typename P> JoinParams join_params(const P& p, int max_len, int splits, int share, int tile) {
   JoinParams j{};
-  j.part_o = part_o, j.part_ml = part_ml, j.o = o, j.lse = lse, j.q_lens = q_lens, j.q_lens_stride = q_lens_stride;
-  j.map = map, j.B = B, j.splits = splits;
+  j.part_o = p.part_o, j.part_ml = p.part_ml, j.o = p.o, j.lse = p.lse;
+  j.lens = p.lens, j.q_lens = p.q_lens, j.lens_stride = p.lens_stride, j.q_lens_stride = p.q_lens_stride;
+  j.map = p.map, j.B = p.B, j.max_len = max_len, j.splits = splits, j.share = share, j.tile = tile;
+  const RowMap& map = p.map;
   j.by_rows = chunk_div(map.rows());
   j.by_heads = chunk_div(map.Hkv);
   return j;
@@ -212,6 +215,9 @@ int kv_cross_forward(const void* q, const void* k, const void* v, const int32_t*
     p.by_pairs = chunk_div((int)c.nbh); p.by_row_tiles = chunk_div(1); p.by_heads = chunk_div(Hkv);
     p.part_o = part_o; p.part_ml = part_ml;
     if (int rc = KV_LAUNCH(launch_rows, p)) return rc;
+    if (c.fwd.splits == 1) return KV_OK;
+    const JoinParams j = join_params(p, Tk, c.fwd.splits, c.fwd.share, 32);
+    return KV_LAUNCH(launch_join, j);
   } else if (c.long_rows && Tk > 0 && rows_fit(qs, Tq, dtype)) {
     LongFwd p{};
     p.q = q; p.k = k; p.v = v; p.o = o; p.lse = lse;
@@ -236,10 +242,10 @@ int kv_cross_forward(const void* q, const void* k, const void* v, const int32_t*
     p.work = work_map(c.nbh, tiles, c.fwd, Hkv, tiles_first(tiles));
     p.part_o = part_o; p.part_ml = part_ml;
     if (int rc = KV_LAUNCH(launch_cross_fwd, p)) return rc;
+    if (c.fwd.splits == 1) return KV_OK;
+    const JoinParams j = join_params(p, Tk, c.fwd.splits, c.fwd.share, c.key_tile);
+    return KV_LAUNCH(launch_join, j);
   }
-  if (c.fwd.splits == 1) return KV_OK;
-  const JoinParams j = join_params(part_o, part_ml, o, lse, q_lens, q_lens_stride, map, B, c.fwd.splits);
-  return KV_LAUNCH(launch_join, j);
 }
 
 int64_t kv_cross_backward_workspace(int B, int Hq, int Hkv, int Tq, int Tk, int D, int dtype) {
@@ -392,16 +398,17 @@ int kv_paged_forward(const void* q, const void* k_pages, const void* v_pages, co
   }
   // chunks matter below the longest length only
   const int most = width * page_size;
-  p.C = std::max(1, std::min(context_size, most));
-  p.R = std::min(back_contexts, most);
-  p.cdiv = chunk_div(p.C);
+  p.win.C = std::max(1, std::min(context_size, most));
+  p.win.R = std::min(back_contexts, most);
+  p.win.cdiv = chunk_div(p.win.C);
   p.splits = c.splits; p.share = c.share; p.row_tiles = (int)c.row_tiles;
   p.by_pairs = chunk_div((int)c.nbh); p.by_row_tiles = chunk_div(p.row_tiles); p.by_heads = chunk_div(Hkv);
   p.part_o = (float*)workspace;
   p.part_ml = p.part_o + c.splits * c.nbh * c.rows * D;
   if (int rc = KV_LAUNCH(launch_rows_paged, p)) return rc;
   if (c.splits == 1) return KV_OK;
-  const JoinParams j = join_params(p.part_o, p.part_ml, o, lse, new_lens, new_lens_stride, p.map, B, c.splits);
+  JoinParams j = join_params(p, p.max_len, c.splits, c.share, 32);
+  j.win = p.win;
   return KV_LAUNCH(launch_join, j);
 }
 

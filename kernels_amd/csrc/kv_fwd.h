@@ -126,10 +126,7 @@ __global__ __launch_bounds__(NW * 64, (D * sizeof(T) == 512 ? (sizeof(T) == 2 ? 
 
   int t0, t1;
   part_of(p.work, (L + TK - 1) / TK, split, t0, t1);
-  if (p.work.splits > 1 && t0 >= t1) {
-    if (row < live && h == 0) p.part_ml[part_row * 2] = -INFINITY, p.part_ml[part_row * 2 + 1] = 0.0f;
-    return;
-  }
+  if (p.work.splits > 1 && t0 >= t1) return;   // (the joining kernel knows how many parts there are)
   // never exactly 0, so that a masked score of -inf stays -inf after scaling
   const float sl2e = fmaxf(fabsf(p.scale_log2e), 1e-30f);
   Frag qf[NF];

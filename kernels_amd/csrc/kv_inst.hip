@@ -100,8 +100,14 @@ template <> int launch_cross_dkdv<ElemT, KV_DGROUP>(const BwdParams& p, int D, h
 }
 #elif KV_KIND == 3
 template <int D, int NW, bool PAGED> static int launch_rows_shape(const RowsParams& p, int64_t blocks, hipStream_t st) {
+  constexpr int row_bytes = D * (int)sizeof(ElemT), lds = RowsShape<ElemT, D, NW>::bytes(PAGED), places = CUS * (163840 / lds);
+  if constexpr (row_bytes >= 128) {
+    static LdsLimit state;
+    if (p.splits > 1 && by_length(p.B, p.row_tiles, row_bytes) && blocks >= 2 * places)
+      return launch(rows_by_length_kernel<ElemT, D, NW, PAGED>, places, NW * 64, lds, state, p, st);
+  }
   static LdsLimit state;
-  return launch(rows_kernel<ElemT, D, NW, PAGED>, blocks, NW * 64, RowsShape<ElemT, D, NW>::bytes(PAGED), state, p, st);
+  return launch(rows_kernel<ElemT, D, NW, PAGED>, blocks, NW * 64, lds, state, p, st);
 }
 template <bool PAGED> static int launch_rows_any(const RowsParams& p, int D, hipStream_t st) {
   return by_head_dim(D, [&](auto d) {

@@ -89,20 +89,26 @@ inline bool long_keys(int64_t key_heads, int64_t rows, int64_t Tk) { return rows
 inline bool few_rows(int64_t rows) { return rows <= 32; }
 // How its keys are divided, from the sizes of the call: at most n tiles of 32 keys for each of `units` workgroups of `rows` rows.  A share is
 // what leaves one workgroup for each CU, from four tiles on; short runs are not divided (the joining kernel takes about 4 us), and shares of
-// many workgroups stay short, so that long sequences of a batch spread over the CUs that short ones have left.  float32 is bound by its matrix
+// many workgroups stay short, so that long sequences of a batch spread over the CUs that short ones have left: 16 tiles where workgroups go
+// through the parts that there are (by_length), else 32, as parts that the lengths leave empty have workgroups then.  float32 is bound by its matrix
 // instructions and gains by every division, down to one tile to a wave (128 units of 63 tiles, D = 64: 55 us in one share, 37 in two; 2 units of
 // 13, D = 128 38 in one, 11.7 in seven; 32 of 10, D = 64 12.1 and 8.8).
 // One token per sequence, in us for shares of 4, 8, 16, 32, 64, 128 tiles (* chosen), 16-bit elements, D = 128, four waves: 8 units of 63
 // tiles 9.5*, 9.7, 12.0, 15.9, 22.3; of 1000 60.9, 45.9, 34.9, 28.0*, 32.2, 49.7; 32 units of 63 16.2, 12.6*, 14.2, 18.1, 25.1; of 250 49.7, 36.7, 29.6,
 // 26.7*, 32.2, 50.2; 128 units of 16 16.3, 13.1, 11.0*; of 63 45.2, 35.7, 29.8, 26.9*, 28.9; two waves: 512 units of 16 33.4, 29.9, 23.8*; of
-// 63 121, 111, 105, 99.7, 94.5*; of up to 256, ragged: shares of 32 109*, 64 118.  D = 64, four waves: 8 units of 63 8.3*, 8.3, 9.9, 12.7, 16.5; 32 of 63
+// 63 121, 111, 105, 99.7, 94.5*.  By length, shares of 12, 16*, 24, 32, 64: 64 sequences x 8 key heads of lengths log-uniform from 64 to 8192 98.7, 95.2, 95.6, 99.6,
+// 117 (a workgroup for each part: 117, 112, 107, 107, 115); 16 x 8 31.5, 31.0, 31.1, 35.8, 60.4; 8 x 8 23.2, 21.6, 24.8, 30.7, 28.8; all of 8192 62.5, 58.3, 62.7, 54.8, 55.0; 2 x 8
+// of 131072 208, 208, 206, 196, 192 and 187 with 128* (D = 32, 28 x 12 of up to 15484 80, 80, 76, 75, 71, a workgroup
+// for each part of 32 69*).  D = 64, four waves: 8 units of 63 8.3*, 8.3, 9.9, 12.7, 16.5; 32 of 63
 // 9.9, 9.0*, 10.7, 13.6, 17.4; 512 units of 63 78.3, 63.3, 57.5, 54.4, 49.2*; eight waves: 128 units of 63 35.3, 24.4, 20.6, 16.9, 15.3* (four: 19.7).
-inline int rows_share(int64_t units, int rows, int64_t n, int row_bytes, bool f32) {
+inline bool by_length(int64_t B, int64_t row_tiles, int row_bytes) { return B <= MAX_BY_LENGTH && row_tiles == 1 && row_bytes >= 128; }
+inline int rows_share(int64_t units, int rows, int64_t n, int row_bytes, bool f32, bool by_length) {
   const int64_t least = !f32 || row_bytes <= 256 ? 4 : row_bytes == 512 ? 2 : 1;
   if (n <= (f32 ? 2 * least : row_bytes <= 128 ? 32 : 16)) return (int)std::max<int64_t>(n, 1);
   int64_t share = std::max(least, ceil_div(units * n, CUS));
   if (2 * share >= n && n <= 64 && !f32) return (int)n;
-  if (share > 32 && units * ceil_div(n, 32) >= 4 * CUS) share = 32;
+  const int64_t most_of_many = by_length ? 16 : 32;
+  if ((units >= 48 || !by_length) && share > most_of_many && units * ceil_div(n, most_of_many) >= 4 * CUS) share = most_of_many;
   share = std::min<int64_t>(share, 128);
   // at most 256 parts to add up, and 256 MiB of them (the chunks of many long sequences)
   const int64_t part = units * rows * (row_bytes / (f32 ? 4 : 2) + 2) * 4;

@@ -5,11 +5,39 @@
 // tokens) and a run of keys.  Its waves go through tiles of 32 keys by themselves, every NW-th each, without a barrier: a wave keeps ST
 // tiles of K and V on their way into LDS of its own, at addresses that each lane forms for its row, and joins the other waves at the end.
 // The products are those of the tile kernels, on matrix instructions whatever the number of rows: at one row they run
-// at a tenth of what the memory needs.
+// at a tenth of what the memory needs.  Batches of many lengths leave most of the parts that a sequence may have empty: with a workgroup for each
+// (1 us even if empty, in a place of the few that the rings leave), shares had to be long, and the last ones ran alone; so the workgroups of
+// rows_by_length_kernel find the parts that there are from the lengths (us, bfloat16, one token: 64 x 8 key heads, lengths log-uniform from
+// 64 to 8192, D = 128 107 -> 96, 4.9 TB/s; 16 x 8 40 -> 31; all of 8192 99 -> 105; float32 32 x 8, up to 3000 242 -> 100).
 #pragma once
 #include "kv_fwd.h"
 
 namespace kv {
+
+// What the rows of a sequence see, of its first L keys: all of them (C = 0), or, in streaming, those of a row's chunk of C and the R chunks
+// before it.
+struct Windows {
+  int C, R;
+  ChunkDiv cdiv;
+};
+// Keys [lo, hi) of row r; the rows are those of the last `tokens` positions.
+SA_BOTH void window_of(const Windows& w, const RowMap& map, int L, int tokens, int r, int& lo, int& hi) {
+  int t, g;
+  map.split(r, t, g);
+  const int at = L - tokens + t, chunk = at < 0 ? 0 : div_by(at, w.cdiv);
+  lo = (chunk > w.R ? chunk - w.R : 0) * w.C;
+  hi = at < 0 ? 0 : (chunk + 1) * w.C < L ? (chunk + 1) * w.C : L;
+}
+// Tiles [first, last) of `tile` keys that some of the `used` rows from r0 on see.
+SA_BOTH void tiles_seen(const Windows& w, const RowMap& map, int L, int tokens, int r0, int used, int tile, int& first, int& last) {
+  int lo = 0, hi = L, ignored;
+  if (w.C > 0) {
+    window_of(w, map, L, tokens, r0, lo, ignored);
+    window_of(w, map, L, tokens, r0 + used - 1, ignored, hi);
+  }
+  first = lo / tile, last = (hi + tile - 1) / tile;
+  last = last > first ? last : first;
+}
 
 struct RowsParams {
   const void *q, *k, *v;
@@ -27,10 +55,9 @@ struct RowsParams {
   int64_t table_sb;
   int width, num_pages, page;
   ChunkDiv by_page;
-  int C, R;              // windows, as in streaming attention
-  ChunkDiv cdiv;
+  Windows win;
   // division of the work
-  int splits, share;     // share: tiles of 32 keys in a split
+  int splits, share;     // the most parts that the tiles of 32 keys of a row tile are divided into, and the most tiles of a part
   int row_tiles;
   ChunkDiv by_pairs, by_row_tiles, by_heads;
   float* part_o;         // [splits, B * Hkv, rows, D]
@@ -50,26 +77,35 @@ template <typename T, int D, int NW> struct RowsShape {
   }
 };
 
+constexpr int MAX_BY_LENGTH = 256;   // sequences
+// The sum of x over this lane and those before it.
+SA_DEV int wave_prefix_sum(int x) {
+  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);   // from one lane below, in rows of 16
+  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);   // two
+  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);   // four
+  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);   // eight
+  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);   // the last lane of rows 0 and 2 to rows 1 and 3
+  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);   // lane 31 to rows 2 and 3
+  return x;
+}
+
+// One part of the keys of 32 rows (r0 and following) of (b, hk).
 template <typename T, int D, int NW, bool PAGED>
-__global__ __launch_bounds__(NW * 64) void rows_kernel(const RowsParams p) {
+SA_DEV void rows_part(const RowsParams& p, char* smem_raw, int b, int hk, int split, int r0) {
   using G = Geom<T, D>;
   using S = RowsShape<T, D, NW>;
   using Frag = typename Elem<T>::Frag;
   constexpr int ST = S::ST, NF = G::NF, DB = G::DB, RPI = G::RPI, NI = 32 / RPI, NT = NW * 64;
   constexpr int IN_FLIGHT = (ST - 1) * 2 * NI < 63 ? (ST - 1) * 2 * NI : 63;
   static_assert(ST == 2, "the waits of the last tiles are written for two");
-  extern __shared__ __attribute__((aligned(16))) char smem_raw[];
 
   const int tid = threadIdx.x, lane = tid & 63, c = lane & 31, h = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  // the splits and row tiles of a pair lie a multiple of the pairs apart: on one XCD where eight divides the pairs
-  const int nbh = p.B * p.map.Hkv, x = div_by(blockIdx.x, p.by_pairs), bh = blockIdx.x - x * nbh;
-  const int split = div_by(x, p.by_row_tiles), r0 = (x - split * p.row_tiles) * 32;
-  const int b = div_by(bh, p.by_heads), hk = bh - b * p.map.Hkv;
+  const int nbh = p.B * p.map.Hkv, bh = b * p.map.Hkv + hk, rows = p.map.rows();
   const int L = wave_length(p.lens, p.lens_stride, b, p.max_len);
-  const int tokens = wave_length(p.q_lens, p.q_lens_stride, b, p.map.T), live = tokens * p.map.G, rows = p.map.rows();
-  const int used = live - r0 < 32 ? live - r0 : 32;   // rows of this workgroup that are not padding
+  const int tokens = wave_length(p.q_lens, p.q_lens_stride, b, p.map.T), live = tokens * p.map.G;
   T* const out = reinterpret_cast<T*>(p.o);
+  const int used = live - r0 < 32 ? live - r0 : 32;   // rows of this workgroup that are not padding
   if (p.splits == 1) {   // (with several splits the joining kernel writes the padding)
     const int first = used > 0 ? r0 + used : r0, last = r0 + 32 < rows ? r0 + 32 : rows;
     zero_rows<T, D, NT>(out, p.map, bh, first, last, tid);
@@ -80,29 +116,20 @@ __global__ __launch_bounds__(NW * 64) void rows_kernel(const RowsParams p) {
 
   // windows: of this lane's row (padding has that of the last row), of all rows, of any row
   const int row = r0 + (c < used ? c : used - 1);
-  auto window = [&](int r, int& lo, int& hi) {
-    lo = 0, hi = L;
-    if constexpr (PAGED) {
-      int t, g;
-      p.map.split(r, t, g);
-      const int at = L - tokens + t;
-      const int chunk = at < 0 ? 0 : div_by(at, p.cdiv);
-      lo = (chunk > p.R ? chunk - p.R : 0) * p.C;
-      hi = at < 0 ? 0 : (chunk + 1) * p.C < L ? (chunk + 1) * p.C : L;
-    }
-  };
-  int lo, hi, lo_min, lo_max, hi_min, hi_max;
-  window(row, lo, hi);
-  window(r0, lo_min, hi_min);
-  window(r0 + used - 1, lo_max, hi_max);
-  const int first = lo_min / 32 + split * p.share;
-  int last = (hi_max + 31) / 32;
-  last = last < first + p.share ? last : first + p.share;
-  const int64_t part_row = ((int64_t)split * nbh + bh) * rows + r0;
-  if (first >= last && p.splits > 1) {
-    if (tid < used) p.part_ml[(part_row + tid) * 2] = -INFINITY, p.part_ml[(part_row + tid) * 2 + 1] = 0.0f;
-    return;
+  int lo = 0, hi = L, lo_min = 0, lo_max = 0, hi_min = L, hi_max = L, first, last;
+  if constexpr (PAGED) {
+    window_of(p.win, p.map, L, tokens, row, lo, hi);
+    window_of(p.win, p.map, L, tokens, r0, lo_min, hi_min);
+    window_of(p.win, p.map, L, tokens, r0 + used - 1, lo_max, hi_max);
   }
+  first = lo_min / 32, last = (hi_max + 31) / 32;
+  if (p.splits > 1) {
+    const int n = last > first ? last - first : 0, parts = parts_of(n, p.share);
+    if (split >= parts) return;
+    last = first + (int)((int64_t)n * (split + 1) / parts);
+    first += (int)((int64_t)n * split / parts);
+  }
+  const int64_t part_row = ((int64_t)split * nbh + bh) * rows + r0;
 
   char* const own = smem_raw + wave * (S::RING + (PAGED ? S::ENTRIES + S::OFFSETS : 0));
   T* const ring = reinterpret_cast<T*>(own);
@@ -230,15 +257,57 @@ __global__ __launch_bounds__(NW * 64) void rows_kernel(const RowsParams p) {
   }
 }
 
+// A workgroup for each part that there may be.
+template <typename T, int D, int NW, bool PAGED>
+__global__ __launch_bounds__(NW * 64) void rows_kernel(const RowsParams p) {
+  extern __shared__ __attribute__((aligned(16))) char smem_raw[];
+  // the splits and row tiles of a pair lie a multiple of the pairs apart: on one XCD where eight divides the pairs
+  const int x = div_by(blockIdx.x, p.by_pairs), split = div_by(x, p.by_row_tiles);
+  const int bh = blockIdx.x - x * (p.B * p.map.Hkv), b = div_by(bh, p.by_heads);
+  rows_part<T, D, NW, PAGED>(p, smem_raw, b, bh - b * p.map.Hkv, split, (x - split * p.row_tiles) * 32);
+}
+// By length: as many workgroups as there are places; each takes the parts that lie the grid apart, of those that the lengths leave, whatever
+// sequence they are of.  Lane l holds, of the sequences l, l + 64, ..., how many parts there are up to and with each.
+template <typename T, int D, int NW, bool PAGED>
+__global__ __launch_bounds__(NW * 64) void rows_by_length_kernel(const RowsParams p) {
+  extern __shared__ __attribute__((aligned(16))) char smem_raw[];
+  constexpr int GROUPS = MAX_BY_LENGTH / 64;
+  const int lane = threadIdx.x & 63;
+  int upto[GROUPS], total = 0;
+#pragma unroll
+  for (int j = 0; j < GROUPS; ++j) {
+    const int b = j * 64 + lane, tokens = b < p.B ? clamped_length(p.q_lens, p.q_lens_stride, b, p.map.T) : 0;
+    int first = 0, last = 0;
+    if (tokens > 0)
+      tiles_seen(p.win, p.map, clamped_length(p.lens, p.lens_stride, b, p.max_len), tokens, 0, tokens * p.map.G, 32, first, last);
+    upto[j] = total + wave_prefix_sum(parts_of(last - first, p.share));
+    total = __builtin_amdgcn_readlane(upto[j], 63);
+  }
+  for (int id = blockIdx.x; id < total * p.map.Hkv; id += gridDim.x) {
+    const int part = div_by(id, p.by_heads);
+    int b = 0, split = part;   // b: the sequences that end before the part
+#pragma unroll
+    for (int j = 0; j < GROUPS; ++j) {
+      const int done = __builtin_popcountll(__builtin_amdgcn_ballot_w64(upto[j] <= part));
+      b += done;
+      if (done > 0) split = part - __builtin_amdgcn_readlane(upto[j], done - 1);
+    }
+    rows_part<T, D, NW, PAGED>(p, smem_raw, b, id - part * p.map.Hkv, split, 0);
+    __syncthreads();   // the next part's rings lie over the waves' results
+  }
+}
+
 // ---- joining --------------------------------------------------------------------------------------------------------
 struct JoinParams {
   const float *part_o, *part_ml;   // [splits, B * Hkv, rows, D], [splits, B * Hkv, rows, 2]
   void* o;
   float* lse;
-  const int32_t* q_lens;
-  int64_t q_lens_stride;
+  const int32_t *lens, *q_lens;
+  int64_t lens_stride, q_lens_stride;
   RowMap map;
-  int B, splits;
+  Windows win;
+  int B, max_len;
+  int splits, share, tile;         // as the parts were made: runs of tiles of `tile` keys
   ChunkDiv by_rows, by_heads;
 };
 
@@ -252,23 +321,30 @@ __global__ __launch_bounds__((SLOTS * D / 4 > 256 ? SLOTS * D / 4 : 256)) void j
   const int rows = p.map.rows();
   const int64_t all = (int64_t)p.B * p.map.Hkv * rows, id = (int64_t)blockIdx.x * RPB + in_block;
   const bool inside = id < all;
-  int bh = 0, row = 0, live = 0;
+  int bh = 0, row = 0, live = 0, parts = 0;
   if (inside) {
     bh = div_by((int)id, p.by_rows), row = (int)id - bh * rows;
-    live = clamped_length(p.q_lens, p.q_lens_stride, div_by(bh, p.by_heads), p.map.T) * p.map.G;
+    const int b = div_by(bh, p.by_heads), L = clamped_length(p.lens, p.lens_stride, b, p.max_len);
+    const int tokens = clamped_length(p.q_lens, p.q_lens_stride, b, p.map.T), r0 = row & ~31;
+    live = tokens * p.map.G;
+    if (row < live) {
+      int first, last;
+      tiles_seen(p.win, p.map, L, tokens, r0, live - r0 < 32 ? live - r0 : 32, p.tile, first, last);
+      parts = parts_of(last - first, p.share);
+    }
   }
   float m = -INFINITY, l = 0.0f;
   f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
   if (row < live) {
-    // a few splits at a time, whose loads are on their way together; a split that has seen nothing has left no O
+    // a few parts at a time, whose loads are on their way together; rows that have seen nothing in a part have a sum of 0
     constexpr int U = 4;
     const float* ml = p.part_ml + id * 2;
-    for (int s0 = slot; s0 < p.splits; s0 += SLOTS * U) {
+    for (int s0 = slot; s0 < parts; s0 += SLOTS * U) {
       float ms[U], ls[U], top = m;
       f32x4 os[U];
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        const bool there = s0 + u * SLOTS < p.splits;
+        const bool there = s0 + u * SLOTS < parts;
         const int64_t s = there ? s0 + u * SLOTS : s0;   // (no branch around the loads)
         ms[u] = ml[s * all * 2];
         ls[u] = there ? ml[s * all * 2 + 1] : 0.0f;

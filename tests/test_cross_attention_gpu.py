@@ -59,6 +59,25 @@ def test_few_rows(dtype, D, Hq, Hkv, Tq, Tk, lens):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("D", [64, 128])
+def test_one_token_of_many_lengths(dtype, D):
+    """Many sequences, whose parts the workgroups find from the lengths."""
+    B, Hq, Hkv, Tk = 72, 8, 4, 3200
+    g = torch.Generator().manual_seed(5)
+    lens = torch.randint(0, Tk + 1, (B,), generator=g).to(torch.int32)
+    lens[0], lens[1], lens[63], lens[64], lens[-1] = 0, Tk, 1, 2049, 0
+    q, k, v, _ = _inputs(B, Hq, Hkv, 1, Tk, D, dtype)
+    o, lse = cross_attention(q.to(DEV), k.to(DEV), v.to(DEV), lens.to(DEV), return_lse=True)
+    some = [0, 1, 2, 62, 63, 64, 65, B - 1]
+    want = kv_oracle.cross(q[some], k[some], v[some], lens[some])
+    kv_oracle.assert_within("o", o[some], want["o"])
+    kv_oracle.assert_within("lse", lse[some], want["lse"])
+    order = torch.randperm(B, generator=g)
+    again = cross_attention(q[order].to(DEV), k[order].to(DEV), v[order].to(DEV), lens[order].to(DEV))
+    assert torch.equal(again.cpu(), o.cpu()[order])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("D", [32, 64, 128, 256])
 @pytest.mark.parametrize("Tq,Tk,lens,q_lens", [(40, 1500, [1500, 260], None), (1500, 40, [40, 3], [1300, 1500]),
                                                (700, 900, [900, 0], [1, 700])])

@@ -238,6 +238,34 @@ def test_every_division_of_the_work(dtype, D, B, T):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("D", [32, 64, 128])
+@pytest.mark.parametrize("B,T,C,R", [(70, 1, 1, None), (200, 1, 1, None), (129, 2, 1, 2500), (66, 3, 64, 40), (256, 1, 1, None)])
+def test_parts_by_length(dtype, D, B, T, C, R):
+    """Batches of every length, whose parts the workgroups find from the lengths: some sequences against the oracle, and all against
+    the same call with the sequences in another order."""
+    Hkv, longest = 4, 3100
+    g = torch.Generator().manual_seed(B + T)
+    lens = torch.randint(0, 400, (B,), generator=g)
+    lens[torch.randperm(B, generator=g)[:9]] = torch.tensor([longest, 0, 1, 2999, 512, 513, 1024, 2048, 1600])
+    lens[0], lens[-1], lens[63], lens[64] = 0, 3000, 2500, 700
+    new_lens = None if T == 1 else torch.randint(0, T + 1, (B,), generator=g).to(torch.int32)
+    q = _q(B, 2 * Hkv, T, D, dtype)
+    k, v, table = _cache(lens.tolist(), Hkv, D, 16, dtype)
+    lens = lens.to(torch.int32)
+    on = _gpu(q, k, v, table, lens)
+    new = None if new_lens is None else new_lens.to(DEV)
+    o, lse = paged_attention(*on, C, R, None, new, return_lse=True)
+    some = [0, 1, 2, 62, 63, 64, B - 2, B - 1, int(lens.argmax())]
+    want = kv_oracle.paged(q[some], k, v, table[some], lens[some], C, R, None, None if new_lens is None else new_lens[some])
+    kv_oracle.assert_within("o", o[some], want["o"])
+    kv_oracle.assert_within("lse", lse[some], want["lse"])
+    order = torch.randperm(B, generator=g).to(DEV)
+    again, _ = paged_attention(on[0][order], on[1], on[2], on[3][order], on[4][order], C, R, None, None if new is None else new[order], return_lse=True)
+    assert torch.equal(again, o[order])
+    assert torch.isfinite(o).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("D", [16, 64, 256])
 @pytest.mark.parametrize("T,page,lens,new_lens", [(1, 16, [1, 40, 16, 17], None), (5, 3, [5, 9, 40, 3], [5, 0, 2, 5]),
                                                   (70, 16, [70, 200, 71, 100], [70, 1, 64, 33]), (4, 16, [2, 100, 400, 1], None)])
