@@ -12,6 +12,8 @@
  *     multiples of 16 bytes and not negative, base pointers 16-byte aligned; the time stride is not 0 where there is more than one
  *     row.  The rows of one head of k and v are addressed with 32-bit byte offsets: (Tk + 1024) * time_stride * element_size < 2^32,
  *     and those of q and d_o in the backward likewise where Hq == Hkv, else KV_ERR_TOO_LARGE.  Outputs are contiguous.
+ *     KV_ERR_TOO_LARGE too where a launch of the call would have 2^32 threads or more (about 2^23 pairs of a batch entry and a key head times tiles
+ *     of 128 rows, or keys in the backward, and up).
  *   - dtype: 0 = float32, 1 = float16, 2 = bfloat16.  D in {16,32,64,128,256}.
  *   - lens, q_lens, new_lens: int32 per batch entry with a stride in elements, or NULL = the whole length; values are clamped to
  *     [0, length].  Positions beyond a length are never used, whatever they hold.

@@ -73,6 +73,7 @@ struct CrossPlan {
   int key_tile, dq_key_tile, row_tile;   // of the forward, dQ, dK and dV
   bool few, long_rows, long_keys;        // the rows kernel; the hand-scheduled forward and dQ; dK and dV
   int64_t fwd_bytes, stats_bytes, dq_bytes, bwd_bytes;
+  int fwd_rc, bwd_rc;                    // KV_ERR_TOO_LARGE where a launch of the forward, or of the backward, would have too many threads
 };
 // KV_ERR_TOO_LARGE where a count of the kernels would pass 31 bits
 int plan_cross(CrossPlan& c, int B, int Hq, int Hkv, int Tq, int Tk, int D, int dtype) {
@@ -82,11 +83,13 @@ int plan_cross(CrossPlan& c, int B, int Hq, int Hkv, int Tq, int Tk, int D, int 
   if (B == 0 || Hq == 0) return KV_OK;
   c.nbh = (int64_t)B * Hkv;
   c.rows = (int64_t)(Hq / Hkv) * Tq;
-  if (c.nbh > kMostBlocks || c.rows > kMostBlocks - 1024 || Tk > kMostBlocks - 1024) return KV_ERR_TOO_LARGE;
+  if (c.nbh > kMostCount || c.rows > kMostCount - 1024 || Tk > kMostCount - 1024) return KV_ERR_TOO_LARGE;
   c.fwd = c.dq = c.dkdv = Shares{1, 1};
-  if (Tq == 0)   // nothing but zeros for dK and dV
-    return c.nbh * ceil_div(Tk, TILE_ROWS) > kMostBlocks ? KV_ERR_TOO_LARGE : KV_OK;
-  const int row_bytes = D * elem_size(dtype);
+  const int row_bytes = D * elem_size(dtype), key_threads = dtype != 0 && D == 256 ? 512 : 256;
+  if (Tq == 0) {   // nothing but zeros for dK and dV
+    c.bwd_rc = launchable(c.nbh * ceil_div(Tk, TILE_ROWS), key_threads) ? KV_OK : KV_ERR_TOO_LARGE;
+    return KV_OK;
+  }
   c.key_tile = c.row_tile = row_bytes <= 256 ? 64 : 32;
   c.dq_key_tile = elem_size(dtype) == 2 ? 64 : c.key_tile;
   const int64_t row_tiles = ceil_div(c.rows, TILE_ROWS), key_tiles = ceil_div(Tk, TILE_ROWS);
@@ -103,9 +106,12 @@ int plan_cross(CrossPlan& c, int B, int Hq, int Hkv, int Tq, int Tk, int D, int 
   }
   if (!c.long_rows) c.dq = tile_shares(c.nbh * row_tiles, ceil_div(Tk, c.dq_key_tile), row_places(row_bytes), false, dtype == 0);
   c.dkdv = tile_shares(c.nbh * key_tiles, ceil_div(c.rows, c.row_tile), key_places(row_bytes), true, dtype == 0);
-  if (c.nbh * std::max(row_tiles * std::max(c.fwd.splits, c.dq.splits), key_tiles * c.dkdv.splits) > kMostBlocks) return KV_ERR_TOO_LARGE;
-  if (std::max(c.fwd.splits, c.dq.splits) > 1 && c.nbh * c.rows > kMostBlocks) return KV_ERR_TOO_LARGE;
-  if (c.dkdv.splits > 1 && c.nbh * Tk > kMostBlocks) return KV_ERR_TOO_LARGE;
+  const int64_t fwd_blocks = c.nbh * (c.few ? 1 : row_tiles) * c.fwd.splits;   // (the hand-scheduled kernels have fewer)
+  const int fwd_threads = c.few ? 64 * rows_waves(row_bytes, dtype == 0, fwd_blocks, c.fwd.share) : 256;
+  if (!launchable(fwd_blocks, fwd_threads)) c.fwd_rc = KV_ERR_TOO_LARGE;
+  if (!launchable(c.nbh * row_tiles * c.dq.splits, 256) || !launchable(c.nbh * key_tiles * c.dkdv.splits, key_threads)) c.bwd_rc = KV_ERR_TOO_LARGE;
+  if (std::max(c.fwd.splits, c.dq.splits) > 1 && c.nbh * c.rows > kMostCount) return KV_ERR_TOO_LARGE;
+  if (c.dkdv.splits > 1 && c.nbh * Tk > kMostCount) return KV_ERR_TOO_LARGE;
   if (c.fwd.splits > 1) c.fwd_bytes = c.fwd.splits * c.nbh * c.rows * (D + 2) * 4;
   c.stats_bytes = ceil_div(c.nbh * c.rows * 4, 256) * 256;
   const int64_t dq = c.dq.splits > 1 ? c.dq.splits * c.nbh * c.rows * D * 4 : 0;
@@ -148,7 +154,7 @@ int plan_paged(PagedPlan& c, int B, int Hq, int Hkv, int T, int D, int page, int
   const int G = Hq / Hkv;
   c.nbh = (int64_t)B * Hkv;
   c.rows = (int64_t)G * T;
-  if (c.nbh > kMostBlocks || c.rows > kMostBlocks - 1024) return KV_ERR_TOO_LARGE;
+  if (c.nbh > kMostCount || c.rows > kMostCount - 1024) return KV_ERR_TOO_LARGE;
   c.row_tiles = ceil_div(c.rows, 32);
   // the most keys that the rows of a tile see together: those of R + 1 chunks for each chunk that its tokens lie in
   const int64_t tokens = std::min<int64_t>(T, 31 / G + 2), chunks = ceil_div(tokens - 1, C) + 1;
@@ -157,7 +163,9 @@ int plan_paged(PagedPlan& c, int B, int Hq, int Hkv, int T, int D, int page, int
   const int row_bytes = D * elem_size(dtype);
   c.share = rows_share(c.nbh * c.row_tiles, (int)std::min<int64_t>(c.rows, 32), tiles, row_bytes, dtype == 0, by_length(B, c.row_tiles, row_bytes));
   c.splits = (int)std::max<int64_t>(1, ceil_div(tiles, c.share));
-  if (c.nbh * c.row_tiles * c.splits > kMostBlocks || (c.splits > 1 && c.nbh * c.rows > kMostBlocks)) return KV_ERR_TOO_LARGE;
+  const int64_t blocks = c.nbh * c.row_tiles * c.splits;
+  if (!launchable(blocks, 64 * rows_waves(row_bytes, dtype == 0, blocks, c.share))) return KV_ERR_TOO_LARGE;
+  if (c.splits > 1 && c.nbh * c.rows > kMostCount) return KV_ERR_TOO_LARGE;
   if (c.splits > 1) c.bytes = c.splits * c.nbh * c.rows * (D + 2) * 4;
   return KV_OK;
 }
@@ -181,7 +189,7 @@ extern "C" {
 int64_t kv_cross_forward_workspace(int B, int Hq, int Hkv, int Tq, int Tk, int D, int dtype) {
   CrossPlan c;
   if (int rc = plan_cross(c, B, Hq, Hkv, Tq, Tk, D, dtype)) return rc;
-  return c.fwd_bytes;
+  return c.fwd_rc ? c.fwd_rc : c.fwd_bytes;
 }
 
 int kv_cross_forward(const void* q, const void* k, const void* v, const int32_t* lens, int64_t lens_stride, const int32_t* q_lens,
@@ -190,6 +198,7 @@ int kv_cross_forward(const void* q, const void* k, const void* v, const int32_t*
                      void* stream) {
   CrossPlan c;
   if (int rc = plan_cross(c, B, Hq, Hkv, Tq, Tk, D, dtype)) return rc;
+  if (c.fwd_rc) return c.fwd_rc;
   if (B == 0 || Hq == 0 || Tq == 0) return KV_OK;
   if (int rc = check_layout(q, qs, dtype, Tq, false)) return rc;
   if (Tk > 0) {
@@ -251,7 +260,7 @@ int kv_cross_forward(const void* q, const void* k, const void* v, const int32_t*
 int64_t kv_cross_backward_workspace(int B, int Hq, int Hkv, int Tq, int Tk, int D, int dtype) {
   CrossPlan c;
   if (int rc = plan_cross(c, B, Hq, Hkv, Tq, Tk, D, dtype)) return rc;
-  return c.bwd_bytes;
+  return c.bwd_rc ? c.bwd_rc : c.bwd_bytes;
 }
 
 int kv_cross_backward(const void* q, const void* k, const void* v, const int32_t* lens, int64_t lens_stride, const int32_t* q_lens,
@@ -261,6 +270,7 @@ int kv_cross_backward(const void* q, const void* k, const void* v, const int32_t
                       void* stream) {
   CrossPlan c;
   if (int rc = plan_cross(c, B, Hq, Hkv, Tq, Tk, D, dtype)) return rc;
+  if (c.bwd_rc) return c.bwd_rc;
   if (B == 0 || Hq == 0) return KV_OK;
   if (Tq > 0) {
     const bool one_head = Hq == Hkv;
@@ -438,7 +448,7 @@ int kv_paged_append(const void* k, const void* v, void* k_pages, void* v_pages, 
   p.vp_sp = vps[0] * es; p.vp_sh = vps[1] * es; p.vp_st = vps[2] * es;
   p.B = B; p.H = H; p.T = T; p.width = width; p.num_pages = num_pages; p.page = page_size;
   p.chunks = (int)(D * es / 16);
-  if ((int64_t)B * H > kMostBlocks || (int64_t)B * H * T > kMostBlocks / p.chunks) return KV_ERR_TOO_LARGE;
+  if ((int64_t)B * H > kMostCount || (int64_t)B * H * T > kMostCount / p.chunks) return KV_ERR_TOO_LARGE;
   p.total = (int64_t)B * H * T * p.chunks;
   p.by_chunks = chunk_div(p.chunks); p.by_tokens = chunk_div(T); p.by_heads = chunk_div(H); p.by_page = chunk_div(page_size);
   const bool streaming = p.total * 32 > (int64_t(32) << 20);   // more than the L2s of all XCDs hold

@@ -35,7 +35,7 @@ template <typename K> static int raise_lds(K kernel, size_t bytes, LdsLimit& sta
 }
 template <typename K, typename P>
 static int launch(K kernel, int64_t blocks, int threads, size_t lds, LdsLimit& state, const P& p, hipStream_t st, int layers = 1) {
-  if (blocks > kMostBlocks) return KV_ERR_TOO_LARGE;
+  if (!launchable(blocks, threads)) return KV_ERR_TOO_LARGE;   // (the host has refused it before the first launch of a call)
   if (blocks == 0) return KV_OK;
   if (int rc = raise_lds(kernel, lds, state)) return rc;
   kernel<<<dim3((unsigned)blocks, layers), dim3(threads), lds, st>>>(p);

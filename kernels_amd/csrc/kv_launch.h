@@ -34,7 +34,9 @@ template <typename T> int launch_long_fwd(const LongFwd& p, hipStream_t st);
 template <typename T> int launch_long_dq(const LongBwd& p, hipStream_t st);
 template <typename T> int launch_long_dkdv(const LongBwd& p, hipStream_t st);
 
-constexpr int64_t kMostBlocks = 0x7fffffff;
+constexpr int64_t kMostCount = 0x7fffffff;   // pairs, rows, keys: what the kernels count in 31 bits
+// The runtime takes fewer than 2^32 threads along a dimension of a grid.
+inline bool launchable(int64_t blocks, int threads) { return blocks <= 0xffffffffLL / threads; }
 inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 constexpr int TILE_ROWS = 128;   // rows (or keys) of a workgroup of the tile kernels: four waves of 32
