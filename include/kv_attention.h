@@ -14,6 +14,7 @@
  *     and those of q and d_o in the backward likewise where Hq == Hkv, else KV_ERR_TOO_LARGE.  Outputs are contiguous.
  *     KV_ERR_TOO_LARGE too where a launch of the call would have 2^32 threads or more (about 2^23 pairs of a batch entry and a key head times tiles
  *     of 128 rows, or keys in the backward, and up).
+ *   - sm_scale is a number within 2^127 on either side of 0, else KV_ERR_ARG.
  *   - dtype: 0 = float32, 1 = float16, 2 = bfloat16.  D in {16,32,64,128,256}.
  *   - lens, q_lens, new_lens: int32 per batch entry with a stride in elements, or NULL = the whole length; values are clamped to
  *     [0, length].  Positions beyond a length are never used, whatever they hold.

@@ -28,6 +28,8 @@ int check_layout(const void* p, const int64_t* s, int dtype, int64_t n, bool off
   if (offsets32 && s[2] > ((int64_t(1) << 32) - 1) / es / (n + 1024)) return KV_ERR_TOO_LARGE;
   return KV_OK;
 }
+// Times log2(e) it has to be a number of float32.
+int check_scale(float sm_scale) { return fabsf(sm_scale) <= 0x1p127f ? KV_OK : KV_ERR_ARG; }
 int check_out(const void* p) { return !p ? KV_ERR_ARG : (reinterpret_cast<uintptr_t>(p) & 15u) ? KV_ERR_LAYOUT : KV_OK; }
 
 template <typename F> int by_dtype(int dtype, F&& f) {
@@ -199,6 +201,7 @@ int kv_cross_forward(const void* q, const void* k, const void* v, const int32_t*
   CrossPlan c;
   if (int rc = plan_cross(c, B, Hq, Hkv, Tq, Tk, D, dtype)) return rc;
   if (c.fwd_rc) return c.fwd_rc;
+  if (int rc = check_scale(sm_scale)) return rc;
   if (B == 0 || Hq == 0 || Tq == 0) return KV_OK;
   if (int rc = check_layout(q, qs, dtype, Tq, false)) return rc;
   if (Tk > 0) {
@@ -271,6 +274,7 @@ int kv_cross_backward(const void* q, const void* k, const void* v, const int32_t
   CrossPlan c;
   if (int rc = plan_cross(c, B, Hq, Hkv, Tq, Tk, D, dtype)) return rc;
   if (c.bwd_rc) return c.bwd_rc;
+  if (int rc = check_scale(sm_scale)) return rc;
   if (B == 0 || Hq == 0) return KV_OK;
   if (Tq > 0) {
     const bool one_head = Hq == Hkv;
@@ -383,6 +387,7 @@ int kv_paged_forward(const void* q, const void* k_pages, const void* v_pages, co
   PagedPlan c;
   if (int rc = plan_paged(c, B, Hq, Hkv, T, D, page_size, width, context_size, back_contexts, dtype)) return rc;
   if (num_pages < 0) return KV_ERR_ARG;
+  if (int rc = check_scale(sm_scale)) return rc;
   if (B == 0 || Hq == 0 || T == 0) return KV_OK;
   if (int rc = check_layout(q, qs, dtype, T, false)) return rc;
   if (!lens) return KV_ERR_ARG;
@@ -462,7 +467,7 @@ const char* kv_error_string(int code) {
     case KV_ERR_DTYPE: return "unsupported dtype id (0 = float32, 1 = float16, 2 = bfloat16)";
     case KV_ERR_HEAD_DIM: return "head dimension must be one of 16, 32, 64, 128, 256";
     case KV_ERR_ARG: return "invalid argument (null pointer, negative size, Hq not a multiple of Hkv, page_size or context_size < 1, "
-                            "back_contexts < 0)";
+                            "back_contexts < 0, a scale beyond 2^127)";
     case KV_ERR_LAYOUT: return "unsupported layout (dim stride must be 1; pointers and strides 16-byte aligned, strides not negative)";
     case KV_ERR_TOO_LARGE: return "problem too large for one launch";
     case KV_ERR_WORKSPACE: return "workspace missing or smaller than the *_workspace function says";

@@ -94,6 +94,7 @@ bool alike(const Tensor& a, const Tensor& b) { return a.device() == b.device() &
 bool is_lengths(const OptTensor& l, const Tensor& q) {
   return !l || (l->scalar_type() == at::kInt && l->dim() == 1 && l->size(0) == q.size(0) && l->device() == q.device());
 }
+bool is_scale(double sm_scale) { return std::fabs(sm_scale) <= 0x1p127; }   // times log2(e) in float32's range
 bool small(int64_t n) { return n <= 0x7fffffff; }
 bool small_sizes(const Tensor& t) { return small(t.size(0)) && small(t.size(1)) && small(t.size(2)); }
 
@@ -101,7 +102,7 @@ bool is_cross(const Tensor& q, const Tensor& k, const Tensor& v, const OptTensor
   if (q.dim() != 4 || k.dim() != 4 || dtype_id(q) < 0 || !known_head_dim(q.size(3)) || !alike(q, k) || !alike(q, v)) return false;
   if (v.sizes() != k.sizes() || k.size(0) != q.size(0) || k.size(3) != q.size(3) || k.size(1) < 1 || q.size(1) < 1 || q.size(1) % k.size(1) != 0)
     return false;
-  return small_sizes(q) && small_sizes(k) && is_lengths(lens, q) && is_lengths(q_lens, q) && std::isfinite(sm_scale);
+  return small_sizes(q) && small_sizes(k) && is_lengths(lens, q) && is_lengths(q_lens, q) && is_scale(sm_scale);
 }
 bool is_cache(const Tensor& x, const Tensor& k_pages, const Tensor& v_pages, const Tensor& table, const Tensor& lens,
               const OptTensor& new_lens) {
@@ -341,7 +342,7 @@ std::tuple<Tensor, Tensor> paged_forward_gpu(const Tensor& q, const Tensor& k_pa
                                              const Tensor& lens, int64_t context_size, int64_t back_contexts, double sm_scale,
                                              const OptTensor& new_lens, bool return_lse) {
   if (C10_UNLIKELY(!(is_cache(q, k_pages, v_pages, page_table, lens, new_lens) && q.size(1) % k_pages.size(1) == 0 && context_size >= 1 &&
-                     back_contexts >= 0 && std::isfinite(sm_scale)))) {
+                     back_contexts >= 0 && is_scale(sm_scale)))) {
     Gil gil;
     explain("_validate_paged", {THPVariable_Wrap(q), THPVariable_Wrap(k_pages), THPVariable_Wrap(v_pages), THPVariable_Wrap(page_table),
                                 THPVariable_Wrap(lens), PyLong_FromLongLong(context_size), PyLong_FromLongLong(back_contexts),

@@ -20,6 +20,7 @@ except ImportError as e:
 HEAD_DIMS = (16, 32, 64, 128, 256)
 DTYPES = (torch.float32, torch.float16, torch.bfloat16)
 MOST_POSITIONS = 1 << 30   # page_table.shape[1] * page size
+MOST_SCALE = 2.0 ** 127    # the kernels take it times log2(e), in float32
 _INT32 = 2 ** 31 - 1
 
 
@@ -27,6 +28,11 @@ def _check_lengths(name, lens, q):
     assert lens is None or (lens.dtype == torch.int32 and lens.ndim == 1 and len(lens) == q.shape[0]), \
         f"{name} must be int32 of shape (batch,)"
     assert lens is None or lens.device == q.device, f"{name} must be on the device of q"
+
+
+def _check_scale(sm_scale):
+    assert math.isfinite(sm_scale), "sm_scale must be finite"
+    assert abs(sm_scale) <= MOST_SCALE, "sm_scale must lie within 2**127 on either side of 0"
 
 
 def _check_heads(q, k, v):
@@ -48,7 +54,7 @@ def _validate_cross(q, k, v, lens, q_lens, sm_scale, *others):
     assert k.shape[0] == q.shape[0], "k and v need q's batch size"
     _check_lengths("lens", lens, q)
     _check_lengths("q_lens", q_lens, q)
-    assert math.isfinite(sm_scale), "sm_scale must be finite"
+    _check_scale(sm_scale)
     for t in others:
         assert t.shape == q.shape, "o and dO need q's shape"
         assert t.device == q.device, "o and dO must be on the device of q"
@@ -75,7 +81,7 @@ def _validate_cache(x, k_pages, v_pages, page_table, lens, new_lens):
 def _validate_paged(q, k_pages, v_pages, page_table, lens, context_size, back_contexts, sm_scale, new_lens):
     _validate_cache(q, k_pages, v_pages, page_table, lens, new_lens)
     assert back_contexts >= 0 and context_size >= 1
-    assert math.isfinite(sm_scale), "sm_scale must be finite"
+    _check_scale(sm_scale)
 
 
 def _validate_append(k, v, k_pages, v_pages, page_table, lens, new_lens):
