@@ -54,21 +54,17 @@ SA_DEV void mul_rows(f32x16 (&acc)[NB], const T* tile, int row0, const typename 
   }
 }
 
-// acc[m][x][c] += sum_r tile[row0 + r][m * 32 + x] * P[r][c] over the 32 rows from row0 on; P is rounded to T.
+// acc[m][x][c] += sum_r tile[row0 + r][m * 32 + x] * P[r][c] over the 32 rows from row0 on: float32 (16-bit elements: sa::mma_tr_n).
 template <typename T, int D, int DB> SA_DEV void mul_tr(f32x16 (&acc)[DB], const T* tile, int row0, const f32x16& P, int lane) {
   using G = Geom<T, D>;
-  static_assert(DB == G::DB, "one accumulator per 32 columns");
-  if constexpr (Elem<T>::HALF) {
-    sa::mma_tr<T, D>(acc, tile, row0 / 32, P, lane);
-  } else {
-    const int h = lane >> 5, c = D < 32 ? lane & 15 : lane & 31;   // D = 16: the product's rows from 16 on repeat the first
+  static_assert(!Elem<T>::HALF && DB == G::DB, "float32, one accumulator per 32 columns");
+  const int h = lane >> 5, c = D < 32 ? lane & 15 : lane & 31;   // D = 16: the product's rows from 16 on repeat the first
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const int row = row0 + sa::crow(i, h);
+  for (int i = 0; i < 16; ++i) {
+    const int row = row0 + sa::crow(i, h);
 #pragma unroll
-      for (int m = 0; m < DB; ++m)
-        acc[m] = __builtin_amdgcn_mfma_f32_32x32x2f32(tile[G::off(row, m * 32 + c)], P[i], acc[m], 0, 0, 0);
-    }
+    for (int m = 0; m < DB; ++m)
+      acc[m] = __builtin_amdgcn_mfma_f32_32x32x2f32(tile[G::off(row, m * 32 + c)], P[i], acc[m], 0, 0, 0);
   }
 }
 

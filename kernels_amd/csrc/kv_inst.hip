@@ -101,7 +101,9 @@ template <> int launch_cross_dkdv<ElemT, KV_DGROUP>(const BwdParams& p, int D, h
 #elif KV_KIND == 3
 template <int D, int NW, bool PAGED> static int launch_rows_shape(const RowsParams& p, int64_t blocks, hipStream_t st) {
   constexpr int row_bytes = D * (int)sizeof(ElemT), lds = RowsShape<ElemT, D, NW>::bytes(PAGED), places = CUS * (163840 / lds);
-  if constexpr (row_bytes >= 128) {
+  // by length where there are many workgroups: only the waves that many workgroups have
+  if constexpr (row_bytes >= 128 && NW == rows_waves(row_bytes, sizeof(ElemT) == 4, 2 * CUS, 1)) {
+    static_assert(2 * places >= 2 * CUS, "many in the sense of rows_waves");
     static LdsLimit state;
     if (p.splits > 1 && by_length(p.B, p.row_tiles, row_bytes) && blocks >= 2 * places)
       return launch(rows_by_length_kernel<ElemT, D, NW, PAGED>, places, NW * 64, lds, state, p, st);

@@ -121,7 +121,7 @@ inline int rows_share(int64_t units, int rows, int64_t n, int row_bytes, bool f3
 // shares or a CU for each (float16, us, four -> eight: 8 units of 10 tiles 6.1 -> 5.8; 16 of 22 8.2 -> 7.5), else four.  256 bytes: two where there is more than one workgroup for each place, so that one begins while the other one is in its
 // run (512 units of 16 tiles 27.1 -> 23.8 us), else four; float32, whose matrix instructions take their time, always four: two waves of two
 // workgroups may share a SIMD (128 units of 63 tiles 38 -> 54).
-inline int rows_waves(int row_bytes, bool f32, int64_t workgroups, int share) {
+constexpr int rows_waves(int row_bytes, bool f32, int64_t workgroups, int share) {
   const bool many = workgroups >= 2 * CUS;
   if (row_bytes == 128) return (!many && share >= 24) || (workgroups <= CUS && share > 8) ? 8 : 4;
   if (row_bytes == 256) return many && !f32 ? 2 : 4;
