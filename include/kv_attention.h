@@ -78,7 +78,8 @@ int64_t kv_paged_forward_workspace(int B, int Hq, int Hkv, int T, int D, int pag
  * Token i of the n = new_lens[b] (or T) new ones is at position at = lens[b] - n + i and sees the positions j < lens[b] with
  * 0 <= at / context_size - j / context_size <= back_contexts: what row `at` of sa_forward sees.  context_size 1 is causal, and with back_contexts
  * = w a window of w + 1 positions; a token whose position is negative sees nothing.  width * page_size <= 2^30.
- * O and LSE as in kv_cross_forward.  The bits of a sequence's result depend on the sizes of the call, not on the other sequences.
+ * O and LSE as in kv_cross_forward.  The bits of a sequence's result depend on the sizes of the call (B, T, width * page_size), not on the
+ * lengths or values of the other sequences.
  * A value that is not finite, at a position that one new token sees, reaches the other tokens of its sequence in the call. */
 int kv_paged_forward(const void* q, const void* k_pages, const void* v_pages,
                      const int32_t* page_table, int64_t table_stride, const int32_t* lens, int64_t lens_stride,

@@ -90,10 +90,15 @@ inline bool long_keys(int64_t key_heads, int64_t rows, int64_t Tk) { return rows
 // The rows kernel serves up to 32 rows of a key head.
 inline bool few_rows(int64_t rows) { return rows <= 32; }
 // How its keys are divided, from the sizes of the call: at most n tiles of 32 keys for each of `units` workgroups of `rows` rows.  A share is
-// what leaves one workgroup for each CU, from four tiles on; short runs are not divided (the joining kernel takes about 4 us), and shares of
+// what leaves one workgroup for each CU if every sequence has all n tiles (a table that is much wider than its sequences leaves few workgroups:
+// 8 units of 4096 positions, D = 128, 16-bit 10.7 us in a table of 4096, 17.9 in one of 32768, 47 in one of 131072), from four tiles on; short
+// runs are not divided (the joining kernel takes about 4 us), and shares of
 // many workgroups stay short, so that long sequences of a batch spread over the CUs that short ones have left: 16 tiles where workgroups go
-// through the parts that there are (by_length), else 32, as parts that the lengths leave empty have workgroups then.  float32 is bound by its matrix
-// instructions and gains by every division, down to one tile to a wave (128 units of 63 tiles, D = 64: 55 us in one share, 37 in two; 2 units of
+// through the parts that there are (by_length), else 32, as parts that the lengths leave empty have workgroups then.  By length this begins at 48
+// units: fewer keep their shares of up to 128 (us, -> 16 tiles, D = 128, 16-bit: all of 131072 4 x 8 368 -> 398, 5 x 8 470 -> 496, 3 x 8 303 -> 305;
+// from half of 131072 on 4 x 8 314 -> 325, 3 x 8 290 -> 255; log-uniform up to 32768 5 x 8 67 -> 59, 12 x 2 40 -> 24, up to 131072 5 x 8 182 -> 186, 12 x 2
+// 117 -> 71); from 48 on 6 x 8 log-uniform up to 131072 211 -> 184, all of 32768 156 -> 155, of 131072 546 -> 588; 8 x 8 log-uniform
+// up to 32768 115 -> 62.  float32 is bound by its matrix instructions and gains by every division, down to one tile to a wave (128 units of 63 tiles, D = 64: 55 us in one share, 37 in two; 2 units of
 // 13, D = 128 38 in one, 11.7 in seven; 32 of 10, D = 64 12.1 and 8.8).
 // One token per sequence, in us for shares of 4, 8, 16, 32, 64, 128 tiles (* chosen), 16-bit elements, D = 128, four waves: 8 units of 63
 // tiles 9.5*, 9.7, 12.0, 15.9, 22.3; of 1000 60.9, 45.9, 34.9, 28.0*, 32.2, 49.7; 32 units of 63 16.2, 12.6*, 14.2, 18.1, 25.1; of 250 49.7, 36.7, 29.6,

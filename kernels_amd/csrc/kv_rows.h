@@ -7,8 +7,10 @@
 // The products are those of the tile kernels, on matrix instructions whatever the number of rows: at one row they run
 // at a tenth of what the memory needs.  Batches of many lengths leave most of the parts that a sequence may have empty: with a workgroup for each
 // (1 us even if empty, in a place of the few that the rings leave), shares had to be long, and the last ones ran alone; so the workgroups of
-// rows_by_length_kernel find the parts that there are from the lengths (us, bfloat16, one token: 64 x 8 key heads, lengths log-uniform from
-// 64 to 8192, D = 128 107 -> 96, 4.9 TB/s; 16 x 8 40 -> 31; all of 8192 99 -> 105; float32 32 x 8, up to 3000 242 -> 100).
+// rows_by_length_kernel find the parts that there are from the lengths.  One token, D = 128, us with a workgroup for each part -> by length: bfloat16,
+// lengths log-uniform from 64 to 8192, 64 x 8 key heads 104 -> 95 (4.6 TB/s), 16 x 8 43 -> 31; float32, 32 x 8, log-uniform up to 3000 243 -> 100, from
+// 1500 on 246 -> 228.  Sequences of one length pay for the gaps between the parts of a workgroup: bfloat16, all of 8192 16 x 8 99 -> 104, 64 x 8
+// 363 -> 386; float32, all of 3000 248 -> 282.
 #pragma once
 #include "kv_fwd.h"
 

@@ -73,9 +73,13 @@ def paged_attention(
 
     Tokens beyond ``new_lens[b]`` give 0 and log-sum-exp 0; a token that sees no position gives 0 and log-sum-exp -inf.  What the cache holds
     where no token sees it does not matter.  (A value that is not finite, seen by one of several new tokens, reaches the others of
-    its sequence.)  The bits of a sequence's result depend on the sizes of the call, not on the lengths or values of other sequences.
-    Forward only.  Can be captured into a HIP graph after one call of the same sizes and type outside the capture.  Meant for few new
-    tokens: a whole prompt runs faster through :func:`streaming_attention.streaming_attention`, beside a :func:`paged_append`.
+    its sequence.)  The bits of a sequence's result depend on the sizes of the call (the batch, the tokens, the table's width), not on the lengths or
+    values of other sequences.  Forward only.  Can be captured into a HIP graph after one call of the same sizes and type outside the capture.
+
+    Meant for few new tokens, in a table about as wide as its sequences are long: the work is divided by the table's width, and one or a few
+    sequences of a table many times wider take several times as long as in a narrow one.  Prompts and further turns are served in any number
+    of tokens and any head layout, at about a third of the rate of a large matrix product; a prompt of a sequence of its own, with as many key heads
+    as heads, runs faster through :func:`streaming_attention.streaming_attention`, beside a :func:`paged_append`.
     """
     if back_contexts is None:
         back_contexts = _NO_LIMIT
