@@ -6,8 +6,8 @@ namespace kv {
 
 // Token i of n = new_lens[b] of sequence b goes to position lens[b] - n + i.  Positions below 0 or past the table, and pages that are not there, are
 // left out.  Bytes only: one thread moves sixteen of K and sixteen of V; consecutive threads go through the chunks of a row, then the tokens of
-// a head.  Bound by memory: prompts of up to 2048 tokens for 8 sequences of 8 heads, D = 128, bfloat16 (67 MB read and written) 12.4-15.0 us,
-// 4.5-5.4 TB/s over several GPUs, with stores past the caches; on one of them 12.9, and 16.1 with plain stores, which a call keeps whose rows stay in
+// a head.  Bound by memory: prompts of up to 2048 tokens for 8 sequences of 8 heads, D = 128, bfloat16 (67 MB read and written) 10.9-15.0 us,
+// 4.5-6.2 TB/s over several GPUs, with stores past the caches; on one of them 12.9, and 16.1 with plain stores, which a call keeps whose rows stay in
 // the L2 for the attention that follows; two or four pieces to a thread took 19 and 27 there.
 struct AppendParams {
   const char *k, *v;
