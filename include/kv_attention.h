@@ -92,8 +92,8 @@ int kv_paged_forward(const void* q, const void* k_pages, const void* v_pages,
 /* Writes the new tokens k, v [B,H,T,D] into the pages: token i of the n = new_lens[b] (or T) of sequence b to position lens[b] - n + i.
  * Positions below 0 or from width * page_size on, and pages that are not there, are left out.  Where two tokens of a call have the
  * same place (two sequences that share a page), it holds either of them afterwards, or sixteen bytes of one beside sixteen of
- * the other.  The strides of the pages are not 0 where there is more than one page or head.  B * H * T * D * element_size < 2^35, else
- * KV_ERR_TOO_LARGE. */
+ * the other.  k and v do not overlap the pages.  The strides of the pages are not 0 where there is more than one page or head.
+ * B * H * T * D * element_size < 2^35, else KV_ERR_TOO_LARGE. */
 int kv_paged_append(const void* k, const void* v, void* k_pages, void* v_pages,
                     const int32_t* page_table, int64_t table_stride, const int32_t* lens, int64_t lens_stride,
                     const int32_t* new_lens, int64_t new_lens_stride,

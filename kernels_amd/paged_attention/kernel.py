@@ -108,7 +108,8 @@ def paged_append(
     ``lens[b]`` counts the new tokens already: token ``i`` of the ``n = new_lens[b]`` (or all) new ones goes to position ``lens[b] - n + i``.
     Positions below 0 or past the table, and pages that are not there, are left out; everything else in the cache stays
     as it is.  A page that sequences share (a common prefix) must not be written by more than one of them in a call: which of two values
-    for one place stays is not defined.  Records no gradient: call it under ``torch.no_grad()`` or on detached tensors.
+    for one place stays is not defined; nor is what is written from ``k`` and ``v`` that overlap the pages.  Records no gradient: call it under
+    ``torch.no_grad()`` or on detached tensors.
     """
     if ops.takes_native_call(k, v, k_pages, v_pages, page_table, lens, new_lens):
         if _eager_append(k, v, k_pages, v_pages, page_table, lens, new_lens) is not NotImplemented:
