@@ -1,6 +1,7 @@
 /* C ABI of libkv_attention.so -- hand-written gfx950 (MI355X) kernels for attention over keys that are not the
  * queries' own: an encoder's states (cross attention, forward and backward) and a cache in pages (the newest tokens of
- * every sequence), and the writing of new tokens into the pages.
+ * every sequence, or trees of drafted ones), the writing of new tokens into the pages, and what comes before attention: norms of queries
+ * and keys for each head and the rotation by position.
  *
  * Common rules
  *   - Every pointer is a device pointer owned by the caller.  Nothing is allocated, freed or synchronised here: each call
@@ -100,6 +101,66 @@ int kv_paged_append(const void* k, const void* v, void* k_pages, void* v_pages,
                     const int64_t* k_strides, const int64_t* v_strides,
                     const int64_t* k_page_strides, const int64_t* v_page_strides,
                     int B, int H, int T, int D, int num_pages, int page_size, int width, int dtype, void* stream);
+
+/* Trees of drafted tokens over the cache: as kv_paged_forward, but token i of the n new ones sees all positions before them, below lens[b] - n, and of
+ * the new tokens those j with tree[b][i][j] != 0: bytes at the strides int64[3] (batch, token, token; a batch stride of 0 is one tree for all).
+ * A token whose position lens[b] - n + i is negative sees nothing, and is not seen. */
+int64_t kv_paged_tree_forward_workspace(int B, int Hq, int Hkv, int T, int D, int page_size, int width, int dtype);
+int kv_paged_tree_forward(const void* q, const void* k_pages, const void* v_pages,
+                          const int32_t* page_table, int64_t table_stride, const int32_t* lens, int64_t lens_stride,
+                          const int32_t* new_lens, int64_t new_lens_stride, const void* tree, const int64_t* tree_strides,
+                          void* o, float* lse, void* workspace, int64_t workspace_bytes,
+                          const int64_t* q_strides, const int64_t* k_strides, const int64_t* v_strides,
+                          int B, int Hq, int Hkv, int T, int D, int num_pages, int page_size, int width,
+                          float sm_scale, int dtype, void* stream);
+
+/* Keeps accepted tokens: K and V of position first[b] + kept[b][i] go to position first[b] + i, for i = 0, 1, ... up to the first entry that is
+ * negative or not above the one before it, or M of them.  kept: int32 at the strides int64[2] (batch, entry).  Where the one or the other position is below
+ * 0, past the table or on a page that is not there, the place stays as it is.  Pages that a call writes are of one sequence each. */
+int kv_paged_keep(void* k_pages, void* v_pages, const int32_t* page_table, int64_t table_stride,
+                  const int32_t* first, int64_t first_stride, const int32_t* kept, const int64_t* kept_strides,
+                  const int64_t* k_page_strides, const int64_t* v_page_strides,
+                  int B, int H, int M, int D, int num_pages, int page_size, int width, int dtype, void* stream);
+
+/* Norms of queries and keys for each head and the rotation by position.  A row x (D channels) of q [B,Hq,T,D] or k [B,Hkv,T,D] becomes
+ *   y = x * w / sqrt(mean(x^2) + eps)      eps 0: y = x, and no weights
+ * and of its first `rot` channels the pairs (a, b) become (a cos - b sin, b cos + a sin): channels i and i + rot / 2, or 2 i and 2 i + 1 if interleaved,
+ * with cos[at][i] and sin[at][i].  at: positions[b][t] at the strides int64[2], or t where positions is NULL.
+ * rot: a multiple of 16 up to D.  cos, sin: float32 [table_rows, rot / 2], rows a multiple of 4 elements apart, 16-byte aligned.  Weights: [D] of the element
+ * type, or float32 where weights_f32 is set, 16-byte aligned, or NULL (ones).  Tokens from lens[b] on, and tokens whose position the table does not
+ * have, are padding: their rows are 0, they are not read and pass no gradient on.  q_out and k_out are contiguous and written whole.
+ * Sums are float32; results are rounded once.  Any Hq (up to 32767) and Hkv (16383), B * T < 2^31, else KV_ERR_TOO_LARGE. */
+int kv_qk_norm_rope(const void* q, const void* k, const float* cos, const float* sin, int64_t cos_stride, int64_t sin_stride,
+                    const void* q_weight, const void* k_weight, int weights_f32,
+                    const int32_t* lens, int64_t lens_stride, const int32_t* positions, const int64_t* position_strides,
+                    void* q_out, void* k_out, const int64_t* q_strides, const int64_t* k_strides,
+                    int B, int Hq, int Hkv, int T, int D, int rot, int table_rows, int interleaved, float eps, int dtype, void* stream);
+
+/* Bytes of workspace for kv_qk_norm_rope_backward where it is asked for gradients of weights. */
+int64_t kv_qk_norm_rope_backward_workspace(int B, int Hq, int Hkv, int T, int D, int dtype);
+
+/* dq, dk and, where the pointers are not NULL, the gradients of the weights (in the weights' type) from those of q_out and k_out. */
+int kv_qk_norm_rope_backward(const void* q, const void* k, const void* d_q_out, const void* d_k_out,
+                             const float* cos, const float* sin, int64_t cos_stride, int64_t sin_stride,
+                             const void* q_weight, const void* k_weight, int weights_f32,
+                             const int32_t* lens, int64_t lens_stride, const int32_t* positions, const int64_t* position_strides,
+                             void* dq, void* dk, void* dq_weight, void* dk_weight, void* workspace, int64_t workspace_bytes,
+                             const int64_t* q_strides, const int64_t* k_strides, const int64_t* dq_out_strides, const int64_t* dk_out_strides,
+                             int B, int Hq, int Hkv, int T, int D, int rot, int table_rows, int interleaved, float eps, int dtype, void* stream);
+
+/* kv_paged_append with norms and rotation on the way: q turned into q_out (contiguous, zeros from new_lens[b] on), k turned into the pages, v as it
+ * is.  The position of a token's angles is positions[b][i], or where the token goes if positions is NULL; a token whose position the table of
+ * angles does not have is left out of the pages, and its q_out is 0. */
+int kv_paged_append_rope(const void* q, const void* k, const void* v, void* q_out, void* k_pages, void* v_pages,
+                         const int32_t* page_table, int64_t table_stride, const int32_t* lens, int64_t lens_stride,
+                         const int32_t* new_lens, int64_t new_lens_stride,
+                         const float* cos, const float* sin, int64_t cos_stride, int64_t sin_stride,
+                         const void* q_weight, const void* k_weight, int weights_f32,
+                         const int32_t* positions, const int64_t* position_strides,
+                         const int64_t* q_strides, const int64_t* k_strides, const int64_t* v_strides,
+                         const int64_t* k_page_strides, const int64_t* v_page_strides,
+                         int B, int Hq, int Hkv, int T, int D, int num_pages, int page_size, int width,
+                         int rot, int table_rows, int interleaved, float eps, int dtype, void* stream);
 
 /* Human-readable text for a return code of the functions above (static storage). */
 const char* kv_error_string(int code);

@@ -1,45 +1,13 @@
 // extern "C" surface of libkv_attention.so: argument checks, workspace layout, parameter packing and dispatch on the element
 // type.  See include/kv_attention.h for the contract.
 #include "kv_append.h"
+#include "kv_check.h"
 #include "kv_launch.h"
 
 using namespace kv;
 
 namespace {
 
-constexpr float kLog2e = 1.4426950408889634f;
-
-int elem_size(int dtype) { return dtype == 0 ? 4 : 2; }
-
-int check_sizes(int B, int Hq, int Hkv, int D, int dtype) {
-  if (dtype < 0 || dtype > 2) return KV_ERR_DTYPE;
-  if (D != 16 && D != 32 && D != 64 && D != 128 && D != 256) return KV_ERR_HEAD_DIM;
-  if (B < 0 || Hq < 0 || Hkv < 0 || (Hkv == 0) != (Hq == 0) || (Hkv > 0 && Hq % Hkv != 0)) return KV_ERR_ARG;
-  return KV_OK;
-}
-// n rows; offsets32: addressed with 32-bit byte offsets from the first one
-int check_layout(const void* p, const int64_t* s, int dtype, int64_t n, bool offsets32) {
-  if (!p || !s) return KV_ERR_ARG;
-  const int64_t es = elem_size(dtype), vec = 16 / es;
-  if (s[3] != 1 || (reinterpret_cast<uintptr_t>(p) & 15u)) return KV_ERR_LAYOUT;
-  for (int i = 0; i < 3; ++i)
-    if (s[i] % vec != 0 || s[i] < 0) return KV_ERR_LAYOUT;
-  if (s[2] == 0 && n > 1) return KV_ERR_LAYOUT;
-  if (offsets32 && s[2] > ((int64_t(1) << 32) - 1) / es / (n + 1024)) return KV_ERR_TOO_LARGE;
-  return KV_OK;
-}
-// Times log2(e) it has to be a number of float32.
-int check_scale(float sm_scale) { return fabsf(sm_scale) <= 0x1p127f ? KV_OK : KV_ERR_ARG; }
-int check_out(const void* p) { return !p ? KV_ERR_ARG : (reinterpret_cast<uintptr_t>(p) & 15u) ? KV_ERR_LAYOUT : KV_OK; }
-
-template <typename F> int by_dtype(int dtype, F&& f) {
-  switch (dtype) {
-    case 0: return f(float{});
-    case 1: return f(_Float16{});
-    case 2: return f(__bf16{});
-  }
-  return KV_ERR_DTYPE;
-}
 #define KV_LAUNCH(fn, p)                                                     \
   by_dtype(dtype, [&](auto tag) {                                            \
     using E = decltype(tag);                                                 \
@@ -124,11 +92,6 @@ int plan_cross(CrossPlan& c, int B, int Hq, int Hkv, int Tq, int Tk, int D, int 
 }
 // The rows of one head within 32-bit byte offsets: what the hand-scheduled kernels need of q and d_o.
 bool rows_fit(const int64_t* s, int64_t n, int dtype) { return s[2] <= ((int64_t(1) << 32) - 1) / elem_size(dtype) / (n + 1024); }
-int check_workspace(void* workspace, int64_t have, int64_t need) {
-  if (need == 0) return KV_OK;
-  if (!workspace || have < need) return KV_ERR_WORKSPACE;
-  return (reinterpret_cast<uintptr_t>(workspace) & 15u) ? KV_ERR_LAYOUT : KV_OK;
-}
 
 // The hand-scheduled forward and dQ: a workgroup owns LONG_ROWS queries of one head; the heads of a key head follow each other.
 template <typename P> void long_sides(P& p, int B, int Hq, int Hkv, int Tq, int Tk) {
@@ -182,6 +145,30 @@ template <typename P> JoinParams join_params(const P& p, int max_len, int splits
   j.by_rows = chunk_div(map.rows());
   j.by_heads = chunk_div(map.Hkv);
   return j;
+}
+
+// The rows kernel's parameters, without windows; width 0: no page can be there.
+RowsParams paged_rows(const PagedPlan& c, const void* q, const void* k_pages, const void* v_pages, const int32_t* page_table, int64_t table_stride,
+                      const int32_t* lens, int64_t lens_stride, const int32_t* new_lens, int64_t new_lens_stride, void* o, float* lse,
+                      void* workspace, const int64_t* qs, const int64_t* ks, const int64_t* vs, int B, int Hq, int Hkv, int T, int D,
+                      int num_pages, int page_size, int width, float sm_scale) {
+  RowsParams p{};
+  p.q = q; p.k = k_pages; p.v = v_pages; p.o = o; p.lse = lse;
+  p.lens = lens; p.q_lens = new_lens; p.lens_stride = lens_stride; p.q_lens_stride = new_lens_stride;
+  p.q_sb = qs[0]; p.q_sh = qs[1]; p.q_st = qs[2];
+  p.map = row_map(Hkv, Hq / Hkv, T); p.B = B; p.scale_log2e = sm_scale * kLog2e;
+  p.page = page_size; p.by_page = chunk_div(page_size);
+  if (width > 0) {
+    p.k_sp = ks[0]; p.k_sh = ks[1]; p.k_st = ks[2];
+    p.v_sp = vs[0]; p.v_sh = vs[1]; p.v_st = vs[2];
+    p.table = page_table; p.table_sb = table_stride; p.width = width; p.num_pages = num_pages;
+    p.max_len = width * page_size;
+  }
+  p.splits = c.splits; p.share = c.share; p.row_tiles = (int)c.row_tiles;
+  p.by_pairs = chunk_div((int)c.nbh); p.by_row_tiles = chunk_div(p.row_tiles); p.by_heads = chunk_div(Hkv);
+  p.part_o = (float*)workspace;
+  p.part_ml = p.part_o + c.splits * c.nbh * c.rows * D;
+  return p;
 }
 
 }  // namespace
@@ -399,32 +386,51 @@ int kv_paged_forward(const void* q, const void* k_pages, const void* v_pages, co
   }
   if (int rc = check_out(o)) return rc;
   if (int rc = check_workspace(workspace, workspace_bytes, c.bytes)) return rc;
-  RowsParams p{};
-  p.q = q; p.k = k_pages; p.v = v_pages; p.o = o; p.lse = lse;
-  p.lens = lens; p.q_lens = new_lens; p.lens_stride = lens_stride; p.q_lens_stride = new_lens_stride;
-  p.q_sb = qs[0]; p.q_sh = qs[1]; p.q_st = qs[2];
-  p.map = row_map(Hkv, Hq / Hkv, T); p.B = B; p.scale_log2e = sm_scale * kLog2e;
-  p.page = page_size; p.by_page = chunk_div(page_size);
-  if (!empty) {
-    p.k_sp = ks[0]; p.k_sh = ks[1]; p.k_st = ks[2];
-    p.v_sp = vs[0]; p.v_sh = vs[1]; p.v_st = vs[2];
-    p.table = page_table; p.table_sb = table_stride; p.width = width; p.num_pages = num_pages;
-    p.max_len = width * page_size;
-  }
+  RowsParams p = paged_rows(c, q, k_pages, v_pages, page_table, table_stride, lens, lens_stride, new_lens, new_lens_stride, o, lse, workspace,
+                            qs, ks, vs, B, Hq, Hkv, T, D, empty ? 0 : num_pages, page_size, empty ? 0 : width, sm_scale);
   // chunks matter below the longest length only
   const int most = width * page_size;
   p.win.C = std::max(1, std::min(context_size, most));
   p.win.R = std::min(back_contexts, most);
   p.win.cdiv = chunk_div(p.win.C);
-  p.splits = c.splits; p.share = c.share; p.row_tiles = (int)c.row_tiles;
-  p.by_pairs = chunk_div((int)c.nbh); p.by_row_tiles = chunk_div(p.row_tiles); p.by_heads = chunk_div(Hkv);
-  p.part_o = (float*)workspace;
-  p.part_ml = p.part_o + c.splits * c.nbh * c.rows * D;
   if (int rc = KV_LAUNCH(launch_rows_paged, p)) return rc;
   if (c.splits == 1) return KV_OK;
   JoinParams j = join_params(p, p.max_len, c.splits, c.share, 32);
   j.win = p.win;
   return KV_LAUNCH(launch_join, j);
+}
+
+int64_t kv_paged_tree_forward_workspace(int B, int Hq, int Hkv, int T, int D, int page_size, int width, int dtype) {
+  PagedPlan c;
+  if (int rc = plan_paged(c, B, Hq, Hkv, T, D, page_size, width, 1, 0x7fffffff, dtype)) return rc;
+  return c.bytes;
+}
+
+int kv_paged_tree_forward(const void* q, const void* k_pages, const void* v_pages, const int32_t* page_table, int64_t table_stride,
+                          const int32_t* lens, int64_t lens_stride, const int32_t* new_lens, int64_t new_lens_stride, const void* tree,
+                          const int64_t* ts, void* o, float* lse, void* workspace, int64_t workspace_bytes, const int64_t* qs, const int64_t* ks,
+                          const int64_t* vs, int B, int Hq, int Hkv, int T, int D, int num_pages, int page_size, int width, float sm_scale,
+                          int dtype, void* stream) {
+  PagedPlan c;
+  if (int rc = plan_paged(c, B, Hq, Hkv, T, D, page_size, width, 1, 0x7fffffff, dtype)) return rc;
+  if (num_pages < 0) return KV_ERR_ARG;
+  if (int rc = check_scale(sm_scale)) return rc;
+  if (B == 0 || Hq == 0 || T == 0) return KV_OK;
+  if (int rc = check_layout(q, qs, dtype, T, false)) return rc;
+  if (!lens || !tree || !ts) return KV_ERR_ARG;
+  const bool empty = num_pages == 0 || width == 0;   // no page can be there: no key is seen
+  if (!empty) {
+    if (!page_table) return KV_ERR_ARG;
+    if (int rc = check_layout(k_pages, ks, dtype, page_size, false)) return rc;
+    if (int rc = check_layout(v_pages, vs, dtype, page_size, false)) return rc;
+  }
+  if (int rc = check_out(o)) return rc;
+  if (int rc = check_workspace(workspace, workspace_bytes, c.bytes)) return rc;
+  RowsParams p = paged_rows(c, q, k_pages, v_pages, page_table, table_stride, lens, lens_stride, new_lens, new_lens_stride, o, lse, workspace,
+                            qs, ks, vs, B, Hq, Hkv, T, D, empty ? 0 : num_pages, page_size, empty ? 0 : width, sm_scale);
+  p.tree = Tree{(const uint8_t*)tree, ts[0], ts[1], ts[2]};
+  if (int rc = KV_LAUNCH(launch_rows_tree, p)) return rc;
+  return c.splits > 1 ? KV_LAUNCH(launch_join, join_params(p, p.max_len, c.splits, c.share, 32)) : KV_OK;
 }
 
 int kv_paged_append(const void* k, const void* v, void* k_pages, void* v_pages, const int32_t* page_table, int64_t table_stride,
@@ -458,6 +464,34 @@ int kv_paged_append(const void* k, const void* v, void* k_pages, void* v_pages, 
   p.by_chunks = chunk_div(p.chunks); p.by_tokens = chunk_div(T); p.by_heads = chunk_div(H); p.by_page = chunk_div(page_size);
   const bool streaming = p.total * 32 > (int64_t(32) << 20);   // more than the L2s of all XCDs hold
   (streaming ? append_kernel<true> : append_kernel<false>)<<<dim3((unsigned)ceil_div(p.total, 256)), dim3(256), 0, (hipStream_t)stream>>>(p);
+  return (int)hipGetLastError();
+}
+
+int kv_paged_keep(void* k_pages, void* v_pages, const int32_t* page_table, int64_t table_stride, const int32_t* first, int64_t first_stride,
+                  const int32_t* kept, const int64_t* kept_strides, const int64_t* kps, const int64_t* vps, int B, int H, int M, int D,
+                  int num_pages, int page_size, int width, int dtype, void* stream) {
+  if (int rc = check_sizes(B, H, H, D, dtype)) return rc;
+  if (M < 0 || num_pages < 0 || page_size < 1 || width < 0) return KV_ERR_ARG;
+  if ((int64_t)width * page_size > (int64_t(1) << 30)) return KV_ERR_TOO_LARGE;
+  if (B == 0 || H == 0 || M == 0 || num_pages == 0 || width == 0) return KV_OK;
+  if (int rc = check_layout(k_pages, kps, dtype, page_size, false)) return rc;
+  if (int rc = check_layout(v_pages, vps, dtype, page_size, false)) return rc;
+  if (!first || !kept || !kept_strides || !page_table) return KV_ERR_ARG;
+  for (const int64_t* s : {kps, vps})   // each place of the cache its own
+    if ((s[0] == 0 && num_pages > 1) || (s[1] == 0 && H > 1)) return KV_ERR_LAYOUT;
+  const int64_t es = elem_size(dtype);
+  KeepParams p{};
+  p.k_pages = (char*)k_pages; p.v_pages = (char*)v_pages;
+  p.first = first; p.kept = kept; p.table = page_table;
+  p.first_stride = first_stride; p.kept_sb = kept_strides[0]; p.kept_si = kept_strides[1]; p.table_sb = table_stride;
+  p.kp_sp = kps[0] * es; p.kp_sh = kps[1] * es; p.kp_st = kps[2] * es;
+  p.vp_sp = vps[0] * es; p.vp_sh = vps[1] * es; p.vp_st = vps[2] * es;
+  p.B = B; p.H = H; p.M = M; p.width = width; p.num_pages = num_pages; p.page = page_size;
+  p.chunks = (int)(D * es / 16);
+  if ((int64_t)B * H > kMostCount / p.chunks) return KV_ERR_TOO_LARGE;
+  p.total = (int64_t)B * H * p.chunks;
+  p.by_chunks = chunk_div(p.chunks); p.by_heads = chunk_div(H); p.by_page = chunk_div(page_size);
+  keep_kernel<<<dim3((unsigned)ceil_div(p.total, 256), 2), dim3(256), 0, (hipStream_t)stream>>>(p);
   return (int)hipGetLastError();
 }
 

@@ -1,4 +1,4 @@
-// The keys and values of new tokens into a cache in pages.
+// The keys and values of new tokens into a cache in pages, and accepted ones to the front of them.
 #pragma once
 #include "kv_common.h"
 
@@ -44,6 +44,58 @@ template <bool STREAMING> __global__ __launch_bounds__(256) void append_kernel(c
   } else {
     *reinterpret_cast<u32x4*>(kp) = kx;
     *reinterpret_cast<u32x4*>(vp) = vx;
+  }
+}
+
+// ---- accepted tokens --------------------------------------------------------------------------------------------------
+// K and V of position first[b] + kept[b][i] to first[b] + i, for i = 0, 1, ... as long as the entries are not negative and ascend.  Bytes only.  An
+// entry is never below its place, so what is read for one place is not written by a place before it: a thread goes through
+// the places of one sixteen bytes of one head, a few loads ahead of its stores, and needs no other thread.
+struct KeepParams {
+  char *k_pages, *v_pages;
+  const int32_t *first, *kept, *table;
+  int64_t first_stride, kept_sb, kept_si, table_sb;
+  int64_t kp_sp, kp_sh, kp_st, vp_sp, vp_sh, vp_st;   // bytes
+  int B, H, M, width, num_pages, page, chunks;
+  int64_t total;          // B * H * chunks of a row
+  ChunkDiv by_chunks, by_heads, by_page;
+};
+static __global__ __launch_bounds__(256) void keep_kernel(const KeepParams p) {
+  const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (id >= p.total) return;
+  const bool values = blockIdx.y == 1;
+  const int bh = div_by((int)id, p.by_chunks), chunk = (int)id - bh * p.chunks, b = div_by(bh, p.by_heads), hd = bh - b * p.H;
+  char* const base = values ? p.v_pages + hd * p.vp_sh + chunk * 16 : p.k_pages + hd * p.kp_sh + chunk * 16;
+  const int64_t sp = values ? p.vp_sp : p.kp_sp, st = values ? p.vp_st : p.kp_st;
+  const int64_t first = p.first[b * p.first_stride], most = (int64_t)p.width * p.page;
+  auto place = [&](int64_t at) -> char* {   // or null: it is not there
+    if (at < 0 || at >= most) return nullptr;
+    const int entry = div_by((int)at, p.by_page);
+    const int32_t page = p.table[b * p.table_sb + entry];
+    return (uint32_t)page < (uint32_t)p.num_pages ? base + page * sp + ((int)at - entry * p.page) * st : nullptr;
+  };
+  constexpr int U = 4;
+  int before = -1;
+  for (int i0 = 0; i0 < p.M; i0 += U) {
+    u32x4 x[U];
+    char* to[U];
+    int n = 0;             // places of these that are on the path
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      to[u] = nullptr;
+      if (n < u || i0 + u >= p.M) continue;
+      const int32_t j = p.kept[b * p.kept_sb + (i0 + u) * p.kept_si];
+      if (j <= before) continue;
+      before = j, n = u + 1;
+      if (j == i0 + u) continue;
+      const char* const from = place(first + j);
+      to[u] = from ? place(first + i0 + u) : nullptr;
+      if (to[u]) x[u] = *reinterpret_cast<const u32x4*>(from);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (to[u]) *reinterpret_cast<u32x4*>(to[u]) = x[u];
+    if (n < U) return;
   }
 }
 

@@ -98,33 +98,34 @@ template <> int launch_cross_dkdv<ElemT, KV_DGROUP>(const BwdParams& p, int D, h
     }
   });
 }
-#elif KV_KIND == 3
-template <int D, int NW, bool PAGED> static int launch_rows_shape(const RowsParams& p, int64_t blocks, hipStream_t st) {
+#elif KV_KIND == 3 || KV_KIND == 5
+template <int D, int NW, bool PAGED, bool TREE> static int launch_rows_shape(const RowsParams& p, int64_t blocks, hipStream_t st) {
   constexpr int row_bytes = D * (int)sizeof(ElemT), lds = RowsShape<ElemT, D, NW>::bytes(PAGED), places = CUS * (163840 / lds);
   // by length where there are many workgroups: only the waves that many workgroups have
   if constexpr (row_bytes >= 128 && NW == rows_waves(row_bytes, sizeof(ElemT) == 4, 2 * CUS, 1)) {
     static_assert(2 * places >= 2 * CUS, "many in the sense of rows_waves");
     static LdsLimit state;
     if (p.splits > 1 && by_length(p.B, p.row_tiles, row_bytes) && blocks >= 2 * places)
-      return launch(rows_by_length_kernel<ElemT, D, NW, PAGED>, places, NW * 64, lds, state, p, st);
+      return launch(rows_by_length_kernel<ElemT, D, NW, PAGED, TREE>, places, NW * 64, lds, state, p, st);
   }
   static LdsLimit state;
-  return launch(rows_kernel<ElemT, D, NW, PAGED>, blocks, NW * 64, lds, state, p, st);
+  return launch(rows_kernel<ElemT, D, NW, PAGED, TREE>, blocks, NW * 64, lds, state, p, st);
 }
-template <bool PAGED> static int launch_rows_any(const RowsParams& p, int D, hipStream_t st) {
+template <bool PAGED, bool TREE> static int launch_rows_any(const RowsParams& p, int D, hipStream_t st) {
   return by_head_dim(D, [&](auto d) {
     constexpr int DD = decltype(d)::value, ROW = DD * (int)sizeof(ElemT);
     const int64_t blocks = (int64_t)p.B * p.map.Hkv * p.row_tiles * p.splits;
     const int waves = rows_waves(ROW, sizeof(ElemT) == 4, blocks, p.share);
     if constexpr (ROW == 128)
-      if (waves == 8) return launch_rows_shape<DD, 8, PAGED>(p, blocks, st);
+      if (waves == 8) return launch_rows_shape<DD, 8, PAGED, TREE>(p, blocks, st);
     if constexpr (ROW == 256 && sizeof(ElemT) == 2)
-      if (waves == 2) return launch_rows_shape<DD, 2, PAGED>(p, blocks, st);
-    return launch_rows_shape<DD, ROW <= 256 ? 4 : ROW == 512 ? 2 : 1, PAGED>(p, blocks, st);
+      if (waves == 2) return launch_rows_shape<DD, 2, PAGED, TREE>(p, blocks, st);
+    return launch_rows_shape<DD, ROW <= 256 ? 4 : ROW == 512 ? 2 : 1, PAGED, TREE>(p, blocks, st);
   });
 }
-template <> int launch_rows<ElemT, KV_DGROUP>(const RowsParams& p, int D, hipStream_t st) { return launch_rows_any<false>(p, D, st); }
-template <> int launch_rows_paged<ElemT, KV_DGROUP>(const RowsParams& p, int D, hipStream_t st) { return launch_rows_any<true>(p, D, st); }
+#if KV_KIND == 3
+template <> int launch_rows<ElemT, KV_DGROUP>(const RowsParams& p, int D, hipStream_t st) { return launch_rows_any<false, false>(p, D, st); }
+template <> int launch_rows_paged<ElemT, KV_DGROUP>(const RowsParams& p, int D, hipStream_t st) { return launch_rows_any<true, false>(p, D, st); }
 template <> int launch_join<ElemT, KV_DGROUP>(const JoinParams& p, int D, hipStream_t st) {
   return by_head_dim(D, [&](auto d) {
     constexpr int DD = decltype(d)::value;
@@ -144,6 +145,9 @@ template <> int launch_sum<ElemT, KV_DGROUP>(const SumParams& p, int D, hipStrea
     return launch(sum_kernel<ElemT, DD>, ceil_div((int64_t)p.B * p.Hkv * rows, 256 / (DD / 4)), 256, 0, none, p, st, queries + 2 * keys);
   });
 }
+#else
+template <> int launch_rows_tree<ElemT, KV_DGROUP>(const RowsParams& p, int D, hipStream_t st) { return launch_rows_any<true, true>(p, D, st); }
+#endif
 #elif KV_KIND == 4 && !defined(SA_NO_ASM_KERNELS)
 constexpr size_t long_stages(int n, size_t tile_rows) { return n * 2 * tile_rows * 128 * sizeof(ElemT); }
 static int64_t long_blocks(const sa::TileMap& m) { return (int64_t)m.nbh * m.n_tiles; }

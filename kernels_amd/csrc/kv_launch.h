@@ -18,6 +18,7 @@ template <typename T, int DGROUP> int launch_cross_dq(const BwdParams& p, int D,
 template <typename T, int DGROUP> int launch_cross_dkdv(const BwdParams& p, int D, hipStream_t st);
 template <typename T, int DGROUP> int launch_rows(const RowsParams& p, int D, hipStream_t st);
 template <typename T, int DGROUP> int launch_rows_paged(const RowsParams& p, int D, hipStream_t st);
+template <typename T, int DGROUP> int launch_rows_tree(const RowsParams& p, int D, hipStream_t st);
 template <typename T, int DGROUP> int launch_join(const JoinParams& p, int D, hipStream_t st);
 template <typename T, int DGROUP> int launch_sum(const SumParams& p, int D, hipStream_t st);
 

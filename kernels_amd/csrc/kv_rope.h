@@ -1,0 +1,369 @@
+// What comes before attention: norms of queries and keys for each head, the rotation of their channels by position, and both on the way
+// into a cache in pages.
+//
+// A row is one token of one head, x of D channels.  y = x r w with r = 1 / sqrt(mean(x^2) + eps) and the weights w (r = w = 1 without norms);
+// the first `rot` channels of y go in pairs (a, b), which are turned by the angle of the token's position: (a c - b s, b c + a s).  Backward,
+// with g turned back by the angle (h = g w): dx = r (h - x r mean(h x r)) and dw = the sum over rows of g x r.
+//
+// Bound by memory: every row is read once and written once (twice read, the gradient and x, in the backward).  Two chunks of sixteen
+// bytes to a lane, so that both sides of a pair are a lane's own, whether pairs are neighbours or halves; what lies past `rot`
+// follows in neighbouring chunks.  The lanes of a row add up its squares among themselves.  A group of lanes keeps its token and goes
+// through heads, so that cosines, sines (64 bytes of float32 to 32 of x) and weights are fetched once for several rows.
+#pragma once
+#include "kv_common.h"
+
+namespace kv {
+
+// How D channels lie over lanes; 256 threads work on GROUPS tokens.
+template <typename T, int D> struct RopeLanes {
+  static constexpr int V = Elem<T>::VEC, LANES = D / (2 * V), GROUPS = 256 / LANES;
+};
+
+struct RopeSide {          // q or k
+  const void *x, *g;       // g: the gradient of the turned rows (backward)
+  void* out;               // contiguous [B, heads, T, D]: the turned rows, or the gradient of x
+  const void* weight;      // [D] or null
+  int64_t sb, sh, st, g_sb, g_sh, g_st;
+  int heads;
+};
+struct RopeTable {
+  const float *cos, *sin;  // [rows, rot / 2]
+  int64_t cos_st, sin_st;
+  int rows, rot;
+};
+struct RopeParams {
+  RopeSide q, k;
+  RopeTable table;
+  const int32_t *lens, *positions;   // or null: all of T, and 0, 1, ...
+  int64_t lens_stride, pos_sb, pos_st;
+  int B, T;
+  float eps;               // 0: no norms
+  bool weights_f32;
+  int chunk, q_chunks;     // heads that a workgroup goes through; layers of the grid that are q's
+  ChunkDiv by_tokens;
+  float* part;             // backward: [layers, gridDim.x, D] sums of dw, or null
+};
+
+// Elements of a lane's two chunks: offsets a and b, V each.
+template <typename T, int D, bool INTER> struct RopeLane {
+  static constexpr int V = RopeLanes<T, D>::V;
+  int a, b, pair;          // pair: of its V cosines and sines
+  bool turned;
+  SA_DEV RopeLane(int lane, int rot) {
+    pair = V * lane;
+    turned = 2 * pair < rot;
+    a = INTER || !turned ? 2 * pair : pair;
+    b = INTER || !turned ? a + V : rot / 2 + pair;
+  }
+};
+template <typename T> SA_DEV void unpack(float* x, const T* from) {
+  const auto f = *reinterpret_cast<const typename Elem<T>::Frag*>(from);
+#pragma unroll
+  for (int e = 0; e < Elem<T>::VEC; ++e) x[e] = (float)f[e];
+}
+template <typename T, bool STREAMING> SA_DEV void pack(T* to, const float* x) {
+  typename Elem<T>::Frag f;
+#pragma unroll
+  for (int e = 0; e < Elem<T>::VEC; ++e) f[e] = (T)x[e];
+  if constexpr (STREAMING) sa::store_streaming(to, __builtin_bit_cast(u32x4, f));
+  else *reinterpret_cast<typename Elem<T>::Frag*>(to) = f;
+}
+template <int V> SA_DEV void load_floats(float (&x)[V], const float* from) {
+#pragma unroll
+  for (int e = 0; e < V; e += 4) {
+    const f32x4 f = *reinterpret_cast<const f32x4*>(from + e);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[e + i] = f[i];
+  }
+}
+// The weights of a lane's channels, in their type or in float32.
+template <typename T, int V> SA_DEV void load_weights(float (&w)[2 * V], const void* weight, bool f32, int a, int b) {
+#pragma unroll
+  for (int e = 0; e < 2 * V; ++e) w[e] = 1.0f;
+  if (!weight) return;
+  if (f32) {
+    const float* p = reinterpret_cast<const float*>(weight);
+    load_floats<V>(reinterpret_cast<float(&)[V]>(w[0]), p + a);
+    load_floats<V>(reinterpret_cast<float(&)[V]>(w[V]), p + b);
+  } else {
+    unpack<T>(w, reinterpret_cast<const T*>(weight) + a);
+    unpack<T>(w + V, reinterpret_cast<const T*>(weight) + b);
+  }
+}
+// The sum over the LANES lanes of a row, in all of them.
+template <int LANES> SA_DEV float row_sum(float x) {
+  auto add = [&](auto ctrl) { x += __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), decltype(ctrl)::value, 0xf, 0xf, false)); };
+  if constexpr (LANES >= 2) add(std::integral_constant<int, 0xB1>{});    // the neighbour
+  if constexpr (LANES >= 4) add(std::integral_constant<int, 0x4E>{});    // the other pair of four
+  if constexpr (LANES >= 8) add(std::integral_constant<int, 0x141>{});   // eight, mirrored
+  if constexpr (LANES >= 16) add(std::integral_constant<int, 0x140>{});  // sixteen, mirrored
+  if constexpr (LANES >= 32) x += __shfl_xor(x, 16);
+  return x;
+}
+template <bool INTER, int V> SA_DEV void turn(float (&x)[2 * V], const float (&c)[V], const float (&s)[V]) {
+#pragma unroll
+  for (int e = 0; e < V; ++e) {
+    const int i = INTER ? 2 * e : e, j = INTER ? 2 * e + 1 : V + e;
+    const float a = x[i], b = x[j];
+    x[i] = a * c[e] - b * s[e];
+    x[j] = b * c[e] + a * s[e];
+  }
+}
+// x -> the turned row
+template <int D, int LANES, bool INTER, int V>
+SA_DEV void norm_and_turn(float (&x)[2 * V], const float (&w)[2 * V], const float (&c)[V], const float (&s)[V], bool turned, float eps) {
+  if (eps > 0.0f) {
+    float sum = 0.0f;
+#pragma unroll
+    for (int e = 0; e < 2 * V; ++e) sum += x[e] * x[e];
+    const float r = rsqrtf(row_sum<LANES>(sum) * (1.0f / D) + eps);
+#pragma unroll
+    for (int e = 0; e < 2 * V; ++e) x[e] *= r * w[e];
+  }
+  if (turned) turn<INTER>(x, c, s);
+}
+
+// The token of a group of lanes: where it is, and the row of the table.
+struct RopeToken {
+  int b, t, at;
+  bool live;               // not padding, and at a position that the table has
+};
+SA_DEV RopeToken rope_token(const RopeParams& p, int token) {
+  RopeToken x;
+  x.b = div_by(token, p.by_tokens), x.t = token - x.b * p.T;
+  x.at = p.positions ? p.positions[x.b * p.pos_sb + x.t * p.pos_st] : x.t;
+  x.live = x.t < clamped_length(p.lens, p.lens_stride, x.b, p.T) && (uint32_t)x.at < (uint32_t)p.table.rows;
+  return x;
+}
+template <int V> SA_DEV void load_angles(float (&c)[V], float (&s)[V], const RopeTable& table, int at, int pair) {
+  load_floats<V>(c, table.cos + at * table.cos_st + pair);
+  load_floats<V>(s, table.sin + at * table.sin_st + pair);
+}
+
+template <typename T, int D, bool INTER> __global__ __launch_bounds__(256) void rope_kernel(const RopeParams p) {
+  using L = RopeLanes<T, D>;
+  constexpr int V = L::V, U = 4;   // rows on their way together
+  const RopeLane<T, D, INTER> lane(threadIdx.x % L::LANES, p.table.rot);
+  const bool keys = (int)blockIdx.y >= p.q_chunks;
+  const RopeSide& side = keys ? p.k : p.q;
+  const int h0 = ((int)blockIdx.y - (keys ? p.q_chunks : 0)) * p.chunk, h1 = h0 + p.chunk < side.heads ? h0 + p.chunk : side.heads;
+  const int64_t step = (int64_t)gridDim.x * L::GROUPS, tokens = (int64_t)p.B * p.T;
+  float w[2 * V];
+  load_weights<T, V>(w, side.weight, p.weights_f32, lane.a, lane.b);
+  for (int64_t id = (int64_t)blockIdx.x * L::GROUPS + threadIdx.x / L::LANES; id < tokens; id += step) {
+    const RopeToken token = rope_token(p, (int)id);
+    const T* x = reinterpret_cast<const T*>(side.x) + token.b * side.sb + token.t * side.st;
+    T* out = reinterpret_cast<T*>(side.out) + ((int64_t)token.b * side.heads * p.T + token.t) * D;
+    float c[V], s[V];
+    if (token.live && lane.turned) load_angles<V>(c, s, p.table, token.at, lane.pair);
+    for (int h = h0; h < h1; h += U) {
+      float rows[U][2 * V];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int head = h + u < h1 ? h + u : h1 - 1;
+        if (token.live) {
+          unpack<T>(rows[u], x + head * side.sh + lane.a);
+          unpack<T>(rows[u] + V, x + head * side.sh + lane.b);
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (h + u >= h1) break;
+        if (token.live) norm_and_turn<D, L::LANES, INTER, V>(rows[u], w, c, s, lane.turned, p.eps);
+        else
+#pragma unroll
+          for (int e = 0; e < 2 * V; ++e) rows[u][e] = 0.0f;
+        T* const to = out + (int64_t)(h + u) * p.T * D;
+        pack<T, false>(to + lane.a, rows[u]);
+        pack<T, false>(to + lane.b, rows[u] + V);
+      }
+    }
+  }
+}
+
+// Gradients of x, and in p.part each workgroup's sums of those of the weights, in the order of its tokens and then of its groups of lanes.
+template <typename T, int D, bool INTER> __global__ __launch_bounds__(256) void rope_backward_kernel(const RopeParams p) {
+  using L = RopeLanes<T, D>;
+  constexpr int V = L::V, U = 2;
+  __shared__ __attribute__((aligned(16))) float sums[L::GROUPS * D];
+  const RopeLane<T, D, INTER> lane(threadIdx.x % L::LANES, p.table.rot);
+  const bool keys = (int)blockIdx.y >= p.q_chunks, norm = p.eps > 0.0f;
+  const RopeSide& side = keys ? p.k : p.q;
+  const int h0 = ((int)blockIdx.y - (keys ? p.q_chunks : 0)) * p.chunk, h1 = h0 + p.chunk < side.heads ? h0 + p.chunk : side.heads;
+  const int64_t step = (int64_t)gridDim.x * L::GROUPS, tokens = (int64_t)p.B * p.T;
+  float w[2 * V], dw[2 * V];
+  load_weights<T, V>(w, side.weight, p.weights_f32, lane.a, lane.b);
+#pragma unroll
+  for (int e = 0; e < 2 * V; ++e) dw[e] = 0.0f;
+  for (int64_t id = (int64_t)blockIdx.x * L::GROUPS + threadIdx.x / L::LANES; id < tokens; id += step) {
+    const RopeToken token = rope_token(p, (int)id);
+    const T* x = reinterpret_cast<const T*>(side.x) + token.b * side.sb + token.t * side.st;
+    const T* g = reinterpret_cast<const T*>(side.g) + token.b * side.g_sb + token.t * side.g_st;
+    T* out = reinterpret_cast<T*>(side.out) + ((int64_t)token.b * side.heads * p.T + token.t) * D;
+    float c[V], s[V];
+    if (token.live && lane.turned) {
+      load_angles<V>(c, s, p.table, token.at, lane.pair);
+#pragma unroll
+      for (int e = 0; e < V; ++e) s[e] = -s[e];
+    }
+    for (int h = h0; h < h1; h += U) {
+      float xs[U][2 * V], gs[U][2 * V];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int head = h + u < h1 ? h + u : h1 - 1;
+        if (token.live) {
+          unpack<T>(gs[u], g + head * side.g_sh + lane.a);
+          unpack<T>(gs[u] + V, g + head * side.g_sh + lane.b);
+          if (norm) {
+            unpack<T>(xs[u], x + head * side.sh + lane.a);
+            unpack<T>(xs[u] + V, x + head * side.sh + lane.b);
+          }
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (h + u >= h1) break;
+        if (token.live) {
+          if (lane.turned) turn<INTER>(gs[u], c, s);
+          if (norm) {
+            float squares = 0.0f, dot = 0.0f;
+#pragma unroll
+            for (int e = 0; e < 2 * V; ++e) squares += xs[u][e] * xs[u][e];
+            const float r = rsqrtf(row_sum<L::LANES>(squares) * (1.0f / D) + p.eps);
+#pragma unroll
+            for (int e = 0; e < 2 * V; ++e) {
+              xs[u][e] *= r;
+              dw[e] += gs[u][e] * xs[u][e];
+              gs[u][e] *= w[e];
+              dot += gs[u][e] * xs[u][e];
+            }
+            const float mean = row_sum<L::LANES>(dot) * (1.0f / D);
+#pragma unroll
+            for (int e = 0; e < 2 * V; ++e) gs[u][e] = r * (gs[u][e] - xs[u][e] * mean);
+          }
+        } else {
+#pragma unroll
+          for (int e = 0; e < 2 * V; ++e) gs[u][e] = 0.0f;
+        }
+        T* const to = out + (int64_t)(h + u) * p.T * D;
+        pack<T, false>(to + lane.a, gs[u]);
+        pack<T, false>(to + lane.b, gs[u] + V);
+      }
+    }
+  }
+  if (!p.part) return;
+  float* const own = sums + threadIdx.x / L::LANES * D;
+#pragma unroll
+  for (int e = 0; e < V; ++e) own[lane.a + e] = dw[e], own[lane.b + e] = dw[V + e];
+  __syncthreads();
+  if (threadIdx.x < D) {
+    float sum = 0.0f;
+    for (int i = 0; i < L::GROUPS; ++i) sum += sums[i * D + threadIdx.x];
+    p.part[((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * D + threadIdx.x] = sum;
+  }
+}
+
+// The workgroups' sums, added up: sixteen channels of q's weights or k's to a workgroup.
+struct RopeSumParams {
+  const float* part;
+  void *dq, *dk;           // [D] or null
+  int q_parts, k_parts, D;
+  bool f32;
+};
+template <typename T> __global__ __launch_bounds__(256) void rope_sum_kernel(const RopeSumParams p) {
+  __shared__ __attribute__((aligned(16))) f32x4 sums[256];
+  const bool keys = blockIdx.y == 1;
+  void* const out = keys ? p.dk : p.dq;
+  if (!out) return;
+  const int n = keys ? p.k_parts : p.q_parts, d = (int)blockIdx.x * 16 + threadIdx.x % 4 * 4;
+  const float* part = p.part + (keys ? (int64_t)p.q_parts * p.D : 0) + d;
+  f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
+  for (int i = threadIdx.x / 4; i < n; i += 64) sum += *reinterpret_cast<const f32x4*>(part + (int64_t)i * p.D);
+  sums[threadIdx.x] = sum;
+  __syncthreads();
+  if (threadIdx.x >= 4) return;
+  for (int i = 1; i < 64; ++i) sum += sums[i * 4 + threadIdx.x];
+  if (p.f32) *reinterpret_cast<f32x4*>(reinterpret_cast<float*>(out) + d) = sum;
+  else sa::store4<T>(reinterpret_cast<T*>(out) + d, sum[0], sum[1], sum[2], sum[3]);
+}
+
+// ---- into the pages ---------------------------------------------------------------------------------------------------
+// Token i of n = new_lens[b] of sequence b goes to position lens[b] - n + i, its angle is that of its entry in `positions`, or of that position.  k is
+// turned and v as it is; q is turned into a tensor of its own.
+struct AppendRopeParams {
+  const void *q, *k, *v;
+  void *q_out, *k_pages, *v_pages;    // q_out contiguous [B, Hq, T, D]
+  const void *q_weight, *k_weight;
+  RopeTable table;
+  const int32_t *lens, *new_lens, *positions, *page_table;
+  int64_t lens_stride, new_lens_stride, pos_sb, pos_st, table_sb;
+  int64_t q_sb, q_sh, q_st, k_sb, k_sh, k_st, v_sb, v_sh, v_st;
+  int64_t kp_sp, kp_sh, kp_st, vp_sp, vp_sh, vp_st;
+  int B, Hq, Hkv, T, width, num_pages, page;
+  float eps;
+  bool weights_f32;
+  int chunk, q_chunks, k_chunks;      // layers of the grid: q's, k's, then v's
+  ChunkDiv by_tokens, by_page;
+};
+template <typename T, int D, bool INTER> __global__ __launch_bounds__(256) void append_rope_kernel(const AppendRopeParams p) {
+  using L = RopeLanes<T, D>;
+  constexpr int V = L::V, U = 4;
+  const int layer = blockIdx.y, kind = layer < p.q_chunks ? 0 : layer < p.q_chunks + p.k_chunks ? 1 : 2;
+  const RopeLane<T, D, INTER> lane(threadIdx.x % L::LANES, kind == 2 ? 0 : p.table.rot);
+  const int heads = kind == 0 ? p.Hq : p.Hkv, h0 = (layer - (kind == 0 ? 0 : kind == 1 ? p.q_chunks : p.q_chunks + p.k_chunks)) * p.chunk;
+  const int h1 = h0 + p.chunk < heads ? h0 + p.chunk : heads;
+  const T* const from = reinterpret_cast<const T*>(kind == 0 ? p.q : kind == 1 ? p.k : p.v);
+  const int64_t sb = kind == 0 ? p.q_sb : kind == 1 ? p.k_sb : p.v_sb, sh = kind == 0 ? p.q_sh : kind == 1 ? p.k_sh : p.v_sh;
+  const int64_t st = kind == 0 ? p.q_st : kind == 1 ? p.k_st : p.v_st;
+  const int64_t step = (int64_t)gridDim.x * L::GROUPS, tokens = (int64_t)p.B * p.T;
+  const float eps = kind == 2 ? 0.0f : p.eps;
+  float w[2 * V];
+  load_weights<T, V>(w, kind == 0 ? p.q_weight : kind == 1 ? p.k_weight : nullptr, p.weights_f32, lane.a, lane.b);
+  for (int64_t id = (int64_t)blockIdx.x * L::GROUPS + threadIdx.x / L::LANES; id < tokens; id += step) {
+    const int b = div_by((int)id, p.by_tokens), t = (int)id - b * p.T;
+    const int n = clamped_length(p.new_lens, p.new_lens_stride, b, p.T);
+    const int64_t place = (int64_t)p.lens[b * p.lens_stride] - n + t;
+    const int64_t at = p.positions ? p.positions[b * p.pos_sb + t * p.pos_st] : place;
+    const bool live = t < n && at >= 0 && at < p.table.rows;
+    T* to;
+    int64_t to_sh;
+    if (kind == 0) {
+      to = reinterpret_cast<T*>(p.q_out) + ((int64_t)b * heads * p.T + t) * D;
+      to_sh = (int64_t)p.T * D;
+    } else {
+      if (!live || place < 0 || place >= (int64_t)p.width * p.page) continue;
+      const int entry = div_by((int)place, p.by_page), slot = (int)place - entry * p.page;
+      const int32_t page = p.page_table[b * p.table_sb + entry];
+      if ((uint32_t)page >= (uint32_t)p.num_pages) continue;
+      to = kind == 1 ? reinterpret_cast<T*>(p.k_pages) + page * p.kp_sp + slot * p.kp_st : reinterpret_cast<T*>(p.v_pages) + page * p.vp_sp + slot * p.vp_st;
+      to_sh = kind == 1 ? p.kp_sh : p.vp_sh;
+    }
+    const T* x = from + b * sb + t * st;
+    float c[V], s[V];
+    if (live && lane.turned) load_angles<V>(c, s, p.table, (int)at, lane.pair);
+    for (int h = h0; h < h1; h += U) {
+      float rows[U][2 * V];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int head = h + u < h1 ? h + u : h1 - 1;
+        if (live) {
+          unpack<T>(rows[u], x + head * sh + lane.a);
+          unpack<T>(rows[u] + V, x + head * sh + lane.b);
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (h + u >= h1) break;
+        if (live) norm_and_turn<D, L::LANES, INTER, V>(rows[u], w, c, s, lane.turned, eps);
+        else
+#pragma unroll
+          for (int e = 0; e < 2 * V; ++e) rows[u][e] = 0.0f;
+        pack<T, false>(to + (h + u) * to_sh + lane.a, rows[u]);
+        pack<T, false>(to + (h + u) * to_sh + lane.b, rows[u] + V);
+      }
+    }
+  }
+}
+
+}  // namespace kv

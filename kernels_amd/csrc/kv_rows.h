@@ -41,6 +41,39 @@ SA_BOTH void tiles_seen(const Windows& w, const RowMap& map, int L, int tokens, 
   last = last > first ? last : first;
 }
 
+// Which of the new tokens each of them sees: tree[b][i][j], bytes.  What lies before them, all of them see.
+struct Tree {
+  const uint8_t* seen;
+  int64_t sb, si, sj;
+};
+// Of the 32 keys from k0 on, those that a lane's row sees, in the bits of sa::row_mask: token t of n new ones, the first of them at position base
+// (below 0: the sequence is shorter; a token before its beginning sees nothing).
+SA_DEV uint32_t tree_mask(const Tree& tree, int b, int t, int n, int base, int k0, int h) {
+  if (base + t < 0) return 0;
+  uint32_t mask = sa::row_mask(0, base - k0, h);
+  if (base >= k0 + 32) return mask;
+  const uint8_t* const row = tree.seen + b * tree.sb + t * tree.si;
+  uint32_t bits = 0;
+#pragma unroll
+  for (int e = 0; e < 16; ++e) {
+    const int u = k0 + sa::crow(e, h) - base, j = u < 0 ? 0 : u < n ? u : n - 1;
+    const bool sees = row[j * tree.sj] != 0 && u == j;
+    bits |= (sees ? 1u : 0u) << (8 * (e >> 2) + (e & 3));
+  }
+  return mask | bits;
+}
+// Those of the 32 keys that any of the wave's rows sees (not only those of the lane), in the order of the keys.
+SA_DEV uint32_t any_row(uint32_t mask) {
+  uint32_t seen = 0;
+#pragma unroll
+  for (int e = 0; e < 16; ++e) {
+    const uint64_t lanes = __builtin_amdgcn_ballot_w64((sa::keep_bits(mask, e)) != 0);
+    seen |= ((uint32_t)lanes != 0 ? 1u : 0u) << sa::crow(e, 0);
+    seen |= ((uint32_t)(lanes >> 32) != 0 ? 1u : 0u) << sa::crow(e, 1);
+  }
+  return seen;
+}
+
 struct RowsParams {
   const void *q, *k, *v;
   void* o;               // contiguous [B, Hq, T, D]
@@ -58,6 +91,7 @@ struct RowsParams {
   int width, num_pages, page;
   ChunkDiv by_page;
   Windows win;
+  Tree tree;             // of the kernels that go by one, in place of the windows
   // division of the work
   int splits, share;     // the most parts that the tiles of 32 keys of a row tile are divided into, and the most tiles of a part
   int row_tiles;
@@ -91,8 +125,9 @@ SA_DEV int wave_prefix_sum(int x) {
   return x;
 }
 
-// One part of the keys of 32 rows (r0 and following) of (b, hk).
-template <typename T, int D, int NW, bool PAGED>
+// One part of the keys of 32 rows (r0 and following) of (b, hk).  TREE: every row sees the keys before the new tokens, and of those the ones
+// that the tree says.
+template <typename T, int D, int NW, bool PAGED, bool TREE>
 SA_DEV void rows_part(const RowsParams& p, char* smem_raw, int b, int hk, int split, int r0) {
   using G = Geom<T, D>;
   using S = RowsShape<T, D, NW>;
@@ -119,7 +154,12 @@ SA_DEV void rows_part(const RowsParams& p, char* smem_raw, int b, int hk, int sp
   // windows: of this lane's row (padding has that of the last row), of all rows, of any row
   const int row = r0 + (c < used ? c : used - 1);
   int lo = 0, hi = L, lo_min = 0, lo_max = 0, hi_min = L, hi_max = L, first, last;
-  if constexpr (PAGED) {
+  int token = 0;   // of this lane's row
+  if constexpr (TREE) {
+    int ignored;
+    p.map.split(row, token, ignored);
+    hi_min = L - tokens;
+  } else if constexpr (PAGED) {
     window_of(p.win, p.map, L, tokens, row, lo, hi);
     window_of(p.win, p.map, L, tokens, r0, lo_min, hi_min);
     window_of(p.win, p.map, L, tokens, r0 + used - 1, lo_max, hi_max);
@@ -198,12 +238,18 @@ SA_DEV void rows_part(const RowsParams& p, char* smem_raw, int b, int hk, int sp
     const int k0 = tile_key(i);
     bool here = k0 + c >= lo_min && k0 + c < hi_max;   // seen by some row
     if constexpr (PAGED) here = here && present(entries[i % (2 * ST) * 64 + c]);
-    const uint32_t seen = (uint32_t)__builtin_amdgcn_ballot_w64(here);
+    uint32_t seen = (uint32_t)__builtin_amdgcn_ballot_w64(here);
     f32x16 s[1];
     clear(s);
     mul_rows<T, D>(s, keys, 0, qf, lane);
     if (seen != 0xFFFFFFFFu || k0 < lo_max || k0 + 32 > hi_min) {
-      const uint32_t mask = sa::row_mask(lo - k0, hi - k0, h) & (seen >> (4 * h));
+      uint32_t mask;
+      if constexpr (TREE) {
+        mask = tree_mask(p.tree, b, token, tokens, L - tokens, k0, h) & (seen >> (4 * h));
+        if (k0 + 32 > hi_min) seen = any_row(mask);
+      } else {
+        mask = sa::row_mask(lo - k0, hi - k0, h) & (seen >> (4 * h));
+      }
 #pragma unroll
       for (int e = 0; e < 16; ++e) s[0][e] = sa::keep_or_neg_inf(s[0][e], sa::keep_bits(mask, e));
       // what stands in V where no row sees a key may be anything: 0 * NaN is not 0
@@ -260,17 +306,17 @@ SA_DEV void rows_part(const RowsParams& p, char* smem_raw, int b, int hk, int sp
 }
 
 // A workgroup for each part that there may be.
-template <typename T, int D, int NW, bool PAGED>
+template <typename T, int D, int NW, bool PAGED, bool TREE = false>
 __global__ __launch_bounds__(NW * 64) void rows_kernel(const RowsParams p) {
   extern __shared__ __attribute__((aligned(16))) char smem_raw[];
   // the splits and row tiles of a pair lie a multiple of the pairs apart: on one XCD where eight divides the pairs
   const int x = div_by(blockIdx.x, p.by_pairs), split = div_by(x, p.by_row_tiles);
   const int bh = blockIdx.x - x * (p.B * p.map.Hkv), b = div_by(bh, p.by_heads);
-  rows_part<T, D, NW, PAGED>(p, smem_raw, b, bh - b * p.map.Hkv, split, (x - split * p.row_tiles) * 32);
+  rows_part<T, D, NW, PAGED, TREE>(p, smem_raw, b, bh - b * p.map.Hkv, split, (x - split * p.row_tiles) * 32);
 }
 // By length: as many workgroups as there are places; each takes the parts that lie the grid apart, of those that the lengths leave, whatever
 // sequence they are of.  Lane l holds, of the sequences l, l + 64, ..., how many parts there are up to and with each.
-template <typename T, int D, int NW, bool PAGED>
+template <typename T, int D, int NW, bool PAGED, bool TREE = false>
 __global__ __launch_bounds__(NW * 64) void rows_by_length_kernel(const RowsParams p) {
   extern __shared__ __attribute__((aligned(16))) char smem_raw[];
   constexpr int GROUPS = MAX_BY_LENGTH / 64;
@@ -294,7 +340,7 @@ __global__ __launch_bounds__(NW * 64) void rows_by_length_kernel(const RowsParam
       b += done;
       if (done > 0) split = part - __builtin_amdgcn_readlane(upto[j], done - 1);
     }
-    rows_part<T, D, NW, PAGED>(p, smem_raw, b, id - part * p.map.Hkv, split, 0);
+    rows_part<T, D, NW, PAGED, TREE>(p, smem_raw, b, id - part * p.map.Hkv, split, 0);
     __syncthreads();   // the next part's rings lie over the waves' results
   }
 }

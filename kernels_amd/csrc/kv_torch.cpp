@@ -1,43 +1,16 @@
 // Native host side of cross attention and of attention over pages (module kv_attention._native): the dispatcher entries of
-// alexdremov_cross_attention::{forward, backward} and alexdremov_paged_attention::{forward, append}, their autograd, and the eager
+// alexdremov_cross_attention::{forward, backward} and alexdremov_paged_attention::{forward, append, tree_forward, keep}, their autograd, and the eager
 // call path of the public Python functions, as sa_torch.cpp has them for streaming attention.
 //
 // The shared library is opened on the first call, the one that KV_ATTENTION_LIB names or the one beside this module; there is no
 // other implementation.  Invalid arguments are handed to the _validate functions of kv_attention.ops, which name the condition (AssertionError).
-#include <Python.h>
-#include <dlfcn.h>
+#include "kv_torch.h"
 
-#include <mutex>
-#include <string>
-
-#include <ATen/ATen.h>
-#include <c10/core/DeviceGuard.h>
-#include <c10/hip/HIPStream.h>
-#include <torch/csrc/Exceptions.h>
-#include <torch/csrc/autograd/custom_function.h>
-#include <torch/csrc/autograd/python_variable.h>
-#include <torch/library.h>
-
-#include "../../include/kv_attention.h"
+using namespace kv_native;
 
 namespace {
 
-using at::Tensor;
-using c10::SymInt;
-using OptTensor = std::optional<Tensor>;
-
 // ---- the shared library -------------------------------------------------------------------------------------
-struct Api {
-  decltype(&kv_cross_forward) cross_forward;
-  decltype(&kv_cross_forward_workspace) cross_forward_workspace;
-  decltype(&kv_cross_backward) cross_backward;
-  decltype(&kv_cross_backward_workspace) cross_backward_workspace;
-  decltype(&kv_paged_forward) paged_forward;
-  decltype(&kv_paged_forward_workspace) paged_forward_workspace;
-  decltype(&kv_paged_append) paged_append;
-  decltype(&kv_error_string) error_string;
-};
-
 Api open_library() {
   std::string path;
   if (const char* env = getenv("KV_ATTENTION_LIB")) {
@@ -65,119 +38,25 @@ Api open_library() {
   KV_SYMBOL(paged_forward);
   KV_SYMBOL(paged_forward_workspace);
   KV_SYMBOL(paged_append);
+  KV_SYMBOL(paged_append_rope);
+  KV_SYMBOL(paged_tree_forward);
+  KV_SYMBOL(paged_tree_forward_workspace);
+  KV_SYMBOL(paged_keep);
+  KV_SYMBOL(qk_norm_rope);
+  KV_SYMBOL(qk_norm_rope_backward);
+  KV_SYMBOL(qk_norm_rope_backward_workspace);
   KV_SYMBOL(error_string);
 #undef KV_SYMBOL
   return a;
 }
-const Api& api() {
+}  // namespace
+
+const Api& kv_native::api() {
   static const Api a = open_library();   // tried again by the next call if it throws
   return a;
 }
-void check(int64_t rc, const char* what) {
-  TORCH_CHECK(rc >= 0, what, " failed with code ", rc, ": ", api().error_string((int)rc));
-}
-void check_launch(int rc, const char* what) {
-  TORCH_CHECK(rc == 0, what, " failed with code ", rc, ": ", api().error_string(rc));
-}
 
-// ---- argument checks and layout -------------------------------------------------------------------------------
-int dtype_id(const Tensor& t) {
-  switch (t.scalar_type()) {
-    case at::kFloat: return 0;
-    case at::kHalf: return 1;
-    case at::kBFloat16: return 2;
-    default: return -1;
-  }
-}
-bool known_head_dim(int64_t d) { return d == 16 || d == 32 || d == 64 || d == 128 || d == 256; }
-bool alike(const Tensor& a, const Tensor& b) { return a.device() == b.device() && a.scalar_type() == b.scalar_type(); }
-bool is_lengths(const OptTensor& l, const Tensor& q) {
-  return !l || (l->scalar_type() == at::kInt && l->dim() == 1 && l->size(0) == q.size(0) && l->device() == q.device());
-}
-bool is_scale(double sm_scale) { return std::fabs(sm_scale) <= 0x1p127; }   // times log2(e) in float32's range
-bool small(int64_t n) { return n <= 0x7fffffff; }
-bool small_sizes(const Tensor& t) { return small(t.size(0)) && small(t.size(1)) && small(t.size(2)); }
-
-bool is_cross(const Tensor& q, const Tensor& k, const Tensor& v, const OptTensor& lens, const OptTensor& q_lens, double sm_scale) {
-  if (q.dim() != 4 || k.dim() != 4 || dtype_id(q) < 0 || !known_head_dim(q.size(3)) || !alike(q, k) || !alike(q, v)) return false;
-  if (v.sizes() != k.sizes() || k.size(0) != q.size(0) || k.size(3) != q.size(3) || k.size(1) < 1 || q.size(1) < 1 || q.size(1) % k.size(1) != 0)
-    return false;
-  return small_sizes(q) && small_sizes(k) && is_lengths(lens, q) && is_lengths(q_lens, q) && is_scale(sm_scale);
-}
-bool is_cache(const Tensor& x, const Tensor& k_pages, const Tensor& v_pages, const Tensor& table, const Tensor& lens,
-              const OptTensor& new_lens) {
-  if (x.dim() != 4 || k_pages.dim() != 4 || dtype_id(x) < 0 || !known_head_dim(x.size(3)) || !alike(x, k_pages) || !alike(x, v_pages)) return false;
-  if (v_pages.sizes() != k_pages.sizes() || k_pages.size(3) != x.size(3) || k_pages.size(2) < 1 || k_pages.size(1) < 1 || x.size(1) < 1) return false;
-  if (table.dim() != 2 || table.scalar_type() != at::kInt || table.size(0) != x.size(0) || table.device() != x.device()) return false;
-  for (const Tensor* t : {&k_pages, &v_pages}) {   // read and written in place: no copy stands in for them
-    const int64_t vec = 16 / t->element_size();
-    if (t->numel() == 0) continue;
-    if (t->stride(3) != 1 || reinterpret_cast<uintptr_t>(t->const_data_ptr()) % 16 != 0) return false;
-    for (int i = 0; i < 3; ++i)
-      if (t->size(i) > 1 && (t->stride(i) % vec != 0 || t->stride(i) <= 0)) return false;
-  }
-  const int64_t capacity = table.size(1) * k_pages.size(2);
-  return small_sizes(x) && small_sizes(k_pages) && small(table.size(1)) && capacity <= (int64_t(1) << 30) && is_lengths(lens, x) && is_lengths(new_lens, x);
-}
-
-PyObject* wrap(const OptTensor& t) {
-  if (t) return THPVariable_Wrap(*t);
-  Py_RETURN_NONE;
-}
-// Have Python's checks name what is wrong; takes the references.
-[[noreturn]] void explain(const char* function, std::initializer_list<PyObject*> args) {
-  PyObject* tuple = PyTuple_New((Py_ssize_t)args.size());
-  Py_ssize_t i = 0;
-  for (PyObject* a : args) PyTuple_SET_ITEM(tuple, i++, a);
-  PyObject* m = PyImport_ImportModule("kv_attention.ops");
-  PyObject* f = m ? PyObject_GetAttrString(m, function) : nullptr;
-  PyObject* r = f ? PyObject_CallObject(f, tuple) : nullptr;
-  Py_XDECREF(r);
-  Py_XDECREF(f);
-  Py_XDECREF(m);
-  Py_DECREF(tuple);
-  if (PyErr_Occurred()) throw python_error();
-  TORCH_CHECK(false, "unsupported arguments");
-}
-struct Gil {
-  PyGILState_STATE s = PyGILState_Ensure();
-  ~Gil() { PyGILState_Release(s); }
-};
-
-// The tensor itself when the kernels can read it in place (unit stride along the head dimension, the others and the base
-// address multiples of 16 bytes, rows that advance), otherwise a contiguous copy.  Rows of one head are addressed with 32-bit byte offsets.
-Tensor kernel_layout(const Tensor& t) {
-  const int64_t es = t.element_size(), vec = 16 / es, T = t.size(2);
-  const auto s = t.strides();
-  bool ok = (s[3] == 1 || t.size(3) == 1) && reinterpret_cast<uintptr_t>(t.const_data_ptr()) % 16 == 0;
-  for (int i = 0; i < 3; ++i) ok = ok && (t.size(i) <= 1 || s[i] % vec == 0);
-  ok = ok && (T <= 1 || (s[2] > 0 && s[2] <= 0xffffffffLL / es / (T + 1024)));
-  if (ok) return t;
-  return t.is_contiguous() ? t.clone(at::MemoryFormat::Contiguous) : t.contiguous();
-}
-struct Strides {   // a dimension of one element may have any stride: 0 here
-  int64_t s[4];
-  explicit Strides(const Tensor& t) {
-    for (int i = 0; i < 3; ++i) s[i] = t.size(i) > 1 ? t.stride(i) : 0;
-    s[3] = 1;
-  }
-  operator const int64_t*() const { return s; }
-};
-const void* ptr(const Tensor& t) { return t.const_data_ptr(); }
-void* out_ptr(const Tensor& t) { return t.mutable_data_ptr(); }
-struct Lengths {
-  const int32_t* p = nullptr;
-  int64_t stride = 0;
-  explicit Lengths(const OptTensor& l) {
-    if (l) p = l->const_data_ptr<int32_t>(), stride = l->stride(0);
-  }
-};
-int clamp_int(int64_t x) { return (int)std::min<int64_t>(x, 0x7fffffff); }
-void* current_stream(const Tensor& q) { return c10::hip::getCurrentHIPStream(q.device().index()).stream(); }
-// From the caching allocator: a workspace belongs to the call and its stream (or to the graph that captures it).
-Tensor workspace(const Tensor& q, int64_t bytes) { return at::empty({bytes}, q.options().dtype(at::kByte)); }
-Tensor empty_rows(const Tensor& q) { return at::empty({q.size(0), q.size(1), q.size(2)}, q.options().dtype(at::kFloat)); }
-Tensor empty_same(const Tensor& q) { return at::empty(q.sizes(), q.options()); }
+namespace {
 
 // ---- cross attention --------------------------------------------------------------------------------------------
 void validate_cross(const Tensor& q, const Tensor& k, const Tensor& v, const OptTensor& lens, const OptTensor& q_lens, double sm_scale,
@@ -247,9 +126,6 @@ std::tuple<Tensor, Tensor, Tensor> cross_backward_gpu(const Tensor& q, const Ten
   return {std::move(dq), std::move(dk), std::move(dv)};
 }
 
-template <typename F> const c10::TypedOperatorHandle<F> find_op(const char* name) {
-  return c10::Dispatcher::singleton().findSchemaOrThrow(name, "").template typed<F>();
-}
 using CrossForward = std::tuple<Tensor, Tensor>(const Tensor&, const Tensor&, const Tensor&, const OptTensor&, const OptTensor&, double, bool);
 using CrossBackward = std::tuple<Tensor, Tensor, Tensor>(const Tensor&, const Tensor&, const Tensor&, const OptTensor&, const OptTensor&,
                                                          const Tensor&, const Tensor&, const Tensor&, double);
@@ -260,18 +136,6 @@ const c10::TypedOperatorHandle<CrossForward>& cross_forward_op() {
 const c10::TypedOperatorHandle<CrossBackward>& cross_backward_op() {
   static const auto op = find_op<CrossBackward>("alexdremov_cross_attention::backward");
   return op;
-}
-
-bool wants_grad(std::initializer_list<const Tensor*> ts) {
-  if (!at::GradMode::is_enabled()) return false;
-  for (const Tensor* t : ts)
-    if (t->requires_grad()) return true;
-  return false;
-}
-bool has_tangent(std::initializer_list<const Tensor*> ts) {
-  for (const Tensor* t : ts)
-    if (t->_fw_grad(0).defined()) return true;
-  return false;
 }
 
 // Saves q, k, v, O, LSE and the lengths and hands dO to the backward op.  No gradient flows through the log-sum-exp: it leaves through
@@ -354,7 +218,7 @@ std::tuple<Tensor, Tensor> paged_forward_gpu(const Tensor& q, const Tensor& k_pa
   if (q.numel() == 0) return {std::move(o), std::move(lse)};
   const Api& a = api();
   const Tensor qk = kernel_layout(q);
-  const Tensor table = page_table.size(1) <= 1 || page_table.stride(1) == 1 ? page_table : page_table.contiguous();
+  const Tensor table = unit_rows(page_table);
   const int B = (int)q.size(0), Hq = (int)q.size(1), T = (int)q.size(2), D = (int)q.size(3);
   const int N = (int)k_pages.size(0), Hkv = (int)k_pages.size(1), page = (int)k_pages.size(2), W = (int)table.size(1);
   const int C = clamp_int(context_size), R = clamp_int(back_contexts);
@@ -383,13 +247,69 @@ void paged_append_gpu(const Tensor& k, const Tensor& v, const Tensor& k_pages, c
     if (!t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
   if (k.numel() == 0 || k_pages.numel() == 0 || page_table.numel() == 0) return;
   const Tensor kk = kernel_layout(k), vk = kernel_layout(v);
-  const Tensor table = page_table.size(1) <= 1 || page_table.stride(1) == 1 ? page_table : page_table.contiguous();
+  const Tensor table = unit_rows(page_table);
   const Lengths l(lens), nl(new_lens);
   check_launch(api().paged_append(ptr(kk), ptr(vk), out_ptr(k_pages), out_ptr(v_pages), table.const_data_ptr<int32_t>(), table.stride(0), l.p,
                                   l.stride, nl.p, nl.stride, Strides(kk), Strides(vk), Strides(k_pages), Strides(v_pages), (int)k.size(0),
                                   (int)k.size(1), (int)k.size(2), (int)k.size(3), (int)k_pages.size(0), (int)k_pages.size(2),
                                   (int)table.size(1), dtype_id(k), current_stream(k)),
                "kv_paged_append");
+}
+
+bool is_tree(const Tensor& tree, const Tensor& q) {
+  const int64_t d = tree.dim();
+  return (d == 2 || (d == 3 && tree.size(0) == q.size(0))) && tree.scalar_type() == at::kBool && tree.device() == q.device() &&
+         tree.size(-1) == q.size(2) && tree.size(-2) == q.size(2);
+}
+std::tuple<Tensor, Tensor> tree_forward_gpu(const Tensor& q, const Tensor& k_pages, const Tensor& v_pages, const Tensor& page_table,
+                                            const Tensor& lens, const Tensor& tree, double sm_scale, const OptTensor& new_lens,
+                                            bool return_lse) {
+  if (C10_UNLIKELY(!(is_cache(q, k_pages, v_pages, page_table, lens, new_lens) && q.size(1) % k_pages.size(1) == 0 && is_tree(tree, q) &&
+                     is_scale(sm_scale)))) {
+    Gil gil;
+    explain("_validate_tree", {THPVariable_Wrap(q), THPVariable_Wrap(k_pages), THPVariable_Wrap(v_pages), THPVariable_Wrap(page_table),
+                               THPVariable_Wrap(lens), THPVariable_Wrap(tree), PyFloat_FromDouble(sm_scale), wrap(new_lens)});
+  }
+  const c10::OptionalDeviceGuard guard(q.device());
+  Tensor o = empty_same(q);
+  Tensor lse = return_lse ? empty_rows(q) : at::empty({0});
+  if (q.numel() == 0) return {std::move(o), std::move(lse)};
+  const Api& a = api();
+  const Tensor qk = kernel_layout(q), table = unit_rows(page_table);
+  const int B = (int)q.size(0), Hq = (int)q.size(1), T = (int)q.size(2), D = (int)q.size(3);
+  const int N = (int)k_pages.size(0), Hkv = (int)k_pages.size(1), page = (int)k_pages.size(2), W = (int)table.size(1);
+  const int64_t bytes = a.paged_tree_forward_workspace(B, Hq, Hkv, T, D, page, W, dtype_id(q));
+  check(bytes, "kv_paged_tree_forward");
+  const Tensor ws = bytes > 0 ? workspace(q, bytes) : Tensor();
+  const Lengths l(lens), nl(new_lens);
+  const int64_t tree_strides[3] = {tree.dim() == 3 ? tree.stride(0) : 0, tree.stride(-2), tree.stride(-1)};
+  check_launch(a.paged_tree_forward(ptr(qk), ptr(k_pages), ptr(v_pages), table.const_data_ptr<int32_t>(), table.stride(0), l.p, l.stride, nl.p,
+                                    nl.stride, ptr(tree), tree_strides, out_ptr(o), return_lse ? (float*)out_ptr(lse) : nullptr,
+                                    bytes > 0 ? out_ptr(ws) : nullptr, bytes, Strides(qk), Strides(k_pages), Strides(v_pages), B, Hq, Hkv, T, D,
+                                    N, page, W, (float)sm_scale, dtype_id(q), current_stream(q)),
+               "kv_paged_tree_forward");
+  return {std::move(o), std::move(lse)};
+}
+
+void paged_keep_gpu(const Tensor& k_pages, const Tensor& v_pages, const Tensor& page_table, const Tensor& first, const Tensor& kept) {
+  if (C10_UNLIKELY(!(is_pages(k_pages, v_pages, page_table) && first.dim() == 1 && kept.dim() == 2 && first.scalar_type() == at::kInt &&
+                     kept.scalar_type() == at::kInt && first.size(0) == page_table.size(0) && kept.size(0) == page_table.size(0) &&
+                     small(kept.size(1)) && first.device() == k_pages.device() && kept.device() == k_pages.device()))) {
+    Gil gil;
+    explain("_validate_keep", {THPVariable_Wrap(k_pages), THPVariable_Wrap(v_pages), THPVariable_Wrap(page_table), THPVariable_Wrap(first),
+                               THPVariable_Wrap(kept)});
+  }
+  const c10::OptionalDeviceGuard guard(k_pages.device());
+  for (const Tensor* t : {&k_pages, &v_pages})
+    if (!t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
+  if (k_pages.numel() == 0 || page_table.numel() == 0 || kept.numel() == 0) return;
+  const Tensor table = unit_rows(page_table);
+  const int64_t kept_strides[2] = {kept.stride(0), kept.stride(1)};
+  check_launch(api().paged_keep(out_ptr(k_pages), out_ptr(v_pages), table.const_data_ptr<int32_t>(), table.stride(0), first.const_data_ptr<int32_t>(),
+                                first.stride(0), kept.const_data_ptr<int32_t>(), kept_strides, Strides(k_pages), Strides(v_pages),
+                                (int)table.size(0), (int)k_pages.size(1), (int)kept.size(1), (int)k_pages.size(3), (int)k_pages.size(0),
+                                (int)k_pages.size(2), (int)table.size(1), dtype_id(k_pages), current_stream(k_pages)),
+               "kv_paged_keep");
 }
 
 using PagedForward = std::tuple<Tensor, Tensor>(const Tensor&, const Tensor&, const Tensor&, const Tensor&, const Tensor&, SymInt, SymInt,
@@ -401,6 +321,18 @@ const c10::TypedOperatorHandle<PagedForward>& paged_forward_op() {
 }
 const c10::TypedOperatorHandle<PagedAppend>& paged_append_op() {
   static const auto op = find_op<PagedAppend>("alexdremov_paged_attention::append");
+  return op;
+}
+
+using TreeForward = std::tuple<Tensor, Tensor>(const Tensor&, const Tensor&, const Tensor&, const Tensor&, const Tensor&, const Tensor&, double,
+                                               const OptTensor&, bool);
+using PagedKeep = void(const Tensor&, const Tensor&, const Tensor&, const Tensor&, const Tensor&);
+const c10::TypedOperatorHandle<TreeForward>& tree_forward_op() {
+  static const auto op = find_op<TreeForward>("alexdremov_paged_attention::tree_forward");
+  return op;
+}
+const c10::TypedOperatorHandle<PagedKeep>& paged_keep_op() {
+  static const auto op = find_op<PagedKeep>("alexdremov_paged_attention::keep");
   return op;
 }
 
@@ -433,6 +365,32 @@ std::tuple<Tensor, Tensor> paged_forward_autograd(const Tensor& q, const Tensor&
                                    return_lse, &lse);
   return {std::move(o), std::move(lse)};
 }
+struct TreeAttention : torch::autograd::Function<TreeAttention> {
+  static Tensor forward(torch::autograd::AutogradContext*, const Tensor& q, const Tensor& k_pages, const Tensor& v_pages,
+                        const Tensor& page_table, const Tensor& lens, const Tensor& tree, double sm_scale, const OptTensor& new_lens,
+                        bool return_lse, Tensor* lse_out) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    auto [o, lse] = tree_forward_op().call(q, k_pages, v_pages, page_table, lens, tree, sm_scale, new_lens, return_lse);
+    *lse_out = std::move(lse);
+    return o;
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext*, torch::autograd::variable_list) {
+    TORCH_CHECK(false, "Trying to backward through alexdremov_paged_attention.tree_forward.default but no autograd formula was registered: "
+                       "attention over pages is forward only");
+  }
+};
+std::tuple<Tensor, Tensor> tree_forward_autograd(const Tensor& q, const Tensor& k_pages, const Tensor& v_pages, const Tensor& page_table,
+                                                 const Tensor& lens, const Tensor& tree, double sm_scale, const OptTensor& new_lens,
+                                                 bool return_lse) {
+  TORCH_CHECK_NOT_IMPLEMENTED(!has_tangent({&q, &k_pages, &v_pages}), "alexdremov_paged_attention::tree_forward has no forward-mode derivative");
+  if (!wants_grad({&q, &k_pages, &v_pages})) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    return tree_forward_op().call(q, k_pages, v_pages, page_table, lens, tree, sm_scale, new_lens, return_lse);
+  }
+  Tensor lse;
+  Tensor o = TreeAttention::apply(q, k_pages, v_pages, page_table, lens, tree, sm_scale, new_lens, return_lse, &lse);
+  return {std::move(o), std::move(lse)};
+}
 // The cache takes values, no history.
 void paged_append_autograd(const Tensor& k, const Tensor& v, const Tensor& k_pages, const Tensor& v_pages, const Tensor& page_table,
                            const Tensor& lens, const OptTensor& new_lens) {
@@ -443,31 +401,17 @@ void paged_append_autograd(const Tensor& k, const Tensor& v, const Tensor& k_pag
   paged_append_op().call(k, v, k_pages, v_pages, page_table, lens, new_lens);
 }
 
+void paged_keep_autograd(const Tensor& k_pages, const Tensor& v_pages, const Tensor& page_table, const Tensor& first, const Tensor& kept) {
+  TORCH_CHECK_NOT_IMPLEMENTED(!has_tangent({&k_pages, &v_pages}), "alexdremov_paged_attention::keep has no forward-mode derivative");
+  TORCH_CHECK(!wants_grad({&k_pages, &v_pages}),
+              "alexdremov_paged_attention::keep records no gradient: call it under torch.no_grad() or on detached tensors");
+  at::AutoDispatchBelowADInplaceOrView below;
+  paged_keep_op().call(k_pages, v_pages, page_table, first, kept);
+}
+
 // ---- eager call path of the public functions ------------------------------------------------------------------------
 // As in sa_torch.cpp: arguments come positionally and complete; one that is not of the plain type returns NotImplemented, and the Python functions
 // call the op itself, which converts or refuses it.
-bool tensor_arg(PyObject* x, Tensor& t) {
-  if (!THPVariable_Check(x)) return false;
-  t = THPVariable_Unpack(x);
-  return true;
-}
-bool optional_arg(PyObject* x, OptTensor& t) {
-  if (x == Py_None) return true;
-  if (!THPVariable_Check(x)) return false;
-  t = THPVariable_Unpack(x);
-  return true;
-}
-bool int_arg(PyObject* x, int64_t& value) {
-  int overflow = 0;
-  if (!PyLong_CheckExact(x)) return false;
-  value = PyLong_AsLongLongAndOverflow(x, &overflow);
-  return overflow == 0;
-}
-bool scale_arg(PyObject* x, const Tensor& q, double& value) {
-  if (q.dim() < 1 || (x != Py_None && !PyFloat_CheckExact(x))) return false;
-  value = x == Py_None ? 1.0 / std::sqrt((double)q.size(-1)) : PyFloat_AS_DOUBLE(x);
-  return true;
-}
 PyObject* result(const std::tuple<Tensor, Tensor>& r, bool return_lse) {
   PyObject* o = THPVariable_Wrap(std::get<0>(r));
   if (!return_lse || !o) return o;
@@ -532,10 +476,49 @@ PyObject* py_paged_append(PyObject*, PyObject* const* args, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// paged_tree_attention(q, k_pages, v_pages, page_table, lens, tree, sm_scale or None, new_lens, return_lse)
+PyObject* py_paged_tree_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  Tensor q, k, v, table, lens, tree;
+  OptTensor new_lens;
+  double sm_scale;
+  if (n != 9 || !tensor_arg(args[0], q) || !tensor_arg(args[1], k) || !tensor_arg(args[2], v) || !tensor_arg(args[3], table) ||
+      !tensor_arg(args[4], lens) || !tensor_arg(args[5], tree) || !scale_arg(args[6], q, sm_scale) || !optional_arg(args[7], new_lens) ||
+      !PyBool_Check(args[8]))
+    Py_RETURN_NOTIMPLEMENTED;
+  const bool return_lse = args[8] == Py_True;
+  std::tuple<Tensor, Tensor> r;
+  {
+    pybind11::gil_scoped_release no_gil;
+    r = tree_forward_op().call(q, k, v, table, lens, tree, sm_scale, new_lens, return_lse);
+  }
+  return result(r, return_lse);
+  END_HANDLE_TH_ERRORS
+}
+
+// paged_keep(k_pages, v_pages, page_table, first, kept)
+PyObject* py_paged_keep(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  Tensor k, v, table, first, kept;
+  if (n != 5 || !tensor_arg(args[0], k) || !tensor_arg(args[1], v) || !tensor_arg(args[2], table) || !tensor_arg(args[3], first) ||
+      !tensor_arg(args[4], kept))
+    Py_RETURN_NOTIMPLEMENTED;
+  {
+    pybind11::gil_scoped_release no_gil;
+    paged_keep_op().call(k, v, table, first, kept);
+  }
+  Py_RETURN_NONE;
+  END_HANDLE_TH_ERRORS
+}
+
 PyMethodDef methods[] = {
     {"cross_attention", (PyCFunction)(void (*)())py_cross_attention, METH_FASTCALL, nullptr},
     {"paged_attention", (PyCFunction)(void (*)())py_paged_attention, METH_FASTCALL, nullptr},
     {"paged_append", (PyCFunction)(void (*)())py_paged_append, METH_FASTCALL, nullptr},
+    {"paged_append_rope", (PyCFunction)(void (*)())py_paged_append_rope, METH_FASTCALL, nullptr},
+    {"paged_tree_attention", (PyCFunction)(void (*)())py_paged_tree_attention, METH_FASTCALL, nullptr},
+    {"paged_keep", (PyCFunction)(void (*)())py_paged_keep, METH_FASTCALL, nullptr},
+    {"qk_norm_rope", (PyCFunction)(void (*)())py_qk_norm_rope, METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_native", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
@@ -562,14 +545,22 @@ TORCH_LIBRARY(alexdremov_paged_attention, m) {
         {at::Tag::pt2_compliant_tag});
   m.def("append(Tensor k, Tensor v, Tensor(a!) k_pages, Tensor(b!) v_pages, Tensor page_table, Tensor lens, Tensor? new_lens) -> ()",
         {at::Tag::pt2_compliant_tag});
+  m.def("tree_forward(Tensor q, Tensor k_pages, Tensor v_pages, Tensor page_table, Tensor lens, Tensor tree, float sm_scale, Tensor? new_lens, "
+        "bool return_lse) -> (Tensor, Tensor)",
+        {at::Tag::pt2_compliant_tag});
+  m.def("keep(Tensor(a!) k_pages, Tensor(b!) v_pages, Tensor page_table, Tensor first, Tensor kept) -> ()", {at::Tag::pt2_compliant_tag});
 }
 TORCH_LIBRARY_IMPL(alexdremov_paged_attention, CUDA, m) {
   m.impl("forward", TORCH_FN(paged_forward_gpu));
   m.impl("append", TORCH_FN(paged_append_gpu));
+  m.impl("tree_forward", TORCH_FN(tree_forward_gpu));
+  m.impl("keep", TORCH_FN(paged_keep_gpu));
 }
 TORCH_LIBRARY_IMPL(alexdremov_paged_attention, Autograd, m) {
   m.impl("forward", TORCH_FN(paged_forward_autograd));
   m.impl("append", TORCH_FN(paged_append_autograd));
+  m.impl("tree_forward", TORCH_FN(tree_forward_autograd));
+  m.impl("keep", TORCH_FN(paged_keep_autograd));
 }
 
 PyMODINIT_FUNC PyInit__native() { return PyModule_Create(&module); }

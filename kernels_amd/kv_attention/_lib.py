@@ -26,6 +26,15 @@ SIGNATURES = {
     "kv_paged_forward_workspace": [_i32] * 10,
     "kv_paged_forward": [_vp] * 3 + _lengths * 3 + [_vp, _vp, _vp, _i64] + [_st] * 3 + [_i32] * 10 + [_f32, _i32, _vp],
     "kv_paged_append": [_vp] * 4 + _lengths * 3 + [_st] * 4 + [_i32] * 8 + [_vp],
+    "kv_paged_tree_forward_workspace": [_i32] * 8,
+    "kv_paged_tree_forward": [_vp] * 3 + _lengths * 3 + [_vp, _st] + [_vp, _vp, _vp, _i64] + [_st] * 3 + [_i32] * 8 + [_f32, _i32, _vp],
+    "kv_paged_keep": [_vp] * 2 + _lengths * 2 + [_vp, _st] + [_st] * 2 + [_i32] * 8 + [_vp],
+    "kv_qk_norm_rope": [_vp] * 4 + [_i64] * 2 + [_vp] * 2 + [_i32] + _lengths + [_vp, _st] + [_vp] * 2 + [_st] * 2 + [_i32] * 8 + [_f32, _i32, _vp],
+    "kv_qk_norm_rope_backward_workspace": [_i32] * 6,
+    "kv_qk_norm_rope_backward": [_vp] * 6 + [_i64] * 2 + [_vp] * 2 + [_i32] + _lengths + [_vp, _st] + [_vp] * 5 + [_i64] + [_st] * 4 + [_i32] * 8
+                                + [_f32, _i32, _vp],
+    "kv_paged_append_rope": [_vp] * 6 + _lengths * 3 + [_vp] * 2 + [_i64] * 2 + [_vp] * 2 + [_i32] + [_vp, _st] + [_st] * 5 + [_i32] * 11
+                            + [_f32, _i32, _vp],
     "kv_error_string": [_i32],
 }
 

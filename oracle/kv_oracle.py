@@ -145,3 +145,95 @@ def assert_within(name, got, want_bound, finite=True):
         at = tuple(int(i) for i in at)
         raise AssertionError(f"{name}: {int(bad.sum())} of {bad.numel()} out of bounds, worst at {at}: "
                              f"{float(got[at])} instead of {float(want[at])}, bound {float(bound[at])}")
+
+
+def tree(q, k_pages, v_pages, table, lens, seen_tokens, scale=None, new_lens=None):
+    """{name: (value, bound)} of o and lse of drafted tokens; all tensors on the CPU."""
+    B, Hq, T, D = q.shape
+    N, Hkv, page, _ = k_pages.shape
+    G, width = Hq // Hkv, table.shape[1]
+    scale = D ** -0.5 if scale is None else scale
+    res = {"o": [torch.zeros(q.shape, dtype=torch.float64) for _ in range(2)],
+           "lse": [torch.zeros(q.shape[:3], dtype=torch.float64) for _ in range(2)]}
+    for b in range(B):
+        L = min(max(int(lens[b]), 0), width * page)
+        n = T if new_lens is None else min(max(int(new_lens[b]), 0), T)
+        entry = table[b].long()[torch.arange(L) // page] if L else torch.zeros(0, dtype=torch.long)
+        there = (entry >= 0) & (entry < N)
+        keys, values = (x[entry.clamp(0, max(N - 1, 0)), :, torch.arange(L) % page].double().transpose(0, 1) if N and L else
+                        torch.zeros(Hkv, L, D, dtype=torch.float64) for x in (k_pages, v_pages))
+        keys, values = (torch.where(there[None, :, None], x, 0.0) for x in (keys, values))
+        seen = torch.zeros(n, L, dtype=torch.bool)
+        for i in range(n):
+            if L - n + i < 0:
+                continue
+            seen[i, :max(L - n, 0)] = True
+            for j in range(n):
+                if L - n + j >= 0:
+                    seen[i, L - n + j] = bool((seen_tokens if seen_tokens.dim() == 2 else seen_tokens[b])[i, j])
+        seen &= there
+        for h in range(Hq):
+            r = _head(q[b, h, :n].double(), keys[h // G], values[h // G], seen, scale, q.dtype)
+            for name in res:
+                for i in range(2):
+                    res[name][i][b, h, :n] = r[name][i]
+    return {n: tuple(x) for n, x in res.items()}
+
+
+# ---- norms and rotation -----------------------------------------------------------------------------------------------
+# With e = 2^-24: a sum of D squares is off by D e at most, its root by half of that, r by two units in the last place more (4 e); y = x (r w) has
+# two roundings.  A turned channel is two products and their difference, 3 e of the magnitudes.
+
+def _pairs(x, rot, interleaved):
+    return (x[..., 0:rot:2], x[..., 1:rot:2]) if interleaved else (x[..., :rot // 2], x[..., rot // 2:rot])
+
+
+def _join(a, b, rest, interleaved):
+    return torch.cat(((torch.stack((a, b), -1).flatten(-2) if interleaved else torch.cat((a, b), -1)), rest), -1)
+
+
+def _turn(x, err, cos, sin, interleaved):
+    """The turned rows and the bound on their error, without a final rounding."""
+    rot = 2 * cos.shape[-1]
+    (a, b), (ea, eb) = _pairs(x, rot, interleaved), _pairs(err, rot, interleaved)
+    c, s = cos.abs(), sin.abs()
+    value = _join(a * cos - b * sin, b * cos + a * sin, x[..., rot:], interleaved)
+    bound = _join(ea * c + eb * s + 3 * E32 * (a.abs() * c + b.abs() * s), eb * c + ea * s + 3 * E32 * (b.abs() * c + a.abs() * s),
+                  err[..., rot:], interleaved)
+    return value, bound
+
+
+def rope_rows(x, cos, sin, weight=None, eps=None, interleaved=False, g=None):
+    """x [..., n, D] with cos and sin [..., n, rot / 2] that broadcast to it: (value, bound) of the turned rows; with g, the gradient of those, a dict of
+    "out", "dx" and "dw" (over all rows)."""
+    dtype, D = x.dtype, x.shape[-1]
+    x, cos, sin = x.double(), cos.double(), sin.double()
+    w = torch.ones(D, dtype=torch.float64) if weight is None else weight.double()
+    final, tiny = HALF_STEP[dtype], TINY[dtype]
+    r = torch.ones_like(x[..., :1]) if eps is None else (x.square().mean(-1, keepdim=True) + eps).rsqrt()
+    rel = 0.0 if eps is None else (D / 2 + 6) * E32          # of r, and with one rounding more of x r
+    unit = x * r
+    y = unit * w
+    out, err = _turn(y, y.abs() * (rel + (2 * E32 if eps is not None else 0.0)), cos, sin, interleaved)
+    res = {"out": (out, err + final * out.abs() + tiny)}
+    if g is None:
+        return res["out"]
+    g = g.double()
+    gy, eg = _turn(g, torch.zeros_like(g), cos, -sin, interleaved)
+    if eps is None:
+        res["dx"] = (gy, eg + final * gy.abs() + tiny)
+        return res
+    rel_u = rel + E32
+    h, eh = gy * w, eg * w.abs() + E32 * (gy * w).abs()
+    m = (h * unit).mean(-1, keepdim=True)
+    em = ((h * unit).abs() * (rel_u + (D + 2) * E32) + eh * unit.abs()).mean(-1, keepdim=True)
+    dx = r * (h - unit * m)
+    edx = r * (eh + unit.abs() * em + (unit * m).abs() * rel_u + 2 * E32 * (h.abs() + (unit * m).abs())) + (rel + E32) * dx.abs()
+    res["dx"] = (dx, edx + final * dx.abs() + tiny)
+    if weight is not None:
+        t = gy * unit
+        dims = tuple(range(x.dim() - 1))
+        dw, rows = t.sum(dims), t.numel() // D
+        final_w = HALF_STEP[weight.dtype]
+        res["dw"] = (dw, (eg * unit.abs() + t.abs() * (rel_u + E32 * (rows + 2))).sum(dims) + final_w * dw.abs() + TINY[weight.dtype])
+    return res
