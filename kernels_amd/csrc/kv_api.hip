@@ -107,7 +107,7 @@ template <typename P> void long_sides(P& p, int B, int Hq, int Hkv, int Tq, int 
 // How the rows kernel goes through the pages.
 struct PagedPlan {
   int64_t nbh, rows, row_tiles, bytes;
-  int splits, share;
+  int splits, share, tile;   // at most that many parts, of up to `share` tiles of `tile` keys
 };
 int plan_paged(PagedPlan& c, int B, int Hq, int Hkv, int T, int D, int page, int width, int C, int R, int dtype) {
   if (int rc = check_sizes(B, Hq, Hkv, D, dtype)) return rc;
@@ -119,6 +119,7 @@ int plan_paged(PagedPlan& c, int B, int Hq, int Hkv, int T, int D, int page, int
   const int G = Hq / Hkv;
   c.nbh = (int64_t)B * Hkv;
   c.rows = (int64_t)G * T;
+  c.tile = 32;
   if (c.nbh > kMostCount || c.rows > kMostCount - 1024) return KV_ERR_TOO_LARGE;
   c.row_tiles = ceil_div(c.rows, 32);
   // the most keys that the rows of a tile see together: those of R + 1 chunks for each chunk that its tokens lie in
@@ -132,6 +133,22 @@ int plan_paged(PagedPlan& c, int B, int Hq, int Hkv, int T, int D, int page, int
   if (!launchable(blocks, 64 * rows_waves(row_bytes, dtype == 0, blocks, c.share))) return KV_ERR_TOO_LARGE;
   if (c.splits > 1 && c.nbh * c.rows > kMostCount) return KV_ERR_TOO_LARGE;
   if (c.splits > 1) c.bytes = c.splits * c.nbh * c.rows * (D + 2) * 4;
+  return KV_OK;
+}
+
+// Trees: the rows kernel, or tiles of rows.
+int plan_tree(PagedPlan& c, int B, int Hq, int Hkv, int T, int D, int page, int width, int dtype) {
+  if (int rc = plan_paged(c, B, Hq, Hkv, T, D, page, width, 1, 0x7fffffff, dtype)) return rc;
+  if (few_rows(c.rows)) return KV_OK;
+  const int row_bytes = D * elem_size(dtype), waves = tree_waves(c.rows);
+  c.tile = row_bytes <= 256 ? 64 : 32;
+  c.row_tiles = ceil_div(c.rows, waves * 32);
+  const int64_t tiles = ceil_div((int64_t)width * page, c.tile);
+  c.share = tree_share(c.nbh * c.row_tiles, tiles);
+  c.splits = (int)std::max<int64_t>(1, ceil_div(tiles, c.share));
+  if (!launchable(c.nbh * c.row_tiles * c.splits, waves * 64)) return KV_ERR_TOO_LARGE;
+  if (c.splits > 1 && c.nbh * c.rows > kMostCount) return KV_ERR_TOO_LARGE;
+  c.bytes = c.splits > 1 ? c.splits * c.nbh * c.rows * (D + 2) * 4 : 0;
   return KV_OK;
 }
 
@@ -402,7 +419,7 @@ int kv_paged_forward(const void* q, const void* k_pages, const void* v_pages, co
 
 int64_t kv_paged_tree_forward_workspace(int B, int Hq, int Hkv, int T, int D, int page_size, int width, int dtype) {
   PagedPlan c;
-  if (int rc = plan_paged(c, B, Hq, Hkv, T, D, page_size, width, 1, 0x7fffffff, dtype)) return rc;
+  if (int rc = plan_tree(c, B, Hq, Hkv, T, D, page_size, width, dtype)) return rc;
   return c.bytes;
 }
 
@@ -412,7 +429,7 @@ int kv_paged_tree_forward(const void* q, const void* k_pages, const void* v_page
                           const int64_t* vs, int B, int Hq, int Hkv, int T, int D, int num_pages, int page_size, int width, float sm_scale,
                           int dtype, void* stream) {
   PagedPlan c;
-  if (int rc = plan_paged(c, B, Hq, Hkv, T, D, page_size, width, 1, 0x7fffffff, dtype)) return rc;
+  if (int rc = plan_tree(c, B, Hq, Hkv, T, D, page_size, width, dtype)) return rc;
   if (num_pages < 0) return KV_ERR_ARG;
   if (int rc = check_scale(sm_scale)) return rc;
   if (B == 0 || Hq == 0 || T == 0) return KV_OK;
@@ -429,8 +446,8 @@ int kv_paged_tree_forward(const void* q, const void* k_pages, const void* v_page
   RowsParams p = paged_rows(c, q, k_pages, v_pages, page_table, table_stride, lens, lens_stride, new_lens, new_lens_stride, o, lse, workspace,
                             qs, ks, vs, B, Hq, Hkv, T, D, empty ? 0 : num_pages, page_size, empty ? 0 : width, sm_scale);
   p.tree = Tree{(const uint8_t*)tree, ts[0], ts[1], ts[2]};
-  if (int rc = KV_LAUNCH(launch_rows_tree, p)) return rc;
-  return c.splits > 1 ? KV_LAUNCH(launch_join, join_params(p, p.max_len, c.splits, c.share, 32)) : KV_OK;
+  if (int rc = few_rows(c.rows) ? KV_LAUNCH(launch_rows_tree, p) : KV_LAUNCH(launch_tree, p)) return rc;
+  return c.splits > 1 ? KV_LAUNCH(launch_join, join_params(p, p.max_len, c.splits, c.share, c.tile)) : KV_OK;
 }
 
 int kv_paged_append(const void* k, const void* v, void* k_pages, void* v_pages, const int32_t* page_table, int64_t table_stride,

@@ -148,6 +148,17 @@ template <> int launch_sum<ElemT, KV_DGROUP>(const SumParams& p, int D, hipStrea
 #else
 template <> int launch_rows_tree<ElemT, KV_DGROUP>(const RowsParams& p, int D, hipStream_t st) { return launch_rows_any<true, true>(p, D, st); }
 #endif
+#elif KV_KIND == 6
+template <int D, int NW> static int launch_tree_shape(const RowsParams& p, hipStream_t st) {
+  static LdsLimit state;
+  return launch(tree_kernel<ElemT, D, NW>, (int64_t)p.B * p.map.Hkv * p.row_tiles * p.splits, NW * 64, TreeShape<ElemT, D, NW>::bytes(), state, p, st);
+}
+template <> int launch_tree<ElemT, KV_DGROUP>(const RowsParams& p, int D, hipStream_t st) {
+  return by_head_dim(D, [&](auto d) {
+    constexpr int DD = decltype(d)::value;
+    return tree_waves(p.map.rows()) == 2 ? launch_tree_shape<DD, 2>(p, st) : launch_tree_shape<DD, 4>(p, st);
+  });
+}
 #elif KV_KIND == 4 && !defined(SA_NO_ASM_KERNELS)
 constexpr size_t long_stages(int n, size_t tile_rows) { return n * 2 * tile_rows * 128 * sizeof(ElemT); }
 static int64_t long_blocks(const sa::TileMap& m) { return (int64_t)m.nbh * m.n_tiles; }

@@ -5,6 +5,7 @@
 #include "../../include/kv_attention.h"
 #include "kv_bwd.h"
 #include "kv_rows.h"
+#include "kv_tree.h"
 #ifndef SA_NO_ASM_KERNELS
 #include "sa_bwd3.h"
 #include "sa_bwd4.h"
@@ -19,6 +20,7 @@ template <typename T, int DGROUP> int launch_cross_dkdv(const BwdParams& p, int 
 template <typename T, int DGROUP> int launch_rows(const RowsParams& p, int D, hipStream_t st);
 template <typename T, int DGROUP> int launch_rows_paged(const RowsParams& p, int D, hipStream_t st);
 template <typename T, int DGROUP> int launch_rows_tree(const RowsParams& p, int D, hipStream_t st);
+template <typename T, int DGROUP> int launch_tree(const RowsParams& p, int D, hipStream_t st);
 template <typename T, int DGROUP> int launch_join(const JoinParams& p, int D, hipStream_t st);
 template <typename T, int DGROUP> int launch_sum(const SumParams& p, int D, hipStream_t st);
 
@@ -132,6 +134,15 @@ constexpr int rows_waves(int row_bytes, bool f32, int64_t workgroups, int share)
   if (row_bytes == 128) return (!many && share >= 24) || (workgroups <= CUS && share > 8) ? 8 : 4;
   if (row_bytes == 256) return many && !f32 ? 2 : 4;
   return row_bytes < 128 ? 4 : row_bytes == 512 ? 2 : 1;
+}
+
+
+// Trees of more rows: waves of 32 rows of a workgroup, and how many tiles (of 64 keys, 32 where rows take more than 256 bytes) a part has.
+constexpr int tree_waves(int64_t rows) { return rows <= 64 ? 2 : 4; }
+inline int tree_share(int64_t workgroups, int64_t tiles) {
+  int64_t share = std::max<int64_t>(4, ceil_div(workgroups * tiles, 2 * CUS));
+  if (getenv("TREE_SHARE")) share = atoi(getenv("TREE_SHARE"));
+  return (int)std::min<int64_t>(std::max<int64_t>(tiles, 1), share);
 }
 
 }  // namespace kv
