@@ -107,6 +107,7 @@ template <typename P> void long_sides(P& p, int B, int Hq, int Hkv, int Tq, int 
 // How the rows kernel goes through the pages.
 struct PagedPlan {
   int64_t nbh, rows, row_tiles, bytes;
+  bool by_rows;              // trees: the rows kernel, or that of tiles
   int splits, share, tile;   // at most that many parts, of up to `share` tiles of `tile` keys
 };
 int plan_paged(PagedPlan& c, int B, int Hq, int Hkv, int T, int D, int page, int width, int C, int R, int dtype) {
@@ -139,14 +140,18 @@ int plan_paged(PagedPlan& c, int B, int Hq, int Hkv, int T, int D, int page, int
 // Trees: the rows kernel, or tiles of rows.
 int plan_tree(PagedPlan& c, int B, int Hq, int Hkv, int T, int D, int page, int width, int dtype) {
   if (int rc = plan_paged(c, B, Hq, Hkv, T, D, page, width, 1, 0x7fffffff, dtype)) return rc;
-  if (few_rows(c.rows)) return KV_OK;
   const int row_bytes = D * elem_size(dtype), waves = tree_waves(c.rows);
+  c.by_rows = tree_by_rows(c.nbh, c.rows, ceil_div((int64_t)width * page, 32), row_bytes, dtype == 0);
+  if (c.by_rows) return KV_OK;
   c.tile = row_bytes <= 256 ? 64 : 32;
   c.row_tiles = ceil_div(c.rows, waves * 32);
   const int64_t tiles = ceil_div((int64_t)width * page, c.tile);
-  c.share = tree_share(c.nbh * c.row_tiles, tiles);
+  c.share = tree_share(c.nbh * c.row_tiles, tiles, row_bytes, waves);
+  // at most 256 MiB of parts
+  const int64_t part = c.nbh * c.rows * (D + 2) * 4;
+  c.share = (int)std::max<int64_t>(c.share, ceil_div(tiles, std::max<int64_t>(1, (256 << 20) / part)));
   c.splits = (int)std::max<int64_t>(1, ceil_div(tiles, c.share));
-  if (!launchable(c.nbh * c.row_tiles * c.splits, waves * 64)) return KV_ERR_TOO_LARGE;
+  if (!launchable(c.nbh * c.row_tiles * c.splits, waves * 128)) return KV_ERR_TOO_LARGE;
   if (c.splits > 1 && c.nbh * c.rows > kMostCount) return KV_ERR_TOO_LARGE;
   c.bytes = c.splits > 1 ? c.splits * c.nbh * c.rows * (D + 2) * 4 : 0;
   return KV_OK;
@@ -446,8 +451,11 @@ int kv_paged_tree_forward(const void* q, const void* k_pages, const void* v_page
   RowsParams p = paged_rows(c, q, k_pages, v_pages, page_table, table_stride, lens, lens_stride, new_lens, new_lens_stride, o, lse, workspace,
                             qs, ks, vs, B, Hq, Hkv, T, D, empty ? 0 : num_pages, page_size, empty ? 0 : width, sm_scale);
   p.tree = Tree{(const uint8_t*)tree, ts[0], ts[1], ts[2]};
-  if (int rc = few_rows(c.rows) ? KV_LAUNCH(launch_rows_tree, p) : KV_LAUNCH(launch_tree, p)) return rc;
-  return c.splits > 1 ? KV_LAUNCH(launch_join, join_params(p, p.max_len, c.splits, c.share, c.tile)) : KV_OK;
+  if (int rc = c.by_rows ? KV_LAUNCH(launch_rows_tree, p) : KV_LAUNCH(launch_tree, p)) return rc;
+  if (c.splits == 1) return KV_OK;
+  JoinParams j = join_params(p, p.max_len, c.splits, c.share, c.tile);
+  j.one_slot = c.nbh * c.rows >= 512;   // 16384 rows of up to 16 parts, D = 128: 22 -> 9 us
+  return KV_LAUNCH(launch_join, j);
 }
 
 int kv_paged_append(const void* k, const void* v, void* k_pages, void* v_pages, const int32_t* page_table, int64_t table_stride,

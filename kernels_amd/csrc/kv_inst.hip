@@ -131,7 +131,7 @@ template <> int launch_join<ElemT, KV_DGROUP>(const JoinParams& p, int D, hipStr
     constexpr int DD = decltype(d)::value;
     static LdsLimit none;
     const int64_t rows = (int64_t)p.B * p.map.Hkv * p.map.rows();
-    if (p.splits <= 8) return launch(join_kernel<ElemT, DD, 1>, ceil_div(rows, 256 / (DD / 4)), 256, 0, none, p, st);
+    if (p.splits <= 8 || p.one_slot) return launch(join_kernel<ElemT, DD, 1>, ceil_div(rows, 256 / (DD / 4)), 256, 0, none, p, st);
     constexpr int NT = 8 * DD / 4 > 256 ? 8 * DD / 4 : 256;
     return launch(join_kernel<ElemT, DD, 8>, ceil_div(rows, NT / (8 * DD / 4)), NT, 0, none, p, st);
   });
@@ -149,14 +149,22 @@ template <> int launch_sum<ElemT, KV_DGROUP>(const SumParams& p, int D, hipStrea
 template <> int launch_rows_tree<ElemT, KV_DGROUP>(const RowsParams& p, int D, hipStream_t st) { return launch_rows_any<true, true>(p, D, st); }
 #endif
 #elif KV_KIND == 6
-template <int D, int NW> static int launch_tree_shape(const RowsParams& p, hipStream_t st) {
+template <int D, int WR, int WK, bool WHOLE> static int launch_tree_pages(const RowsParams& p, hipStream_t st) {
+  using S = TreeShape<ElemT, D, WR, WK, WHOLE>;
   static LdsLimit state;
-  return launch(tree_kernel<ElemT, D, NW>, (int64_t)p.B * p.map.Hkv * p.row_tiles * p.splits, NW * 64, TreeShape<ElemT, D, NW>::bytes(), state, p, st);
+  return launch(tree_kernel<ElemT, D, WR, WK, WHOLE>, (int64_t)p.B * p.map.Hkv * p.row_tiles * p.splits, S::NW * 64, S::bytes(), state, p, st);
+}
+template <int D, int WR, int WK> static int launch_tree_shape(const RowsParams& p, hipStream_t st) {
+  constexpr int rows = TreeShape<ElemT, D, WR, WK, true>::GROUP;   // offsets in a page have 32 bits
+  const int64_t most = (int64_t(1) << 31) / (int64_t)sizeof(ElemT);
+  const bool whole = p.page % rows == 0 && std::max(p.k_sp, p.v_sp) < most && std::max(p.k_st, p.v_st) < most / std::max(p.page, rows);
+  return whole ? launch_tree_pages<D, WR, WK, true>(p, st) : launch_tree_pages<D, WR, WK, false>(p, st);
 }
 template <> int launch_tree<ElemT, KV_DGROUP>(const RowsParams& p, int D, hipStream_t st) {
   return by_head_dim(D, [&](auto d) {
     constexpr int DD = decltype(d)::value;
-    return tree_waves(p.map.rows()) == 2 ? launch_tree_shape<DD, 2>(p, st) : launch_tree_shape<DD, 4>(p, st);
+    constexpr int blocks = fwd_tile<ElemT, DD>() / 32;
+    return tree_waves(p.map.rows()) == 2 ? launch_tree_shape<DD, 2, blocks>(p, st) : launch_tree_shape<DD, 4, 1>(p, st);
   });
 }
 #elif KV_KIND == 4 && !defined(SA_NO_ASM_KERNELS)

@@ -46,21 +46,43 @@ struct Tree {
   const uint8_t* seen;
   int64_t sb, si, sj;
 };
-// Of the 32 keys from k0 on, those that a lane's row sees, in the bits of sa::row_mask: token t of n new ones, the first of them at position base
-// (below 0: the sequence is shorter; a token before its beginning sees nothing).
-SA_DEV uint32_t tree_mask(const Tree& tree, int b, int t, int n, int base, int k0, int h) {
-  if (base + t < 0) return 0;
-  uint32_t mask = sa::row_mask(0, base - k0, h);
-  if (base >= k0 + 32) return mask;
-  const uint8_t* const row = tree.seen + b * tree.sb + t * tree.si;
+// Of the 32 keys from k0 on, those that a lane's row sees, in the bits of sa::row_mask: token t of n new ones (of T), the first of them at position base
+// (below 0: the sequence is shorter; a token before its beginning sees nothing).  A lane needs four runs of four keys; they are fetched together, words
+// where a row's bytes are neighbours (a byte at a time, one after the other, took 2 us and more for each 32 keys).
+SA_DEV uint32_t tree_mask(const Tree& tree, int T, int b, int t, int n, int base, int k0, int h) {
   uint32_t bits = 0;
+  if (base < k0 + 32) {
+    const uint8_t* const row = tree.seen + b * tree.sb + t * tree.si;
+    uint32_t run[4];
+    if (tree.sj == 1 && T >= 4) {
 #pragma unroll
-  for (int e = 0; e < 16; ++e) {
-    const int u = k0 + sa::crow(e, h) - base, j = u < 0 ? 0 : u < n ? u : n - 1;
-    const bool sees = row[j * tree.sj] != 0 && u == j;
-    bits |= (sees ? 1u : 0u) << (8 * (e >> 2) + (e & 3));
+      for (int g = 0; g < 4; ++g) {
+        const int u = k0 + 8 * g + 4 * h - base;
+        __builtin_memcpy(&run[g], row + (u < 0 ? 0 : u < T - 4 ? u : T - 4), 4);
+      }
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {   // what was fetched from beside the run to its place
+        const int u = k0 + 8 * g + 4 * h - base, late = u > T - 4 ? u - (T - 4) : 0, early = u < 0 ? -u : 0;
+        run[g] = late > 3 || early > 3 ? 0 : run[g] >> (8 * late) << (8 * early);
+      }
+    } else {
+      uint32_t one[16];
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const int u = k0 + sa::crow(e, h) - base;
+        one[e] = row[(u < 0 ? 0 : u < T ? u : T - 1) * tree.sj];
+      }
+#pragma unroll
+      for (int g = 0; g < 4; ++g) run[g] = one[4 * g] | one[4 * g + 1] << 8 | one[4 * g + 2] << 16 | one[4 * g + 3] << 24;
+    }
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {   // four bytes that are not 0 -> four bits
+      const uint32_t set = (((run[g] & 0x7f7f7f7fu) + 0x7f7f7f7fu) | run[g]) >> 7 & 0x01010101u;
+      bits |= set * 0x01020408u >> 24 << (8 * g);
+    }
+    bits &= sa::row_mask(base - k0, base + n - k0, h);   // (the bits past the drafted ones: clamped neighbours)
   }
-  return mask | bits;
+  return base + t < 0 ? 0 : bits | sa::row_mask(0, base - k0, h);
 }
 // Those of the 32 keys that any of the wave's rows sees (not only those of the lane), in the order of the keys.
 SA_DEV uint32_t any_row(uint32_t mask) {
@@ -125,6 +147,12 @@ SA_DEV int wave_prefix_sum(int x) {
   return x;
 }
 
+// The first tile of the part `split` of n, as in part_of: mostly a division of 32 bits (one of 64 takes 0.3 us).
+SA_BOTH int part_start(int n, int parts, int split) {
+  const uint64_t x = (uint64_t)(uint32_t)n * (uint32_t)split;
+  return x >> 32 ? (int)(x / (uint32_t)parts) : (int)((uint32_t)x / (uint32_t)parts);
+}
+
 // One part of the keys of 32 rows (r0 and following) of (b, hk).  TREE: every row sees the keys before the new tokens, and of those the ones
 // that the tree says.
 template <typename T, int D, int NW, bool PAGED, bool TREE>
@@ -168,8 +196,13 @@ SA_DEV void rows_part(const RowsParams& p, char* smem_raw, int b, int hk, int sp
   if (p.splits > 1) {
     const int n = last > first ? last - first : 0, parts = parts_of(n, p.share);
     if (split >= parts) return;
-    last = first + (int)((int64_t)n * (split + 1) / parts);
-    first += (int)((int64_t)n * split / parts);
+    if constexpr (TREE) {
+      last = first + part_start(n, parts, split + 1);
+      first += part_start(n, parts, split);
+    } else {
+      last = first + (int)((int64_t)n * (split + 1) / parts);
+      first += (int)((int64_t)n * split / parts);
+    }
   }
   const int64_t part_row = ((int64_t)split * nbh + bh) * rows + r0;
 
@@ -245,7 +278,7 @@ SA_DEV void rows_part(const RowsParams& p, char* smem_raw, int b, int hk, int sp
     if (seen != 0xFFFFFFFFu || k0 < lo_max || k0 + 32 > hi_min) {
       uint32_t mask;
       if constexpr (TREE) {
-        mask = tree_mask(p.tree, b, token, tokens, L - tokens, k0, h) & (seen >> (4 * h));
+        mask = tree_mask(p.tree, p.map.T, b, token, tokens, L - tokens, k0, h) & (seen >> (4 * h));
         if (k0 + 32 > hi_min) seen = any_row(mask);
       } else {
         mask = sa::row_mask(lo - k0, hi - k0, h) & (seen >> (4 * h));
@@ -356,6 +389,7 @@ struct JoinParams {
   Windows win;
   int B, max_len;
   int splits, share, tile;         // as the parts were made: runs of tiles of `tile` keys
+  bool one_slot;                   // many rows: one set of threads to a row however many parts it has
   ChunkDiv by_rows, by_heads;
 };
 
