@@ -8,7 +8,9 @@
 // Bound by memory: every row is read once and written once (twice read, the gradient and x, in the backward).  Two chunks of sixteen
 // bytes to a lane, so that both sides of a pair are a lane's own, whether pairs are neighbours or halves; what lies past `rot`
 // follows in neighbouring chunks.  The lanes of a row add up its squares among themselves.  A group of lanes keeps its token and goes
-// through heads, so that cosines, sines (64 bytes of float32 to 32 of x) and weights are fetched once for several rows.
+// through heads, so that cosines, sines (64 bytes of float32 to 32 of x) and weights are fetched once for several rows; one row at a time: two or four
+// on their way together cost registers, and with them waves (2 x 40 heads x 8192, D = 128, forward and backward 163 us; with two and one rows 185, four and two 190,
+// eight and four 209, before stores past the caches).  2 x 40 x 8192, D = 128, bfloat16: forward 336 MB read and written in 65-71 us, 4.7-5.2 TB/s.
 #pragma once
 #include "kv_common.h"
 
@@ -44,16 +46,21 @@ struct RopeParams {
   float* part;             // backward: [layers, gridDim.x, D] sums of dw, or null
 };
 
-// Elements of a lane's two chunks: offsets a and b, V each.
+// A lane's two chunks of V elements.  Both sides of a pair are a lane's own; and the first chunks of a row's lanes follow each other, as do the second
+// ones, wherever the pairs allow it (halves: where all channels are turned), so that a store covers half of a row.
 template <typename T, int D, bool INTER> struct RopeLane {
   static constexpr int V = RopeLanes<T, D>::V;
-  int a, b, pair;          // pair: of its V cosines and sines
-  bool turned;
+  int a, b;
+  bool a_turned, b_turned;
   SA_DEV RopeLane(int lane, int rot) {
-    pair = V * lane;
-    turned = 2 * pair < rot;
-    a = INTER || !turned ? 2 * pair : pair;
-    b = INTER || !turned ? a + V : rot / 2 + pair;
+    if constexpr (INTER) {
+      a = V * lane, b = D / 2 + V * lane;
+      a_turned = a < rot, b_turned = b < rot;
+    } else {
+      a_turned = b_turned = 2 * V * lane < rot;
+      a = a_turned ? V * lane : 2 * V * lane;
+      b = a_turned ? rot / 2 + V * lane : a + V;
+    }
   }
 };
 template <typename T> SA_DEV void unpack(float* x, const T* from) {
@@ -68,12 +75,13 @@ template <typename T, bool STREAMING> SA_DEV void pack(T* to, const float* x) {
   if constexpr (STREAMING) sa::store_streaming(to, __builtin_bit_cast(u32x4, f));
   else *reinterpret_cast<typename Elem<T>::Frag*>(to) = f;
 }
-template <int V> SA_DEV void load_floats(float (&x)[V], const float* from) {
+template <int N> SA_DEV void load_floats(float* x, const float* from) {
+  typedef float Part __attribute__((ext_vector_type(N < 4 ? N : 4)));
 #pragma unroll
-  for (int e = 0; e < V; e += 4) {
-    const f32x4 f = *reinterpret_cast<const f32x4*>(from + e);
+  for (int e = 0; e < N; e += 4) {
+    const Part f = *reinterpret_cast<const Part*>(from + e);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) x[e + i] = f[i];
+    for (int i = 0; i < (N < 4 ? N : 4); ++i) x[e + i] = f[i];
   }
 }
 // The weights of a lane's channels, in their type or in float32.
@@ -83,8 +91,8 @@ template <typename T, int V> SA_DEV void load_weights(float (&w)[2 * V], const v
   if (!weight) return;
   if (f32) {
     const float* p = reinterpret_cast<const float*>(weight);
-    load_floats<V>(reinterpret_cast<float(&)[V]>(w[0]), p + a);
-    load_floats<V>(reinterpret_cast<float(&)[V]>(w[V]), p + b);
+    load_floats<V>(w, p + a);
+    load_floats<V>(w + V, p + b);
   } else {
     unpack<T>(w, reinterpret_cast<const T*>(weight) + a);
     unpack<T>(w + V, reinterpret_cast<const T*>(weight) + b);
@@ -100,18 +108,27 @@ template <int LANES> SA_DEV float row_sum(float x) {
   if constexpr (LANES >= 32) x += __shfl_xor(x, 16);
   return x;
 }
-template <bool INTER, int V> SA_DEV void turn(float (&x)[2 * V], const float (&c)[V], const float (&s)[V]) {
+// The pairs of a lane: elements 2 e and 2 e + 1 of its two chunks (INTER), or e of each.
+template <bool INTER, int V> SA_DEV void turn(float (&x)[2 * V], const float (&c)[V], const float (&s)[V], bool a_turned, bool b_turned) {
+  auto pairs = [&](int first, int last) {
 #pragma unroll
-  for (int e = 0; e < V; ++e) {
-    const int i = INTER ? 2 * e : e, j = INTER ? 2 * e + 1 : V + e;
-    const float a = x[i], b = x[j];
-    x[i] = a * c[e] - b * s[e];
-    x[j] = b * c[e] + a * s[e];
+    for (int e = first; e < last; ++e) {
+      const int i = INTER ? 2 * e : e, j = INTER ? 2 * e + 1 : V + e;
+      const float a = x[i], b = x[j];
+      x[i] = a * c[e] - b * s[e];
+      x[j] = b * c[e] + a * s[e];
+    }
+  };
+  if constexpr (INTER) {
+    if (a_turned) pairs(0, V / 2);
+    if (b_turned) pairs(V / 2, V);
+  } else if (a_turned) {
+    pairs(0, V);
   }
 }
 // x -> the turned row
-template <int D, int LANES, bool INTER, int V>
-SA_DEV void norm_and_turn(float (&x)[2 * V], const float (&w)[2 * V], const float (&c)[V], const float (&s)[V], bool turned, float eps) {
+template <int D, int LANES, bool INTER, int V, typename Lane>
+SA_DEV void norm_and_turn(float (&x)[2 * V], const float (&w)[2 * V], const float (&c)[V], const float (&s)[V], const Lane& lane, float eps) {
   if (eps > 0.0f) {
     float sum = 0.0f;
 #pragma unroll
@@ -120,7 +137,7 @@ SA_DEV void norm_and_turn(float (&x)[2 * V], const float (&w)[2 * V], const floa
 #pragma unroll
     for (int e = 0; e < 2 * V; ++e) x[e] *= r * w[e];
   }
-  if (turned) turn<INTER>(x, c, s);
+  turn<INTER>(x, c, s, lane.a_turned, lane.b_turned);
 }
 
 // The token of a group of lanes: where it is, and the row of the table.
@@ -135,14 +152,20 @@ SA_DEV RopeToken rope_token(const RopeParams& p, int token) {
   x.live = x.t < clamped_length(p.lens, p.lens_stride, x.b, p.T) && (uint32_t)x.at < (uint32_t)p.table.rows;
   return x;
 }
-template <int V> SA_DEV void load_angles(float (&c)[V], float (&s)[V], const RopeTable& table, int at, int pair) {
-  load_floats<V>(c, table.cos + at * table.cos_st + pair);
-  load_floats<V>(s, table.sin + at * table.sin_st + pair);
+template <bool INTER, int V, typename Lane> SA_DEV void load_angles(float (&c)[V], float (&s)[V], const RopeTable& table, int at, const Lane& lane) {
+  const float *cos = table.cos + at * table.cos_st, *sin = table.sin + at * table.sin_st;
+  if constexpr (INTER) {
+    if (lane.a_turned) load_floats<V / 2>(c, cos + lane.a / 2), load_floats<V / 2>(s, sin + lane.a / 2);
+    if (lane.b_turned) load_floats<V / 2>(c + V / 2, cos + lane.b / 2), load_floats<V / 2>(s + V / 2, sin + lane.b / 2);
+  } else if (lane.a_turned) {
+    load_floats<V>(c, cos + lane.a);
+    load_floats<V>(s, sin + lane.a);
+  }
 }
 
-template <typename T, int D, bool INTER> __global__ __launch_bounds__(256) void rope_kernel(const RopeParams p) {
+template <typename T, int D, bool INTER, bool STREAMING> __global__ __launch_bounds__(256) void rope_kernel(const RopeParams p) {
   using L = RopeLanes<T, D>;
-  constexpr int V = L::V, U = 4;   // rows on their way together
+  constexpr int V = L::V;
   const RopeLane<T, D, INTER> lane(threadIdx.x % L::LANES, p.table.rot);
   const bool keys = (int)blockIdx.y >= p.q_chunks;
   const RopeSide& side = keys ? p.k : p.q;
@@ -152,39 +175,29 @@ template <typename T, int D, bool INTER> __global__ __launch_bounds__(256) void 
   load_weights<T, V>(w, side.weight, p.weights_f32, lane.a, lane.b);
   for (int64_t id = (int64_t)blockIdx.x * L::GROUPS + threadIdx.x / L::LANES; id < tokens; id += step) {
     const RopeToken token = rope_token(p, (int)id);
-    const T* x = reinterpret_cast<const T*>(side.x) + token.b * side.sb + token.t * side.st;
-    T* out = reinterpret_cast<T*>(side.out) + ((int64_t)token.b * side.heads * p.T + token.t) * D;
-    float c[V], s[V];
-    if (token.live && lane.turned) load_angles<V>(c, s, p.table, token.at, lane.pair);
-    for (int h = h0; h < h1; h += U) {
-      float rows[U][2 * V];
+    const T* x = reinterpret_cast<const T*>(side.x) + token.b * side.sb + token.t * side.st + h0 * side.sh;
+    T* out = reinterpret_cast<T*>(side.out) + (((int64_t)token.b * side.heads + h0) * p.T + token.t) * D;
+    float c[V], s[V], row[2 * V];
+    if (token.live) load_angles<INTER>(c, s, p.table, token.at, lane);
+    for (int h = h0; h < h1; ++h, x += side.sh, out += (int64_t)p.T * D) {
+      if (token.live) {
+        unpack<T>(row, x + lane.a);
+        unpack<T>(row + V, x + lane.b);
+        norm_and_turn<D, L::LANES, INTER, V>(row, w, c, s, lane, p.eps);
+      } else {
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int head = h + u < h1 ? h + u : h1 - 1;
-        if (token.live) {
-          unpack<T>(rows[u], x + head * side.sh + lane.a);
-          unpack<T>(rows[u] + V, x + head * side.sh + lane.b);
-        }
+        for (int e = 0; e < 2 * V; ++e) row[e] = 0.0f;
       }
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        if (h + u >= h1) break;
-        if (token.live) norm_and_turn<D, L::LANES, INTER, V>(rows[u], w, c, s, lane.turned, p.eps);
-        else
-#pragma unroll
-          for (int e = 0; e < 2 * V; ++e) rows[u][e] = 0.0f;
-        T* const to = out + (int64_t)(h + u) * p.T * D;
-        pack<T, false>(to + lane.a, rows[u]);
-        pack<T, false>(to + lane.b, rows[u] + V);
-      }
+      pack<T, STREAMING>(out + lane.a, row);
+      pack<T, STREAMING>(out + lane.b, row + V);
     }
   }
 }
 
 // Gradients of x, and in p.part each workgroup's sums of those of the weights, in the order of its tokens and then of its groups of lanes.
-template <typename T, int D, bool INTER> __global__ __launch_bounds__(256) void rope_backward_kernel(const RopeParams p) {
+template <typename T, int D, bool INTER, bool STREAMING> __global__ __launch_bounds__(256) void rope_backward_kernel(const RopeParams p) {
   using L = RopeLanes<T, D>;
-  constexpr int V = L::V, U = 2;
+  constexpr int V = L::V;
   __shared__ __attribute__((aligned(16))) float sums[L::GROUPS * D];
   const RopeLane<T, D, INTER> lane(threadIdx.x % L::LANES, p.table.rot);
   const bool keys = (int)blockIdx.y >= p.q_chunks, norm = p.eps > 0.0f;
@@ -197,58 +210,46 @@ template <typename T, int D, bool INTER> __global__ __launch_bounds__(256) void 
   for (int e = 0; e < 2 * V; ++e) dw[e] = 0.0f;
   for (int64_t id = (int64_t)blockIdx.x * L::GROUPS + threadIdx.x / L::LANES; id < tokens; id += step) {
     const RopeToken token = rope_token(p, (int)id);
-    const T* x = reinterpret_cast<const T*>(side.x) + token.b * side.sb + token.t * side.st;
-    const T* g = reinterpret_cast<const T*>(side.g) + token.b * side.g_sb + token.t * side.g_st;
-    T* out = reinterpret_cast<T*>(side.out) + ((int64_t)token.b * side.heads * p.T + token.t) * D;
-    float c[V], s[V];
-    if (token.live && lane.turned) {
-      load_angles<V>(c, s, p.table, token.at, lane.pair);
+    const T* x = reinterpret_cast<const T*>(side.x) + token.b * side.sb + token.t * side.st + h0 * side.sh;
+    const T* g = reinterpret_cast<const T*>(side.g) + token.b * side.g_sb + token.t * side.g_st + h0 * side.g_sh;
+    T* out = reinterpret_cast<T*>(side.out) + (((int64_t)token.b * side.heads + h0) * p.T + token.t) * D;
+    float c[V], s[V], xs[2 * V], gs[2 * V];
+    if (token.live) {
+      load_angles<INTER>(c, s, p.table, token.at, lane);
 #pragma unroll
       for (int e = 0; e < V; ++e) s[e] = -s[e];
     }
-    for (int h = h0; h < h1; h += U) {
-      float xs[U][2 * V], gs[U][2 * V];
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int head = h + u < h1 ? h + u : h1 - 1;
-        if (token.live) {
-          unpack<T>(gs[u], g + head * side.g_sh + lane.a);
-          unpack<T>(gs[u] + V, g + head * side.g_sh + lane.b);
-          if (norm) {
-            unpack<T>(xs[u], x + head * side.sh + lane.a);
-            unpack<T>(xs[u] + V, x + head * side.sh + lane.b);
-          }
+    for (int h = h0; h < h1; ++h, x += side.sh, g += side.g_sh, out += (int64_t)p.T * D) {
+      if (token.live) {
+        unpack<T>(gs, g + lane.a);
+        unpack<T>(gs + V, g + lane.b);
+        if (norm) {
+          unpack<T>(xs, x + lane.a);
+          unpack<T>(xs + V, x + lane.b);
         }
-      }
+        turn<INTER>(gs, c, s, lane.a_turned, lane.b_turned);
+        if (norm) {
+          float squares = 0.0f, dot = 0.0f;
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        if (h + u >= h1) break;
-        if (token.live) {
-          if (lane.turned) turn<INTER>(gs[u], c, s);
-          if (norm) {
-            float squares = 0.0f, dot = 0.0f;
+          for (int e = 0; e < 2 * V; ++e) squares += xs[e] * xs[e];
+          const float r = rsqrtf(row_sum<L::LANES>(squares) * (1.0f / D) + p.eps);
 #pragma unroll
-            for (int e = 0; e < 2 * V; ++e) squares += xs[u][e] * xs[u][e];
-            const float r = rsqrtf(row_sum<L::LANES>(squares) * (1.0f / D) + p.eps);
-#pragma unroll
-            for (int e = 0; e < 2 * V; ++e) {
-              xs[u][e] *= r;
-              dw[e] += gs[u][e] * xs[u][e];
-              gs[u][e] *= w[e];
-              dot += gs[u][e] * xs[u][e];
-            }
-            const float mean = row_sum<L::LANES>(dot) * (1.0f / D);
-#pragma unroll
-            for (int e = 0; e < 2 * V; ++e) gs[u][e] = r * (gs[u][e] - xs[u][e] * mean);
+          for (int e = 0; e < 2 * V; ++e) {
+            xs[e] *= r;
+            dw[e] += gs[e] * xs[e];
+            gs[e] *= w[e];
+            dot += gs[e] * xs[e];
           }
-        } else {
+          const float mean = row_sum<L::LANES>(dot) * (1.0f / D);
 #pragma unroll
-          for (int e = 0; e < 2 * V; ++e) gs[u][e] = 0.0f;
+          for (int e = 0; e < 2 * V; ++e) gs[e] = r * (gs[e] - xs[e] * mean);
         }
-        T* const to = out + (int64_t)(h + u) * p.T * D;
-        pack<T, false>(to + lane.a, gs[u]);
-        pack<T, false>(to + lane.b, gs[u] + V);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 2 * V; ++e) gs[e] = 0.0f;
       }
+      pack<T, STREAMING>(out + lane.a, gs);
+      pack<T, STREAMING>(out + lane.b, gs + V);
     }
   }
   if (!p.part) return;
@@ -306,9 +307,9 @@ struct AppendRopeParams {
   int chunk, q_chunks, k_chunks;      // layers of the grid: q's, k's, then v's
   ChunkDiv by_tokens, by_page;
 };
-template <typename T, int D, bool INTER> __global__ __launch_bounds__(256) void append_rope_kernel(const AppendRopeParams p) {
+template <typename T, int D, bool INTER, bool STREAMING> __global__ __launch_bounds__(256) void append_rope_kernel(const AppendRopeParams p) {
   using L = RopeLanes<T, D>;
-  constexpr int V = L::V, U = 4;
+  constexpr int V = L::V;
   const int layer = blockIdx.y, kind = layer < p.q_chunks ? 0 : layer < p.q_chunks + p.k_chunks ? 1 : 2;
   const RopeLane<T, D, INTER> lane(threadIdx.x % L::LANES, kind == 2 ? 0 : p.table.rot);
   const int heads = kind == 0 ? p.Hq : p.Hkv, h0 = (layer - (kind == 0 ? 0 : kind == 1 ? p.q_chunks : p.q_chunks + p.k_chunks)) * p.chunk;
@@ -339,29 +340,21 @@ template <typename T, int D, bool INTER> __global__ __launch_bounds__(256) void 
       to = kind == 1 ? reinterpret_cast<T*>(p.k_pages) + page * p.kp_sp + slot * p.kp_st : reinterpret_cast<T*>(p.v_pages) + page * p.vp_sp + slot * p.vp_st;
       to_sh = kind == 1 ? p.kp_sh : p.vp_sh;
     }
-    const T* x = from + b * sb + t * st;
-    float c[V], s[V];
-    if (live && lane.turned) load_angles<V>(c, s, p.table, (int)at, lane.pair);
-    for (int h = h0; h < h1; h += U) {
-      float rows[U][2 * V];
+    const T* x = from + b * sb + t * st + h0 * sh;
+    to += h0 * to_sh;
+    float c[V], s[V], row[2 * V];
+    if (live) load_angles<INTER>(c, s, p.table, (int)at, lane);
+    for (int h = h0; h < h1; ++h, x += sh, to += to_sh) {
+      if (live) {
+        unpack<T>(row, x + lane.a);
+        unpack<T>(row + V, x + lane.b);
+        norm_and_turn<D, L::LANES, INTER, V>(row, w, c, s, lane, eps);
+      } else {
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int head = h + u < h1 ? h + u : h1 - 1;
-        if (live) {
-          unpack<T>(rows[u], x + head * sh + lane.a);
-          unpack<T>(rows[u] + V, x + head * sh + lane.b);
-        }
+        for (int e = 0; e < 2 * V; ++e) row[e] = 0.0f;
       }
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        if (h + u >= h1) break;
-        if (live) norm_and_turn<D, L::LANES, INTER, V>(rows[u], w, c, s, lane.turned, eps);
-        else
-#pragma unroll
-          for (int e = 0; e < 2 * V; ++e) rows[u][e] = 0.0f;
-        pack<T, false>(to + (h + u) * to_sh + lane.a, rows[u]);
-        pack<T, false>(to + (h + u) * to_sh + lane.b, rows[u] + V);
-      }
+      pack<T, STREAMING>(to + lane.a, row);
+      pack<T, STREAMING>(to + lane.b, row + V);
     }
   }
 }

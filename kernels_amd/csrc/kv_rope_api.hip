@@ -26,12 +26,6 @@ int check_weights(const void* q_weight, const void* k_weight, float eps) {
   return ((reinterpret_cast<uintptr_t>(q_weight) | reinterpret_cast<uintptr_t>(k_weight)) & 15u) ? KV_ERR_LAYOUT : KV_OK;
 }
 
-// Workgroups of the backward leave a row of sums each.
-constexpr int64_t kBackwardBlocks = 2048;
-RopeGrid backward_grid(int B, int Hq, int Hkv, int T, int D, int dtype) {
-  return rope_grid((int64_t)B * T, Hq, Hkv, D, elem_size(dtype), kBackwardBlocks);
-}
-
 }  // namespace
 
 extern "C" {
@@ -64,15 +58,16 @@ int kv_qk_norm_rope(const void* q, const void* k, const float* cos, const float*
   if (positions) p.pos_sb = position_strides[0], p.pos_st = position_strides[1];
   p.B = B; p.T = T; p.eps = eps; p.weights_f32 = weights_f32 != 0;
   p.by_tokens = chunk_div(T);
-  const RopeGrid g = rope_grid((int64_t)B * T, Hq, Hkv, D, elem_size(dtype), 1 << 22);
+  const RopeGrid g = forward_grid((int64_t)B * T, Hq, Hkv, D, elem_size(dtype));
   p.chunk = g.chunk; p.q_chunks = g.q_chunks;
-  return by_dtype(dtype, [&](auto tag) { return launch_rope<decltype(tag)>(p, g, D, interleaved != 0, (hipStream_t)stream); });
+  const bool streaming = past_caches((int64_t)B * (Hq + Hkv) * T, D, rot, interleaved != 0, elem_size(dtype));
+  return by_dtype(dtype, [&](auto tag) { return launch_rope<decltype(tag)>(p, g, D, interleaved != 0, streaming, (hipStream_t)stream); });
 }
 
 int64_t kv_qk_norm_rope_backward_workspace(int B, int Hq, int Hkv, int T, int D, int dtype) {
   if (int rc = check_rope(B, Hq, Hkv, T, D, 16, 0, 0.0f, dtype)) return rc;
   if (B == 0 || T == 0 || Hq + Hkv == 0) return 0;
-  const RopeGrid g = backward_grid(B, Hq, Hkv, T, D, dtype);
+  const RopeGrid g = backward_grid((int64_t)B * T, Hq, Hkv, D, elem_size(dtype));
   return (int64_t)g.blocks * (g.q_chunks + g.k_chunks) * D * 4;
 }
 
@@ -87,7 +82,7 @@ int kv_qk_norm_rope_backward(const void* q, const void* k, const void* d_q_out, 
   if ((dq_weight && !q_weight) || (dk_weight && !k_weight)) return KV_ERR_ARG;
   if (((reinterpret_cast<uintptr_t>(dq_weight) | reinterpret_cast<uintptr_t>(dk_weight)) & 15u) != 0) return KV_ERR_LAYOUT;
   if (int rc = check_weights(q_weight, k_weight, eps)) return rc;
-  const RopeGrid g = backward_grid(B, std::max(Hq, 0), std::max(Hkv, 0), T, D, dtype);
+  const RopeGrid g = backward_grid((int64_t)B * T, Hq, Hkv, D, elem_size(dtype));
   RopeParams p{};
   const bool any = B > 0 && T > 0 && Hq + Hkv > 0;
   if (any) {
@@ -118,7 +113,8 @@ int kv_qk_norm_rope_backward(const void* q, const void* k, const void* d_q_out, 
     p.by_tokens = chunk_div(T);
     p.chunk = g.chunk; p.q_chunks = g.q_chunks;
     p.part = weights ? (float*)workspace : nullptr;
-    if (int rc = by_dtype(dtype, [&](auto tag) { return launch_rope_backward<decltype(tag)>(p, g, D, interleaved != 0, (hipStream_t)stream); }))
+    const bool streaming = past_caches((int64_t)B * (Hq + Hkv) * T, D, rot, interleaved != 0, elem_size(dtype));
+    if (int rc = by_dtype(dtype, [&](auto tag) { return launch_rope_backward<decltype(tag)>(p, g, D, interleaved != 0, streaming, (hipStream_t)stream); }))
       return rc;
   }
   if (!weights) return KV_OK;
@@ -173,9 +169,10 @@ int kv_paged_append_rope(const void* q, const void* k, const void* v, void* q_ou
   p.B = B; p.Hq = Hq; p.Hkv = cache ? Hkv : 0; p.T = T; p.width = width; p.num_pages = num_pages; p.page = page_size;
   p.eps = eps;
   p.by_tokens = chunk_div(T); p.by_page = chunk_div(page_size);
-  const RopeGrid g = rope_grid((int64_t)B * T, Hq, p.Hkv, D, elem_size(dtype), 1 << 22);
+  const RopeGrid g = forward_grid((int64_t)B * T, Hq, p.Hkv, D, elem_size(dtype));
   p.chunk = g.chunk; p.q_chunks = g.q_chunks; p.k_chunks = g.k_chunks;
-  return by_dtype(dtype, [&](auto tag) { return launch_append_rope<decltype(tag)>(p, g, D, interleaved != 0, (hipStream_t)stream); });
+  const bool streaming = past_caches((int64_t)B * (Hq + 2 * p.Hkv) * T, D, rot, interleaved != 0, elem_size(dtype));
+  return by_dtype(dtype, [&](auto tag) { return launch_append_rope<decltype(tag)>(p, g, D, interleaved != 0, streaming, (hipStream_t)stream); });
 }
 
 }  // extern "C"

@@ -14,8 +14,9 @@ using ElemT = __bf16;
 #error "KV_DTYPE_ID must be 0, 1 or 2"
 #endif
 
-template <typename F> static int by_shape(int D, bool inter, F&& f) {
-  auto pairs = [&](auto d) { return inter ? f(d, std::true_type{}) : f(d, std::false_type{}); };
+template <typename F> static int by_shape(int D, bool inter, bool streaming, F&& f) {
+  auto stores = [&](auto d, auto i) { return streaming ? f(d, i, std::true_type{}) : f(d, i, std::false_type{}); };
+  auto pairs = [&](auto d) { return inter ? stores(d, std::true_type{}) : stores(d, std::false_type{}); };
   switch (D) {
     case 16: return pairs(std::integral_constant<int, 16>{});
     case 32: return pairs(std::integral_constant<int, 32>{});
@@ -26,15 +27,17 @@ template <typename F> static int by_shape(int D, bool inter, F&& f) {
   return KV_ERR_HEAD_DIM;
 }
 
-template <> int launch_rope<ElemT>(const RopeParams& p, const RopeGrid& g, int D, bool inter, hipStream_t st) {
-  return by_shape(D, inter, [&](auto d, auto i) {
-    rope_kernel<ElemT, decltype(d)::value, decltype(i)::value><<<dim3(g.blocks, g.q_chunks + g.k_chunks), dim3(256), 0, st>>>(p);
+template <> int launch_rope<ElemT>(const RopeParams& p, const RopeGrid& g, int D, bool inter, bool streaming, hipStream_t st) {
+  return by_shape(D, inter, streaming, [&](auto d, auto i, auto s) {
+    rope_kernel<ElemT, decltype(d)::value, decltype(i)::value, decltype(s)::value>
+        <<<dim3(g.blocks, g.q_chunks + g.k_chunks), dim3(256), 0, st>>>(p);
     return (int)hipGetLastError();
   });
 }
-template <> int launch_rope_backward<ElemT>(const RopeParams& p, const RopeGrid& g, int D, bool inter, hipStream_t st) {
-  return by_shape(D, inter, [&](auto d, auto i) {
-    rope_backward_kernel<ElemT, decltype(d)::value, decltype(i)::value><<<dim3(g.blocks, g.q_chunks + g.k_chunks), dim3(256), 0, st>>>(p);
+template <> int launch_rope_backward<ElemT>(const RopeParams& p, const RopeGrid& g, int D, bool inter, bool streaming, hipStream_t st) {
+  return by_shape(D, inter, streaming, [&](auto d, auto i, auto s) {
+    rope_backward_kernel<ElemT, decltype(d)::value, decltype(i)::value, decltype(s)::value>
+        <<<dim3(g.blocks, g.q_chunks + g.k_chunks), dim3(256), 0, st>>>(p);
     return (int)hipGetLastError();
   });
 }
@@ -42,9 +45,10 @@ template <> int launch_rope_sum<ElemT>(const RopeSumParams& p, hipStream_t st) {
   rope_sum_kernel<ElemT><<<dim3(p.D / 16, 2), dim3(256), 0, st>>>(p);
   return (int)hipGetLastError();
 }
-template <> int launch_append_rope<ElemT>(const AppendRopeParams& p, const RopeGrid& g, int D, bool inter, hipStream_t st) {
-  return by_shape(D, inter, [&](auto d, auto i) {
-    append_rope_kernel<ElemT, decltype(d)::value, decltype(i)::value><<<dim3(g.blocks, g.q_chunks + 2 * g.k_chunks), dim3(256), 0, st>>>(p);
+template <> int launch_append_rope<ElemT>(const AppendRopeParams& p, const RopeGrid& g, int D, bool inter, bool streaming, hipStream_t st) {
+  return by_shape(D, inter, streaming, [&](auto d, auto i, auto s) {
+    append_rope_kernel<ElemT, decltype(d)::value, decltype(i)::value, decltype(s)::value>
+        <<<dim3(g.blocks, g.q_chunks + 2 * g.k_chunks), dim3(256), 0, st>>>(p);
     return (int)hipGetLastError();
   });
 }

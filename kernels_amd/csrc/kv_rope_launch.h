@@ -10,22 +10,34 @@ namespace kv {
 struct RopeGrid {
   int chunk, q_chunks, k_chunks, blocks;
 };
-template <typename T> int launch_rope(const RopeParams& p, const RopeGrid& g, int D, bool inter, hipStream_t st);
-template <typename T> int launch_rope_backward(const RopeParams& p, const RopeGrid& g, int D, bool inter, hipStream_t st);
+template <typename T> int launch_rope(const RopeParams& p, const RopeGrid& g, int D, bool inter, bool streaming, hipStream_t st);
+template <typename T> int launch_rope_backward(const RopeParams& p, const RopeGrid& g, int D, bool inter, bool streaming, hipStream_t st);
 template <typename T> int launch_rope_sum(const RopeSumParams& p, hipStream_t st);
-template <typename T> int launch_append_rope(const AppendRopeParams& p, const RopeGrid& g, int D, bool inter, hipStream_t st);
+template <typename T> int launch_append_rope(const AppendRopeParams& p, const RopeGrid& g, int D, bool inter, bool streaming, hipStream_t st);
 
 constexpr int64_t kMostTokens = 0x7fffffff;   // of all sequences: what the kernels count in 31 bits
 inline int64_t rope_tokens_per_block(int D, int elem_size) { return 256 * 32 / (D * elem_size); }   // two chunks of 16 bytes to a lane
-inline RopeGrid rope_grid(int64_t tokens, int Hq, int Hkv, int D, int elem_size, int64_t most_blocks) {
+// A workgroup goes through up to eight heads, fewer where that leaves fewer than `split` workgroups, and a layer has at most most_blocks / layers of them, which go
+// through the tokens.  The backward splits down to 512 and keeps to 1024, whose sums it adds up (forward and backward captured, us, split to 2048 ->
+// 512: 2 x 20 heads x 1024, D = 128 21.5 -> 19.1; 32 x 24 x 200, D = 64 30.0 -> 26.4; at most 2048 -> 1024: 2 x 40 x 8192, D = 128 167 -> 163).
+inline RopeGrid rope_grid(int64_t tokens, int Hq, int Hkv, int D, int elem_size, int64_t split, int64_t most_blocks) {
   const int64_t groups = (tokens + rope_tokens_per_block(D, elem_size) - 1) / rope_tokens_per_block(D, elem_size);
   RopeGrid g{};
   g.chunk = 8;
-  while (g.chunk > 1 && groups * ((Hq + Hkv + g.chunk - 1) / g.chunk) < 2048) g.chunk /= 2;
+  while (g.chunk > 1 && groups * ((Hq + Hkv + g.chunk - 1) / g.chunk) < split) g.chunk /= 2;
   g.q_chunks = (Hq + g.chunk - 1) / g.chunk;
   g.k_chunks = (Hkv + g.chunk - 1) / g.chunk;
   g.blocks = (int)std::max<int64_t>(1, std::min(groups, most_blocks / (g.q_chunks + g.k_chunks)));
   return g;
+}
+inline RopeGrid forward_grid(int64_t tokens, int Hq, int Hkv, int D, int elem_size) { return rope_grid(tokens, Hq, Hkv, D, elem_size, 2048, 1 << 22); }
+inline RopeGrid backward_grid(int64_t tokens, int Hq, int Hkv, int D, int elem_size) { return rope_grid(tokens, Hq, Hkv, D, elem_size, 512, 1024); }
+
+// Stores past the caches, where a call reads and writes more than the L2s of all XCDs hold and each store covers whole lines (of 128 bytes, half of a
+// row).  In us, plain -> past the caches, bfloat16: 2 x 40 heads x 8192, D = 128, forward 76 -> 71, with gradients 189 -> 163; 2 x 2048 of them 20.9 -> 16.5;
+// prompts of up to 2048 tokens of 8 sequences into pages 72 -> 65; half of the channels turned (64 bytes to a line) 80 -> 89.
+inline bool past_caches(int64_t rows, int D, int rot, bool inter, int elem_size) {
+  return D * elem_size >= 256 && (inter || rot == D) && 2 * rows * D * elem_size > (int64_t(32) << 20);
 }
 
 }  // namespace kv
