@@ -68,34 +68,41 @@ static __global__ __launch_bounds__(256) void keep_kernel(const KeepParams p) {
   char* const base = values ? p.v_pages + hd * p.vp_sh + chunk * 16 : p.k_pages + hd * p.kp_sh + chunk * 16;
   const int64_t sp = values ? p.vp_sp : p.kp_sp, st = values ? p.vp_st : p.kp_st;
   const int64_t first = p.first[b * p.first_stride], most = (int64_t)p.width * p.page;
-  auto place = [&](int64_t at) -> char* {   // or null: it is not there
-    if (at < 0 || at >= most) return nullptr;
-    const int entry = div_by((int)at, p.by_page);
-    const int32_t page = p.table[b * p.table_sb + entry];
-    return (uint32_t)page < (uint32_t)p.num_pages ? base + page * sp + ((int)at - entry * p.page) * st : nullptr;
-  };
-  constexpr int U = 4;
+  constexpr int U = 8;     // entries, then the pages of both places, then the bytes are on their way together; no branches around loads
   int before = -1;
   for (int i0 = 0; i0 < p.M; i0 += U) {
+    int32_t entry[U], page[2 * U];
+    int64_t at[2 * U];     // places that are read, and written; -1 past the table
     u32x4 x[U];
-    char* to[U];
-    int n = 0;             // places of these that are on the path
+#pragma unroll
+    for (int u = 0; u < U; ++u) entry[u] = p.kept[b * p.kept_sb + (i0 + u < p.M ? i0 + u : p.M - 1) * p.kept_si];
+    bool on = true;        // still on the path
+    uint32_t path = 0;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      to[u] = nullptr;
-      if (n < u || i0 + u >= p.M) continue;
-      const int32_t j = p.kept[b * p.kept_sb + (i0 + u) * p.kept_si];
-      if (j <= before) continue;
-      before = j, n = u + 1;
-      if (j == i0 + u) continue;
-      const char* const from = place(first + j);
-      to[u] = from ? place(first + i0 + u) : nullptr;
-      if (to[u]) x[u] = *reinterpret_cast<const u32x4*>(from);
+      on = on && i0 + u < p.M && entry[u] > before;
+      before = on ? entry[u] : before;
+      path |= (on ? 1u : 0u) << u;
+      at[u] = first + entry[u], at[U + u] = first + i0 + u;
     }
 #pragma unroll
+    for (int v = 0; v < 2 * U; ++v) {
+      at[v] = at[v] >= 0 && at[v] < most ? at[v] : -1;
+      page[v] = p.table[b * p.table_sb + div_by(at[v] < 0 ? 0 : (int)at[v], p.by_page)];
+    }
+#pragma unroll
+    for (int v = 0; v < 2 * U; ++v) {   // to bytes from the base; what has no place, the first bytes (they are there, and not used)
+      const bool there = at[v] >= 0 && (uint32_t)page[v] < (uint32_t)p.num_pages;
+      if (!there) path &= ~(1u << v % U);
+      const int k = there ? (int)at[v] : 0;
+      at[v] = there ? page[v] * sp + (k - div_by(k, p.by_page) * p.page) * st : 0;
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) x[u] = *reinterpret_cast<const u32x4*>(base + at[u]);
+#pragma unroll
     for (int u = 0; u < U; ++u)
-      if (to[u]) *reinterpret_cast<u32x4*>(to[u]) = x[u];
-    if (n < U) return;
+      if (path >> u & 1) *reinterpret_cast<u32x4*>(base + at[U + u]) = x[u];
+    if (!on) return;
   }
 }
 
