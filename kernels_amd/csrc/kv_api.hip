@@ -454,7 +454,7 @@ int kv_paged_tree_forward(const void* q, const void* k_pages, const void* v_page
   if (int rc = c.by_rows ? KV_LAUNCH(launch_rows_tree, p) : KV_LAUNCH(launch_tree, p)) return rc;
   if (c.splits == 1) return KV_OK;
   JoinParams j = join_params(p, p.max_len, c.splits, c.share, c.tile);
-  j.one_slot = c.nbh * c.rows >= 512;   // 16384 rows of up to 16 parts, D = 128: 22 -> 9 us
+  j.one_slot = c.nbh * c.rows >= 4096;   // 16384 rows of up to 16 parts, D = 128: 22 -> 9 us; 512 of 64: 4.4 -> 8
   return KV_LAUNCH(launch_join, j);
 }
 
