@@ -230,8 +230,9 @@ template <typename T, int D, int WR, int WK, bool WHOLE> SA_DEV void tree_part(c
 template <typename T, int D, int WR, int WK, bool WHOLE> __global__ __launch_bounds__(WR * WK * 64) void tree_kernel(const RowsParams p) {
   extern __shared__ __attribute__((aligned(16))) char smem_raw[];
   const int x = div_by(blockIdx.x, p.by_pairs), split = div_by(x, p.by_row_tiles);
-  const int bh = blockIdx.x - x * (p.B * p.map.Hkv), b = div_by(bh, p.by_heads);
-  tree_part<T, D, WR, WK, WHOLE>(p, smem_raw, b, bh - b * p.map.Hkv, split, (x - split * p.row_tiles) * WR * 32);
+  const int bh = blockIdx.x - x * (p.B * p.map.Hkv), in_order = div_by(bh, p.by_heads);
+  const int b = split & 1 ? p.B - 1 - in_order : in_order;
+  tree_part<T, D, WR, WK, WHOLE>(p, smem_raw, b, bh - in_order * p.map.Hkv, split, (x - split * p.row_tiles) * WR * 32);
 }
 
 }  // namespace kv
