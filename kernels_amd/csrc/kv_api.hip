@@ -448,14 +448,14 @@ int kv_paged_tree_forward(const void* q, const void* k_pages, const void* v_page
   }
   if (int rc = check_out(o)) return rc;
   if (int rc = check_workspace(workspace, workspace_bytes, c.bytes)) return rc;
-  RowsParams p = paged_rows(c, q, k_pages, v_pages, page_table, table_stride, lens, lens_stride, new_lens, new_lens_stride, o, lse, workspace,
-                            qs, ks, vs, B, Hq, Hkv, T, D, empty ? 0 : num_pages, page_size, empty ? 0 : width, sm_scale);
+  TreeParams p{paged_rows(c, q, k_pages, v_pages, page_table, table_stride, lens, lens_stride, new_lens, new_lens_stride, o, lse, workspace,
+                            qs, ks, vs, B, Hq, Hkv, T, D, empty ? 0 : num_pages, page_size, empty ? 0 : width, sm_scale)};
   p.tree = Tree{(const uint8_t*)tree, ts[0], ts[1], ts[2]};
   if (int rc = c.by_rows ? KV_LAUNCH(launch_rows_tree, p) : KV_LAUNCH(launch_tree, p)) return rc;
   if (c.splits == 1) return KV_OK;
-  JoinParams j = join_params(p, p.max_len, c.splits, c.share, c.tile);
-  j.one_slot = c.nbh * c.rows >= 4096;   // 16384 rows of up to 16 parts, D = 128: 22 -> 9 us; 512 of 64: 4.4 -> 8
-  return KV_LAUNCH(launch_join, j);
+  const JoinParams j = join_params(p, p.max_len, c.splits, c.share, c.tile);
+  // many rows fill the GPU by themselves: 16384 of up to 16 parts, D = 128 22 -> 9 us; 512 of 64: 4.4 -> 8
+  return c.nbh * c.rows >= 4096 ? KV_LAUNCH(launch_join_many, j) : KV_LAUNCH(launch_join, j);
 }
 
 int kv_paged_append(const void* k, const void* v, void* k_pages, void* v_pages, const int32_t* page_table, int64_t table_stride,

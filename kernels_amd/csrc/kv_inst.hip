@@ -99,7 +99,7 @@ template <> int launch_cross_dkdv<ElemT, KV_DGROUP>(const BwdParams& p, int D, h
   });
 }
 #elif KV_KIND == 3 || KV_KIND == 5
-template <int D, int NW, bool PAGED, bool TREE> static int launch_rows_shape(const RowsParams& p, int64_t blocks, hipStream_t st) {
+template <int D, int NW, bool PAGED, bool TREE> static int launch_rows_shape(const RowsParamsOf<TREE>& p, int64_t blocks, hipStream_t st) {
   constexpr int row_bytes = D * (int)sizeof(ElemT), lds = RowsShape<ElemT, D, NW>::bytes(PAGED), places = CUS * (163840 / lds);
   // by length where there are many workgroups: only the waves that many workgroups have
   if constexpr (row_bytes >= 128 && NW == rows_waves(row_bytes, sizeof(ElemT) == 4, 2 * CUS, 1)) {
@@ -111,7 +111,7 @@ template <int D, int NW, bool PAGED, bool TREE> static int launch_rows_shape(con
   static LdsLimit state;
   return launch(rows_kernel<ElemT, D, NW, PAGED, TREE>, blocks, NW * 64, lds, state, p, st);
 }
-template <bool PAGED, bool TREE> static int launch_rows_any(const RowsParams& p, int D, hipStream_t st) {
+template <bool PAGED, bool TREE> static int launch_rows_any(const RowsParamsOf<TREE>& p, int D, hipStream_t st) {
   return by_head_dim(D, [&](auto d) {
     constexpr int DD = decltype(d)::value, ROW = DD * (int)sizeof(ElemT);
     const int64_t blocks = (int64_t)p.B * p.map.Hkv * p.row_tiles * p.splits;
@@ -131,7 +131,7 @@ template <> int launch_join<ElemT, KV_DGROUP>(const JoinParams& p, int D, hipStr
     constexpr int DD = decltype(d)::value;
     static LdsLimit none;
     const int64_t rows = (int64_t)p.B * p.map.Hkv * p.map.rows();
-    if (p.splits <= 8 || p.one_slot) return launch(join_kernel<ElemT, DD, 1>, ceil_div(rows, 256 / (DD / 4)), 256, 0, none, p, st);
+    if (p.splits <= 8) return launch(join_kernel<ElemT, DD, 1>, ceil_div(rows, 256 / (DD / 4)), 256, 0, none, p, st);
     constexpr int NT = 8 * DD / 4 > 256 ? 8 * DD / 4 : 256;
     return launch(join_kernel<ElemT, DD, 8>, ceil_div(rows, NT / (8 * DD / 4)), NT, 0, none, p, st);
   });
@@ -146,25 +146,32 @@ template <> int launch_sum<ElemT, KV_DGROUP>(const SumParams& p, int D, hipStrea
   });
 }
 #else
-template <> int launch_rows_tree<ElemT, KV_DGROUP>(const RowsParams& p, int D, hipStream_t st) { return launch_rows_any<true, true>(p, D, st); }
+template <> int launch_rows_tree<ElemT, KV_DGROUP>(const TreeParams& p, int D, hipStream_t st) { return launch_rows_any<true, true>(p, D, st); }
 #endif
 #elif KV_KIND == 6
-template <int D, int WR, int WK, bool WHOLE> static int launch_tree_pages(const RowsParams& p, hipStream_t st) {
+template <int D, int WR, int WK, bool WHOLE> static int launch_tree_pages(const TreeParams& p, hipStream_t st) {
   using S = TreeShape<ElemT, D, WR, WK, WHOLE>;
   static LdsLimit state;
   return launch(tree_kernel<ElemT, D, WR, WK, WHOLE>, (int64_t)p.B * p.map.Hkv * p.row_tiles * p.splits, S::NW * 64, S::bytes(), state, p, st);
 }
-template <int D, int WR, int WK> static int launch_tree_shape(const RowsParams& p, hipStream_t st) {
+template <int D, int WR, int WK> static int launch_tree_shape(const TreeParams& p, hipStream_t st) {
   constexpr int rows = TreeShape<ElemT, D, WR, WK, true>::GROUP;   // offsets in a page have 32 bits
   const int64_t most = (int64_t(1) << 31) / (int64_t)sizeof(ElemT);
   const bool whole = p.page % rows == 0 && std::max(p.k_sp, p.v_sp) < most && std::max(p.k_st, p.v_st) < most / std::max(p.page, rows);
   return whole ? launch_tree_pages<D, WR, WK, true>(p, st) : launch_tree_pages<D, WR, WK, false>(p, st);
 }
-template <> int launch_tree<ElemT, KV_DGROUP>(const RowsParams& p, int D, hipStream_t st) {
+template <> int launch_tree<ElemT, KV_DGROUP>(const TreeParams& p, int D, hipStream_t st) {
   return by_head_dim(D, [&](auto d) {
     constexpr int DD = decltype(d)::value;
     constexpr int blocks = fwd_tile<ElemT, DD>() / 32;
     return tree_waves(p.map.rows()) == 2 ? launch_tree_shape<DD, 2, blocks>(p, st) : launch_tree_shape<DD, 4, 1>(p, st);
+  });
+}
+template <> int launch_join_many<ElemT, KV_DGROUP>(const JoinParams& p, int D, hipStream_t st) {
+  return by_head_dim(D, [&](auto d) {
+    constexpr int DD = decltype(d)::value;
+    static LdsLimit none;
+    return launch(join_kernel<ElemT, DD, 1>, ceil_div((int64_t)p.B * p.map.Hkv * p.map.rows(), 256 / (DD / 4)), 256, 0, none, p, st);
   });
 }
 #elif KV_KIND == 4 && !defined(SA_NO_ASM_KERNELS)

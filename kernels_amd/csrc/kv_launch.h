@@ -19,9 +19,10 @@ template <typename T, int DGROUP> int launch_cross_dq(const BwdParams& p, int D,
 template <typename T, int DGROUP> int launch_cross_dkdv(const BwdParams& p, int D, hipStream_t st);
 template <typename T, int DGROUP> int launch_rows(const RowsParams& p, int D, hipStream_t st);
 template <typename T, int DGROUP> int launch_rows_paged(const RowsParams& p, int D, hipStream_t st);
-template <typename T, int DGROUP> int launch_rows_tree(const RowsParams& p, int D, hipStream_t st);
-template <typename T, int DGROUP> int launch_tree(const RowsParams& p, int D, hipStream_t st);
+template <typename T, int DGROUP> int launch_rows_tree(const TreeParams& p, int D, hipStream_t st);
+template <typename T, int DGROUP> int launch_tree(const TreeParams& p, int D, hipStream_t st);
 template <typename T, int DGROUP> int launch_join(const JoinParams& p, int D, hipStream_t st);
+template <typename T, int DGROUP> int launch_join_many(const JoinParams& p, int D, hipStream_t st);   // one set of threads to a row, however many parts
 template <typename T, int DGROUP> int launch_sum(const SumParams& p, int D, hipStream_t st);
 
 // The hand-scheduled kernels of streaming attention on another sequence's keys: 16-bit elements, head dimension 128.  -DSA_NO_ASM_KERNELS

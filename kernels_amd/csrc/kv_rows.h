@@ -113,7 +113,6 @@ struct RowsParams {
   int width, num_pages, page;
   ChunkDiv by_page;
   Windows win;
-  Tree tree;             // of the kernels that go by one, in place of the windows
   // division of the work
   int splits, share;     // the most parts that the tiles of 32 keys of a row tile are divided into, and the most tiles of a part
   int row_tiles;
@@ -121,6 +120,11 @@ struct RowsParams {
   float* part_o;         // [splits, B * Hkv, rows, D]
   float* part_ml;        // [splits, B * Hkv, rows, 2]
 };
+
+struct TreeParams : RowsParams {
+  Tree tree;             // in place of the windows
+};
+template <bool TREE> using RowsParamsOf = std::conditional_t<TREE, TreeParams, RowsParams>;
 
 // A wave's rings take 16 KiB at rows of 128 bytes; a workgroup has NW waves (rows_waves in kv_launch.h).
 template <typename T, int D, int NW> struct RowsShape {
@@ -156,7 +160,7 @@ SA_BOTH int part_start(int n, int parts, int split) {
 // One part of the keys of 32 rows (r0 and following) of (b, hk).  TREE: every row sees the keys before the new tokens, and of those the ones
 // that the tree says.
 template <typename T, int D, int NW, bool PAGED, bool TREE>
-SA_DEV void rows_part(const RowsParams& p, char* smem_raw, int b, int hk, int split, int r0) {
+SA_DEV void rows_part(const RowsParamsOf<TREE>& p, char* smem_raw, int b, int hk, int split, int r0) {
   using G = Geom<T, D>;
   using S = RowsShape<T, D, NW>;
   using Frag = typename Elem<T>::Frag;
@@ -340,7 +344,7 @@ SA_DEV void rows_part(const RowsParams& p, char* smem_raw, int b, int hk, int sp
 
 // A workgroup for each part that there may be.
 template <typename T, int D, int NW, bool PAGED, bool TREE = false>
-__global__ __launch_bounds__(NW * 64) void rows_kernel(const RowsParams p) {
+__global__ __launch_bounds__(NW * 64) void rows_kernel(const RowsParamsOf<TREE> p) {
   extern __shared__ __attribute__((aligned(16))) char smem_raw[];
   // the splits and row tiles of a pair lie a multiple of the pairs apart: on one XCD where eight divides the pairs
   const int x = div_by(blockIdx.x, p.by_pairs), split = div_by(x, p.by_row_tiles);
@@ -350,7 +354,7 @@ __global__ __launch_bounds__(NW * 64) void rows_kernel(const RowsParams p) {
 // By length: as many workgroups as there are places; each takes the parts that lie the grid apart, of those that the lengths leave, whatever
 // sequence they are of.  Lane l holds, of the sequences l, l + 64, ..., how many parts there are up to and with each.
 template <typename T, int D, int NW, bool PAGED, bool TREE = false>
-__global__ __launch_bounds__(NW * 64) void rows_by_length_kernel(const RowsParams p) {
+__global__ __launch_bounds__(NW * 64) void rows_by_length_kernel(const RowsParamsOf<TREE> p) {
   extern __shared__ __attribute__((aligned(16))) char smem_raw[];
   constexpr int GROUPS = MAX_BY_LENGTH / 64;
   const int lane = threadIdx.x & 63;
@@ -389,7 +393,6 @@ struct JoinParams {
   Windows win;
   int B, max_len;
   int splits, share, tile;         // as the parts were made: runs of tiles of `tile` keys
-  bool one_slot;                   // many rows: one set of threads to a row however many parts it has
   ChunkDiv by_rows, by_heads;
 };
 

@@ -29,7 +29,7 @@ template <typename T, int D, int WR, int WK, bool WHOLE> struct TreeShape {
 };
 
 // The part `split` of the keys, for rows r0 and following of (b, hk).  WHOLE: sixteen rows (and those of a copy) lie in one page.
-template <typename T, int D, int WR, int WK, bool WHOLE> SA_DEV void tree_part(const RowsParams& p, char* smem_raw, int b, int hk, int split, int r0) {
+template <typename T, int D, int WR, int WK, bool WHOLE> SA_DEV void tree_part(const TreeParams& p, char* smem_raw, int b, int hk, int split, int r0) {
   using G = Geom<T, D>;
   using S = TreeShape<T, D, WR, WK, WHOLE>;
   using Frag = typename Elem<T>::Frag;
@@ -227,7 +227,7 @@ template <typename T, int D, int WR, int WK, bool WHOLE> SA_DEV void tree_part(c
 }
 
 // A workgroup for each part that there may be.
-template <typename T, int D, int WR, int WK, bool WHOLE> __global__ __launch_bounds__(WR * WK * 64) void tree_kernel(const RowsParams p) {
+template <typename T, int D, int WR, int WK, bool WHOLE> __global__ __launch_bounds__(WR * WK * 64) void tree_kernel(const TreeParams p) {
   extern __shared__ __attribute__((aligned(16))) char smem_raw[];
   const int x = div_by(blockIdx.x, p.by_pairs), split = div_by(x, p.by_row_tiles);
   const int bh = blockIdx.x - x * (p.B * p.map.Hkv), in_order = div_by(bh, p.by_heads);
