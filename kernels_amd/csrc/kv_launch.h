@@ -137,10 +137,9 @@ constexpr int rows_waves(int row_bytes, bool f32, int64_t workgroups, int share)
   return row_bytes < 128 ? 4 : row_bytes == 512 ? 2 : 1;
 }
 
-
 // Trees: the rows kernel up to 32 rows of a key head and for little work altogether (blocks of 32 rows times tiles of 32 keys: few for each wave
 // of the GPU), else the tile kernel.  Rows -> tiles, in us, D = 128, bfloat16: 64 rows, 8 key heads of 1000 12.3 -> 15.3, of 4096 14.9 -> 16.1; 256 rows, 8 of
-// 4096 (8192 blocks) 22.3 -> 23.9; 64 rows, 96 of 2000 (12096) 27.9 -> 25.7; 128 rows, 16 of 8192 31.5 -> 26.8; 256 rows, 64 of 8192 201 -> 92.  D = 256: 40
+// 4096 (8192 blocks) 22.3 -> 23.9; 64 rows, 96 of 2000 (12096) 27.9 -> 25.7; 128 rows, 16 of 8192 31.5 -> 27; 256 rows, 64 of 8192 201 -> 92.  D = 256: 40
 // rows, 16 of 500 18.7-25 -> 20, 64 of 2000 45-72 -> 32.  float32: 40 rows, 32 of 1000, D = 64 (2048) 15.2 -> 20.7; 256 rows, 16 of 2000, D = 128 95 -> 56.
 inline bool tree_by_rows(int64_t units, int64_t rows, int64_t tiles, int row_bytes, bool f32) {
   const int64_t blocks = units * ceil_div(rows, 32) * tiles;
@@ -152,10 +151,11 @@ inline bool tree_by_rows(int64_t units, int64_t rows, int64_t tiles, int row_byt
 constexpr int tree_waves(int64_t rows) { return rows <= 64 ? 2 : 4; }
 // Tiles (of 64 keys, or of 32 where rows take more than 256 bytes) of a part: what leaves a workgroup for each place, at least eight, or four where
 // those leave half of the CUs without one, at most 2048 keys (1024 for four waves at D <= 64): a part writes and reads again 520 bytes for each of its rows at
-// D = 128, an eighth of the keys and values of 2048 for 128 rows.  In us for shares of 4, 8, 16, 32, 64 tiles (* chosen), bfloat16: 64 rows, D = 128, 256
-// key heads log-uniform up to 8192 83, 63, 56, 50*, 85; from 4096 on 263, 208, 184, 172*, 168; from 1 on 167, 137, 120, 124*, 122; 96 of 2000 31.7, 25.7*,
-// 27.5, 37.1; 256 rows, 64 of 8192 198, 138, 108, 95*, 116; 128 rows, 16 of 8192 31.7, 27.2*, 34.2, 52.8; D = 64: 48 rows, 256 up to 4096 56, 50, 50,
-// 44*, 58; 100 rows, 256 from 1 to 4000 59, 53, 48*, 59, 73; D = 256: 80 rows, 64 of up to 2000 66, 50, 42*, 62.
+// D = 128, an eighth of the keys and values of 2048 for 128 rows.  In us for shares of 4, 8, 16, 32 tiles (* chosen), means over three sets of
+// lengths, bfloat16: 64 rows, D = 128, 256 key heads of 8192 307, 273, 236, 217*; from 4096 on 240, 212, 190, 178*; from 1 on 174, 154, 135, 136*; log-uniform
+// 87, 76, 69, 65*; 96 of 2000 37, 28*, 28, 38; 256 rows, 64 of 8192 172, 134, 108, 95*, log-uniform 71, 62, 56, 72*; 128 rows, 128 of 4096 120, 92, 79*, 67,
+// from 1 on 68, 55, 50*, 58, log-uniform 46, 40, 45*, 57; 240 rows, 15 of 6000 43, 36*, 36, 55; D = 64: 60 rows, 192 of 4000 55, 46, 41*, 41, log-uniform 28, 24, 26*, 36;
+// 100 rows, 128 of 4000 55, 46, 42*, 50; D = 256: 80 rows, 64 of up to 2000 66, 50, 42*, 62.
 inline int tree_share(int64_t workgroups, int64_t tiles, int row_bytes, int waves) {
   const int64_t places = waves == 2 ? (row_bytes <= 128 ? 3 : 2) : (row_bytes <= 128 ? 3 : row_bytes == 256 ? 2 : 1);
   const int64_t least = workgroups * ceil_div(tiles, 8) > CUS / 2 ? 8 : 4;

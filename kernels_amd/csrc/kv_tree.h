@@ -1,9 +1,19 @@
-// Trees of drafted tokens over a cache in pages, from 33 rows of a key head on (up to 32: kv_rows.h).
+// Trees of drafted tokens over a cache in pages, for more than 32 rows of a key head (few rows, and little work: kv_rows.h).
 //
-// The tile kernel of kv_fwd.h with keys in pages: NW waves of 32 rows share tiles of TK keys, which go through LDS once for all of them, in two
-// stages.  Each lane forms the place of one key of the next tile from its page, and hands it to the lanes that copy that row.  Every row sees the
-// keys before the drafted tokens, so masks are formed only where a tile reaches those, or where pages are missing; there the waves also tell
-// each other which keys some row sees, and values that none does become zeros.
+//   O = softmax(scale * Q K^T) V over the keys before the drafted tokens and those of the drafted ones that the tree names
+//
+// The tile kernel of kv_fwd.h with keys in pages: waves of 32 rows share tiles of TK keys, which go through LDS once for all of them, in two stages, so
+// that K and V are read from memory once for 64 or 128 rows.  WR waves have rows of their own; up to 64 rows WK = 2 waves share each block of rows, one
+// half of a tile's keys each, and add up their sums at the end: a tile's chain of products and exponentials, of which a wave can hide little, is half as
+// long.  Each lane forms the place of one key of the next tile from its page.  WHOLE (pages of a multiple of sixteen positions): places are handed on in scalar
+// registers, one for sixteen rows; other pages through LDS, one for each row.  Every row sees the keys before the drafted tokens, so masks are
+// formed only where a tile reaches those, or where pages are missing; there the waves also tell each other which keys some row sees, and values
+// that none does become zeros.
+//
+// Bound by memory up to 64 rows, by vector and matrix instructions, which hardly overlap, above: 64 rows, D = 128, bfloat16, 256 key heads of 8192 (1.07 GB)
+// 217 us, 5.0 TB/s, log-uniform up to 8192 52-91 us for 38-69 us of a copy's rate; 256 rows, 64 of 8192 92 us, 0.75 PFLOP/s, matrix units busy 43 %, vector units 43 %
+// of the time.  64 rows in us: two waves of rows alone 64 (log-uniform) and 187 (from 4096 on), with places in scalar registers 59 and 179, two waves to each block
+// of rows 52 and 172.
 #pragma once
 #include "kv_rows.h"
 
@@ -231,6 +241,7 @@ template <typename T, int D, int WR, int WK, bool WHOLE> __global__ __launch_bou
   extern __shared__ __attribute__((aligned(16))) char smem_raw[];
   const int x = div_by(blockIdx.x, p.by_pairs), split = div_by(x, p.by_row_tiles);
   const int bh = blockIdx.x - x * (p.B * p.map.Hkv), in_order = div_by(bh, p.by_heads);
+  // the second parts of the sequences in reverse order: the places of a CU go to parts of different sequences (log-uniform up to 8192 69-101 -> 62-92 us)
   const int b = split & 1 ? p.B - 1 - in_order : in_order;
   tree_part<T, D, WR, WK, WHOLE>(p, smem_raw, b, bh - in_order * p.map.Hkv, split, (x - split * p.row_tiles) * WR * 32);
 }
