@@ -27,7 +27,7 @@ inline RopeGrid rope_grid(int64_t tokens, int Hq, int Hkv, int D, int elem_size,
   while (g.chunk > 1 && groups * ((Hq + Hkv + g.chunk - 1) / g.chunk) < split) g.chunk /= 2;
   g.q_chunks = (Hq + g.chunk - 1) / g.chunk;
   g.k_chunks = (Hkv + g.chunk - 1) / g.chunk;
-  g.blocks = (int)std::max<int64_t>(1, std::min(groups, most_blocks / (g.q_chunks + g.k_chunks)));
+  g.blocks = (int)std::max<int64_t>(1, std::min(groups, most_blocks / std::max(1, g.q_chunks + g.k_chunks)));
   return g;
 }
 inline RopeGrid forward_grid(int64_t tokens, int Hq, int Hkv, int D, int elem_size) { return rope_grid(tokens, Hq, Hkv, D, elem_size, 2048, 1 << 22); }

@@ -78,6 +78,19 @@ def test_rope_codes(lib):
     assert lib.kv_qk_norm_rope_backward_workspace(64, 64, 64, 1 << 16, 256, 0) <= 1 << 24   # sums of workgroups, not of tokens
 
 
+def test_rope_without_heads(lib):
+    """No query or key heads, or neither: nothing to do, whatever else stands there."""
+    def call(B, T):
+        return lib.kv_qk_norm_rope_backward(None, None, None, None, None, None, 0, 0, None, None, 0, None, 0, None, None, None, None, None, None,
+                                            None, 0, None, None, None, None, B, 0, 0, T, 64, 64, 0, 0, 1e-6, 2, None)
+
+    for B, T in ((1, 8), (0, 8), (3, 0)):
+        assert call(B, T) == 0
+        assert lib.kv_qk_norm_rope_backward_workspace(B, 0, 0, T, 64, 2) == 0
+        assert lib.kv_qk_norm_rope(None, None, None, None, 0, 0, None, None, 0, None, 0, None, None, None, None, None, None, B, 0, 0, T, 64, 64, 0, 0,
+                                   1e-6, 2, None) == 0
+
+
 def test_tree_and_keep_codes(lib):
     buf, p = _buffer()
     st, three = _strides(8 * 64, 8 * 64, 64, 1), _strides(1, 1, 1)
