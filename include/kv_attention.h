@@ -116,7 +116,8 @@ int kv_paged_tree_forward(const void* q, const void* k_pages, const void* v_page
 
 /* Keeps accepted tokens: K and V of position first[b] + kept[b][i] go to position first[b] + i, for i = 0, 1, ... up to the first entry that is
  * negative or not above the one before it, or M of them.  kept: int32 at the strides int64[2] (batch, entry).  Where the one or the other position is below
- * 0, past the table or on a page that is not there, the place stays as it is.  Pages that a call writes are of one sequence each. */
+ * 0, past the table or on a page that is not there, the place stays as it is.  Pages that a call writes stand once in the table, and K and V are
+ * one cache or do not overlap. */
 int kv_paged_keep(void* k_pages, void* v_pages, const int32_t* page_table, int64_t table_stride,
                   const int32_t* first, int64_t first_stride, const int32_t* kept, const int64_t* kept_strides,
                   const int64_t* k_page_strides, const int64_t* v_page_strides,

@@ -516,7 +516,9 @@ int kv_paged_keep(void* k_pages, void* v_pages, const int32_t* page_table, int64
   if ((int64_t)B * H > kMostCount / p.chunks) return KV_ERR_TOO_LARGE;
   p.total = (int64_t)B * H * p.chunks;
   p.by_chunks = chunk_div(p.chunks); p.by_heads = chunk_div(H); p.by_page = chunk_div(page_size);
-  keep_kernel<<<dim3((unsigned)ceil_div(p.total, 256), 2), dim3(256), 0, (hipStream_t)stream>>>(p);
+  // keys that are the values too move once: the second set of threads would read what the first has written
+  const bool one = k_pages == v_pages && p.kp_sp == p.vp_sp && p.kp_sh == p.vp_sh && p.kp_st == p.vp_st;
+  keep_kernel<<<dim3((unsigned)ceil_div(p.total, 256), one ? 1 : 2), dim3(256), 0, (hipStream_t)stream>>>(p);
   return (int)hipGetLastError();
 }
 

@@ -145,7 +145,8 @@ def paged_append_rope(
     :func:`paged_tree_attention`.
 
     Args:
-        q, k, v, k_pages, v_pages, page_table, lens, new_lens: as for :func:`paged_append` and :func:`paged_attention`
+        q, k, v, k_pages, v_pages, page_table, lens, new_lens: as for :func:`paged_append` and :func:`paged_attention`; the pages
+            of keys and values, and what goes into them, must not overlap
         cos, sin, q_weight, k_weight, eps, interleaved: as for :func:`qk_norm_rope.qk_norm_rope`; no norms by default
         positions: ``(batch, tokens)`` int32 positions of the angles, or None: where the token goes, ``lens[b] - n + i``.  Drafted tokens of a tree
             stand behind each other in the cache, but each at the position of its depth
@@ -235,8 +236,9 @@ def paged_keep(
             first entry that is negative (-1 behind a shorter path) or not above the one before it: a token's ancestors stand before it
 
     ``first[b]`` and the number of kept tokens make the new length, which the caller counts.  Entries whose old or new place is not there (past the
-    table, on a missing page) are left out; everything else in the cache stays as it is.  Pages that a call writes must not be shared
-    between sequences.  Records no gradient.
+    table, on a missing page) are left out; everything else in the cache stays as it is.  Pages that a call writes must stand
+    in the table once, and the pages of keys and values must be the same or not overlap.  Records no gradient: call it under
+    ``torch.no_grad()`` or on detached tensors.
     """
     if ops.takes_native_call(k_pages, v_pages, page_table, first, kept):
         if _eager_keep(k_pages, v_pages, page_table, first, kept) is not NotImplemented:

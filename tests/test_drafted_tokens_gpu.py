@@ -280,6 +280,21 @@ def test_append_rope_without_a_cache():
         assert torch.equal(paged_append_rope(q, k, k, pages, pages.clone(), table, lens, *tables), want)
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("D", [64, 128])
+def test_values_go_as_they_are(dtype, D):
+    """Every pattern of 16 bits: subnormal numbers, infinities, both zeros; what is not a number stays none."""
+    v = torch.arange(-2 ** 15, 2 ** 15).to(torch.int16).view(dtype).view(1, 1, -1, D)
+    T, page = v.shape[2], 64
+    q = torch.zeros(1, 1, T, D, dtype=dtype)
+    pages = [torch.zeros(T // page, 1, page, D, dtype=dtype, device=DEV) for _ in range(2)]
+    table = torch.arange(T // page, dtype=torch.int32)[None]
+    paged_append_rope(*_gpu(q, q, v), *pages, *_gpu(table, _i32([T]), *_tables(T, 16)), eps=1e-6)
+    got, want = pages[1].cpu().flatten(), v.flatten()
+    nan = want.isnan()
+    assert torch.equal(got.isnan(), nan) and torch.equal(got.view(torch.int16)[~nan], want.view(torch.int16)[~nan])
+
+
 # ---- accepted tokens ------------------------------------------------------------------------------------------------
 
 def _keep_by_hand(k, v, table, first, kept):
@@ -331,6 +346,19 @@ def test_keep_leaves_out_what_has_no_place():
     got = _gpu(k, v)
     paged_keep(*got, *_gpu(table, first, kept))
     assert torch.equal(got[0].cpu(), want[0]) and torch.equal(got[1].cpu(), want[1])
+
+
+@pytest.mark.parametrize("T", [5, 40])
+def test_keep_of_one_cache(T):
+    """Keys that are the values too move once: every entry one place, so that a second move would take the next one's."""
+    k, _, table = _cache([100] * 300, 4, 128, 16, torch.bfloat16)
+    first = torch.arange(300, dtype=torch.int32) % 50
+    kept = torch.arange(1, T + 1, dtype=torch.int32).expand(300, T)
+    want = k.clone()
+    _keep_by_hand(want, want.clone(), table, first, kept)
+    got = k.to(DEV)
+    paged_keep(got, got, *_gpu(table, first, kept))
+    assert torch.equal(got.cpu(), want)
 
 
 # ---- together -------------------------------------------------------------------------------------------------------

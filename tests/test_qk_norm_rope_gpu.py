@@ -4,6 +4,7 @@ import pytest
 import torch
 
 from cross_attention import cross_attention
+from kv_attention import _lib
 from oracle import kv_oracle
 from qk_norm_rope import qk_norm_rope, qk_norm_rope_reference
 from streaming_attention import streaming_attention
@@ -367,6 +368,30 @@ def test_another_stream_and_threads():
     for t in threads:
         t.join()
     assert not wrong
+
+
+def test_the_smallest_eps():
+    """Rows of zeros over a subnormal eps: zeros, and gradients of g w / sqrt(eps)."""
+    q, k = (torch.zeros(1, h, 3, 64, device=DEV, requires_grad=True) for h in (2, 1))
+    cos, sin = torch.ones(3, 32, device=DEV), torch.zeros(3, 32, device=DEV)
+    for eps in (2.0 ** -126, 2.0 ** -140, 2.0 ** -148):
+        out = qk_norm_rope(q, k, cos, sin, eps=eps)
+        assert all(torch.equal(t, torch.zeros_like(t)) for t in out)
+        for grad in torch.autograd.grad(out, (q, k), [torch.ones_like(t) for t in out]):
+            # the root and three products with it: a few roundings of float32
+            assert ((grad.double() * eps ** 0.5 - 1).abs() <= 8 * 2.0 ** -24).all()
+
+
+def test_weights_without_rows():
+    """No sequence, token or head: the C entry leaves zeros in the weights' gradients."""
+    lib = _lib.load()
+    w = torch.ones(64, device=DEV)
+    for B, Hq, Hkv, T in ((0, 2, 1, 8), (2, 2, 1, 0), (2, 0, 0, 8)):
+        got = [torch.full((64,), 7.0, device=DEV) for _ in range(2)]
+        rc = lib.kv_qk_norm_rope_backward(None, None, None, None, None, None, 0, 0, w.data_ptr(), w.data_ptr(), 1, None, 0, None, None, None, None,
+                                          got[0].data_ptr(), got[1].data_ptr(), None, 0, None, None, None, None, B, Hq, Hkv, T, 64, 64, 0, 0, 1e-6,
+                                          2, torch.cuda.current_stream().cuda_stream)
+        assert rc == 0 and all(torch.equal(t, torch.zeros_like(t)) for t in got)
 
 
 def test_more_than_two_to_the_31_elements():
