@@ -69,8 +69,9 @@ template <typename T, int D, int WR, int WK, bool WHOLE> SA_DEV void tree_part(c
   if (p.splits > 1) {
     const int n = t1, parts = parts_of(n, p.share);
     if (split >= parts) return;   // (the joining kernel knows how many parts there are)
-    t0 = part_start(n, parts, split);
-    t1 = part_start(n, parts, split + 1);
+    // the last part's masks take as long as two tiles: 240 rows, 15 key heads of 6000 33.8 -> 32.3 us, 64 rows, 96 of 2000 26.0 -> 23.8, others 0-6 % less
+    t0 = part_start(n + 2, parts, split), t1 = part_start(n + 2, parts, split + 1);
+    t1 = t1 < n ? t1 : n;
   }
   const float sl2e = fmaxf(fabsf(p.scale_log2e), 1e-30f);   // never exactly 0, so that a masked score of -inf stays -inf after scaling
   const T* const kbase = reinterpret_cast<const T*>(p.k) + hk * p.k_sh;
