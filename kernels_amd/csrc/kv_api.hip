@@ -146,7 +146,7 @@ int plan_tree(PagedPlan& c, int B, int Hq, int Hkv, int T, int D, int page, int 
   c.tile = row_bytes <= 256 ? 64 : 32;
   c.row_tiles = ceil_div(c.rows, waves * 32);
   const int64_t tiles = ceil_div((int64_t)width * page, c.tile);
-  c.share = tree_share(c.nbh * c.row_tiles, tiles, row_bytes, waves);
+  c.share = tree_share(c.nbh * c.row_tiles, tiles, row_bytes, waves, dtype == 0);
   // at most 256 MiB of parts
   const int64_t part = c.nbh * c.rows * (D + 2) * 4;
   c.share = (int)std::max<int64_t>(c.share, ceil_div(tiles, std::max<int64_t>(1, (256 << 20) / part)));

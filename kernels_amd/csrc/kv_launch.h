@@ -156,8 +156,14 @@ constexpr int tree_waves(int64_t rows) { return rows <= 64 ? 2 : 4; }
 // 87, 76, 69, 65*; 96 of 2000 37, 28*, 28, 38; 256 rows, 64 of 8192 172, 134, 108, 95*, log-uniform 71, 62, 56, 72*; 128 rows, 128 of 4096 120, 92, 79*, 67,
 // from 1 on 68, 55, 50*, 58, log-uniform 46, 40, 45*, 57; 240 rows, 15 of 6000 43, 36*, 36, 55; D = 64: 60 rows, 192 of 4000 55, 46, 41*, 41, log-uniform 28, 24, 26*, 36;
 // 100 rows, 128 of 4000 55, 46, 42*, 50; D = 256: 80 rows, 64 of up to 2000 66, 50, 42*, 62.
-inline int tree_share(int64_t workgroups, int64_t tiles, int row_bytes, int waves) {
+// Where the workgroups of whole runs of up to 4096 keys fill every place, none is divided: nothing to write and join (runs in two or four parts -> whole, lengths
+// full, from half on, from 1 on, log-uniform: 64 rows, 512 key heads of 4096, D = 128 218 -> 185, 181 -> 154, 129 -> 118, 65 -> 76; 128 rows 248 -> 193, 211 -> 167, 158 -> 132, 96 -> 101; 256 rows
+// 501 -> 387, 416 -> 322, 273 -> 225, 163 -> 144; D = 64, 200 rows, 384 of 4000 206 -> 164, 159 -> 133, 111 -> 103, 78 -> 84).  Of 8192 keys the few longest run alone: 256 rows, 256 key heads 407 -> 363, 323 -> 290,
+// 223 -> 255, 128 -> 213; so do D = 256's of 4096, 60 rows 445 -> 416, 367 -> 346, 262 -> 268, 155 -> 218, D = 32's, 100 rows, 768 of 4000 154 -> 144, 122 -> 115, 80 -> 89, 57 -> 74,
+// and float32's, D = 64, 40 rows, 768 of 4000 487 -> 482, 387 -> 429, 289 -> 279, 183 -> 221.
+inline int tree_share(int64_t workgroups, int64_t tiles, int row_bytes, int waves, bool f32) {
   const int64_t places = waves == 2 ? (row_bytes <= 128 ? 3 : 2) : (row_bytes <= 128 ? 3 : row_bytes == 256 ? 2 : 1);
+  if (!f32 && (row_bytes == 128 || row_bytes == 256) && tiles <= 64 && workgroups >= places * CUS) return (int)std::max<int64_t>(tiles, 1);
   const int64_t least = workgroups * ceil_div(tiles, 8) > CUS / 2 ? 8 : 4;
   const int64_t most = row_bytes > 256 ? 64 : waves == 4 && row_bytes <= 128 ? 16 : 32;
   const int64_t share = std::min(most, std::max(least, ceil_div(workgroups * tiles, places * CUS)));

@@ -27,6 +27,8 @@ def _parts(B, Hq, Hkv, T, D, page, width, dtype):
     least = 8 if groups * _ceil(tiles, 8) > 128 else 4
     most = 64 if row_bytes > 256 else 16 if waves == 4 and row_bytes <= 128 else 32
     share = max(1, min(tiles, min(most, max(least, _ceil(groups * tiles, places * 256)))))
+    if es == 2 and row_bytes in (128, 256) and tiles <= 64 and groups >= places * 256:   # as many whole runs as there are places
+        share = tiles
     share = max(share, _ceil(tiles, max(1, (256 << 20) // (units * rows * (D + 2) * 4))))
     bytes_ = _lib.load().kv_paged_tree_forward_workspace(B, Hq, Hkv, T, D, page, width, DTYPES.index(dtype))
     return _ceil(tiles, share), max(1, bytes_ // (units * rows * (D + 2) * 4))
@@ -71,6 +73,26 @@ def test_tiles_of_long_caches(dtype, D, T, G, page):
     some = torch.tensor([0, 1, 2, 3, 4, 5, B - 1])
     want = kv_oracle.tree(q[some], k, v, table[some], _i32(lens)[some], trees[some])
     o, lse = paged_tree_attention(*_gpu(q, k, v, table, _i32(lens), trees), return_lse=True)
+    kv_oracle.assert_within("o", o[some.to(DEV)], want["o"])
+    kv_oracle.assert_within("lse", lse[some.to(DEV)], want["lse"])
+
+
+@pytest.mark.parametrize("dtype", DTYPES[1:])
+@pytest.mark.parametrize("B,Hkv,T,G,D", [(64, 8, 16, 4, 128), (128, 6, 40, 1, 64), (48, 8, 50, 3, 64), (64, 4, 70, 3, 128)])
+def test_as_many_sequences_as_places(dtype, B, Hkv, T, G, D):
+    """Whole runs, without parts, of every length up to the table's; sequences share their pages."""
+    page, span = 16, 640
+    g = torch.Generator().manual_seed(8)
+    lens = torch.randint(0, span + 1, (B,), generator=g, dtype=torch.int32)
+    lens[:5] = _i32([span, 0, T - 1, 65, 64])
+    k, v, pool = _cache([span] * 4, Hkv, D, page, dtype, width=span // page)
+    table = pool[torch.arange(B) % 4]
+    want, parts = _parts(B, Hkv * G, Hkv, T, D, page, span // page, dtype)
+    assert want == parts == 1
+    q, trees = _q(B, Hkv * G, T, D, dtype), _trees(B, T)
+    o, lse = paged_tree_attention(*_gpu(q, k, v, table, lens, trees), return_lse=True)
+    some = torch.tensor([0, 1, 2, 3, 4, 5, 6, B - 1])
+    want = kv_oracle.tree(q[some], k, v, table[some], lens[some], trees[some])
     kv_oracle.assert_within("o", o[some.to(DEV)], want["o"])
     kv_oracle.assert_within("lse", lse[some.to(DEV)], want["lse"])
 
