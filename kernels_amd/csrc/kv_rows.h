@@ -84,16 +84,16 @@ SA_DEV uint32_t tree_mask(const Tree& tree, int T, int b, int t, int n, int base
   }
   return base + t < 0 ? 0 : bits | sa::row_mask(0, base - k0, h);
 }
-// Those of the 32 keys that any of the wave's rows sees (not only those of the lane), in the order of the keys.
+// Those of the 32 keys that any of the wave's rows sees (not only those of the lane), in the order of the keys.  Joined over the lanes of a half (one vote
+// of the wave for each key took 0.4 us: one tree of 8, 300 keys, D = 64 6.5 -> 6.1, 256 rows, 128 key heads of 500, D = 128 20.1 -> 18.5).
 SA_DEV uint32_t any_row(uint32_t mask) {
-  uint32_t seen = 0;
-#pragma unroll
-  for (int e = 0; e < 16; ++e) {
-    const uint64_t lanes = __builtin_amdgcn_ballot_w64((sa::keep_bits(mask, e)) != 0);
-    seen |= ((uint32_t)lanes != 0 ? 1u : 0u) << sa::crow(e, 0);
-    seen |= ((uint32_t)(lanes >> 32) != 0 ? 1u : 0u) << sa::crow(e, 1);
-  }
-  return seen;
+  int x = (int)(mask & 0x0f0f0f0fu);   // the keys of the lane's half
+  x |= __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);   // as in wave_prefix_sum, up to the lanes 31 and 63
+  x |= __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);
+  x |= __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);
+  x |= __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);
+  x |= __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);
+  return (uint32_t)__builtin_amdgcn_readlane(x, 31) | (uint32_t)__builtin_amdgcn_readlane(x, 63) << 4;
 }
 
 struct RowsParams {
