@@ -138,9 +138,9 @@ constexpr int rows_waves(int row_bytes, bool f32, int64_t workgroups, int share)
 }
 
 // Trees: the rows kernel up to 32 rows of a key head and for little work altogether (blocks of 32 rows times tiles of 32 keys: few for each wave
-// of the GPU), else the tile kernel.  Rows -> tiles, in us, D = 128, bfloat16: 64 rows, 8 key heads of 1000 12.3 -> 15.3, of 4096 14.9 -> 16.1; 256 rows, 8 of
-// 4096 (8192 blocks) 22.3 -> 23.9; 64 rows, 96 of 2000 (12096) 27.9 -> 25.7; 128 rows, 16 of 8192 31.5 -> 27; 256 rows, 64 of 8192 201 -> 92.  D = 256: 40
-// rows, 16 of 500 18.7-25 -> 20, 64 of 2000 45-72 -> 32.  float32: 40 rows, 32 of 1000, D = 64 (2048) 15.2 -> 20.7; 256 rows, 16 of 2000, D = 128 95 -> 56.
+// of the GPU), else the tile kernel.  Rows -> tiles, in us, D = 128, bfloat16: 64 rows, 8 key heads of 1000 11.7 -> 13.5, of 4096 14.1 -> 15.4, 32 of 4096 (8192
+// blocks) 23.1 -> 20.8; 256 rows, 8 of 4096 (8192) 21.5 -> 23.9; 64 rows, 96 of 2000 (12096) 27.9 -> 23.5; 128 rows, 16 of 8192 31.5 -> 26.3; 256 rows, 64 of 8192 201 -> 92.  D = 256: 40
+// rows, 16 of 500 18.7-25 -> 17.6, 64 of 2000 45-72 -> 32.  float32: 40 rows, 32 of 1000, D = 64 (2048) 14.9 -> 20.9; 256 rows, 16 of 2000, D = 128 95 -> 56.
 inline bool tree_by_rows(int64_t units, int64_t rows, int64_t tiles, int row_bytes, bool f32) {
   const int64_t blocks = units * ceil_div(rows, 32) * tiles;
   return rows <= 32 || (f32 ? row_bytes <= 512 && blocks <= 4096 : row_bytes <= 256 && blocks <= 8192);
