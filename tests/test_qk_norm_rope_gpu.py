@@ -394,6 +394,32 @@ def test_weights_without_rows():
         assert rc == 0 and all(torch.equal(t, torch.zeros_like(t)) for t in got)
 
 
+@pytest.mark.parametrize("dtype,D,rot,interleaved", [
+    (torch.bfloat16, 256, 128, False), (torch.float16, 256, 64, False), (torch.float32, 128, 64, False), (torch.float16, 128, 128, False),
+    (torch.bfloat16, 128, 64, False), (torch.bfloat16, 128, 32, True), (torch.float32, 64, 64, False), (torch.float16, 256, 256, True)])
+def test_large_calls_give_what_small_ones_give(dtype, D, rot, interleaved):
+    """More than the caches hold, with stores past them where a store covers whole lines: the same bits as in pieces, forward and backward."""
+    B, H = 2, 16
+    T = (20 << 20) // (B * (H + 2) * D * dtype.itemsize) + 3
+    g = torch.Generator(device=DEV).manual_seed(4)
+    q, k = (torch.randn(B, h, T, D, generator=g, device=DEV).to(dtype).requires_grad_() for h in (H, 2))
+    up = [torch.randn(x.shape, generator=g, device=DEV).to(dtype) for x in (q, k)]
+    w = (1 + 0.2 * torch.randn(D, generator=g, device=DEV)).to(dtype)
+    tables = [t.to(DEV) for t in _tables(T, rot)]
+    lens = _i32([T, T - T // 3]).to(DEV)
+    out = qk_norm_rope(q, k, *tables, w, w, lens=lens, interleaved=interleaved)
+    grads = torch.autograd.grad(out, (q, k), up)
+    for t0 in range(0, T, -(-T // 5)):
+        t1 = min(T, t0 + -(-T // 5))
+        part = [x.detach()[:, :, t0:t1].requires_grad_() for x in (q, k)]
+        at = torch.arange(t0, t1, dtype=torch.int32, device=DEV).expand(B, -1)
+        got = qk_norm_rope(*part, *tables, w, w, lens=(lens - t0).clamp(min=0).int(), positions=at, interleaved=interleaved)
+        for a, b in zip(got, out):
+            assert torch.equal(a, b[:, :, t0:t1])
+        for a, b in zip(torch.autograd.grad(got, part, [x[:, :, t0:t1] for x in up]), grads):
+            assert torch.equal(a, b[:, :, t0:t1])
+
+
 def test_more_than_two_to_the_31_elements():
     g = torch.Generator(device=DEV).manual_seed(11)
     B, Hq, Hkv, T, D = 4, 40, 2, 110000, 128
