@@ -146,11 +146,13 @@ struct RopeToken {
   int b, t, at;
   bool live;               // not padding, and at a position that the table has
 };
-SA_DEV RopeToken rope_token(const RopeParams& p, int token) {
+// (tokens behind the last one: not live, in place of the last)
+SA_DEV RopeToken rope_token(const RopeParams& p, int64_t id, int64_t tokens) {
   RopeToken x;
+  const int token = (int)(id < tokens ? id : tokens - 1);
   x.b = div_by(token, p.by_tokens), x.t = token - x.b * p.T;
   x.at = p.positions ? p.positions[x.b * p.pos_sb + x.t * p.pos_st] : x.t;
-  x.live = x.t < clamped_length(p.lens, p.lens_stride, x.b, p.T) && (uint32_t)x.at < (uint32_t)p.table.rows;
+  x.live = id < tokens && x.t < clamped_length(p.lens, p.lens_stride, x.b, p.T) && (uint32_t)x.at < (uint32_t)p.table.rows;
   return x;
 }
 template <bool INTER, int V, typename Lane> SA_DEV void load_angles(float (&c)[V], float (&s)[V], const RopeTable& table, int at, const Lane& lane) {
@@ -164,6 +166,60 @@ template <bool INTER, int V, typename Lane> SA_DEV void load_angles(float (&c)[V
   }
 }
 
+// Where a lane's two chunks of a row go.  Rows of 128 bytes: the groups of lanes of two tokens that follow each other exchange a chunk (in the order of
+// lanes that the half mirror gives), so that each store covers whole rows.  In us, with a half of a row to a store -> whole rows -> past the caches, D = 64, 16 bits: 4 x
+// 32 heads x 8192 forward 66 -> 60 -> 58, 8 x 24 x 1500-3000 38 -> 34.5 -> 25.5; with gradients 8 x 32 x 4096 150 -> 126, prompts of up to 2048 tokens of 8 sequences into pages 46 -> 27.
+template <typename T, int D, bool INTER> struct RowStore {
+  using L = RopeLanes<T, D>;
+  static constexpr bool PAIRS = L::LANES == 4;
+  // The tokens from here on that the loop of a group has to take part in: both of a pair, or its own.
+  SA_DEV static int64_t leader(int64_t id) { return PAIRS ? id & ~int64_t(1) : id; }
+  T *first, *second;
+  bool has_first, has_second, odd = false;
+  SA_DEV static int other(int x) { return __builtin_amdgcn_update_dpp(0, x, 0x141, 0xf, 0xf, false); }
+  // to: this group's row; there: it is to be written
+  SA_DEV RowStore(T* to, bool there, int64_t id, int rot, const RopeLane<T, D, INTER>& lane) {
+    if constexpr (PAIRS) {
+      const RopeLane<T, D, INTER> mirrored(L::LANES - 1 - threadIdx.x % L::LANES, rot);
+      const uint64_t own = reinterpret_cast<uint64_t>(to);
+      T* const others = reinterpret_cast<T*>((uint64_t)(uint32_t)other((int)(own >> 32)) << 32 | (uint32_t)other((int)own));
+      const bool others_there = other(there ? 1 : 0) != 0;
+      odd = id & 1;
+      first = odd ? others + mirrored.b : to + lane.a;
+      second = odd ? to + lane.b : others + mirrored.a;
+      has_first = odd ? others_there : there;
+      has_second = odd ? there : others_there;
+    } else {
+      first = to + lane.a, second = to + lane.b;
+      has_first = has_second = there;
+    }
+  }
+  template <bool STREAMING> SA_DEV void put(const float* x) const {
+    constexpr int V = L::V;
+    if constexpr (PAIRS) {
+      typename Elem<T>::Frag a, b;
+#pragma unroll
+      for (int e = 0; e < V; ++e) a[e] = (T)x[e], b[e] = (T)x[V + e];
+      u32x4 one = __builtin_bit_cast(u32x4, a), two = __builtin_bit_cast(u32x4, b);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const uint32_t got = (uint32_t)other((int)(odd ? one[e] : two[e]));
+        one[e] = odd ? got : one[e], two[e] = odd ? two[e] : got;
+      }
+      auto store = [](T* to, const u32x4& v) {
+        if constexpr (STREAMING) sa::store_streaming(to, v);
+        else *reinterpret_cast<u32x4*>(to) = v;
+      };
+      if (has_first) store(first, one);
+      if (has_second) store(second, two);
+    } else if (has_first) {
+      pack<T, STREAMING>(first, x);
+      pack<T, STREAMING>(second, x + V);
+    }
+  }
+  SA_DEV void next(int64_t step) { first += step, second += step; }
+};
+
 template <typename T, int D, bool INTER, bool STREAMING> __global__ __launch_bounds__(256) void rope_kernel(const RopeParams p) {
   using L = RopeLanes<T, D>;
   constexpr int V = L::V;
@@ -174,13 +230,13 @@ template <typename T, int D, bool INTER, bool STREAMING> __global__ __launch_bou
   const int64_t step = (int64_t)gridDim.x * L::GROUPS, tokens = (int64_t)p.B * p.T;
   float w[2 * V];
   load_weights<T, V>(w, side.weight, p.weights_f32, lane.a, lane.b);
-  for (int64_t id = (int64_t)blockIdx.x * L::GROUPS + threadIdx.x / L::LANES; id < tokens; id += step) {
-    const RopeToken token = rope_token(p, (int)id);
+  for (int64_t id = (int64_t)blockIdx.x * L::GROUPS + threadIdx.x / L::LANES; RowStore<T, D, INTER>::leader(id) < tokens; id += step) {
+    const RopeToken token = rope_token(p, id, tokens);
     const T* x = reinterpret_cast<const T*>(side.x) + token.b * side.sb + token.t * side.st + h0 * side.sh;
-    T* out = reinterpret_cast<T*>(side.out) + (((int64_t)token.b * side.heads + h0) * p.T + token.t) * D;
+    RowStore<T, D, INTER> to(reinterpret_cast<T*>(side.out) + (((int64_t)token.b * side.heads + h0) * p.T + token.t) * D, id < tokens, id, p.table.rot, lane);
     float c[V], s[V], row[2 * V];
     if (token.live) load_angles<INTER>(c, s, p.table, token.at, lane);
-    for (int h = h0; h < h1; ++h, x += side.sh, out += (int64_t)p.T * D) {
+    for (int h = h0; h < h1; ++h, x += side.sh, to.next((int64_t)p.T * D)) {
       if (token.live) {
         unpack<T>(row, x + lane.a);
         unpack<T>(row + V, x + lane.b);
@@ -189,8 +245,7 @@ template <typename T, int D, bool INTER, bool STREAMING> __global__ __launch_bou
 #pragma unroll
         for (int e = 0; e < 2 * V; ++e) row[e] = 0.0f;
       }
-      pack<T, STREAMING>(out + lane.a, row);
-      pack<T, STREAMING>(out + lane.b, row + V);
+      to.template put<STREAMING>(row);
     }
   }
 }
@@ -209,18 +264,18 @@ template <typename T, int D, bool INTER, bool STREAMING> __global__ __launch_bou
   load_weights<T, V>(w, side.weight, p.weights_f32, lane.a, lane.b);
 #pragma unroll
   for (int e = 0; e < 2 * V; ++e) dw[e] = 0.0f;
-  for (int64_t id = (int64_t)blockIdx.x * L::GROUPS + threadIdx.x / L::LANES; id < tokens; id += step) {
-    const RopeToken token = rope_token(p, (int)id);
+  for (int64_t id = (int64_t)blockIdx.x * L::GROUPS + threadIdx.x / L::LANES; RowStore<T, D, INTER>::leader(id) < tokens; id += step) {
+    const RopeToken token = rope_token(p, id, tokens);
     const T* x = reinterpret_cast<const T*>(side.x) + token.b * side.sb + token.t * side.st + h0 * side.sh;
     const T* g = reinterpret_cast<const T*>(side.g) + token.b * side.g_sb + token.t * side.g_st + h0 * side.g_sh;
-    T* out = reinterpret_cast<T*>(side.out) + (((int64_t)token.b * side.heads + h0) * p.T + token.t) * D;
+    RowStore<T, D, INTER> to(reinterpret_cast<T*>(side.out) + (((int64_t)token.b * side.heads + h0) * p.T + token.t) * D, id < tokens, id, p.table.rot, lane);
     float c[V], s[V], xs[2 * V], gs[2 * V];
     if (token.live) {
       load_angles<INTER>(c, s, p.table, token.at, lane);
 #pragma unroll
       for (int e = 0; e < V; ++e) s[e] = -s[e];
     }
-    for (int h = h0; h < h1; ++h, x += side.sh, g += side.g_sh, out += (int64_t)p.T * D) {
+    for (int h = h0; h < h1; ++h, x += side.sh, g += side.g_sh, to.next((int64_t)p.T * D)) {
       if (token.live) {
         unpack<T>(gs, g + lane.a);
         unpack<T>(gs + V, g + lane.b);
@@ -249,8 +304,7 @@ template <typename T, int D, bool INTER, bool STREAMING> __global__ __launch_bou
 #pragma unroll
         for (int e = 0; e < 2 * V; ++e) gs[e] = 0.0f;
       }
-      pack<T, STREAMING>(out + lane.a, gs);
-      pack<T, STREAMING>(out + lane.b, gs + V);
+      to.template put<STREAMING>(gs);
     }
   }
   if (!p.part) return;
@@ -322,30 +376,33 @@ template <typename T, int D, bool INTER, bool STREAMING> __global__ __launch_bou
   const float eps = kind == 2 ? 0.0f : p.eps;
   float w[2 * V];
   load_weights<T, V>(w, kind == 0 ? p.q_weight : kind == 1 ? p.k_weight : nullptr, p.weights_f32, lane.a, lane.b);
-  for (int64_t id = (int64_t)blockIdx.x * L::GROUPS + threadIdx.x / L::LANES; id < tokens; id += step) {
-    const int b = div_by((int)id, p.by_tokens), t = (int)id - b * p.T;
+  for (int64_t id = (int64_t)blockIdx.x * L::GROUPS + threadIdx.x / L::LANES; RowStore<T, D, INTER>::leader(id) < tokens; id += step) {
+    const int token = (int)(id < tokens ? id : tokens - 1), b = div_by(token, p.by_tokens), t = token - b * p.T;
     const int n = clamped_length(p.new_lens, p.new_lens_stride, b, p.T);
     const int64_t place = (int64_t)p.lens[b * p.lens_stride] - n + t;
     const int64_t at = p.positions ? p.positions[b * p.pos_sb + t * p.pos_st] : place;
-    const bool live = t < n && at >= 0 && at < p.table.rows;
-    T* to;
-    int64_t to_sh;
+    const bool live = id < tokens && t < n && at >= 0 && at < p.table.rows;
+    T* own = nullptr;
+    int64_t own_sh = (int64_t)p.T * D;
+    bool there = id < tokens;
     if (kind == 0) {
-      to = reinterpret_cast<T*>(p.q_out) + ((int64_t)b * heads * p.T + t) * D;
-      to_sh = (int64_t)p.T * D;
+      own = reinterpret_cast<T*>(p.q_out) + (((int64_t)b * heads + h0) * p.T + t) * D;
     } else {
-      if (!live || place < 0 || place >= (int64_t)p.width * p.page) continue;
-      const int entry = div_by((int)place, p.by_page), slot = (int)place - entry * p.page;
-      const int32_t page = p.page_table[b * p.table_sb + entry];
-      if ((uint32_t)page >= (uint32_t)p.num_pages) continue;
-      to = kind == 1 ? reinterpret_cast<T*>(p.k_pages) + page * p.kp_sp + slot * p.kp_st : reinterpret_cast<T*>(p.v_pages) + page * p.vp_sp + slot * p.vp_st;
-      to_sh = kind == 1 ? p.kp_sh : p.vp_sh;
+      own_sh = kind == 1 ? p.kp_sh : p.vp_sh;
+      there = live && place >= 0 && place < (int64_t)p.width * p.page;
+      if (there) {
+        const int entry = div_by((int)place, p.by_page), slot = (int)place - entry * p.page;
+        const int32_t page = p.page_table[b * p.table_sb + entry];
+        there = (uint32_t)page < (uint32_t)p.num_pages;
+        own = (kind == 1 ? reinterpret_cast<T*>(p.k_pages) + page * p.kp_sp + slot * p.kp_st : reinterpret_cast<T*>(p.v_pages) + page * p.vp_sp + slot * p.vp_st) + h0 * own_sh;
+      }
+      if (!RowStore<T, D, INTER>::PAIRS && !there) continue;
     }
+    RowStore<T, D, INTER> to(own, there, id, kind == 2 ? 0 : p.table.rot, lane);
     const T* x = from + b * sb + t * st + h0 * sh;
-    to += h0 * to_sh;
     float c[V], s[V], row[2 * V];
     if (live) load_angles<INTER>(c, s, p.table, (int)at, lane);
-    for (int h = h0; h < h1; ++h, x += sh, to += to_sh) {
+    for (int h = h0; h < h1; ++h, x += sh, to.next(own_sh)) {
       if (live) {
         unpack<T>(row, x + lane.a);
         unpack<T>(row + V, x + lane.b);
@@ -354,8 +411,7 @@ template <typename T, int D, bool INTER, bool STREAMING> __global__ __launch_bou
 #pragma unroll
         for (int e = 0; e < 2 * V; ++e) row[e] = 0.0f;
       }
-      pack<T, STREAMING>(to + lane.a, row);
-      pack<T, STREAMING>(to + lane.b, row + V);
+      to.template put<STREAMING>(row);
     }
   }
 }
