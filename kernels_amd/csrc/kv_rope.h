@@ -169,13 +169,15 @@ template <bool INTER, int V, typename Lane> SA_DEV void load_angles(float (&c)[V
 // Where a lane's two chunks of a row go.  Rows of 128 bytes: the groups of lanes of two tokens that follow each other exchange a chunk (in the order of
 // lanes that the half mirror gives), so that each store covers whole rows.  In us, with a half of a row to a store -> whole rows -> past the caches, D = 64, 16 bits: 4 x
 // 32 heads x 8192 forward 66 -> 60 -> 58, 8 x 24 x 1500-3000 38 -> 34.5 -> 25.5; with gradients 8 x 32 x 4096 150 -> 126, prompts of up to 2048 tokens of 8 sequences into pages 46 -> 27.
-template <typename T, int D, bool INTER> struct RowStore {
+// Likewise the halves of a row of 256 bytes of which half is turned, in calls that store past the caches: D = 128, 2 x 40 x 8192 forward 81 -> 71, with gradients 191 -> 163, prompts into
+// pages 77 -> 64 (64 bytes to a store and plain -> whole lines past the caches).
+template <typename T, int D, bool INTER, bool STREAMING> struct RowStore {
   using L = RopeLanes<T, D>;
-  static constexpr bool PAIRS = L::LANES == 4;
+  static constexpr bool PAIRS = L::LANES == 4, HALVES = L::LANES == 8 && !INTER && STREAMING;
   // The tokens from here on that the loop of a group has to take part in: both of a pair, or its own.
   SA_DEV static int64_t leader(int64_t id) { return PAIRS ? id & ~int64_t(1) : id; }
   T *first, *second;
-  bool has_first, has_second, odd = false;
+  bool has_first, has_second, exchanged = PAIRS, odd = false;
   SA_DEV static int other(int x) { return __builtin_amdgcn_update_dpp(0, x, 0x141, 0xf, 0xf, false); }
   // to: this group's row; there: it is to be written
   SA_DEV RowStore(T* to, bool there, int64_t id, int rot, const RopeLane<T, D, INTER>& lane) {
@@ -192,20 +194,26 @@ template <typename T, int D, bool INTER> struct RowStore {
     } else {
       first = to + lane.a, second = to + lane.b;
       has_first = has_second = there;
+      if constexpr (HALVES) {
+        exchanged = 2 * rot == D, odd = threadIdx.x & 4;
+        const RopeLane<T, D, INTER> mirrored(L::LANES - 1 - threadIdx.x % L::LANES, rot);
+        if (exchanged) first = to + (odd ? mirrored.b : lane.a), second = to + (odd ? lane.b : mirrored.a);
+      }
     }
   }
-  template <bool STREAMING> SA_DEV void put(const float* x) const {
+  SA_DEV void put(const float* x) const {
     constexpr int V = L::V;
-    if constexpr (PAIRS) {
+    if constexpr (PAIRS || HALVES) {
       typename Elem<T>::Frag a, b;
 #pragma unroll
       for (int e = 0; e < V; ++e) a[e] = (T)x[e], b[e] = (T)x[V + e];
       u32x4 one = __builtin_bit_cast(u32x4, a), two = __builtin_bit_cast(u32x4, b);
+      if (exchanged)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const uint32_t got = (uint32_t)other((int)(odd ? one[e] : two[e]));
-        one[e] = odd ? got : one[e], two[e] = odd ? two[e] : got;
-      }
+        for (int e = 0; e < 4; ++e) {
+          const uint32_t got = (uint32_t)other((int)(odd ? one[e] : two[e]));
+          one[e] = odd ? got : one[e], two[e] = odd ? two[e] : got;
+        }
       auto store = [](T* to, const u32x4& v) {
         if constexpr (STREAMING) sa::store_streaming(to, v);
         else *reinterpret_cast<u32x4*>(to) = v;
@@ -220,7 +228,8 @@ template <typename T, int D, bool INTER> struct RowStore {
   SA_DEV void next(int64_t step) { first += step, second += step; }
 };
 
-template <typename T, int D, bool INTER, bool STREAMING> __global__ __launch_bounds__(256) void rope_kernel(const RopeParams p) {
+// (five waves to a SIMD: up to 102 registers, and none spills)
+template <typename T, int D, bool INTER, bool STREAMING> __global__ __launch_bounds__(256, 5) void rope_kernel(const RopeParams p) {
   using L = RopeLanes<T, D>;
   constexpr int V = L::V;
   const RopeLane<T, D, INTER> lane(threadIdx.x % L::LANES, p.table.rot);
@@ -230,10 +239,10 @@ template <typename T, int D, bool INTER, bool STREAMING> __global__ __launch_bou
   const int64_t step = (int64_t)gridDim.x * L::GROUPS, tokens = (int64_t)p.B * p.T;
   float w[2 * V];
   load_weights<T, V>(w, side.weight, p.weights_f32, lane.a, lane.b);
-  for (int64_t id = (int64_t)blockIdx.x * L::GROUPS + threadIdx.x / L::LANES; RowStore<T, D, INTER>::leader(id) < tokens; id += step) {
+  for (int64_t id = (int64_t)blockIdx.x * L::GROUPS + threadIdx.x / L::LANES; RowStore<T, D, INTER, STREAMING>::leader(id) < tokens; id += step) {
     const RopeToken token = rope_token(p, id, tokens);
     const T* x = reinterpret_cast<const T*>(side.x) + token.b * side.sb + token.t * side.st + h0 * side.sh;
-    RowStore<T, D, INTER> to(reinterpret_cast<T*>(side.out) + (((int64_t)token.b * side.heads + h0) * p.T + token.t) * D, id < tokens, id, p.table.rot, lane);
+    RowStore<T, D, INTER, STREAMING> to(reinterpret_cast<T*>(side.out) + (((int64_t)token.b * side.heads + h0) * p.T + token.t) * D, id < tokens, id, p.table.rot, lane);
     float c[V], s[V], row[2 * V];
     if (token.live) load_angles<INTER>(c, s, p.table, token.at, lane);
     for (int h = h0; h < h1; ++h, x += side.sh, to.next((int64_t)p.T * D)) {
@@ -245,7 +254,7 @@ template <typename T, int D, bool INTER, bool STREAMING> __global__ __launch_bou
 #pragma unroll
         for (int e = 0; e < 2 * V; ++e) row[e] = 0.0f;
       }
-      to.template put<STREAMING>(row);
+      to.put(row);
     }
   }
 }
@@ -264,11 +273,11 @@ template <typename T, int D, bool INTER, bool STREAMING> __global__ __launch_bou
   load_weights<T, V>(w, side.weight, p.weights_f32, lane.a, lane.b);
 #pragma unroll
   for (int e = 0; e < 2 * V; ++e) dw[e] = 0.0f;
-  for (int64_t id = (int64_t)blockIdx.x * L::GROUPS + threadIdx.x / L::LANES; RowStore<T, D, INTER>::leader(id) < tokens; id += step) {
+  for (int64_t id = (int64_t)blockIdx.x * L::GROUPS + threadIdx.x / L::LANES; RowStore<T, D, INTER, STREAMING>::leader(id) < tokens; id += step) {
     const RopeToken token = rope_token(p, id, tokens);
     const T* x = reinterpret_cast<const T*>(side.x) + token.b * side.sb + token.t * side.st + h0 * side.sh;
     const T* g = reinterpret_cast<const T*>(side.g) + token.b * side.g_sb + token.t * side.g_st + h0 * side.g_sh;
-    RowStore<T, D, INTER> to(reinterpret_cast<T*>(side.out) + (((int64_t)token.b * side.heads + h0) * p.T + token.t) * D, id < tokens, id, p.table.rot, lane);
+    RowStore<T, D, INTER, STREAMING> to(reinterpret_cast<T*>(side.out) + (((int64_t)token.b * side.heads + h0) * p.T + token.t) * D, id < tokens, id, p.table.rot, lane);
     float c[V], s[V], xs[2 * V], gs[2 * V];
     if (token.live) {
       load_angles<INTER>(c, s, p.table, token.at, lane);
@@ -304,7 +313,7 @@ template <typename T, int D, bool INTER, bool STREAMING> __global__ __launch_bou
 #pragma unroll
         for (int e = 0; e < 2 * V; ++e) gs[e] = 0.0f;
       }
-      to.template put<STREAMING>(gs);
+      to.put(gs);
     }
   }
   if (!p.part) return;
@@ -376,7 +385,7 @@ template <typename T, int D, bool INTER, bool STREAMING> __global__ __launch_bou
   const float eps = kind == 2 ? 0.0f : p.eps;
   float w[2 * V];
   load_weights<T, V>(w, kind == 0 ? p.q_weight : kind == 1 ? p.k_weight : nullptr, p.weights_f32, lane.a, lane.b);
-  for (int64_t id = (int64_t)blockIdx.x * L::GROUPS + threadIdx.x / L::LANES; RowStore<T, D, INTER>::leader(id) < tokens; id += step) {
+  for (int64_t id = (int64_t)blockIdx.x * L::GROUPS + threadIdx.x / L::LANES; RowStore<T, D, INTER, STREAMING>::leader(id) < tokens; id += step) {
     const int token = (int)(id < tokens ? id : tokens - 1), b = div_by(token, p.by_tokens), t = token - b * p.T;
     const int n = clamped_length(p.new_lens, p.new_lens_stride, b, p.T);
     const int64_t place = (int64_t)p.lens[b * p.lens_stride] - n + t;
@@ -396,9 +405,9 @@ template <typename T, int D, bool INTER, bool STREAMING> __global__ __launch_bou
         there = (uint32_t)page < (uint32_t)p.num_pages;
         own = (kind == 1 ? reinterpret_cast<T*>(p.k_pages) + page * p.kp_sp + slot * p.kp_st : reinterpret_cast<T*>(p.v_pages) + page * p.vp_sp + slot * p.vp_st) + h0 * own_sh;
       }
-      if (!RowStore<T, D, INTER>::PAIRS && !there) continue;
+      if (!RowStore<T, D, INTER, STREAMING>::PAIRS && !there) continue;
     }
-    RowStore<T, D, INTER> to(own, there, id, kind == 2 ? 0 : p.table.rot, lane);
+    RowStore<T, D, INTER, STREAMING> to(own, there, id, kind == 2 ? 0 : p.table.rot, lane);
     const T* x = from + b * sb + t * st + h0 * sh;
     float c[V], s[V], row[2 * V];
     if (live) load_angles<INTER>(c, s, p.table, (int)at, lane);
@@ -411,7 +420,7 @@ template <typename T, int D, bool INTER, bool STREAMING> __global__ __launch_bou
 #pragma unroll
         for (int e = 0; e < 2 * V; ++e) row[e] = 0.0f;
       }
-      to.template put<STREAMING>(row);
+      to.put(row);
     }
   }
 }

@@ -33,14 +33,14 @@ inline RopeGrid rope_grid(int64_t tokens, int Hq, int Hkv, int D, int elem_size,
 inline RopeGrid forward_grid(int64_t tokens, int Hq, int Hkv, int D, int elem_size) { return rope_grid(tokens, Hq, Hkv, D, elem_size, 2048, 1 << 22); }
 inline RopeGrid backward_grid(int64_t tokens, int Hq, int Hkv, int D, int elem_size) { return rope_grid(tokens, Hq, Hkv, D, elem_size, 512, 1024); }
 
-// Stores past the caches, where a call reads and writes more than the L2s of all XCDs hold and each store covers whole lines of 128 bytes (rows of 128: RowStore; else half of a
-// row; halves, some of the channels turned: half of those and half of the others).  In us, plain -> past the caches, bfloat16: 2 x 40
-// heads x 8192, D = 128, forward 76 -> 71, with gradients 189 -> 163; 2 x 2048 of them 20.9 -> 16.5; prompts of up to 2048 tokens of 8 sequences into pages 72 -> 65; half of
-// the channels turned, 2 x 40 x 4096, D = 256 forward 78 -> 74, with gradients 187 -> 167, into pages 77 -> 74, float32, D = 128 182 -> 160; with 64 bytes to a line, D = 128, bfloat16 81 -> 82, 192 -> 178, into pages 76 -> 77,
-// a quarter turned 152 -> 174, three quarters forward 82 -> 105.
+// Stores past the caches, where a call reads and writes more than the L2s of all XCDs hold and each store covers whole lines of 128 bytes: rows of 128 (RowStore), halves of longer
+// rows; halves as pairs, some of the channels turned: half of those and half of the others, or a row of 256 bytes half of which is turned (RowStore).  In us, plain -> past the caches,
+// bfloat16: 2 x 40 heads x 8192, D = 128, forward 76 -> 71, with gradients 189 -> 163; 2 x 2048 of them 20.9 -> 16.5; prompts of up to 2048 tokens of 8 sequences into pages
+// 72 -> 65; half of the channels turned, 2 x 40 x 4096, D = 256 forward 78 -> 74, with gradients 187 -> 167, into pages 77 -> 74, float32, D = 128 182 -> 160; with stores of parts
+// of lines, D = 128, a quarter turned 152 -> 174, three quarters forward 82 -> 105.
 inline bool past_caches(int64_t rows, int D, int rot, bool inter, int elem_size) {
   const bool lines = inter ? D * elem_size % 256 == 0 : rot * elem_size % 256 == 0 && (D - rot) * elem_size % 256 == 0;
-  return (lines || D * elem_size == 128) && 2 * rows * D * elem_size > (int64_t(32) << 20);
+  return (lines || D * elem_size == 128 || (D * elem_size == 256 && 2 * rot == D)) && 2 * rows * D * elem_size > (int64_t(32) << 20);
 }
 
 }  // namespace kv
