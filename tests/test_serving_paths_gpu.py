@@ -1,0 +1,42 @@
+"""Norms, rotation, pages and trees on the GPU in calls that are large enough for ways through the kernels of their own: stores past the caches,
+the exchange of chunks between lanes, workgroups that find their parts by the lengths."""
+import pytest
+import torch
+
+from paged_attention import paged_append_rope
+from tests.test_drafted_tokens_gpu import _tables
+from tests.test_paged_attention_gpu import DEV, DTYPES
+
+pytestmark = pytest.mark.gpu
+
+
+def _past_caches(rows, D, dtype):
+    """More than the caches hold, read and written."""
+    return 2 * rows * D * dtype.itemsize > 32 << 20
+
+
+def _bits(x):
+    return x.view({2: torch.int16, 4: torch.int32}[x.element_size()])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("D,rot", [(16, 16), (64, 64), (64, 32), (128, 128), (128, 64), (256, 128)])
+@pytest.mark.parametrize("T", [5, 40001])
+@pytest.mark.parametrize("eps", [None, 1e-6])
+def test_values_keep_every_bit(dtype, D, rot, T, eps):
+    """Any bits: numbers, infinities, subnormal numbers, zeros of both signs, and what is not a number, with its sign and all that it carries."""
+    g = torch.Generator(device=DEV).manual_seed(7)
+    bits = torch.int16 if dtype.itemsize == 2 else torch.int32
+    info = torch.iinfo(bits)
+    v = torch.randint(info.min, info.max + 1, (1, 2, T, D), generator=g, device=DEV, dtype=torch.int64).to(bits).view(dtype)
+    v[:, :, ::3] = torch.randint(1, 1 << (7 if dtype == torch.bfloat16 else 10), v[:, :, ::3].shape, generator=g, device=DEV).to(bits).bitwise_or(
+        {torch.bfloat16: 0x7F80, torch.float16: 0x7C00, torch.float32: 0x7F800000}[dtype]).view(dtype)   # not numbers, the quiet bit not set in most
+    assert T < 100 or D < 64 or _past_caches(6 * T, D, dtype)
+    q = torch.zeros(1, 2, T, D, dtype=dtype, device=DEV)
+    page, tables = 64, [t.to(DEV) for t in _tables(T, rot)]
+    width = -(-T // page)
+    pages = [torch.zeros(width, 2, page, D, dtype=dtype, device=DEV) for _ in range(2)]
+    table = torch.arange(width, dtype=torch.int32, device=DEV)[None]
+    paged_append_rope(q, q, v, *pages, table, torch.tensor([T], dtype=torch.int32, device=DEV), *tables, eps=eps)
+    got = pages[1].transpose(0, 1).reshape(2, width * page, D)[:, :T]
+    assert torch.equal(_bits(got), _bits(v[0]))
