@@ -32,6 +32,7 @@ Tensor table_layout(const Tensor& t) {
                   reinterpret_cast<uintptr_t>(t.const_data_ptr()) % 16 == 0;
   return ok ? t : t.clone(at::MemoryFormat::Contiguous);
 }
+Tensor rows_layout(const Tensor& t) { return kernel_layout(t, false); }   // rows of a long projection may lie any distance apart
 OptTensor weight_layout(const OptTensor& w) {
   if (!w || ((w->stride(0) == 1) && reinterpret_cast<uintptr_t>(w->const_data_ptr()) % 16 == 0)) return w;
   return w->clone(at::MemoryFormat::Contiguous);
@@ -78,7 +79,7 @@ std::tuple<Tensor, Tensor> rope_forward_gpu(const Tensor& q, const Tensor& k, co
   const c10::OptionalDeviceGuard guard(q.device());
   Tensor q_out = empty_same(q), k_out = empty_same(k);
   if (q.numel() == 0) return {std::move(q_out), std::move(k_out)};
-  const Tensor qk = kernel_layout(q), kk = kernel_layout(k), ct = table_layout(cos), st = table_layout(sin);
+  const Tensor qk = rows_layout(q), kk = rows_layout(k), ct = table_layout(cos), st = table_layout(sin);
   const OptTensor wq = weight_layout(q_weight), wk = weight_layout(k_weight);
   const Lengths l(lens);
   const Positions pos(positions);
@@ -106,9 +107,9 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> rope_backward_gpu(const Tensor& d_q, 
     return {std::move(dq), std::move(dk), std::move(dwq), std::move(dwk)};
   }
   const Api& a = api();
-  const Tensor qk = kernel_layout(q), kk = kernel_layout(k), ct = table_layout(cos), st = table_layout(sin);
+  const Tensor qk = rows_layout(q), kk = rows_layout(k), ct = table_layout(cos), st = table_layout(sin);
   // the upstream gradient may arrive in another type and with arbitrary strides
-  const Tensor gq = kernel_layout(d_q.to(q.scalar_type())), gk = kernel_layout(d_k.to(q.scalar_type()));
+  const Tensor gq = rows_layout(d_q.to(q.scalar_type())), gk = rows_layout(d_k.to(q.scalar_type()));
   const OptTensor wq = weight_layout(q_weight), wk = weight_layout(k_weight);
   const int B = (int)q.size(0), Hq = (int)q.size(1), Hkv = (int)k.size(1), T = (int)q.size(2), D = (int)q.size(3);
   const int64_t bytes = weights ? a.qk_norm_rope_backward_workspace(B, Hq, Hkv, T, D, dtype_id(q)) : 0;
@@ -230,7 +231,7 @@ Tensor append_rope_gpu(const Tensor& q, const Tensor& k, const Tensor& v, const 
     if (!t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
   Tensor q_out = empty_same(q);
   if (q.numel() == 0) return q_out;
-  const Tensor qk = kernel_layout(q), kk = kernel_layout(k), vk = kernel_layout(v), ct = table_layout(cos), st = table_layout(sin);
+  const Tensor qk = rows_layout(q), kk = rows_layout(k), vk = rows_layout(v), ct = table_layout(cos), st = table_layout(sin);
   const Tensor table = unit_rows(page_table);
   const OptTensor wq = weight_layout(q_weight), wk = weight_layout(k_weight);
   const Lengths l(lens), nl(new_lens);

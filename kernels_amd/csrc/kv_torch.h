@@ -123,13 +123,13 @@ struct Gil {
 };
 
 // The tensor itself when the kernels can read it in place (unit stride along the head dimension, the others and the base
-// address multiples of 16 bytes, rows that advance), otherwise a contiguous copy.  Rows of one head are addressed with 32-bit byte offsets.
-inline Tensor kernel_layout(const Tensor& t) {
+// address multiples of 16 bytes, rows that advance), otherwise a contiguous copy.  offsets32: rows of one head are addressed with 32-bit byte offsets.
+inline Tensor kernel_layout(const Tensor& t, bool offsets32 = true) {
   const int64_t es = t.element_size(), vec = 16 / es, T = t.size(2);
   const auto s = t.strides();
   bool ok = (s[3] == 1 || t.size(3) == 1) && reinterpret_cast<uintptr_t>(t.const_data_ptr()) % 16 == 0;
   for (int i = 0; i < 3; ++i) ok = ok && (t.size(i) <= 1 || s[i] % vec == 0);
-  ok = ok && (T <= 1 || (s[2] > 0 && s[2] <= 0xffffffffLL / es / (T + 1024)));
+  ok = ok && (T <= 1 || (s[2] > 0 && (!offsets32 || s[2] <= 0xffffffffLL / es / (T + 1024))));
   if (ok) return t;
   return t.is_contiguous() ? t.clone(at::MemoryFormat::Contiguous) : t.contiguous();
 }

@@ -40,3 +40,46 @@ def test_values_keep_every_bit(dtype, D, rot, T, eps):
     paged_append_rope(q, q, v, *pages, table, torch.tensor([T], dtype=torch.int32, device=DEV), *tables, eps=eps)
     got = pages[1].transpose(0, 1).reshape(2, width * page, D)[:, :T]
     assert torch.equal(_bits(got), _bits(v[0]))
+
+
+def _allocated(call):
+    """(result, bytes that the call allocated at most)"""
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    torch.cuda.reset_peak_memory_stats()
+    out = call()
+    torch.cuda.synchronize()
+    return out, torch.cuda.max_memory_allocated() - before
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_rows_any_distance_apart(dtype):
+    """Rows of a head further apart than 32-bit byte offsets reach: read in place, the bits of a contiguous copy."""
+    Hq, Hkv, T, D = 4, 2, 600, 64
+    step = (1 << 32) // dtype.itemsize // (T + 1000) // 64 * 64
+    assert step * T * dtype.itemsize > 1 << 30 and step * (T + 1024) * dtype.itemsize > 1 << 32
+    g = torch.Generator(device=DEV).manual_seed(1)
+    far = torch.empty(step * T, dtype=dtype, device=DEV).as_strided((1, 2 * (Hq + 2 * Hkv), T, D), (0, D, step, 1))
+    far.copy_(torch.randn(far.shape, generator=g, device=DEV))
+    near = far.contiguous()
+    tables, lens = [t.to(DEV) for t in _tables(T, D)], torch.tensor([T], dtype=torch.int32, device=DEV)
+    w = torch.rand(D, generator=g, device=DEV).to(dtype)
+    forward, backward = torch.ops.alexdremov_qk_norm_rope.forward, torch.ops.alexdremov_qk_norm_rope.backward
+    page = 40
+    table = torch.arange(T // page, dtype=torch.int32, device=DEV)[None]
+    empty = torch.zeros(T // page, Hkv, page, D, dtype=dtype, device=DEV)
+    results = []
+    for x in (near, far):
+        q, k, v, dq, dk, _ = x.split([Hq, Hkv, Hkv] * 2, dim=1)
+        pages = [empty.clone(), empty.clone()]
+        calls = [lambda: forward(q, k, *tables, w, w, lens, None, 1e-6, False),
+                 lambda: backward(dq, dk, q, k, *tables, w, w, lens, None, 1e-6, False, False)[:2],
+                 lambda: (paged_append_rope(q, k, v, *pages, table, lens, *tables, w, w, eps=1e-6),)]
+        results.append([])
+        for call in calls:
+            out, most = _allocated(call)
+            copied = x is far and most >= 1.25 * sum(t.numel() * t.element_size() for t in out)
+            assert not copied, most
+            results[-1] += out
+        results[-1] += pages
+    assert all(torch.equal(a, b) and a.any() for a, b in zip(*results))
