@@ -24,7 +24,7 @@ bool is_rotation(const Tensor& q, const Tensor& cos, const Tensor& sin, const Op
                     positions->size(1) != q.size(2) || positions->device() != q.device()))
     return false;
   if (!eps) return !q_weight && !k_weight;
-  return (float)*eps > 0.0f && std::isfinite((float)*eps);
+  return (float)*eps > 0.0f && *eps < 3.4e38;
 }
 // Rows that the kernels can read in place, or a copy.
 Tensor table_layout(const Tensor& t) {

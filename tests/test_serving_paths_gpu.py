@@ -4,6 +4,7 @@ import pytest
 import torch
 
 from paged_attention import paged_append_rope
+from qk_norm_rope import qk_norm_rope
 from tests.test_drafted_tokens_gpu import _tables
 from tests.test_paged_attention_gpu import DEV, DTYPES
 
@@ -83,3 +84,21 @@ def test_rows_any_distance_apart(dtype):
             results[-1] += out
         results[-1] += pages
     assert all(torch.equal(a, b) and a.any() for a, b in zip(*results))
+
+
+@pytest.mark.parametrize("eps", [0.0, -1e-6, 1e-60, 3.4e38, 3.402e38, 1e39, float("inf"), float("nan")])
+def test_eps_that_float32_does_not_hold(eps):
+    """Refused by name, whichever way it is out of range."""
+    q, table = torch.zeros(1, 1, 3, 32, device=DEV), torch.zeros(3, 16, device=DEV)
+    with pytest.raises(AssertionError, match="eps must be a positive number of float32"):
+        qk_norm_rope(q, q, table, table, eps=eps)
+    pages, one = torch.zeros(1, 1, 4, 32, device=DEV), torch.zeros(1, 1, dtype=torch.int32, device=DEV)
+    with pytest.raises(AssertionError, match="eps must be a positive number of float32"):
+        paged_append_rope(q, q, q, pages, pages.clone(), one, one[0] + 3, table, table, eps=eps)
+
+
+def test_the_largest_eps():
+    q = torch.ones(1, 1, 3, 32, device=DEV)
+    out = qk_norm_rope(q, q, torch.ones(3, 16, device=DEV), torch.zeros(3, 16, device=DEV), eps=3.39e38)[0]
+    # the root, a product: some roundings of float32
+    assert ((out.double() * 3.39e38 ** 0.5 - 1).abs() <= 8 * 2.0 ** -24).all()
