@@ -69,12 +69,11 @@ template <typename T> SA_DEV void unpack(float* x, const T* from) {
 #pragma unroll
   for (int e = 0; e < Elem<T>::VEC; ++e) x[e] = (float)f[e];
 }
-template <typename T, bool STREAMING> SA_DEV void pack(T* to, const float* x) {
+template <typename T> SA_DEV u32x4 packed(const float* x) {
   typename Elem<T>::Frag f;
 #pragma unroll
   for (int e = 0; e < Elem<T>::VEC; ++e) f[e] = (T)x[e];
-  if constexpr (STREAMING) sa::store_streaming(to, __builtin_bit_cast(u32x4, f));
-  else *reinterpret_cast<typename Elem<T>::Frag*>(to) = f;
+  return __builtin_bit_cast(u32x4, f);
 }
 template <int N> SA_DEV void load_floats(float* x, const float* from) {
   typedef float Part __attribute__((ext_vector_type(N < 4 ? N : 4)));
@@ -201,33 +200,33 @@ template <typename T, int D, bool INTER, bool STREAMING> struct RowStore {
       }
     }
   }
+  SA_DEV static void store(T* to, const u32x4& v) {
+    if constexpr (STREAMING) sa::store_streaming(to, v);
+    else *reinterpret_cast<u32x4*>(to) = v;
+  }
   SA_DEV void put(const float* x) const {
-    constexpr int V = L::V;
     if constexpr (PAIRS || HALVES) {
-      typename Elem<T>::Frag a, b;
-#pragma unroll
-      for (int e = 0; e < V; ++e) a[e] = (T)x[e], b[e] = (T)x[V + e];
-      put(__builtin_bit_cast(u32x4, a), __builtin_bit_cast(u32x4, b));
+      put(packed<T>(x), packed<T>(x + L::V));
     } else if (has_first) {
-      pack<T, STREAMING>(first, x);
-      pack<T, STREAMING>(second, x + V);
+      store(first, packed<T>(x));
+      store(second, packed<T>(x + L::V));
     }
   }
   // The two chunks as bytes.
   SA_DEV void put(u32x4 one, u32x4 two) const {
-    if constexpr (PAIRS || HALVES)
+    if constexpr (PAIRS || HALVES) {
       if (exchanged)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const uint32_t got = (uint32_t)other((int)(odd ? one[e] : two[e]));
           one[e] = odd ? got : one[e], two[e] = odd ? two[e] : got;
         }
-    auto store = [](T* to, const u32x4& v) {
-      if constexpr (STREAMING) sa::store_streaming(to, v);
-      else *reinterpret_cast<u32x4*>(to) = v;
-    };
-    if (has_first) store(first, one);
-    if (has_second) store(second, two);
+      if (has_first) store(first, one);
+      if (has_second) store(second, two);
+    } else if (has_first) {
+      store(first, one);
+      store(second, two);
+    }
   }
   SA_DEV void next(int64_t step) { first += step, second += step; }
 };
@@ -359,8 +358,7 @@ template <typename T> __global__ __launch_bounds__(256) void rope_sum_kernel(con
 
 // ---- into the pages ---------------------------------------------------------------------------------------------------
 // Token i of n = new_lens[b] of sequence b goes to position lens[b] - n + i, its angle is that of its entry in `positions`, or of that position.  k is
-// turned and v goes as bytes: by way of float32 numbers, signalling NaN of 16 bits would come back quiet (and prompts of up to 2048 tokens of 8 sequences,
-// 32 / 8 heads, D = 128, bfloat16 took 61-65 us instead of 55-57); q is turned into a tensor of its own.
+// turned and v goes as bytes: by way of float32 numbers, signalling NaN of 16 bits would come back quiet; q is turned into a tensor of its own.
 struct AppendRopeParams {
   const void *q, *k, *v;
   void *q_out, *k_pages, *v_pages;    // q_out contiguous [B, Hq, T, D]
@@ -376,7 +374,10 @@ struct AppendRopeParams {
   int chunk, q_chunks, k_chunks;      // layers of the grid: q's, k's, then v's
   ChunkDiv by_tokens, by_page;
 };
-template <typename T, int D, bool INTER, bool STREAMING> __global__ __launch_bounds__(256) void append_rope_kernel(const AppendRopeParams p) {
+// Four waves to a SIMD in 16 bits: told so, the compiler keeps all but 2 to 14 scalar registers (bfloat16, D = 16: 47 to 80) where five waves spill 51 to 81
+// (bfloat16, 32 / 8 heads, D = 128, five -> four, us: prompts of up to 2048 tokens of 8 sequences 63-68 -> 62-66, up to 1024 of 2 13.3 -> 11.6).
+template <typename T, int D, bool INTER, bool STREAMING>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(4, sizeof(T) == 2 ? 4 : 8))) void append_rope_kernel(const AppendRopeParams p) {
   using L = RopeLanes<T, D>;
   constexpr int V = L::V;
   const int layer = blockIdx.y, kind = layer < p.q_chunks ? 0 : layer < p.q_chunks + p.k_chunks ? 1 : 2;
@@ -416,21 +417,16 @@ template <typename T, int D, bool INTER, bool STREAMING> __global__ __launch_bou
     float c[V], s[V], row[2 * V];
     if (live && kind != 2) load_angles<INTER>(c, s, p.table, (int)at, lane);
     for (int h = h0; h < h1; ++h, x += sh, to.next(own_sh)) {
-      if (kind == 2) {
-        u32x4 one = {0, 0, 0, 0}, two = one;
-        if (live) one = *reinterpret_cast<const u32x4*>(x + lane.a), two = *reinterpret_cast<const u32x4*>(x + lane.b);
-        to.put(one, two);
-        continue;
-      }
-      if (live) {
+      u32x4 one = {0, 0, 0, 0}, two = one;
+      if (live && kind == 2) {
+        one = *reinterpret_cast<const u32x4*>(x + lane.a), two = *reinterpret_cast<const u32x4*>(x + lane.b);
+      } else if (live) {
         unpack<T>(row, x + lane.a);
         unpack<T>(row + V, x + lane.b);
         norm_and_turn<D, L::LANES, INTER, V>(row, w, c, s, lane, p.eps);
-      } else {
-#pragma unroll
-        for (int e = 0; e < 2 * V; ++e) row[e] = 0.0f;
+        one = packed<T>(row), two = packed<T>(row + V);
       }
-      to.put(row);
+      to.put(one, two);   // (one call for both: of stores that it joins the compiler has dropped that they go past the caches)
     }
   }
 }
