@@ -15,7 +15,11 @@ using ElemT = __bf16;
 #endif
 
 template <typename F> static int by_shape(int D, bool inter, bool streaming, F&& f) {
-  auto stores = [&](auto d, auto i) { return streaming ? f(d, i, std::true_type{}) : f(d, i, std::false_type{}); };
+  auto stores = [&](auto d, auto i) {
+    if constexpr (may_go_past_caches(decltype(d)::value * (int)sizeof(ElemT)))
+      if (streaming) return f(d, i, std::true_type{});
+    return f(d, i, std::false_type{});
+  };
   auto pairs = [&](auto d) { return inter ? stores(d, std::true_type{}) : stores(d, std::false_type{}); };
   switch (D) {
     case 16: return pairs(std::integral_constant<int, 16>{});

@@ -42,5 +42,6 @@ inline bool past_caches(int64_t rows, int D, int rot, bool inter, int elem_size)
   const bool lines = inter ? D * elem_size % 256 == 0 : rot * elem_size % 256 == 0 && (D - rot) * elem_size % 256 == 0;
   return (lines || D * elem_size == 128 || (D * elem_size == 256 && 2 * rot == D)) && 2 * rows * D * elem_size > (int64_t(32) << 20);
 }
+constexpr bool may_go_past_caches(int row_bytes) { return row_bytes >= 128; }   // the kernels that there are: never so for shorter rows
 
 }  // namespace kv
