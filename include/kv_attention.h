@@ -124,7 +124,7 @@ int kv_paged_keep(void* k_pages, void* v_pages, const int32_t* page_table, int64
                   int B, int H, int M, int D, int num_pages, int page_size, int width, int dtype, void* stream);
 
 /* Norms of queries and keys for each head and the rotation by position.  A row x (D channels) of q [B,Hq,T,D] or k [B,Hkv,T,D] becomes
- *   y = x * w / sqrt(mean(x^2) + eps)      eps 0: y = x, and no weights
+ *   y = x * w / sqrt(mean(x^2) + eps)      eps below 3.4e38; 0: y = x, and no weights
  * and of its first `rot` channels the pairs (a, b) become (a cos - b sin, b cos + a sin): channels i and i + rot / 2, or 2 i and 2 i + 1 if interleaved,
  * with cos[at][i] and sin[at][i].  at: positions[b][t] at the strides int64[2], or t where positions is NULL.
  * rot: a multiple of 16 up to D.  cos, sin: float32 [table_rows, rot / 2], rows a multiple of 4 elements apart, 16-byte aligned.  Weights: [D] of the element

@@ -528,7 +528,7 @@ const char* kv_error_string(int code) {
     case KV_ERR_DTYPE: return "unsupported dtype id (0 = float32, 1 = float16, 2 = bfloat16)";
     case KV_ERR_HEAD_DIM: return "head dimension must be one of 16, 32, 64, 128, 256";
     case KV_ERR_ARG: return "invalid argument (null pointer, negative size, Hq not a multiple of Hkv, page_size or context_size < 1, "
-                            "back_contexts < 0, a scale beyond 2^127)";
+                            "back_contexts < 0, a scale beyond 2^127, rot or eps out of range, weights without norms)";
     case KV_ERR_LAYOUT: return "unsupported layout (dim stride must be 1; pointers and strides 16-byte aligned, strides not negative)";
     case KV_ERR_TOO_LARGE: return "problem too large for one launch";
     case KV_ERR_WORKSPACE: return "workspace missing or smaller than the *_workspace function says";

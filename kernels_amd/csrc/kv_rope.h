@@ -231,7 +231,7 @@ template <typename T, int D, bool INTER, bool STREAMING> struct RowStore {
   SA_DEV void next(int64_t step) { first += step, second += step; }
 };
 
-// (five waves to a SIMD: up to 102 registers, and none spills)
+// (five waves to a SIMD: up to 96 registers, which come in eights, and none spills)
 template <typename T, int D, bool INTER, bool STREAMING> __global__ __launch_bounds__(256, 5) void rope_kernel(const RopeParams p) {
   using L = RopeLanes<T, D>;
   constexpr int V = L::V;

@@ -141,7 +141,7 @@ def paged_append_rope(
     """:func:`paged_append` with what :func:`qk_norm_rope.qk_norm_rope` does on the way: one pass from a projection's output to the cache.
 
     The keys of new tokens are turned by their positions, and with ``eps`` normed for each head first, as they go into the pages, the values
-    go as they are, and the queries, ``(batch, heads, tokens, head_dim)``, come back turned likewise, ready for :func:`paged_attention` or
+    go as they are, bit by bit, and the queries, ``(batch, heads, tokens, head_dim)``, come back turned likewise, ready for :func:`paged_attention` or
     :func:`paged_tree_attention`.
 
     Args:
@@ -207,8 +207,9 @@ def paged_tree_attention(
             its ancestors.  All see the positions before the drafted ones.  Any mask will do; entries of tokens beyond ``new_lens[b]`` are not used
 
     Token ``i`` of the ``n`` drafted ones is in the cache at position ``lens[b] - n + i``, whatever its depth; with the lower triangle as `tree`, this is
-    :func:`paged_attention` with its default, causal windows.  What that function says of padding, of tokens that see nothing, of values that are
-    not finite, of bits and of capturing holds here too.  Forward only.  :func:`paged_keep` moves the accepted tokens together afterwards.
+    :func:`paged_attention` with its default, causal windows.  There are no other windows (chunks, back contexts): every drafted token sees the whole
+    context.  What that function says of padding, of tokens that see nothing, of values that are not finite, of bits, of capturing and of tables much wider
+    than their sequences holds here too.  Forward only.  :func:`paged_keep` moves the accepted tokens together afterwards.
     """
     if ops.takes_native_call(q, k_pages, v_pages, page_table, lens, tree, new_lens):
         result = _eager_tree(q, k_pages, v_pages, page_table, lens, tree, sm_scale, new_lens, return_lse)
