@@ -11,7 +11,7 @@
 // that none does become zeros.
 //
 // Bound by memory up to 64 rows, by vector and matrix instructions, which hardly overlap, above: 64 rows, D = 128, bfloat16, 256 key heads of 8192 (1.07 GB)
-// 217 us, 5.0 TB/s, log-uniform up to 8192 52-91 us for 38-69 us of a copy's rate; 256 rows, 64 of 8192 92 us, 0.75 PFLOP/s, matrix units busy 43 %, vector units 43 %
+// 217 us, 5.0 TB/s, log-uniform up to 8192 52-91 us for 32-58 us at a copy's rate (6.05 TB/s); 256 rows, 64 of 8192 92 us, 0.75 PFLOP/s, matrix units busy 43 %, vector units 43 %
 // of the time.  64 rows in us: two waves of rows alone 64 (log-uniform) and 187 (from 4096 on), with places in scalar registers 59 and 179, two waves to each block
 // of rows 52 and 172.
 #pragma once
